@@ -283,6 +283,82 @@ int moe_mi355x_moe_sublayer_fp8(const void* h, const void* h_add, const void* ln
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * A step over the 8-bit paged KV cache: seqs sequences of which each gets up to max_new new tokens, tokens rows
+ * in all (a captured step's capacity; rows behind the last sequence's are padding), block tables of max_pages
+ * columns, heads query and kv_heads kv heads.  No counterpart in the reference (its cache is contiguous,
+ * unquantised and planned on the host).
+ * seqs <= 4096, tokens <= 262144, 1 <= max_new, 1 <= max_pages <= 2^22, heads / kv_heads <= 16.
+ */
+typedef struct moe_mi355x_plan_shape {
+  int seqs, tokens, max_new, max_pages, heads, kv_heads;
+} moe_mi355x_plan_shape;
+
+/*
+ * Block tables, slots and work lists of a step, built on the GPU from the lengths alone.  Rows are filled in
+ * sequence order: sequence b owns rows cu[b] .. cu[b+1] with cu[b+1] = min(tokens, sum of clamp(new, 0,
+ * max_new) up to b), so what does not fit the rows is left out of the step.
+ *   cached_lens  int32 [seqs]             tokens in the cache (clamped to 0 .. 16 max_pages)
+ *   new_lens     int32 [seqs]             tokens of this step
+ *   block_tables int32 [seqs, max_pages]  in and out: the new pages' entries are written, others left as they
+ *                                         were; sequences must not share a page that gets tokens
+ *   free_pages   int32 [n_free]           taken in order, sequence by sequence; past its end the entries are -1
+ *   plan         plan_bytes >= paged_plan_bytes(shape), 16-byte aligned; read by the entry points below, which
+ *                take the same shape
+ * paged_plan_bytes returns 0 for an unsupported shape, and puts (offsets not null) the positions, in int32 from the
+ * plan's start, of: the pages taken [1] (more than n_free: the list ran out), cu [seqs + 1], the context lengths
+ * with this step's tokens [seqs], the position of each row in its sequence [tokens] and its slot, 16 * page +
+ * position % 16 [tokens]; both -1 for padding rows, the slot also where there is no page.
+ */
+enum { MOE_PLAN_PAGES, MOE_PLAN_CU, MOE_PLAN_CONTEXT, MOE_PLAN_POSITIONS, MOE_PLAN_SLOTS, MOE_PLAN_SECTIONS };
+size_t moe_mi355x_paged_plan_bytes(const moe_mi355x_plan_shape* shape, int32_t* offsets);
+int moe_mi355x_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int32_t* block_tables,
+                          const int32_t* free_pages, int n_free, const moe_mi355x_plan_shape* shape, void* plan,
+                          size_t plan_bytes, void* stream);
+
+/*
+ * Quantising append of a step's keys and values to the 8-bit paged cache: e4m3 codes with one scale per (page,
+ * kv head), the smallest power of two s >= 2^-100 with |x| / s <= 448 for the finite values of the page (infinities
+ * saturate, NaN stays NaN).  A page that begins with this step's tokens is written whole, zeros behind them; in
+ * a page that goes on the scale can only grow, and its codes are then re-coded.  Tokens without a page (a
+ * table entry outside [0, num_pages)) are not kept.
+ *   k, v     bf16 [tokens, kv_heads, 128], rows of a token k_stride / v_stride values apart (multiples of 8)
+ *   k_cache  e4m3 [num_pages, kv_heads, 8, 16, 16]     (dim / 16, token, dim % 16)
+ *   v_cache  e4m3 [num_pages, kv_heads, 2, 4, 64, 4]   (dim / 64, token / 4, dim % 64, token % 4)
+ *   k_scale, v_scale  fp32 [num_pages, kv_heads], powers of two
+ * head_dim == 128, page_size == 16.
+ */
+int moe_mi355x_kv_append_fp8(const void* k, const void* v, long long k_stride, long long v_stride, void* k_cache,
+                             void* v_cache, float* k_scale, float* v_scale, int head_dim, int page_size,
+                             int num_pages, const moe_mi355x_plan_shape* shape, const void* plan, void* stream);
+
+/*
+ * moe_mi355x_kv_append_fp8 from the fused q/k/v projections, with q_norm / k_norm and the rotary embedding at each
+ * row's position (TF/models/qwen3_moe/modeling_qwen3_moe.py:162-171), for prompts and single tokens.  fp32
+ * throughout (the angle position * inv_freq in 64 bits) and one rounding: q to bf16, k and v to their codes.
+ *   qkv      bf16 [tokens, (heads + 2 kv_heads) * 128]  (q heads, then k heads, then v heads)
+ *   q_norm_w, k_norm_w bf16 [128]   inv_freq fp32 [64]   q_out bf16 [tokens, heads, 128] (padding rows: 0)
+ */
+int moe_mi355x_qk_norm_rope_append_fp8(const void* qkv, const void* q_norm_w, const void* k_norm_w,
+                                       const float* inv_freq, float eps, void* q_out, void* k_cache, void* v_cache,
+                                       float* k_scale, float* v_scale, int head_dim, int page_size, int num_pages,
+                                       const moe_mi355x_plan_shape* shape, const void* plan, void* stream);
+
+/*
+ * Causal GQA attention of a step's tokens, prompts' and single ones, over the 8-bit paged cache: for a token at
+ * position p of its sequence and query head h, over the keys 0 .. p of kv head h / (heads / kv_heads),
+ *   out = bf16( softmax(scale * q . K) . V )
+ * with fp32 scores, softmax and sums, and bf16 probabilities in the product with V.  Keys of a page that the table
+ * does not hold (an entry outside [0, num_pages)) are left out; a row without keys and a padding row are 0.
+ *   q   bf16 [tokens, heads, 128], rows of a token q_stride values apart (a multiple of 8)
+ *   out bf16 [tokens, heads, 128]      block_tables as the plan left them      scale finite, > 0
+ */
+size_t moe_mi355x_paged_attn_fp8_workspace_bytes(const moe_mi355x_plan_shape* shape);
+int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache,
+                              const float* k_scale, const float* v_scale, const int32_t* block_tables, int head_dim,
+                              int page_size, int num_pages, float scale, const moe_mi355x_plan_shape* shape,
+                              const void* plan, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing (instrumentation; no counterpart in the reference).  While enabled, each
  * kernel launch of this library is bracketed by hipEvents on its stream; profile_read
  * waits for them and returns the launch count and summed duration (ms) of one slot:

@@ -28,21 +28,27 @@ from .experts import (  # noqa: F401
     swap_moe_blocks,
 )
 from .kernels import (  # noqa: F401
+    PagedPlan,
     align,
     experts_bf16,
     experts_fp8,
     kv_append,
+    kv_append_fp8,
     moe_block_bf16,
     moe_block_fp8,
     moe_sublayer_fp8,
     paged_attention_decode,
+    paged_attention_fp8,
+    paged_plan,
     qk_norm_rope_append,
+    qk_norm_rope_append_fp8,
     linear_bf16,
     rms_norm,
     quantize_act_fp8,
     quantize_weight_fp8,
     route,
     topk_softmax,
+    unpack_kv_fp8,
 )
 
 __version__ = "0.1.0"

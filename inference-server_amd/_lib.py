@@ -16,6 +16,19 @@ _c_int, _c_size, _vp = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
 _fp = ctypes.POINTER(ctypes.c_float)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
+
+
+class PlanShape(ctypes.Structure):
+    """``moe_mi355x_plan_shape``"""
+
+    _fields_ = [(n, _c_int) for n in ("seqs", "tokens", "max_new", "max_pages", "heads", "kv_heads")]
+
+
+# MOE_PLAN_*: sections of a plan that callers read
+PLAN_SECTIONS = ("pages_used", "cu_tokens", "context_lens", "positions", "slots")
+_shape = ctypes.POINTER(PlanShape)
+_c_ll = ctypes.c_longlong
+
 # name -> (restype, argtypes); mirrors include/moe_mi355x.h
 SIGNATURES = {
     "moe_mi355x_error_string": (ctypes.c_char_p, [_c_int]),
@@ -60,6 +73,15 @@ SIGNATURES = {
     "moe_mi355x_moe_sublayer_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
     "moe_mi355x_moe_sublayer_fp8": (_c_int, [_vp, _vp, _vp, ctypes.c_float, _vp, _c_int, _c_int, _c_int, _c_int,
                                              _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "moe_mi355x_paged_plan_bytes": (_c_size, [_shape, _vp]),
+    "moe_mi355x_paged_plan": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _shape, _vp, _c_size, _vp]),
+    "moe_mi355x_kv_append_fp8": (_c_int, [_vp, _vp, _c_ll, _c_ll, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _shape,
+                                          _vp, _vp]),
+    "moe_mi355x_qk_norm_rope_append_fp8": (_c_int, [_vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp,
+                                                    _c_int, _c_int, _c_int, _shape, _vp, _vp]),
+    "moe_mi355x_paged_attn_fp8_workspace_bytes": (_c_size, [_shape]),
+    "moe_mi355x_paged_attn_fp8": (_c_int, [_vp, _c_ll, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int,
+                                           ctypes.c_float, _shape, _vp, _vp, _vp, _c_size, _vp]),
     "moe_mi355x_profile_enable": (_c_int, [_c_int]),
     "moe_mi355x_profile_read": (_c_int, [_c_int, ctypes.POINTER(_c_int), ctypes.POINTER(ctypes.c_double)]),
     "moe_mi355x_profile_slot_name": (ctypes.c_char_p, [_c_int]),

@@ -1,0 +1,627 @@
+// Causal GQA attention over the 8-bit paged KV cache (kv_fp8.h) for a step that mixes prompts, chunks of them and
+// single tokens (paged_plan.h): for token t of a sequence at position p, query head h and kv head h / G,
+//   o = sum_{j <= p} softmax_j(scale q . K_j) V_j
+// with K and V the values that the codes stand for, everything in fp32 but for two operands: the bf16 q, and
+// the probabilities exp(s - max), rounded to bf16 (half a step, 2^-9) for the second MFMA; their sum is
+// formed from the unrounded ones.  The codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8 with the
+// page's power-of-two scale), so both products run on the bf16 MFMAs without a further error.
+//
+// Two kernels, by the rows (tokens x heads of the group) that a sequence has for one kv head:
+//   short: up to 16 rows (a decoding sequence), bound by the cache's bytes.  One workgroup per (sequence, kv
+//     head, run of pages); its 4 waves take pairs of pages round robin, straight from HBM to the MFMA.
+//   tile: more rows (prompts), bound by the MFMA and the softmax.  One workgroup per (128 rows, kv
+//     head); pages are widened to bf16 once per workgroup, in LDS.
+// Rows whose keys are split over several workgroups leave fp32 partial results that the merge kernel joins in key
+// order, so results do not depend on timing.
+#include "kv_fp8.h"
+#include "paged_plan.h"
+
+namespace {
+
+constexpr int kHD = kKvHead;
+constexpr int kPage = kPlanPage;
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kCachePolicyNT = 2;  // the instruction's cache-policy field: nt (streaming)
+constexpr int kPadBlocks = 8;      // workgroups that clear the rows behind the last sequence
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+struct AttnFp8Args {
+  const uint16_t* q;  // [T][Hq][128], rows of a token q_stride values apart
+  long q_stride;
+  const uint8_t *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int32_t* tables;
+  const int32_t* plan;
+  uint16_t* out;         // [T][Hq][128]
+  float *short_o, *short_ml, *tile_o, *tile_ml;  // partial results, by item
+  int num_pages;
+  float scale;  // times log2(e)
+  PlanLayout p;
+};
+
+// A (page, kv head) block; no page: a size of 0, so its loads read zeros and touch no memory.  Word 3 is the
+// 32-bit data format (untyped loads return zeros without one).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint8_t* cache, int page, int Hkv, int g) {
+  const long blk = page < 0 ? 0 : (long)page * Hkv + g;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(cache + blk * kKvBlock), (short)0, page < 0 ? 0 : kKvBlock, 0x00020000);
+}
+template <int POLICY>
+__device__ __forceinline__ uint4 block_load(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, POLICY));
+}
+
+// 8 codes -> 8 bf16 values times the power of two `scale`, exactly
+__device__ __forceinline__ v8bf widen8(uint32_t lo, uint32_t hi, float scale) {
+  const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const v2bf b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const v2bf d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return (v8bf){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Reductions over lanes l, l ^ 16, l ^ 32, l ^ 48, resp. l, l ^ 32 (gfx950's row and half swaps)
+__device__ __forceinline__ float half_max(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float rows_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
+// The bytes of a quad of tokens (4 codes of one dim) of which the first `live` count
+__device__ __forceinline__ uint32_t quad_mask(int live) {
+  return live >= 4 ? 0xffffffffu : live <= 0 ? 0u : (1u << (8 * live)) - 1u;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+}
+
+// ---------------------------------------------------------------------------
+// short: S^T [16 keys x 16 rows] = K [16 x 128] Q^T (4 MFMAs 16x16x32 a page), then
+// O^T [128 x 16 rows] += V^T [128 x 32 keys] P^T (8 MFMAs for two pages).  Lane l has row l & 15 throughout, and
+// of its scores keys 4 (l >> 4) + i of each page, which are the 8 keys that the second MFMA wants from it.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void attn_fp8_short_kernel(AttnFp8Args a) {
+  const PlanLayout& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int Hkv = p.Hkv, G = p.G;
+  const int items = p.S * Hkv;
+  if ((int)blockIdx.x >= items) {  // rows behind the last sequence: zeros
+    const long row = (long)p.Hq * kHD / 8;  // 16-byte pieces of a token
+    const long end = p.T * row;
+    for (long i = a.plan[PH_TOKENS] * row + ((int)blockIdx.x - items) * 256 + threadIdx.x; i < end; i += kPadBlocks * 256)
+      ((uint4*)a.out)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
+  if (item >= a.plan[PH_SHORTS]) return;
+  const int4* it = (const int4*)(a.plan + p.shorts + (long)PI_INTS * item);
+  const int4 i0 = it[0], i1 = it[1];
+  const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
+  const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
+  const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
+  const int parts = __builtin_amdgcn_readfirstlane(i1.z);
+  const int rows = ntok * G;
+
+  // Q^T operand: row lr, dims in the order in which the K block's loads bring them
+  const int row_tok = lr / G, row_head = lr % G;
+  v8bf qop[4];
+  {
+    const bool live = lr < rows;
+    const uint16_t* src = a.q + (tok + (live ? row_tok : 0)) * a.q_stride + (long)(g * G + (live ? row_head : 0)) * kHD;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const uint4 v = *(const uint4*)(src + 64 * (kk >> 1) + 16 * lg + 8 * (kk & 1));
+      qop[kk] = __builtin_bit_cast(v8bf, live ? v : make_uint4(0, 0, 0, 0));
+    }
+  }
+  const int key_end = pos + row_tok + 1;  // of this lane's row
+
+  float m_run = -INFINITY, l_run = 0.f;
+  v4f o[8];  // o[4 j + d][i]: dim 64 j + 16 lg + 4 i + d of row lr
+#pragma unroll
+  for (int n = 0; n < 8; ++n) o[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+
+  const int32_t* table = a.tables + (long)seq * p.max_pages;
+  // 32 pairs of pages at a time: lane l holds the id and the scales of page l & 1 of this wave's pair l >> 1, so
+  // that a page's loads wait for no other
+  for (int first = page0; first < page1; first += 64 * kWaves) {
+    const int mine = first + 2 * (wave + kWaves * (lane >> 1)) + (lane & 1);
+    int my_page = mine < page1 ? table[mine] : -1;
+    if (my_page >= a.num_pages || my_page < 0) my_page = -1;  // a pad or a stale id: an empty page
+    const long my_blk = my_page < 0 ? 0 : (long)my_page * Hkv + g;
+    const float my_ks = a.num_pages > 0 ? a.k_scale[my_blk] : 1.f, my_vs = a.num_pages > 0 ? a.v_scale[my_blk] : 1.f;
+    const int pairs = (min(page1 - first, 64 * kWaves) + 1) / 2;  // of all waves
+    const int n = pairs > wave ? (pairs - wave + kWaves - 1) / kWaves : 0;
+
+    uint4 kr[2][2], vr[2][2];
+    auto page_at = [&](int i, int h) __attribute__((always_inline)) {
+      return i < 32 ? __builtin_amdgcn_readlane(my_page, 2 * i + h) : -1;
+    };
+    auto scale_at = [&](float s, int i, int h) __attribute__((always_inline)) {
+      return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s), 2 * i + h));
+    };
+    // issued unconditionally (a branch around loads makes the compiler wait where it joins)
+    auto load = [&](uint4 (&r)[2][2], const uint8_t* cache, int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const __amdgpu_buffer_rsrc_t rs = block_rsrc(cache, page_at(i, h), Hkv, g);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) r[h][j] = block_load<kCachePolicyNT>(rs, lane * 16 + j * 1024);
+      }
+    };
+    load(kr, a.k_cache, 0);
+    load(vr, a.v_cache, 0);
+    for (int i = 0; i < n; ++i) {
+      v4f s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float ks = scale_at(my_ks, i, h);
+        s[h] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(kr[h][j].x, kr[h][j].y, ks), qop[2 * j], s[h], 0, 0, 0);
+          s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(kr[h][j].z, kr[h][j].w, ks), qop[2 * j + 1], s[h], 0, 0, 0);
+        }
+      }
+      load(kr, a.k_cache, i + 1);
+      const int key0 = (first + 2 * (wave + kWaves * i)) * kPage;
+      const bool all = page_at(i, 0) >= 0 && page_at(i, 1) >= 0 && key0 + 2 * kPage <= pos + 1;  // uniform
+      float sv[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[h][e] = s[h][e] * a.scale;
+      if (!all) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int end = page_at(i, h) < 0 ? 0 : key_end;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sv[h][e] = key0 + kPage * h + 4 * lg + e < end ? sv[h][e] : -INFINITY;
+          // codes behind the last key may be anything, a NaN too: zero them rather than multiply them by zero
+          const uint32_t mask = quad_mask(pos + ntok - (key0 + kPage * h + 4 * lg));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            vr[h][j].x &= mask;
+            vr[h][j].y &= mask;
+            vr[h][j].z &= mask;
+            vr[h][j].w &= mask;
+          }
+        }
+      }
+      float pm = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
+                       fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
+      pm = rows_max(pm);
+      if (__any(pm > m_run)) {  // some row's maximum grows
+        const float m_new = fmaxf(m_run, pm);
+        const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] *= corr;
+      }
+      const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+      float ps = 0.f;
+      v8bf pb;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(sv[h][e] - m_ref);
+          ps += x;
+          pb[4 * h + e] = (__bf16)x;
+        }
+      l_run += ps;  // this lane's keys; the row's lanes are summed at the end
+      const float vs0 = scale_at(my_vs, i, 0), vs1 = scale_at(my_vs, i, 1);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t v0[4] = {vr[0][j].x, vr[0][j].y, vr[0][j].z, vr[0][j].w};
+        const uint32_t v1[4] = {vr[1][j].x, vr[1][j].y, vr[1][j].z, vr[1][j].w};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const v2bf w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v0[d], vs0, false);
+          const v2bf w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v0[d], vs0, true);
+          const v2bf w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v1[d], vs1, false);
+          const v2bf w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v1[d], vs1, true);
+          const v8bf va = {w0[0], w0[1], w1[0], w1[1], w2[0], w2[1], w3[0], w3[1]};
+          o[4 * j + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[4 * j + d], 0, 0, 0);
+        }
+      }
+      load(vr, a.v_cache, i + 1);
+    }
+  }
+  l_run = rows_sum(l_run);
+
+  // join the 4 waves
+  __shared__ float s_m[kWaves][kShortRows], s_l[kWaves][kShortRows];
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][kShortRows][kHD + 4];
+  if (lg == 0) {
+    s_m[wave][lr] = m_run;
+    s_l[wave][lr] = l_run;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *(v4f*)&s_o[wave][lr][64 * j + 16 * lg + 4 * i] = (v4f){o[4 * j][i], o[4 * j + 1][i], o[4 * j + 2][i], o[4 * j + 3][i]};
+  __syncthreads();
+  const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  if (r >= rows) return;
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
+  float wgt[kWaves], L = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    wgt[w] = s_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - M);
+    L += s_l[w][r] * wgt[w];
+  }
+  float acc[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    acc[d] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) acc[d] += s_o[w][r][d0 + d] * wgt[w];
+  }
+  if (parts == 1) {
+    const float inv = M == -INFINITY ? 0.f : 1.0f / L;  // no key at all: zeros
+    uint16_t* dst = a.out + ((long)(tok + r / G) * p.Hq + g * G + r % G) * kHD + d0;
+    *(uint4*)dst = make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv),
+                              pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
+    return;
+  }
+  const long base = ((long)item * Hkv + g) * kShortRows + r;
+  float* dst = a.short_o + base * kHD + d0;
+  *(float4*)dst = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  *(float4*)(dst + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  if ((threadIdx.x & 15) == 0) *(float2*)(a.short_ml + 2 * base) = make_float2(M, L);
+}
+
+// ---------------------------------------------------------------------------
+// tile: 128 rows, 32 a wave, 64 keys (4 pages) a step.  S^T [32 keys x 32 rows] = K Q^T (8 MFMAs 32x32x16
+// per 32 keys), O^T [128 x 32 rows] += V^T [128 x 16 keys] P^T (4 MFMAs a page).  Lane l has row l & 31 and,
+// of a page's keys, 4 (l >> 5) + {0..3, 8..11}: again the 8 that the second MFMA wants from it.
+// In LDS, bf16: K [dim / 8][key 64][8 dims] and V [page][quad & 1][dim slot][8 keys], quads q and q + 2 together;
+// the slot 64 j + 16 d + x of dim 64 j + 4 x + d makes the writes contiguous.  Every read and write of 16
+// bytes is contiguous over the lanes that the LDS serves together.
+// ---------------------------------------------------------------------------
+constexpr int kStepPages = kTileKeys / kPage;
+
+__global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
+  const PlanLayout& p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 31, kg = lane >> 5;
+  const int Hkv = p.Hkv, G = p.G;
+  // neighbours in the launch go to different XCDs (8), so with 2, 4 or 8 kv heads an XCD's L2 holds few heads
+  const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
+  if (item >= a.plan[PH_TILES]) return;
+  const int4* it = (const int4*)(a.plan + p.tiles + (long)PI_INTS * item);
+  const int4 i0 = it[0], i1 = it[1];
+  const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
+  const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
+  const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
+  const int parts = __builtin_amdgcn_readfirstlane(i1.z);
+
+  __shared__ __attribute__((aligned(16))) uint4 s_k[2][kHD / 8][kTileKeys];
+  __shared__ __attribute__((aligned(16))) uint4 s_v[2][kStepPages][2][kHD];
+
+  const int r = 32 * wave + lr;
+  const bool live = r < ntok * G;
+  const int row_tok = min(r / G, ntok - 1);
+  const long row = (long)(tok + row_tok);
+  v8bf qop[8];
+  {
+    const uint16_t* src = a.q + row * a.q_stride + (long)(g * G + r % G) * kHD + 8 * kg;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(v8bf, *(const uint4*)(src + 16 * s));
+  }
+  const int key_end = pos + row_tok + 1;                              // of this lane's row
+  const int all_end = pos + min(32 * wave / G, ntok - 1) + 1;         // keys that every row of the wave sees
+  const int any_end = pos + min((32 * wave + 31) / G, ntok - 1) + 1;  // and that any sees
+
+  float m_run = -INFINITY, l_run = 0.f;
+  v16f o[4];  // o[db][i]: dim slot 32 db + 8 (i / 4) + 4 kg + i % 4 of row lr
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+
+  const int32_t* table = a.tables + (long)seq * p.max_pages;
+  // the ids and scales of 64 pages, one a lane
+  int my_page;
+  float my_ks, my_vs;
+  auto fetch = [&](int first) __attribute__((always_inline)) {
+    const int mine = first + lane;
+    my_page = mine < page1 ? table[mine] : -1;
+    if (my_page >= a.num_pages || my_page < 0) my_page = -1;
+    const long blk = my_page < 0 ? 0 : (long)my_page * Hkv + g;
+    my_ks = a.num_pages > 0 ? a.k_scale[blk] : 1.f;
+    my_vs = a.num_pages > 0 ? a.v_scale[blk] : 1.f;
+  };
+  auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
+  };
+  // a step's codes: K, 16 bytes (16 dims of a token) of pages wave / 2 and 2 + wave / 2; V, of page `wave`
+  // the quads kg and kg + 2 of 4 dims
+  uint4 kr[2], vr[2];
+  float ks[2], vs;
+  const int vj = lane >> 5, vq = (lane >> 4) & 1, vx = lane & 15;
+  auto load = [&](int l) __attribute__((always_inline)) {  // l: the step's first page among the 64
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = l + 2 * h + (wave >> 1);
+      ks[h] = lane_f(my_ks, at);
+      kr[h] = block_load<0>(block_rsrc(a.k_cache, __builtin_amdgcn_readlane(my_page, at), Hkv, g),
+                            (wave & 1) * 1024 + lane * 16);
+    }
+    vs = lane_f(my_vs, l + wave);
+    const __amdgpu_buffer_rsrc_t rv = block_rsrc(a.v_cache, __builtin_amdgcn_readlane(my_page, l + wave), Hkv, g);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) vr[h] = block_load<0>(rv, vj * 1024 + (vq + 2 * h) * 256 + vx * 16);
+  };
+  auto store = [&](int buf, int page) __attribute__((always_inline)) {
+    const int c = 4 * (wave & 1) + (lane >> 4);  // dims 16 c .. +16 of token lane & 15
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = (2 * h + (wave >> 1)) * kPage + (lane & 15);
+      s_k[buf][2 * c][key] = __builtin_bit_cast(uint4, widen8(kr[h].x, kr[h].y, ks[h]));
+      s_k[buf][2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
+    }
+    if ((page + kStepPages) * kPage > pos + ntok) {  // codes behind the last key may be anything, a NaN too
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t mask = quad_mask(pos + ntok - ((page + wave) * kPage + 4 * (vq + 2 * h)));
+        vr[h].x &= mask;
+        vr[h].y &= mask;
+        vr[h].z &= mask;
+        vr[h].w &= mask;
+      }
+    }
+    const uint32_t v0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, v1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      s_v[buf][wave][vq][64 * vj + 16 * d + vx] = __builtin_bit_cast(uint4, widen8(v0[d], v1[d], vs));
+  };
+
+  fetch(page0);
+  load(0);
+  store(0, page0);
+  __syncthreads();
+  int buf = 0;
+  for (int page = page0, l = 0; page < page1; page += kStepPages, buf ^= 1) {
+    const int here = l;  // this step's first page among the 64
+    uint64_t held = __ballot(my_page >= 0) >> here;  // which of its pages there are
+    const bool more = page + kStepPages < page1;
+    l += kStepPages;
+    if (more) {
+      if (l == 64) {
+        l = 0;
+        fetch(page + kStepPages);
+      }
+      load(l);
+    }
+    const int key0 = page * kPage;
+    if (key0 < any_end) {  // wave-uniform
+      v16f s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_k[buf][2 * k + kg][32 * b + lr]), qop[k],
+                                                         s[b], 0, 0, 0);
+      if (key0 + kTileKeys > all_end || (held & 15) != 15) {  // wave-uniform
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = key0 + 32 * b + 8 * (i >> 2) + 4 * kg + (i & 3);
+            const bool ok = key < key_end && ((held >> (2 * b + (i >> 3))) & 1);
+            s[b][i] = ok ? s[b][i] : -INFINITY;
+          }
+      }
+      float pm = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[0][i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pm = fmaxf(pm, s[1][i]);
+      pm = half_max(pm) * a.scale;
+      if (__any(pm > m_run)) {
+        const float m_new = fmaxf(m_run, pm);
+        const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+      }
+      const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+      float ps = 0.f;
+      v8bf pb[4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -m_ref));
+          ps += x;
+          pb[2 * b + (i >> 3)][i & 7] = (__bf16)x;
+        }
+      l_run += ps;
+#pragma unroll
+      for (int g4 = 0; g4 < kStepPages; ++g4)
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_v[buf][g4][kg][32 * d + lr]), pb[g4],
+                                                         o[d], 0, 0, 0);
+    }
+    if (more) store(buf ^ 1, page + kStepPages);
+    __syncthreads();
+  }
+  l_run = half_sum(l_run);
+  if (!live) return;
+  if (parts == 1) {
+    const float inv = m_run == -INFINITY ? 0.f : 1.0f / l_run;  // no key at all: zeros
+    uint16_t* dst = a.out + (row * p.Hq + g * G + r % G) * kHD;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int x = 8 * (i >> 2) + 4 * kg + (i & 3);
+        *(uint2*)(dst + 64 * j + 4 * x) = make_uint2(pack_bf16(o[2 * j][i] * inv, o[2 * j][i + 8] * inv),
+                                                     pack_bf16(o[2 * j + 1][i] * inv, o[2 * j + 1][i + 8] * inv));
+      }
+    return;
+  }
+  const long base = ((long)item * Hkv + g) * kTileRows + r;
+  float* dst = a.tile_o + base * kHD;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = 8 * (i >> 2) + 4 * kg + (i & 3);
+      *(float4*)(dst + 64 * j + 4 * x) = make_float4(o[2 * j][i], o[2 * j][i + 8], o[2 * j + 1][i], o[2 * j + 1][i + 8]);
+    }
+  if (kg == 0) *(float2*)(a.tile_ml + 2 * base) = make_float2(m_run, l_run);
+}
+
+// ---------------------------------------------------------------------------
+// merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order.  One workgroup per (rows,
+// kv head, row): 8 groups of 32 lanes take the items round robin, a lane 4 dims.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
+  const PlanLayout& p = a.p;
+  const int entry = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv, r = blockIdx.y;
+  if (entry >= a.plan[PH_MERGES]) return;
+  const int4 e = *(const int4*)(a.plan + p.merges + 4L * entry);
+  if (r >= e.w * p.G) return;
+  const int ns = abs(e.x), stride = e.x < 0 ? kTileRows : kShortRows;
+  const float* part = e.x < 0 ? a.tile_o : a.short_o;
+  const float* ml = e.x < 0 ? a.tile_ml : a.short_ml;
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  __shared__ float s_m[8], s_l[8];
+  __shared__ __attribute__((aligned(16))) v4f s_o[8][32];
+  float M = -INFINITY, L = 0.f;
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = grp; s < ns; s += 8) {
+    const long base = ((long)(e.y + s) * p.Hkv + g) * stride + r;
+    const float2 x = *(const float2*)(ml + 2 * base);
+    const v4f v = *(const v4f*)(part + base * kHD + 4 * lane);
+    if (x.x == -INFINITY) continue;  // only empty pages
+    const float m_new = fmaxf(M, x.x);
+    const float old = __builtin_amdgcn_exp2f(M - m_new), w = __builtin_amdgcn_exp2f(x.x - m_new);
+    M = m_new;
+    L = L * old + x.y * w;
+    acc = acc * old + v * w;
+  }
+  s_o[grp][lane] = acc;
+  if (lane == 0) {
+    s_m[grp] = M;
+    s_l[grp] = L;
+  }
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+  L = 0.f;
+  acc = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = s_m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i] - M);
+    L += s_l[i] * w;
+    acc += s_o[i][lane] * w;
+  }
+  const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+  uint16_t* dst = a.out + ((long)(e.z + r / p.G) * p.Hq + g * p.G + r % p.G) * kHD + 4 * lane;
+  *(uint2*)dst = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+}
+
+// Partial results: an item's rows and their (max, sum), for both kinds; none where no item is split.
+struct Parts {
+  long shorts, tiles;  // rows
+};
+Parts attn_parts(const PlanLayout& p) {
+  return {p.max_pages > kShortStep ? (long)p.S * p.Hkv * kShortRows : 0,
+          (long)p.max_pages * kPage > kTileMinKeys ? (long)p.split_tiles * p.Hkv * kTileRows : 0};
+}
+
+void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
+  a->short_o = c.take<float>(n.shorts * kHD);
+  a->short_ml = c.take<float>(n.shorts * 2);
+  a->tile_o = c.take<float>(n.tiles * kHD);
+  a->tile_ml = c.take<float>(n.tiles * 2);
+}
+
+bool attn_grid_ok(const PlanLayout& p) {
+  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) && moe_grid_fits((long)p.M * p.Hkv);
+}
+
+}  // namespace
+
+extern "C" size_t moe_mi355x_paged_attn_fp8_workspace_bytes(const moe_mi355x_plan_shape* shape) {
+  if (!plan_shape_ok(shape)) return 0;
+  const PlanLayout p = plan_layout(shape);
+  if (!attn_grid_ok(p)) return 0;
+  WsCarver c(nullptr);
+  AttnFp8Args a{};
+  attn_carve(c, attn_parts(p), &a);
+  return moe_align_up(c.off, 256);
+}
+
+extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache,
+                                         const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                                         int head_dim, int page_size, int num_pages, float scale,
+                                         const moe_mi355x_plan_shape* shape, const void* plan, void* out,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  MOE_RETURN_IF(!plan_shape_ok(shape) || head_dim != kHD || page_size != kPage || num_pages < 0, MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(!(scale > 0.f) || !(scale < INFINITY), MOE_ERR_INVALID_ARG);
+  if (shape->tokens == 0) return MOE_OK;
+  MOE_RETURN_IF(!q || !k_cache || !v_cache || !k_scale || !v_scale || !plan || !out, MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(shape->seqs > 0 && !block_tables, MOE_ERR_INVALID_ARG);
+  const PlanLayout p = plan_layout(shape);
+  MOE_RETURN_IF(!attn_grid_ok(p) || q_stride < (long)p.Hq * kHD, MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(q_stride % 8 || !moe_aligned16(q) || !moe_aligned16(k_cache) || !moe_aligned16(v_cache) ||
+                    !moe_aligned16(plan) || !moe_aligned16(out),
+                MOE_ERR_ALIGNMENT);
+  const size_t need = moe_mi355x_paged_attn_fp8_workspace_bytes(shape);
+  MOE_RETURN_IF(need > 0 && (!workspace || workspace_bytes < need), MOE_ERR_WORKSPACE);
+  AttnFp8Args a{};
+  a.q = (const uint16_t*)q, a.q_stride = q_stride;
+  a.k_cache = (const uint8_t*)k_cache, a.v_cache = (const uint8_t*)v_cache, a.k_scale = k_scale, a.v_scale = v_scale;
+  a.tables = block_tables, a.plan = (const int32_t*)plan, a.out = (uint16_t*)out;
+  a.num_pages = num_pages, a.scale = scale * kLog2e, a.p = p;
+  const Parts parts = attn_parts(p);
+  WsCarver c(workspace);
+  attn_carve(c, parts, &a);
+  hipStream_t s = (hipStream_t)stream;
+  if (p.N > 0) {
+    hipLaunchKernelGGL(attn_fp8_tile_kernel, dim3((unsigned)(p.N * p.Hkv)), dim3(256), 0, s, a);
+    MOE_CHECK_LAUNCH();
+  }
+  hipLaunchKernelGGL(attn_fp8_short_kernel, dim3((unsigned)(p.S * p.Hkv + kPadBlocks)), dim3(256), 0, s, a);
+  MOE_CHECK_LAUNCH();
+  if (parts.shorts + parts.tiles > 0 && p.M > 0) {
+    hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3((unsigned)(p.M * p.Hkv), parts.tiles > 0 ? kTileRows : kShortRows),
+                       dim3(256), 0, s, a);
+    MOE_CHECK_LAUNCH();
+  }
+  return MOE_OK;
+}

@@ -1,0 +1,87 @@
+// The plan of a step over the 8-bit paged KV cache: one int32 buffer that moe_mi355x_paged_plan
+// (paged_plan.hip) fills from the sequences' lengths and that the cache writers (kv_fp8.hip) and the
+// attention (attn_fp8.hip) read.  Sections, each from a multiple of 16 ints:
+//   head    [16]         counts (PH_*)
+//   cu      [B + 1]      first token of each sequence in the step's T rows
+//   context [B]          tokens of each sequence with this step's
+//   pos     [T]          position of each token in its sequence (-1: a row behind the last sequence)
+//   slot    [T]          16 * page + slot of each token (-1: none)
+//   writes  [W][4]       pages that get tokens: {page or -1, first token, its slot, tokens}
+//   shorts  [S][8]       attention items of sequences with few query rows (PI_*)
+//   tiles   [N][8]       attention items of the others: kTileRows query rows (PI_*)
+//   merges  [M][4]       rows whose keys are split over items: {items (< 0: of tiles), first item,
+//                        first token, tokens}
+#pragma once
+
+#include "common.h"
+
+constexpr int kPlanPage = 16;        // tokens per page
+constexpr int kPlanMaxSeqs = 4096;   // a workgroup holds every sequence's offsets in LDS
+constexpr int kPlanMaxTokens = 1 << 18;
+constexpr int kPlanMaxPages = 1 << 22;  // per sequence
+
+constexpr int kShortRows = 16;       // query rows (tokens x heads of the group) of a short item
+constexpr int kTileRows = 128;       // and of a tile
+constexpr int kShortStep = 8;        // pages that a short item's workgroup takes at once
+// Items that short sequences are split into, over all kv heads: the 1024 workgroups that the GPU
+// holds at once.
+constexpr int kShortTarget = 1024;
+// Workgroups that tiles are split for when there are fewer: two per CU, each with kTileMinKeys at least.
+constexpr int kTileTarget = 512;
+constexpr int kTileMinKeys = 512;
+constexpr int kTileKeys = 64;        // keys per step of a tile
+
+enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_MERGES, PH_PAGES, PH_INTS = 16 };
+// page_begin .. page_end: the item's keys; parts: items that share the rows (1: none other)
+enum { PI_SEQ, PI_TOK, PI_NTOK, PI_POS, PI_PAGE0, PI_PAGE1, PI_PARTS, PI_INTS = 8 };
+
+struct PlanLayout {
+  int B, T, max_new, max_pages, Hq, Hkv, G;
+  int tile_tok;               // tokens per tile
+  int W, S, N, M;             // list capacities
+  int split_tiles;            // tiles, and items of tiles, that may hold partial results
+  long cu, ctx, pos, slot, writes, shorts, tiles, merges, ints;  // offsets
+};
+
+static inline bool plan_shape_ok(const moe_mi355x_plan_shape* s) {
+  return s && s->seqs >= 0 && s->seqs <= kPlanMaxSeqs && s->tokens >= 0 && s->tokens <= kPlanMaxTokens &&
+         s->max_new >= 1 && s->max_pages >= 1 && s->max_pages <= kPlanMaxPages && s->heads >= 1 && s->kv_heads >= 1 &&
+         s->kv_heads <= 1024 && s->heads % s->kv_heads == 0 && s->heads / s->kv_heads <= kShortRows;
+}
+
+static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
+  PlanLayout p{};
+  p.B = s->seqs, p.T = s->tokens, p.max_pages = s->max_pages, p.Hq = s->heads, p.Hkv = s->kv_heads;
+  p.max_new = s->max_new < p.T ? s->max_new : p.T;
+  p.G = p.Hq / p.Hkv;
+  p.tile_tok = kTileRows / p.G;
+  const long B = p.B, T = p.T;
+  // a sequence with n new tokens touches at most (n + 30) / 16 pages, and at most n
+  p.W = (int)(T < (T + 30 * B) / 16 ? T : (T + 30 * B) / 16);
+  const long seqs = B < T ? B : T;  // with new tokens
+  const long per = (s->max_pages + kShortStep - 1) / kShortStep;
+  const long by_target = seqs + (kShortTarget + p.Hkv - 1) / p.Hkv, by_pages = seqs * per;
+  p.S = (int)(by_target < by_pages ? by_target : by_pages);
+  // no sequence is long enough for tiles: none
+  const bool tiles = (long)p.max_new * p.G > kShortRows;
+  const long nt = tiles ? T / p.tile_tok + seqs : 0;
+  const long target = (kTileTarget + p.Hkv - 1) / p.Hkv;
+  p.split_tiles = (int)(tiles ? (nt < target ? nt : target) + target : 0);
+  p.N = (int)(nt > p.split_tiles ? nt : p.split_tiles);
+  p.M = (int)(seqs + (nt < target ? nt : target));
+  auto at = [&](long ints) {
+    const long here = p.ints;
+    p.ints += (ints + 15) / 16 * 16;
+    return here;
+  };
+  at(PH_INTS);
+  p.cu = at(B + 1);
+  p.ctx = at(B);
+  p.pos = at(T);
+  p.slot = at(T);
+  p.writes = at(4L * p.W);
+  p.shorts = at((long)PI_INTS * p.S);
+  p.tiles = at((long)PI_INTS * p.N);
+  p.merges = at(4L * p.M);
+  return p;
+}

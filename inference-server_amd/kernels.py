@@ -9,6 +9,9 @@ buffers from the caching allocator, so calls on different streams never share on
 
 from __future__ import annotations
 
+import contextlib
+import ctypes
+
 import torch
 
 from . import _lib
@@ -408,6 +411,253 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                                                 block_tables.data_ptr(), positions.data_ptr(), B, Hkv, HEAD_DIM,
                                                 PAGE_SIZE, block_tables.shape[1], k_cache.shape[0], _stream(k)),
                "kv_append")
+
+
+# ---------------------------------------------------------------------------
+# 8-bit paged KV cache: the plan of a step, the writers, the attention
+# ---------------------------------------------------------------------------
+
+K_BLOCK_FP8 = (HEAD_DIM // 16, PAGE_SIZE, 16)                # dim / 16, token, dim % 16
+V_BLOCK_FP8 = (2, PAGE_SIZE // 4, HEAD_DIM // 2, 4)          # dim / 64, token / 4, dim % 64, token % 4
+PLAN_MAX_SEQS, PLAN_MAX_TOKENS, PLAN_MAX_PAGES = 4096, 1 << 18, 1 << 22
+
+
+def _launch_on(t: torch.Tensor):
+    """Makes t's device the current one for a launch, where it is not."""
+    if torch._C._cuda_getDevice() == t.device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(first: torch.Tensor, **others: torch.Tensor) -> None:
+    for name, t in others.items():
+        if t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+
+
+class PagedPlan:
+    """A step's plan over the 8-bit paged KV cache, as ``paged_plan`` left it on the GPU: which pages and slots
+    its tokens get and how the attention is split up.  Built once a step, used by every layer.
+
+    ``positions`` int32 [T] (-1: padding row), ``slots`` int32 [T] (16 * page + position % 16; -1: none), ``cu_tokens``
+    int32 [B + 1], ``context_lens`` int32 [B] (with the new tokens), ``pages_used`` int32 [1] and ``block_tables``
+    are views of what the GPU holds; the rest is the kernels' own.
+    """
+
+    __slots__ = ("shape", "buffer", "block_tables", "_at", "_ref")
+
+    def __init__(self, shape: _lib.PlanShape, buffer: torch.Tensor, at, block_tables: torch.Tensor):
+        self.shape, self.buffer, self._at, self.block_tables = shape, buffer, at, block_tables
+        self._ref = ctypes.byref(shape)
+
+    def _section(self, name: str, size: int) -> torch.Tensor:
+        first = self._at[_lib.PLAN_SECTIONS.index(name)]
+        return self.buffer[first:first + size]
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._section("positions", self.shape.tokens)
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._section("slots", self.shape.tokens)
+
+    @property
+    def cu_tokens(self) -> torch.Tensor:
+        return self._section("cu_tokens", self.shape.seqs + 1)
+
+    @property
+    def context_lens(self) -> torch.Tensor:
+        return self._section("context_lens", self.shape.seqs)
+
+    @property
+    def pages_used(self) -> torch.Tensor:
+        return self._section("pages_used", 1)
+
+
+def paged_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
+               free_pages: torch.Tensor, num_tokens: int, max_new_tokens: int, num_heads: int, num_kv_heads: int,
+               out: PagedPlan | None = None) -> PagedPlan:
+    """Plans a step of B sequences on the GPU, from lengths that only the GPU needs to know.
+
+    ``cached_lens`` int32 [B]: tokens already cached; ``new_lens`` int32 [B]: this step's (a prompt's, a chunk's, 1
+    for a decoding sequence, 0); ``num_tokens``: rows of the step's tensors (what is not taken is padding, what does not
+    fit is left out); ``max_new_tokens``: no sequence takes more (1 for a decode step).  ``block_tables``
+    int32 [B, max_pages] gets the new pages' entries in place, taken in order from ``free_pages`` int32 [N]
+    (-1 past its end; ``pages_used`` says how many were wanted).  A page that gets tokens belongs to one sequence.
+
+    With ``out``, an earlier plan of the same sizes, that plan's memory is filled again: a captured step keeps one.
+    """
+    _need(cached_lens, "cached_lens", torch.int32, 1)
+    _need(new_lens, "new_lens", torch.int32, 1)
+    _need(block_tables, "block_tables", torch.int32, 2)
+    _need(free_pages, "free_pages", torch.int32, 1)
+    _same_device(cached_lens, new_lens=new_lens, block_tables=block_tables, free_pages=free_pages)
+    B, max_pages = block_tables.shape
+    if cached_lens.shape[0] != B or new_lens.shape[0] != B:
+        raise ValueError("cached_lens and new_lens need one entry per row of block_tables")
+    if B > PLAN_MAX_SEQS or not 0 <= num_tokens <= PLAN_MAX_TOKENS or not 1 <= max_pages <= PLAN_MAX_PAGES:
+        raise ValueError(f"a step has at most {PLAN_MAX_SEQS} sequences, {PLAN_MAX_TOKENS} tokens and "
+                         f"{PLAN_MAX_PAGES} pages a sequence, got {B}, {num_tokens} and {max_pages}")
+    if not 1 <= max_new_tokens < 1 << 31:
+        raise ValueError(f"max_new_tokens must be positive, got {max_new_tokens}")
+    if num_kv_heads < 1 or num_kv_heads > 1024 or num_heads % num_kv_heads or not 1 <= num_heads // num_kv_heads <= 16:
+        raise ValueError(f"num_heads ({num_heads}) must be a multiple of num_kv_heads ({num_kv_heads}, 1 to 1024) with "
+                         "1 to 16 query heads per kv head")
+    if free_pages.shape[0] >= 1 << 31:
+        raise ValueError("free_pages is too long")
+    lib = _lib.load()
+    if out is None:
+        shape = _lib.PlanShape(B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads)
+        at = (ctypes.c_int32 * len(_lib.PLAN_SECTIONS))()
+        nbytes = lib.moe_mi355x_paged_plan_bytes(shape, at)
+        out = PagedPlan(shape, torch.empty(nbytes // 4, dtype=torch.int32, device=cached_lens.device), at, block_tables)
+    else:
+        s = out.shape
+        if (s.seqs, s.tokens, s.max_new, s.max_pages, s.heads, s.kv_heads) != \
+                (B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads):
+            raise ValueError("out is a plan of other sizes")
+        _same_device(cached_lens, out=out.buffer)
+        out.block_tables = block_tables
+    with _launch_on(cached_lens):
+        _lib.check(lib.moe_mi355x_paged_plan(cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
+                                             free_pages.data_ptr(), free_pages.shape[0], out._ref,
+                                             out.buffer.data_ptr(), out.buffer.numel() * 4, _stream(cached_lens)),
+                   "paged_plan")
+    return out
+
+
+def _need_rows(t: torch.Tensor, name: str, tokens: int, heads: int) -> int:
+    """Checks a bf16 [tokens, heads, 128] tensor whose tokens may lie apart (a slice of a fused projection);
+    returns the values from one token to the next."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must have dtype torch.bfloat16, got {t.dtype}")
+    if t.shape != (tokens, heads, HEAD_DIM):
+        raise ValueError(f"{name} must be {(tokens, heads, HEAD_DIM)}, got {tuple(t.shape)}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on a ROCm GPU device, got {t.device}")
+    row = heads * HEAD_DIM
+    if tokens == 0:
+        return row
+    apart, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != HEAD_DIM):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    if tokens == 1:
+        return row
+    if apart < row or apart % 8:
+        raise ValueError(f"{name}: tokens must be a multiple of 8 values apart and not overlap, got {apart}")
+    return apart
+
+
+def _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan) -> int:
+    """The pools of the plan's kv heads; returns their pages."""
+    if not isinstance(plan, PagedPlan):
+        raise TypeError("plan must be a PagedPlan (paged_plan)")
+    _need(k_cache, "k_cache", FP8, 5)
+    _need(v_cache, "v_cache", FP8, 6)
+    _need(k_scale, "k_scale", torch.float32, 2)
+    _need(v_scale, "v_scale", torch.float32, 2)
+    pages, heads = k_cache.shape[0], plan.shape.kv_heads
+    if k_cache.shape != (pages, heads, *K_BLOCK_FP8):
+        raise ValueError(f"k_cache must be [pages, {heads}, 8, 16, 16], got {tuple(k_cache.shape)}")
+    if v_cache.shape != (pages, heads, *V_BLOCK_FP8):
+        raise ValueError(f"v_cache must be [{pages}, {heads}, 2, 4, 64, 4], got {tuple(v_cache.shape)}")
+    if k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
+        raise ValueError(f"k_scale and v_scale must be [{pages}, {heads}]")
+    if pages >= 1 << 27:
+        raise ValueError("a pool has fewer than 2^27 pages")
+    _same_device(plan.buffer, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    return pages
+
+
+def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, plan: PagedPlan) -> None:
+    """Quantises a step's keys and values (bf16 [T, Hkv, 128], tokens may lie apart) into the 8-bit paged
+    cache: e4m3 codes, one power-of-two scale per (page, kv head).  Prompts and single tokens alike.
+
+    ``k_cache`` e4m3 [pages, Hkv, 8, 16, 16] (dim / 16, token, dim % 16), ``v_cache`` e4m3 [pages, Hkv, 2, 4, 64,
+    4] (dim / 64, token / 4, dim % 64, token % 4), ``k_scale`` and ``v_scale`` fp32 [pages, Hkv].  A page that begins
+    is written whole; a page that goes on keeps its scale or, where a new value needs it, gets a larger one and
+    its codes are re-coded.  ``unpack_kv_fp8`` gives the values back.
+    """
+    pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
+    T, Hkv = plan.shape.tokens, plan.shape.kv_heads
+    k_stride = _need_rows(k, "k", T, Hkv)
+    v_stride = _need_rows(v, "v", T, Hkv)
+    _same_device(plan.buffer, k=k, v=v)
+    with _launch_on(k):
+        _lib.check(_lib.load().moe_mi355x_kv_append_fp8(
+            k.data_ptr(), v.data_ptr(), k_stride, v_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), HEAD_DIM, PAGE_SIZE, pages, plan._ref, plan.buffer.data_ptr(), _stream(k)),
+            "kv_append_fp8")
+
+
+def qk_norm_rope_append_fp8(qkv: torch.Tensor, q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor,
+                            inv_freq: torch.Tensor, num_heads: int, num_kv_heads: int, eps: float,
+                            k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                            v_scale: torch.Tensor, plan: PagedPlan) -> torch.Tensor:
+    """q/k RMSNorm, rotary embedding at the plan's positions and ``kv_append_fp8`` in one launch, for a step's prompts
+    and single tokens (modeling_qwen3_moe.py:162-171).  ``qkv`` bf16 [T, (Hq + 2 Hkv) * 128]; returns q bf16
+    [T, Hq, 128] (padding rows: zeros).  fp32 from the projections to the one rounding of each result."""
+    pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
+    s = plan.shape
+    if (num_heads, num_kv_heads) != (s.heads, s.kv_heads):
+        raise ValueError(f"the plan is for {s.heads} query and {s.kv_heads} kv heads")
+    _need(qkv, "qkv", torch.bfloat16, 2)
+    _need(q_norm_weight, "q_norm_weight", torch.bfloat16, 1)
+    _need(k_norm_weight, "k_norm_weight", torch.bfloat16, 1)
+    _need(inv_freq, "inv_freq", torch.float32, 1)
+    if qkv.shape != (s.tokens, (num_heads + 2 * num_kv_heads) * HEAD_DIM):
+        raise ValueError(f"qkv must be [{s.tokens}, (Hq + 2 Hkv) * 128], got {tuple(qkv.shape)}")
+    if q_norm_weight.shape[0] != HEAD_DIM or k_norm_weight.shape[0] != HEAD_DIM or inv_freq.shape[0] != HEAD_DIM // 2:
+        raise ValueError("the norm weights must be [128] and inv_freq [64]")
+    _same_device(plan.buffer, qkv=qkv, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, inv_freq=inv_freq)
+    q = torch.empty((s.tokens, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
+    with _launch_on(qkv):
+        _lib.check(_lib.load().moe_mi355x_qk_norm_rope_append_fp8(
+            qkv.data_ptr(), q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), inv_freq.data_ptr(), float(eps),
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), HEAD_DIM,
+            PAGE_SIZE, pages, plan._ref, plan.buffer.data_ptr(), _stream(qkv)), "qk_norm_rope_append_fp8")
+    return q
+
+
+def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, plan: PagedPlan, scale: float) -> torch.Tensor:
+    """Causal attention of a step's tokens over the 8-bit paged cache, which already holds the step's own keys
+    and values: ``softmax(scale * q . K) . V`` over the keys up to each token's position.  Prompts, chunks of
+    them and single tokens in one call.  ``q`` bf16 [T, Hq, 128] (tokens may lie apart); returns bf16 [T, Hq, 128].
+
+    fp32 scores, softmax and sums.  Keys of pages that the table does not hold are left out; a token without keys
+    and a padding row give zeros."""
+    pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
+    s = plan.shape
+    q_stride = _need_rows(q, "q", s.tokens, s.heads)
+    _same_device(plan.buffer, q=q)
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    lib = _lib.load()
+    out = torch.empty((s.tokens, s.heads, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    nws = lib.moe_mi355x_paged_attn_fp8_workspace_bytes(plan._ref)
+    ws = _ws(nws, q.device)
+    with _launch_on(q):
+        _lib.check(lib.moe_mi355x_paged_attn_fp8(
+            q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            plan.block_tables.data_ptr(), HEAD_DIM, PAGE_SIZE, pages, scale, plan._ref, plan.buffer.data_ptr(),
+            out.data_ptr(), ws.data_ptr(), nws, _stream(q)), "paged_attention_fp8")
+    return out
+
+
+def unpack_kv_fp8(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The values of 8-bit cache pages, K's or V's (told apart by their shape), as fp32 [pages, Hkv, 16, 128] token
+    rows: for a look into the cache, not for the hot path (plain torch, on any device)."""
+    if codes.dtype != FP8 or codes.shape[2:] not in (K_BLOCK_FP8, V_BLOCK_FP8) or scale.shape != codes.shape[:2]:
+        raise ValueError("codes must be an e4m3 K or V pool and scale its [pages, Hkv]")
+    x = codes.float()
+    x = x.permute(0, 1, 3, 2, 4) if codes.dim() == 5 else x.permute(0, 1, 3, 5, 2, 4)
+    return x.reshape(*codes.shape[:2], PAGE_SIZE, HEAD_DIM) * scale[..., None, None]
 
 
 # ---------------------------------------------------------------------------
