@@ -24,6 +24,7 @@ constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCachePolicyNT = 2;  // the instruction's cache-policy field: nt (streaming)
 constexpr int kPadBlocks = 8;      // workgroups that clear the rows behind the last sequence
+constexpr int kMergeBlocks = 1024;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -37,7 +38,8 @@ struct AttnFp8Args {
   uint16_t* out;         // [T][Hq][128]
   float *short_o, *short_ml, *tile_o, *tile_ml;  // partial results, by item
   int num_pages;
-  float scale;  // times log2(e)
+  int merge_rows;  // rows that an entry of the merge list may have
+  float scale;     // times log2(e)
   PlanLayout p;
 };
 
@@ -504,54 +506,72 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order.  One workgroup per (rows,
-// kv head, row): 8 groups of 32 lanes take the items round robin, a lane 4 dims.
+// merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order.  A workgroup takes one
+// (rows, kv head, row) at a time: 8 groups of 32 lanes share the items, a lane 4 dims; four items' loads are in
+// flight at once.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
   const PlanLayout& p = a.p;
-  const int entry = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv, r = blockIdx.y;
-  if (entry >= a.plan[PH_MERGES]) return;
-  const int4 e = *(const int4*)(a.plan + p.merges + 4L * entry);
-  if (r >= e.w * p.G) return;
-  const int ns = abs(e.x), stride = e.x < 0 ? kTileRows : kShortRows;
-  const float* part = e.x < 0 ? a.tile_o : a.short_o;
-  const float* ml = e.x < 0 ? a.tile_ml : a.short_ml;
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   __shared__ float s_m[8], s_l[8];
   __shared__ __attribute__((aligned(16))) v4f s_o[8][32];
-  float M = -INFINITY, L = 0.f;
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = grp; s < ns; s += 8) {
-    const long base = ((long)(e.y + s) * p.Hkv + g) * stride + r;
-    const float2 x = *(const float2*)(ml + 2 * base);
-    const v4f v = *(const v4f*)(part + base * kHD + 4 * lane);
-    if (x.x == -INFINITY) continue;  // only empty pages
-    const float m_new = fmaxf(M, x.x);
-    const float old = __builtin_amdgcn_exp2f(M - m_new), w = __builtin_amdgcn_exp2f(x.x - m_new);
-    M = m_new;
-    L = L * old + x.y * w;
-    acc = acc * old + v * w;
-  }
-  s_o[grp][lane] = acc;
-  if (lane == 0) {
-    s_m[grp] = M;
-    s_l[grp] = L;
-  }
-  __syncthreads();
-  if (grp > 0) return;
+  const long tasks = (long)a.plan[PH_MERGES] * p.Hkv * a.merge_rows;
+  for (long task = blockIdx.x; task < tasks; task += gridDim.x) {  // workgroup-uniform
+    const int r = (int)(task % a.merge_rows), g = (int)(task / a.merge_rows % p.Hkv);
+    const int4 e = *(const int4*)(a.plan + p.merges + 4 * (task / a.merge_rows / p.Hkv));
+    if (r >= e.w * p.G) continue;
+    const int ns = abs(e.x), stride = e.x < 0 ? kTileRows : kShortRows;
+    const float* part = e.x < 0 ? a.tile_o : a.short_o;
+    const float* ml = e.x < 0 ? a.tile_ml : a.short_ml;
+    float M = -INFINITY, L = 0.f;
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = grp; s0 < ns; s0 += 32) {
+      float2 x[4];
+      v4f v[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
-  L = 0.f;
-  acc = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < 4; ++u) {
+        const long base = ((long)(e.y + min(s0 + 8 * u, ns - 1)) * p.Hkv + g) * stride + r;
+        x[u] = *(const float2*)(ml + 2 * base);
+        v[u] = *(const v4f*)(part + base * kHD + 4 * lane);
+      }
+      float m_new = M;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float w = s_m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i] - M);
-    L += s_l[i] * w;
-    acc += s_o[i][lane] * w;
+      for (int u = 0; u < 4; ++u) m_new = fmaxf(m_new, x[u].x);  // the last item again changes nothing
+      if (m_new == -INFINITY) continue;                          // only empty pages so far
+      const float old = __builtin_amdgcn_exp2f(M - m_new);
+      M = m_new;
+      L *= old;
+      acc *= old;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = s0 + 8 * u < ns ? __builtin_amdgcn_exp2f(x[u].x - M) : 0.f;
+        L += x[u].y * w;
+        acc += v[u] * w;
+      }
+    }
+    s_o[grp][lane] = acc;
+    if (lane == 0) {
+      s_m[grp] = M;
+      s_l[grp] = L;
+    }
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+      L = 0.f;
+      acc = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = s_m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i] - M);
+        L += s_l[i] * w;
+        acc += s_o[i][lane] * w;
+      }
+      const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+      uint16_t* dst = a.out + ((long)(e.z + r / p.G) * p.Hq + g * p.G + r % p.G) * kHD + 4 * lane;
+      *(uint2*)dst = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
+    }
+    __syncthreads();  // the sums are read
   }
-  const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-  uint16_t* dst = a.out + ((long)(e.z + r / p.G) * p.Hq + g * p.G + r % p.G) * kHD + 4 * lane;
-  *(uint2*)dst = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
 }
 
 // Partial results: an item's rows and their (max, sum), for both kinds; none where no item is split.
@@ -571,7 +591,7 @@ void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
 }
 
 bool attn_grid_ok(const PlanLayout& p) {
-  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) && moe_grid_fits((long)p.M * p.Hkv);
+  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv);
 }
 
 }  // namespace
@@ -619,8 +639,10 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   hipLaunchKernelGGL(attn_fp8_short_kernel, dim3((unsigned)(p.S * p.Hkv + kPadBlocks)), dim3(256), 0, s, a);
   MOE_CHECK_LAUNCH();
   if (parts.shorts + parts.tiles > 0 && p.M > 0) {
-    hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3((unsigned)(p.M * p.Hkv), parts.tiles > 0 ? kTileRows : kShortRows),
-                       dim3(256), 0, s, a);
+    a.merge_rows = parts.tiles > 0 ? kTileRows : kShortRows;
+    const long tasks = (long)p.M * p.Hkv * a.merge_rows;
+    hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3((unsigned)(tasks < kMergeBlocks ? tasks : kMergeBlocks)), dim3(256), 0, s,
+                       a);
     MOE_CHECK_LAUNCH();
   }
   return MOE_OK;

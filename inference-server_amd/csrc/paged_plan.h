@@ -1,6 +1,6 @@
 // The plan of a step over the 8-bit paged KV cache: one int32 buffer that moe_mi355x_paged_plan
 // (paged_plan.hip) fills from the sequences' lengths and that the cache writers (kv_fp8.hip) and the
-// attention (attn_fp8.hip) read.  Sections, each from a multiple of 16 ints:
+// attention (attn_fp8.hip) read.  Sections, the lists from a multiple of 16 ints:
 //   head    [16]         counts (PH_*)
 //   cu      [B + 1]      first token of each sequence in the step's T rows
 //   context [B]          tokens of each sequence with this step's
@@ -31,7 +31,7 @@ constexpr int kTileTarget = 512;
 constexpr int kTileMinKeys = 512;
 constexpr int kTileKeys = 64;        // keys per step of a tile
 
-enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_MERGES, PH_PAGES, PH_INTS = 16 };
+enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_MERGES, PH_PAGES = 15, PH_INTS };
 // page_begin .. page_end: the item's keys; parts: items that share the rows (1: none other)
 enum { PI_SEQ, PI_TOK, PI_NTOK, PI_POS, PI_PAGE0, PI_PAGE1, PI_PARTS, PI_INTS = 8 };
 
@@ -69,16 +69,16 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   p.split_tiles = (int)(tiles ? (nt < target ? nt : target) + target : 0);
   p.N = (int)(nt > p.split_tiles ? nt : p.split_tiles);
   p.M = (int)(seqs + (nt < target ? nt : target));
+  p.cu = PH_INTS;
+  p.ctx = p.cu + B + 1;
+  p.pos = p.ctx + B;
+  p.slot = p.pos + T;
+  p.ints = (p.slot + T + 15) / 16 * 16;
   auto at = [&](long ints) {
     const long here = p.ints;
     p.ints += (ints + 15) / 16 * 16;
     return here;
   };
-  at(PH_INTS);
-  p.cu = at(B + 1);
-  p.ctx = at(B);
-  p.pos = at(T);
-  p.slot = at(T);
   p.writes = at(4L * p.W);
   p.shorts = at((long)PI_INTS * p.S);
   p.tiles = at((long)PI_INTS * p.N);

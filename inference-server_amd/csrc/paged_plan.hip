@@ -10,13 +10,13 @@
 //
 // One launch.  Every workgroup forms the prefix sums over the sequences by itself (4 B of two arrays
 // each, in LDS afterwards): cheaper than a launch of its own for them.  Workgroup 0 then builds the attention
-// lists, the others take 1024 tokens each.  A new page's table entry and write record come from its first
+// lists, the others take 256 tokens each.  A new page's table entry and write record come from its first
 // token's thread, so nothing waits for anything and every list has one order.
 #include "paged_plan.h"
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / MOE_WAVE;
 
 struct PlanArgs {
@@ -28,27 +28,36 @@ struct PlanArgs {
   PlanLayout p;
 };
 
-// Exclusive prefix sum over the workgroup; *total gets the sum.  Every thread calls it.
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, T* total, T* s_wave) {
+// Exclusive prefix sums of N values over the workgroup; v becomes them, total the sums.  Every thread calls it.
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*s_wave)[kWaves]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T incl = v;
+  int incl[N];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T t = __shfl_up(incl, d);
-    if (lane >= d) incl += t;
-  }
+  for (int k = 0; k < N; ++k) incl[k] = v[k];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int t = __shfl_up(incl[k], d);
+      if (lane >= d) incl[k] += t;
+    }
   __syncthreads();  // the last call's sums are read
-  if (lane == 63) s_wave[wave] = incl;
-  __syncthreads();
-  T before = 0, all = 0;
+  if (lane == 63)
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? s_wave[w] : 0;
-    all += s_wave[w];
+    for (int k = 0; k < N; ++k) s_wave[k][wave] = incl[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < wave ? s_wave[k][w] : 0;
+      all += s_wave[k][w];
+    }
+    total[k] = all;
+    v[k] = before + incl[k] - v[k];
   }
-  *total = all;
-  return before + incl - v;
 }
 
 // The last index i < n with s[i] <= x, for s ascending from s[0] <= x.
@@ -68,71 +77,63 @@ __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPlanPage
 
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   const PlanLayout& p = a.p;
-  __shared__ int s_cu[kPlanMaxSeqs + 1], s_a[kPlanMaxSeqs + 1], s_b[kPlanMaxSeqs + 1];
-  __shared__ long s_sum[kWaves];
-  int* s_isum = (int*)s_sum;
+  // per sequence: tokens cached, first row, and two prefix sums that the workgroup needs
+  __shared__ int s_cached[kPlanMaxSeqs], s_cu[kPlanMaxSeqs + 1], s_a[kPlanMaxSeqs + 1], s_b[kPlanMaxSeqs + 1];
+  __shared__ int s_wave[3][kWaves];
+  __shared__ unsigned long long s_pages, s_keys;
   const int tid = threadIdx.x;
-  const int per = (p.B + kThreads - 1) / kThreads;  // sequences per thread, 4 at most
-  const int b0 = tid * per;
+  const int per = (p.B + kThreads - 1) / kThreads;  // sequences per thread: b0 .. b1
+  const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   const int room = p.max_pages * kPlanPage;
   int32_t* plan = a.plan;
 
-  int c[4], n[4];
-  int sum = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool live = i < per && b0 + i < p.B;
-    c[i] = live ? min(max(a.cached[b0 + i], 0), room) : 0;
-    n[i] = live ? min(max(a.fresh[b0 + i], 0), p.max_new) : 0;
-    sum += n[i];  // <= 4096 * 2^18
+  int first[1] = {0}, total[1];
+  for (int b = b0; b < b1; ++b) {
+    s_cached[b] = min(max(a.cached[b], 0), room);
+    s_b[b] = min(max(a.fresh[b], 0), p.max_new);
+    first[0] += s_b[b];  // <= 4096 * 2^18
   }
-  int total;
-  int at = block_scan(sum, &total, s_isum);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int first = min(at, p.T);
-    at += n[i];
-    n[i] = min(at, p.T) - first;
-    if (i < per && b0 + i < p.B) s_cu[b0 + i] = first;
+  if (tid == 0) s_pages = s_keys = 0;
+  block_scan(first, total, s_wave);
+  total[0] = min(total[0], p.T);
+  for (int b = b0; b < b1; ++b) {
+    s_cu[b] = min(first[0], p.T);
+    first[0] += s_b[b];
   }
-  total = min(total, p.T);
-  if (tid == 0) s_cu[p.B] = total;
+  if (tid == 0) s_cu[p.B] = total[0];
+  const int end = min(first[0], p.T);  // of this thread's last sequence
+  // a thread knows its own sequences' new tokens without waiting for the others
+  auto new_of = [&](int b) __attribute__((always_inline)) { return (b + 1 < b1 ? s_cu[b + 1] : end) - s_cu[b]; };
 
   if (blockIdx.x > 0) {  // tokens: page records and slots
-    int need = 0, touched = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      need += pages_of(min(c[i] + n[i], room)) - pages_of(c[i]);
-      touched += n[i] > 0 ? (c[i] + n[i] - 1) / kPlanPage - c[i] / kPlanPage + 1 : 0;
-    }
-    int all_need, all_touched;
-    int need_at = block_scan(need, &all_need, s_isum);
-    int touched_at = block_scan(touched, &all_touched, s_isum);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i < per && b0 + i < p.B) {
-        s_a[b0 + i] = need_at;
-        s_b[b0 + i] = touched_at;
-        need_at += pages_of(min(c[i] + n[i], room)) - pages_of(c[i]);
-        touched_at += n[i] > 0 ? (c[i] + n[i] - 1) / kPlanPage - c[i] / kPlanPage + 1 : 0;
-      }
+    int at[2] = {0, 0}, all[2];  // new pages, pages that get tokens
+    auto count = [&](int b) __attribute__((always_inline)) {
+      const int c = s_cached[b], n = new_of(b);
+      at[0] += pages_of(min(c + n, room)) - pages_of(c);
+      at[1] += n > 0 ? (c + n - 1) / kPlanPage - c / kPlanPage + 1 : 0;
+    };
+    for (int b = b0; b < b1; ++b) count(b);
+    block_scan(at, all, s_wave);
+    for (int b = b0; b < b1; ++b) {
+      s_a[b] = at[0];
+      s_b[b] = at[1];
+      count(b);
     }
     __syncthreads();
     if (blockIdx.x == 1 && tid == 0) {
-      plan[PH_WRITES] = all_touched;
-      plan[PH_PAGES] = all_need;
+      plan[PH_PAGES] = all[0];
+      plan[PH_WRITES] = all[1];
     }
     const int t = (blockIdx.x - 1) * kThreads + tid;
     if (t >= p.T) return;
-    if (t >= total) {
+    if (t >= total[0]) {
       plan[p.pos + t] = -1;
       plan[p.slot + t] = -1;
       return;
     }
     const int b = last_le(s_cu, p.B, t);  // the last of those that begin at or before t: the one that has tokens
-    const int first = s_cu[b], count = s_cu[b + 1] - first;
-    const int cached = min(max(a.cached[b], 0), room);
-    const int pos = cached + (t - first);
+    const int row0 = s_cu[b], cached = s_cached[b];
+    const int pos = cached + (t - row0);
     const int j = pos / kPlanPage, have = pages_of(cached);
     int page = -1;
     if (j < p.max_pages) {
@@ -147,107 +148,99 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     }
     plan[p.pos + t] = pos;
     plan[p.slot + t] = page < 0 ? -1 : page * kPlanPage + pos % kPlanPage;
-    if (t == first || pos % kPlanPage == 0) {
+    if (t == row0 || pos % kPlanPage == 0) {
       const int w = s_b[b] + j - cached / kPlanPage;
-      const int some = min(kPlanPage - pos % kPlanPage, first + count - t);
+      const int some = min(kPlanPage - pos % kPlanPage, s_cu[b + 1] - t);
       *(int4*)(plan + p.writes + 4L * w) = make_int4(page, t, pos % kPlanPage, some);
     }
     return;
   }
 
   // workgroup 0: offsets, contexts and the attention's lists
-  long short_pages = 0, tile_keys = 0;
-  int tiles = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < per && b0 + i < p.B) {
-      plan[p.cu + b0 + i] = s_cu[b0 + i];
-      plan[p.ctx + b0 + i] = min(c[i] + n[i], room);
-      if (n[i] > 0 && n[i] * p.G <= kShortRows) short_pages += pages_of(min(c[i] + n[i], room));
-      if (n[i] * p.G > kShortRows) {
-        const long nt = (n[i] + p.tile_tok - 1) / p.tile_tok;
-        tiles += (int)nt;
-        tile_keys += nt * c[i] + p.tile_tok * (nt * (nt - 1) / 2) + n[i];
+  int tiles[1] = {0}, all_tiles[1];
+  {
+    unsigned long long pages = 0, keys = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int c = s_cached[b], n = new_of(b), ctx = min(c + n, room);
+      plan[p.cu + b] = s_cu[b];
+      plan[p.ctx + b] = ctx;
+      if (n > 0 && n * p.G <= kShortRows) pages += pages_of(ctx);
+      if (n * p.G > kShortRows) {
+        const long nt = (n + p.tile_tok - 1) / p.tile_tok;
+        tiles[0] += (int)nt;
+        keys += nt * c + p.tile_tok * (nt * (nt - 1) / 2) + n;
       }
     }
+    if (pages) atomicAdd(&s_pages, pages);
+    if (keys) atomicAdd(&s_keys, keys);
   }
-  if (tid == 0) plan[p.cu + p.B] = total;
-  long all_pages, all_keys;
-  int all_tiles;
-  block_scan(short_pages, &all_pages, s_sum);
-  block_scan(tile_keys, &all_keys, s_sum);
-  int tile_at = block_scan(tiles, &all_tiles, s_isum);
+  if (tid == 0) plan[p.cu + p.B] = total[0];
+  block_scan(tiles, all_tiles, s_wave);  // its barriers complete the two sums
   // pages per short item
-  long pps = (all_pages * p.Hkv + kShortTarget - 1) / kShortTarget;
+  long pps = ((long)s_pages * p.Hkv + kShortTarget - 1) / kShortTarget;
   pps = max(pps, 1L) + kShortStep - 1;
   pps = pps / kShortStep * kShortStep;
   // keys per item of a tile; with enough tiles to fill the GPU they are not split
-  long chunk = (all_keys * p.Hkv + kTileTarget - 1) / kTileTarget;
+  long chunk = ((long)s_keys * p.Hkv + kTileTarget - 1) / kTileTarget;
   chunk = (max(chunk, (long)kTileMinKeys) + kTileKeys - 1) / kTileKeys * kTileKeys;
-  if ((long)all_tiles * p.Hkv >= kTileTarget) chunk = 1L << 40;
+  if ((long)all_tiles[0] * p.Hkv >= kTileTarget) chunk = 1L << 40;
 
-  int items = 0, merged = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int pages = pages_of(min(c[i] + n[i], room));
-    const int ns = n[i] > 0 && n[i] * p.G <= kShortRows ? (int)((pages + pps - 1) / pps) : 0;
-    items += ns;
-    merged += ns > 1;
+  auto splits = [&](int b) __attribute__((always_inline)) {
+    const int n = new_of(b);
+    return n > 0 && n * p.G <= kShortRows ? (int)((pages_of(min(s_cached[b] + n, room)) + pps - 1) / pps) : 0;
+  };
+  int at[2] = {0, 0}, all[2];  // short items, merges
+  for (int b = b0; b < b1; ++b) {
+    const int ns = splits(b);
+    at[0] += ns;
+    at[1] += ns > 1;
   }
-  int n_items, n_merged;
-  int item_at = block_scan(items, &n_items, s_isum);
-  int merge_at = block_scan(merged, &n_merged, s_isum);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (!(i < per && b0 + i < p.B)) continue;
-    const int b = b0 + i, pages = pages_of(min(c[i] + n[i], room));
-    const int ns = n[i] > 0 && n[i] * p.G <= kShortRows ? (int)((pages + pps - 1) / pps) : 0;
-    s_a[b] = item_at;
-    s_b[b] = tile_at;
-    if (ns > 1) {
-      *(int4*)(plan + p.merges + 4L * merge_at) = make_int4(ns, item_at, s_cu[b], n[i]);
-      ++merge_at;
-    }
-    item_at += ns;
-    if (n[i] * p.G > kShortRows) tile_at += (n[i] + p.tile_tok - 1) / p.tile_tok;
+  block_scan(at, all, s_wave);
+  for (int b = b0; b < b1; ++b) {
+    const int ns = splits(b), n = new_of(b);
+    s_a[b] = at[0];
+    s_b[b] = tiles[0];
+    if (ns > 1) *(int4*)(plan + p.merges + 4L * at[1]) = make_int4(ns, at[0], s_cu[b], n);
+    at[0] += ns;
+    at[1] += ns > 1;
+    if (n * p.G > kShortRows) tiles[0] += (n + p.tile_tok - 1) / p.tile_tok;
   }
   if (tid == 0) {
-    s_a[p.B] = n_items;
-    s_b[p.B] = all_tiles;
+    s_a[p.B] = all[0];
+    s_b[p.B] = all_tiles[0];
   }
   __syncthreads();
 
-  for (int k = tid; k < n_items; k += kThreads) {
+  for (int k = tid; k < all[0]; k += kThreads) {
     const int b = last_le(s_a, p.B, k);
-    const int first = s_cu[b], count = s_cu[b + 1] - first;
-    const int cached = min(max(a.cached[b], 0), room);
-    const int pages = pages_of(min(cached + count, room)), ns = s_a[b + 1] - s_a[b];
+    const int row0 = s_cu[b], n = s_cu[b + 1] - row0;
+    const int pages = pages_of(min(s_cached[b] + n, room)), ns = s_a[b + 1] - s_a[b];
     // equal shares, each a multiple of what a workgroup takes at once
     const int share = (pages + ns * kShortStep - 1) / (ns * kShortStep) * kShortStep;
     const int page0 = (k - s_a[b]) * share;
     int4* dst = (int4*)(plan + p.shorts + (long)PI_INTS * k);
-    dst[0] = make_int4(b, first, count, cached);
+    dst[0] = make_int4(b, row0, n, s_cached[b]);
     dst[1] = make_int4(page0, min(page0 + share, pages), ns, 0);
   }
 
-  int n_tile_items = 0;
-  for (int k0 = 0; k0 < all_tiles; k0 += kThreads) {  // workgroup-uniform
+  int n_items = 0, n_merged = all[1];
+  for (int k0 = 0; k0 < all_tiles[0]; k0 += kThreads) {  // workgroup-uniform
     const int k = k0 + tid;
     int ns = 0, b = 0, tok = 0, count = 0, pos = 0, keys = 0;
-    if (k < all_tiles) {
+    if (k < all_tiles[0]) {
       b = last_le(s_b, p.B, k);
-      const int first = s_cu[b], n_b = s_cu[b + 1] - first;
+      const int row0 = s_cu[b], n = s_cu[b + 1] - row0;
       // a sequence's last tiles, which have the most keys, first
       const int i = s_b[b + 1] - 1 - k;
-      tok = first + i * p.tile_tok;
-      count = min(p.tile_tok, n_b - i * p.tile_tok);
-      pos = min(max(a.cached[b], 0), room) + i * p.tile_tok;
+      tok = row0 + i * p.tile_tok;
+      count = min(p.tile_tok, n - i * p.tile_tok);
+      pos = s_cached[b] + i * p.tile_tok;
       keys = min(pos + count, room);
       ns = (int)((keys + chunk - 1) / chunk);
     }
-    int round, round_merged;
-    const int item = n_tile_items + block_scan(ns, &round, s_isum);
-    const int merge = n_merged + block_scan(ns > 1 ? 1 : 0, &round_merged, s_isum);
+    int mine[2] = {ns, ns > 1 ? 1 : 0}, round[2];
+    block_scan(mine, round, s_wave);
+    const int item = n_items + mine[0], merge = n_merged + mine[1];
     if (ns > 1) *(int4*)(plan + p.merges + 4L * merge) = make_int4(-ns, item, tok, count);
     for (int s = 0; s < ns; ++s) {
       const int pages = pages_of(keys), step = ns > 1 ? (int)(chunk / kPlanPage) : pages;
@@ -255,13 +248,13 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       dst[0] = make_int4(b, tok, count, pos);
       dst[1] = make_int4(s * step, min((s + 1) * step, pages), ns, 0);
     }
-    n_tile_items += round;
-    n_merged += round_merged;
+    n_items += round[0];
+    n_merged += round[1];
   }
   if (tid == 0) {
-    plan[PH_TOKENS] = total;
-    plan[PH_SHORTS] = n_items;
-    plan[PH_TILES] = n_tile_items;
+    plan[PH_TOKENS] = total[0];
+    plan[PH_SHORTS] = all[0];
+    plan[PH_TILES] = n_items;
     plan[PH_MERGES] = n_merged;
   }
 }

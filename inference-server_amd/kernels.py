@@ -9,8 +9,8 @@ buffers from the caching allocator, so calls on different streams never share on
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -422,17 +422,34 @@ V_BLOCK_FP8 = (2, PAGE_SIZE // 4, HEAD_DIM // 2, 4)          # dim / 64, token /
 PLAN_MAX_SEQS, PLAN_MAX_TOKENS, PLAN_MAX_PAGES = 4096, 1 << 18, 1 << 22
 
 
-def _launch_on(t: torch.Tensor):
-    """Makes t's device the current one for a launch, where it is not."""
-    if torch._C._cuda_getDevice() == t.device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(what: str, device: int, entry, *args) -> None:
+    """One call of an entry point with `device` as the current one (a kernel is launched on the current device)."""
+    if torch._C._cuda_getDevice() == device:
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
+    if rc:
+        _lib.check(rc, what)
 
 
 def _same_device(first: torch.Tensor, **others: torch.Tensor) -> None:
     for name, t in others.items():
         if t.device != first.device:
             raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan_sizes(*sizes: int):
+    """(shape, reference to it, int32 of the plan, sizes of its sections, workspace bytes of its attention)"""
+    lib = _lib.load()
+    shape = _lib.PlanShape(*sizes)
+    at = (ctypes.c_int32 * len(_lib.PLAN_SECTIONS))()
+    ints = lib.moe_mi355x_paged_plan_bytes(ctypes.byref(shape), at) // 4
+    # the sections that callers read follow each other, between the counts and the lists
+    ends = [*at[1:], at[4] + shape.tokens]
+    sections = [at[0], *(e - a for a, e in zip(at, ends)), ints - ends[-1]]
+    return shape, ctypes.byref(shape), ints, sections, lib.moe_mi355x_paged_attn_fp8_workspace_bytes(shape)
 
 
 class PagedPlan:
@@ -444,35 +461,37 @@ class PagedPlan:
     are views of what the GPU holds; the rest is the kernels' own.
     """
 
-    __slots__ = ("shape", "buffer", "block_tables", "_at", "_ref")
+    __slots__ = ("sizes", "buffer", "block_tables", "device", "_shape", "_ref", "_ws_bytes", "_sections", "_views")
 
-    def __init__(self, shape: _lib.PlanShape, buffer: torch.Tensor, at, block_tables: torch.Tensor):
-        self.shape, self.buffer, self._at, self.block_tables = shape, buffer, at, block_tables
-        self._ref = ctypes.byref(shape)
+    def __init__(self, sizes: tuple, buffer: torch.Tensor, block_tables: torch.Tensor):
+        self.sizes, self.buffer, self.block_tables, self.device = sizes, buffer, block_tables, buffer.get_device()
+        self._shape, self._ref, _, self._sections, self._ws_bytes = _plan_sizes(*sizes)
+        self._views = None
 
-    def _section(self, name: str, size: int) -> torch.Tensor:
-        first = self._at[_lib.PLAN_SECTIONS.index(name)]
-        return self.buffer[first:first + size]
+    def _section(self, name: str) -> torch.Tensor:
+        if self._views is None:
+            self._views = self.buffer.split_with_sizes(self._sections)
+        return self._views[1 + _lib.PLAN_SECTIONS.index(name)]
 
     @property
     def positions(self) -> torch.Tensor:
-        return self._section("positions", self.shape.tokens)
+        return self._section("positions")
 
     @property
     def slots(self) -> torch.Tensor:
-        return self._section("slots", self.shape.tokens)
+        return self._section("slots")
 
     @property
     def cu_tokens(self) -> torch.Tensor:
-        return self._section("cu_tokens", self.shape.seqs + 1)
+        return self._section("cu_tokens")
 
     @property
     def context_lens(self) -> torch.Tensor:
-        return self._section("context_lens", self.shape.seqs)
+        return self._section("context_lens")
 
     @property
     def pages_used(self) -> torch.Tensor:
-        return self._section("pages_used", 1)
+        return self._section("pages_used")
 
 
 def paged_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -488,64 +507,65 @@ def paged_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: 
 
     With ``out``, an earlier plan of the same sizes, that plan's memory is filled again: a captured step keeps one.
     """
-    _need(cached_lens, "cached_lens", torch.int32, 1)
-    _need(new_lens, "new_lens", torch.int32, 1)
-    _need(block_tables, "block_tables", torch.int32, 2)
-    _need(free_pages, "free_pages", torch.int32, 1)
-    _same_device(cached_lens, new_lens=new_lens, block_tables=block_tables, free_pages=free_pages)
+    dev = block_tables.get_device() if isinstance(block_tables, torch.Tensor) else -1
+    if not (_fits(block_tables, torch.int32, dev, 2) and _fits(cached_lens, torch.int32, dev, 1) and
+            _fits(new_lens, torch.int32, dev, 1) and _fits(free_pages, torch.int32, dev, 1)):
+        for t, name, ndim in ((block_tables, "block_tables", 2), (cached_lens, "cached_lens", 1), (new_lens, "new_lens", 1),
+                              (free_pages, "free_pages", 1)):
+            _need(t, name, torch.int32, ndim)
+        _same_device(block_tables, cached_lens=cached_lens, new_lens=new_lens, free_pages=free_pages)
     B, max_pages = block_tables.shape
     if cached_lens.shape[0] != B or new_lens.shape[0] != B:
         raise ValueError("cached_lens and new_lens need one entry per row of block_tables")
     if B > PLAN_MAX_SEQS or not 0 <= num_tokens <= PLAN_MAX_TOKENS or not 1 <= max_pages <= PLAN_MAX_PAGES:
-        raise ValueError(f"a step has at most {PLAN_MAX_SEQS} sequences, {PLAN_MAX_TOKENS} tokens and "
+        raise ValueError(f"a step has at most {PLAN_MAX_SEQS} sequences, {PLAN_MAX_TOKENS} tokens and 1 to "
                          f"{PLAN_MAX_PAGES} pages a sequence, got {B}, {num_tokens} and {max_pages}")
     if not 1 <= max_new_tokens < 1 << 31:
         raise ValueError(f"max_new_tokens must be positive, got {max_new_tokens}")
-    if num_kv_heads < 1 or num_kv_heads > 1024 or num_heads % num_kv_heads or not 1 <= num_heads // num_kv_heads <= 16:
+    if not 1 <= num_kv_heads <= 1024 or num_heads % num_kv_heads or not 1 <= num_heads // num_kv_heads <= 16:
         raise ValueError(f"num_heads ({num_heads}) must be a multiple of num_kv_heads ({num_kv_heads}, 1 to 1024) with "
                          "1 to 16 query heads per kv head")
-    if free_pages.shape[0] >= 1 << 31:
+    n_free = free_pages.shape[0]
+    if n_free >= 1 << 31:
         raise ValueError("free_pages is too long")
-    lib = _lib.load()
+    sizes = (B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads)
     if out is None:
-        shape = _lib.PlanShape(B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads)
-        at = (ctypes.c_int32 * len(_lib.PLAN_SECTIONS))()
-        nbytes = lib.moe_mi355x_paged_plan_bytes(shape, at)
-        out = PagedPlan(shape, torch.empty(nbytes // 4, dtype=torch.int32, device=cached_lens.device), at, block_tables)
+        ints = _plan_sizes(*sizes)[2]
+        out = PagedPlan(sizes, torch.empty(ints, dtype=torch.int32, device=block_tables.device), block_tables)
     else:
-        s = out.shape
-        if (s.seqs, s.tokens, s.max_new, s.max_pages, s.heads, s.kv_heads) != \
-                (B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads):
-            raise ValueError("out is a plan of other sizes")
-        _same_device(cached_lens, out=out.buffer)
+        if out.sizes != sizes or out.device != dev:
+            raise ValueError(f"out is a plan of sizes {out.sizes} on device {out.device}, not of {sizes} on {dev}")
         out.block_tables = block_tables
-    with _launch_on(cached_lens):
-        _lib.check(lib.moe_mi355x_paged_plan(cached_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
-                                             free_pages.data_ptr(), free_pages.shape[0], out._ref,
-                                             out.buffer.data_ptr(), out.buffer.numel() * 4, _stream(cached_lens)),
-                   "paged_plan")
+    _launch("paged_plan", dev, _lib.load().moe_mi355x_paged_plan, cached_lens.data_ptr(), new_lens.data_ptr(),
+            block_tables.data_ptr(), free_pages.data_ptr(), n_free, out._ref, out.buffer.data_ptr(),
+            out.buffer.shape[0] * 4, _stream(block_tables))
     return out
 
 
-def _need_rows(t: torch.Tensor, name: str, tokens: int, heads: int) -> int:
-    """Checks a bf16 [tokens, heads, 128] tensor whose tokens may lie apart (a slice of a fused projection);
+def _fits(t, dtype, device: int, ndim: int) -> bool:
+    """What ``_need`` asks for, on GPU `device`, as one test (the errors are ``_need``'s to tell apart)."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device >= 0 and t.dim() == ndim and
+            t.is_contiguous())
+
+
+def _need_rows(t: torch.Tensor, name: str, plan: PagedPlan, heads: int) -> int:
+    """Checks a step's bf16 [tokens, heads, 128] tensor whose tokens may lie apart (a slice of a fused projection);
     returns the values from one token to the next."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must have dtype torch.bfloat16, got {t.dtype}")
+    tokens = plan.sizes[1]
     if t.shape != (tokens, heads, HEAD_DIM):
         raise ValueError(f"{name} must be {(tokens, heads, HEAD_DIM)}, got {tuple(t.shape)}")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name} must be on a ROCm GPU device, got {t.device}")
+    if t.get_device() != plan.device:
+        raise ValueError(f"{name} must be on the plan's device, {plan.buffer.device}, got {t.device}")
     row = heads * HEAD_DIM
-    if tokens == 0:
+    if t.is_contiguous():
         return row
     apart, head, one = t.stride()
     if one != 1 or (heads > 1 and head != HEAD_DIM):
         raise ValueError(f"{name}: a token's heads must be contiguous")
-    if tokens == 1:
-        return row
     if apart < row or apart % 8:
         raise ValueError(f"{name}: tokens must be a multiple of 8 values apart and not overlap, got {apart}")
     return apart
@@ -555,20 +575,23 @@ def _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan) -> int:
     """The pools of the plan's kv heads; returns their pages."""
     if not isinstance(plan, PagedPlan):
         raise TypeError("plan must be a PagedPlan (paged_plan)")
-    _need(k_cache, "k_cache", FP8, 5)
-    _need(v_cache, "v_cache", FP8, 6)
-    _need(k_scale, "k_scale", torch.float32, 2)
-    _need(v_scale, "v_scale", torch.float32, 2)
-    pages, heads = k_cache.shape[0], plan.shape.kv_heads
-    if k_cache.shape != (pages, heads, *K_BLOCK_FP8):
+    dev, heads = plan.device, plan.sizes[5]
+    if not (_fits(k_cache, FP8, dev, 5) and _fits(v_cache, FP8, dev, 6) and _fits(k_scale, torch.float32, dev, 2) and
+            _fits(v_scale, torch.float32, dev, 2)):
+        _need(k_cache, "k_cache", FP8, 5)
+        _need(v_cache, "v_cache", FP8, 6)
+        _need(k_scale, "k_scale", torch.float32, 2)
+        _need(v_scale, "v_scale", torch.float32, 2)
+        _same_device(plan.buffer, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    pages = k_cache.shape[0]
+    if k_cache.shape != (pages, heads, 8, 16, 16):
         raise ValueError(f"k_cache must be [pages, {heads}, 8, 16, 16], got {tuple(k_cache.shape)}")
-    if v_cache.shape != (pages, heads, *V_BLOCK_FP8):
+    if v_cache.shape != (pages, heads, 2, 4, 64, 4):
         raise ValueError(f"v_cache must be [{pages}, {heads}, 2, 4, 64, 4], got {tuple(v_cache.shape)}")
     if k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
         raise ValueError(f"k_scale and v_scale must be [{pages}, {heads}]")
     if pages >= 1 << 27:
         raise ValueError("a pool has fewer than 2^27 pages")
-    _same_device(plan.buffer, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     return pages
 
 
@@ -583,15 +606,12 @@ def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cac
     its codes are re-coded.  ``unpack_kv_fp8`` gives the values back.
     """
     pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
-    T, Hkv = plan.shape.tokens, plan.shape.kv_heads
-    k_stride = _need_rows(k, "k", T, Hkv)
-    v_stride = _need_rows(v, "v", T, Hkv)
-    _same_device(plan.buffer, k=k, v=v)
-    with _launch_on(k):
-        _lib.check(_lib.load().moe_mi355x_kv_append_fp8(
-            k.data_ptr(), v.data_ptr(), k_stride, v_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), HEAD_DIM, PAGE_SIZE, pages, plan._ref, plan.buffer.data_ptr(), _stream(k)),
-            "kv_append_fp8")
+    heads = plan.sizes[5]
+    k_stride = _need_rows(k, "k", plan, heads)
+    v_stride = _need_rows(v, "v", plan, heads)
+    _launch("kv_append_fp8", plan.device, _lib.load().moe_mi355x_kv_append_fp8, k.data_ptr(), v.data_ptr(), k_stride,
+            v_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), HEAD_DIM, PAGE_SIZE,
+            pages, plan._ref, plan.buffer.data_ptr(), _stream(k))
 
 
 def qk_norm_rope_append_fp8(qkv: torch.Tensor, q_norm_weight: torch.Tensor, k_norm_weight: torch.Tensor,
@@ -602,24 +622,26 @@ def qk_norm_rope_append_fp8(qkv: torch.Tensor, q_norm_weight: torch.Tensor, k_no
     and single tokens (modeling_qwen3_moe.py:162-171).  ``qkv`` bf16 [T, (Hq + 2 Hkv) * 128]; returns q bf16
     [T, Hq, 128] (padding rows: zeros).  fp32 from the projections to the one rounding of each result."""
     pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
-    s = plan.shape
-    if (num_heads, num_kv_heads) != (s.heads, s.kv_heads):
-        raise ValueError(f"the plan is for {s.heads} query and {s.kv_heads} kv heads")
-    _need(qkv, "qkv", torch.bfloat16, 2)
-    _need(q_norm_weight, "q_norm_weight", torch.bfloat16, 1)
-    _need(k_norm_weight, "k_norm_weight", torch.bfloat16, 1)
-    _need(inv_freq, "inv_freq", torch.float32, 1)
-    if qkv.shape != (s.tokens, (num_heads + 2 * num_kv_heads) * HEAD_DIM):
-        raise ValueError(f"qkv must be [{s.tokens}, (Hq + 2 Hkv) * 128], got {tuple(qkv.shape)}")
+    _, tokens, _, _, heads, kv_heads = plan.sizes
+    if num_heads != heads or num_kv_heads != kv_heads:
+        raise ValueError(f"the plan is for {heads} query and {kv_heads} kv heads")
+    dev = plan.device
+    if not (_fits(qkv, torch.bfloat16, dev, 2) and _fits(q_norm_weight, torch.bfloat16, dev, 1) and
+            _fits(k_norm_weight, torch.bfloat16, dev, 1) and _fits(inv_freq, torch.float32, dev, 1)):
+        _need(qkv, "qkv", torch.bfloat16, 2)
+        _need(q_norm_weight, "q_norm_weight", torch.bfloat16, 1)
+        _need(k_norm_weight, "k_norm_weight", torch.bfloat16, 1)
+        _need(inv_freq, "inv_freq", torch.float32, 1)
+        _same_device(plan.buffer, qkv=qkv, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, inv_freq=inv_freq)
+    if qkv.shape != (tokens, (heads + 2 * kv_heads) * HEAD_DIM):
+        raise ValueError(f"qkv must be [{tokens}, (Hq + 2 Hkv) * 128], got {tuple(qkv.shape)}")
     if q_norm_weight.shape[0] != HEAD_DIM or k_norm_weight.shape[0] != HEAD_DIM or inv_freq.shape[0] != HEAD_DIM // 2:
         raise ValueError("the norm weights must be [128] and inv_freq [64]")
-    _same_device(plan.buffer, qkv=qkv, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, inv_freq=inv_freq)
-    q = torch.empty((s.tokens, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
-    with _launch_on(qkv):
-        _lib.check(_lib.load().moe_mi355x_qk_norm_rope_append_fp8(
-            qkv.data_ptr(), q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), inv_freq.data_ptr(), float(eps),
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), HEAD_DIM,
-            PAGE_SIZE, pages, plan._ref, plan.buffer.data_ptr(), _stream(qkv)), "qk_norm_rope_append_fp8")
+    q = qkv.new_empty((tokens, heads, HEAD_DIM))
+    _launch("qk_norm_rope_append_fp8", dev, _lib.load().moe_mi355x_qk_norm_rope_append_fp8, qkv.data_ptr(),
+            q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), inv_freq.data_ptr(), float(eps), q.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), HEAD_DIM, PAGE_SIZE, pages,
+            plan._ref, plan.buffer.data_ptr(), _stream(qkv))
     return q
 
 
@@ -632,21 +654,18 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     fp32 scores, softmax and sums.  Keys of pages that the table does not hold are left out; a token without keys
     and a padding row give zeros."""
     pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
-    s = plan.shape
-    q_stride = _need_rows(q, "q", s.tokens, s.heads)
-    _same_device(plan.buffer, q=q)
+    heads = plan.sizes[4]
+    q_stride = _need_rows(q, "q", plan, heads)
     scale = float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    lib = _lib.load()
-    out = torch.empty((s.tokens, s.heads, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    nws = lib.moe_mi355x_paged_attn_fp8_workspace_bytes(plan._ref)
-    ws = _ws(nws, q.device)
-    with _launch_on(q):
-        _lib.check(lib.moe_mi355x_paged_attn_fp8(
-            q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            plan.block_tables.data_ptr(), HEAD_DIM, PAGE_SIZE, pages, scale, plan._ref, plan.buffer.data_ptr(),
-            out.data_ptr(), ws.data_ptr(), nws, _stream(q)), "paged_attention_fp8")
+    out = q.new_empty((plan.sizes[1], heads, HEAD_DIM))
+    nws = plan._ws_bytes
+    ws = plan.buffer.new_empty(nws // 4) if nws else None
+    _launch("paged_attention_fp8", plan.device, _lib.load().moe_mi355x_paged_attn_fp8, q.data_ptr(), q_stride,
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), plan.block_tables.data_ptr(),
+            HEAD_DIM, PAGE_SIZE, pages, scale, plan._ref, plan.buffer.data_ptr(), out.data_ptr(),
+            ws.data_ptr() if nws else None, nws, _stream(q))
     return out
 
 
