@@ -38,8 +38,7 @@ struct AttnFp8Args {
   uint16_t* out;         // [T][Hq][128]
   float *short_o, *short_ml, *tile_o, *tile_ml;  // partial results, by item
   int num_pages;
-  int merge_rows;  // rows that an entry of the merge list may have
-  float scale;     // times log2(e)
+  float scale;  // times log2(e)
   PlanLayout p;
 };
 
@@ -515,14 +514,17 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   __shared__ float s_m[8], s_l[8];
   __shared__ __attribute__((aligned(16))) v4f s_o[8][32];
-  const long tasks = (long)a.plan[PH_MERGES] * p.Hkv * a.merge_rows;
-  for (long task = blockIdx.x; task < tasks; task += gridDim.x) {  // workgroup-uniform
-    const int r = (int)(task % a.merge_rows), g = (int)(task / a.merge_rows % p.Hkv);
-    const int4 e = *(const int4*)(a.plan + p.merges + 4 * (task / a.merge_rows / p.Hkv));
+  const int shorts = a.plan[PH_SHORT_MERGES];
+  const int short_tasks = shorts * p.Hkv * kShortRows, tasks = short_tasks + a.plan[PH_TILE_MERGES] * p.Hkv * kTileRows;
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {  // workgroup-uniform
+    const bool tile = task >= short_tasks;
+    const int stride = tile ? kTileRows : kShortRows, i = tile ? task - short_tasks : task;
+    const int r = i % stride, g = i / stride % p.Hkv;
+    const int4 e = *(const int4*)(a.plan + p.merges + 4L * ((tile ? shorts : 0) + i / stride / p.Hkv));
     if (r >= e.w * p.G) continue;
-    const int ns = abs(e.x), stride = e.x < 0 ? kTileRows : kShortRows;
-    const float* part = e.x < 0 ? a.tile_o : a.short_o;
-    const float* ml = e.x < 0 ? a.tile_ml : a.short_ml;
+    const int ns = e.x;
+    const float* part = tile ? a.tile_o : a.short_o;
+    const float* ml = tile ? a.tile_ml : a.short_ml;
     float M = -INFINITY, L = 0.f;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = grp; s0 < ns; s0 += 32) {
@@ -557,14 +559,14 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
     __syncthreads();
     if (grp == 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+      for (int k = 0; k < 8; ++k) M = fmaxf(M, s_m[k]);
       L = 0.f;
       acc = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = s_m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i] - M);
-        L += s_l[i] * w;
-        acc += s_o[i][lane] * w;
+      for (int k = 0; k < 8; ++k) {
+        const float w = s_m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[k] - M);
+        L += s_l[k] * w;
+        acc += s_o[k][lane] * w;
       }
       const float inv = M == -INFINITY ? 0.f : 1.0f / L;
       uint16_t* dst = a.out + ((long)(e.z + r / p.G) * p.Hq + g * p.G + r % p.G) * kHD + 4 * lane;
@@ -591,7 +593,8 @@ void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
 }
 
 bool attn_grid_ok(const PlanLayout& p) {
-  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv);
+  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) &&
+         moe_grid_fits((long)p.M * p.Hkv * kTileRows);
 }
 
 }  // namespace
@@ -639,8 +642,7 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   hipLaunchKernelGGL(attn_fp8_short_kernel, dim3((unsigned)(p.S * p.Hkv + kPadBlocks)), dim3(256), 0, s, a);
   MOE_CHECK_LAUNCH();
   if (parts.shorts + parts.tiles > 0 && p.M > 0) {
-    a.merge_rows = parts.tiles > 0 ? kTileRows : kShortRows;
-    const long tasks = (long)p.M * p.Hkv * a.merge_rows;
+    const long tasks = (long)p.M * p.Hkv * (parts.tiles > 0 ? kTileRows : kShortRows);
     hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3((unsigned)(tasks < kMergeBlocks ? tasks : kMergeBlocks)), dim3(256), 0, s,
                        a);
     MOE_CHECK_LAUNCH();

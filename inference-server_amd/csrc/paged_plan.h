@@ -9,8 +9,8 @@
 //   writes  [W][4]       pages that get tokens: {page or -1, first token, its slot, tokens}
 //   shorts  [S][8]       attention items of sequences with few query rows (PI_*)
 //   tiles   [N][8]       attention items of the others: kTileRows query rows (PI_*)
-//   merges  [M][4]       rows whose keys are split over items: {items (< 0: of tiles), first item,
-//                        first token, tokens}
+//   merges  [M][4]       rows whose keys are split over items, the short ones' first: {items, first item, first
+//                        token, tokens}
 #pragma once
 
 #include "common.h"
@@ -31,7 +31,7 @@ constexpr int kTileTarget = 512;
 constexpr int kTileMinKeys = 512;
 constexpr int kTileKeys = 64;        // keys per step of a tile
 
-enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_MERGES, PH_PAGES = 15, PH_INTS };
+enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_SHORT_MERGES, PH_TILE_MERGES, PH_PAGES = 15, PH_INTS };
 // page_begin .. page_end: the item's keys; parts: items that share the rows (1: none other)
 enum { PI_SEQ, PI_TOK, PI_NTOK, PI_POS, PI_PAGE0, PI_PAGE1, PI_PARTS, PI_INTS = 8 };
 

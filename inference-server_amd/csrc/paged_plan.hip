@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     int mine[2] = {ns, ns > 1 ? 1 : 0}, round[2];
     block_scan(mine, round, s_wave);
     const int item = n_items + mine[0], merge = n_merged + mine[1];
-    if (ns > 1) *(int4*)(plan + p.merges + 4L * merge) = make_int4(-ns, item, tok, count);
+    if (ns > 1) *(int4*)(plan + p.merges + 4L * merge) = make_int4(ns, item, tok, count);
     for (int s = 0; s < ns; ++s) {
       const int pages = pages_of(keys), step = ns > 1 ? (int)(chunk / kPlanPage) : pages;
       int4* dst = (int4*)(plan + p.tiles + (long)PI_INTS * (item + s));
@@ -255,7 +255,8 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     plan[PH_TOKENS] = total[0];
     plan[PH_SHORTS] = all[0];
     plan[PH_TILES] = n_items;
-    plan[PH_MERGES] = n_merged;
+    plan[PH_SHORT_MERGES] = all[1];
+    plan[PH_TILE_MERGES] = n_merged - all[1];
   }
 }
 
