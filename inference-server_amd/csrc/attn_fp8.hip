@@ -20,11 +20,13 @@ namespace {
 
 constexpr int kHD = kKvHead;
 constexpr int kPage = kPlanPage;
-constexpr int kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCachePolicyNT = 2;  // the instruction's cache-policy field: nt (streaming)
 constexpr int kPadBlocks = 8;      // workgroups that clear the rows behind the last sequence
-constexpr int kMergeBlocks = 1024;
+constexpr int kMergeBlocks = 512;
+constexpr int kMergeFew = 8;
+constexpr int kFewItems = 256;
+constexpr float kSlack = 8.f;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -94,7 +96,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // O^T [128 x 16 rows] += V^T [128 x 32 keys] P^T (8 MFMAs for two pages).  Lane l has row l & 15 throughout, and
 // of its scores keys 4 (l >> 4) + i of each page, which are the 8 keys that the second MFMA wants from it.
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void attn_fp8_short_kernel(AttnFp8Args a) {
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))) void attn_fp8_short_kernel(AttnFp8Args a) {
+  constexpr int kThreads = 64 * kWaves;
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -104,7 +108,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
   if ((int)blockIdx.x >= items) {  // rows behind the last sequence: zeros
     const long row = (long)p.Hq * kHD / 8;  // 16-byte pieces of a token
     const long end = p.T * row;
-    for (long i = a.plan[PH_TOKENS] * row + ((int)blockIdx.x - items) * 256 + threadIdx.x; i < end; i += kPadBlocks * 256)
+    for (long i = a.plan[PH_TOKENS] * row + ((int)blockIdx.x - items) * kThreads + threadIdx.x; i < end;
+         i += kPadBlocks * kThreads)
       ((uint4*)a.out)[i] = make_uint4(0, 0, 0, 0);
     return;
   }
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
       float pm = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
                        fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
       pm = rows_max(pm);
-      if (__any(pm > m_run)) {  // some row's maximum grows
+      if (__any(pm > m_run + kSlack)) {  // as in the tile kernel
         const float m_new = fmaxf(m_run, pm);
         const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
@@ -260,36 +265,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
     for (int i = 0; i < 4; ++i)
       *(v4f*)&s_o[wave][lr][64 * j + 16 * lg + 4 * i] = (v4f){o[4 * j][i], o[4 * j + 1][i], o[4 * j + 2][i], o[4 * j + 3][i]};
   __syncthreads();
-  const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  constexpr int kDims = kShortRows * kHD / kThreads;  // of a row, a thread's
+  const int r = threadIdx.x / (kHD / kDims), d0 = threadIdx.x % (kHD / kDims) * kDims;
   if (r >= rows) return;
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
-  float wgt[kWaves], L = 0.f;
+  float acc[kDims], L = 0.f;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) acc[d] = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    wgt[w] = s_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - M);
-    L += s_l[w][r] * wgt[w];
-  }
-  float acc[8];
+    const float wgt = s_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - M);
+    L += s_l[w][r] * wgt;
 #pragma unroll
-  for (int d = 0; d < 8; ++d) {
-    acc[d] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) acc[d] += s_o[w][r][d0 + d] * wgt[w];
+    for (int d = 0; d < kDims; ++d) acc[d] += s_o[w][r][d0 + d] * wgt;
   }
   if (parts == 1) {
     const float inv = M == -INFINITY ? 0.f : 1.0f / L;  // no key at all: zeros
     uint16_t* dst = a.out + ((long)(tok + r / G) * p.Hq + g * G + r % G) * kHD + d0;
-    *(uint4*)dst = make_uint4(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv),
-                              pack_bf16(acc[4] * inv, acc[5] * inv), pack_bf16(acc[6] * inv, acc[7] * inv));
+#pragma unroll
+    for (int d = 0; d < kDims; d += 2) *(uint32_t*)(dst + d) = pack_bf16(acc[d] * inv, acc[d + 1] * inv);
     return;
   }
   const long base = ((long)item * Hkv + g) * kShortRows + r;
   float* dst = a.short_o + base * kHD + d0;
-  *(float4*)dst = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  *(float4*)(dst + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-  if ((threadIdx.x & 15) == 0) *(float2*)(a.short_ml + 2 * base) = make_float2(M, L);
+#pragma unroll
+  for (int d = 0; d < kDims; d += 2) *(float2*)(dst + d) = make_float2(acc[d], acc[d + 1]);
+  if (d0 == 0) *(float2*)(a.short_ml + 2 * base) = make_float2(M, L);
 }
 
 // ---------------------------------------------------------------------------
@@ -302,6 +305,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void a
 // ---------------------------------------------------------------------------
 constexpr int kStepPages = kTileKeys / kPage;
 
+// Scheduling of the block so far: N MFMAs with V vector instructions behind each, LDS reads kAhead MFMAs ahead
+#ifndef AHEAD
+#define AHEAD 2
+#endif
+#ifndef VA
+#define VA 3
+#endif
+#ifndef VB
+#define VB 5
+#endif
+#define MIX(N, V)                                              \
+  do {                                                         \
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);     \
+    _Pragma("unroll") for (int _i = 0; _i < (N); ++_i) {       \
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
+      if (_i + AHEAD < (N)) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       \
+      __builtin_amdgcn_sched_group_barrier(0x002, (V), 0);     \
+    }                                                          \
+  } while (0)
 __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 63;
@@ -331,38 +353,52 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
 #pragma unroll
     for (int s = 0; s < 8; ++s) qop[s] = __builtin_bit_cast(v8bf, *(const uint4*)(src + 16 * s));
   }
-  const int key_end = pos + row_tok + 1;                              // of this lane's row
-  const int all_end = pos + min(32 * wave / G, ntok - 1) + 1;         // keys that every row of the wave sees
-  const int any_end = pos + min((32 * wave + 31) / G, ntok - 1) + 1;  // and that any sees
+  const int key_end = pos + row_tok + 1;                       // of this lane's row
+  const int all_end = pos + min(32 * wave / G, ntok - 1) + 1;  // keys that every row of the wave sees
 
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_ref = -INFINITY, l_run = 0.f;
   v16f o[4];  // o[db][i]: dim slot 32 db + 8 (i / 4) + 4 kg + i % 4 of row lr
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
+  // Page ids and scales, 64 pages (16 steps) at a time, one a lane; the next 64 are fetched two steps ahead.
   const int32_t* table = a.tables + (long)seq * p.max_pages;
-  // the ids and scales of 64 pages, one a lane
-  int my_page;
-  float my_ks, my_vs;
-  auto fetch = [&](int first) __attribute__((always_inline)) {
+  int my_page, next_page = -1;
+  float my_ks, my_vs, next_ks = 1.f, next_vs = 1.f;
+  auto fetch_ids = [&](int first) __attribute__((always_inline)) {
     const int mine = first + lane;
-    my_page = mine < page1 ? table[mine] : -1;
-    if (my_page >= a.num_pages || my_page < 0) my_page = -1;
-    const long blk = my_page < 0 ? 0 : (long)my_page * Hkv + g;
-    my_ks = a.num_pages > 0 ? a.k_scale[blk] : 1.f;
-    my_vs = a.num_pages > 0 ? a.v_scale[blk] : 1.f;
+    next_page = mine < page1 ? table[mine] : -1;
+  };
+  auto fetch_scales = [&]() __attribute__((always_inline)) {
+    if (next_page >= a.num_pages || next_page < 0) next_page = -1;  // a pad or a stale id: an empty page
+    const long blk = next_page < 0 ? 0 : (long)next_page * Hkv + g;
+    next_ks = a.num_pages > 0 ? a.k_scale[blk] : 1.f;
+    next_vs = a.num_pages > 0 ? a.v_scale[blk] : 1.f;
   };
   auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
   };
-  // a step's codes: K, 16 bytes (16 dims of a token) of pages wave / 2 and 2 + wave / 2; V, of page `wave`
-  // the quads kg and kg + 2 of 4 dims
+  // This thread's codes of a step: K, 16 bytes (16 dims of a token) of pages wave / 2 and 2 + wave / 2; V, of page
+  // `wave` the quads vq and vq + 2 of 4 dims.  K runs a step ahead of V.
   uint4 kr[2], vr[2];
-  float ks[2], vs;
+  float ks[2], vs = 1.f, vs_next = 1.f;
+  int v_page = -1;      // of the step that K was last loaded for
+  uint32_t held = 0;    // which of that step's pages there are
   const int vj = lane >> 5, vq = (lane >> 4) & 1, vx = lane & 15;
-  auto load = [&](int l) __attribute__((always_inline)) {  // l: the step's first page among the 64
+  auto load_k = [&](int step) __attribute__((always_inline)) {
+    const int l = (step & 15) * kStepPages;
+    if (l == 0) {
+      my_page = next_page;
+      my_ks = next_ks;
+      my_vs = next_vs;
+    }
+    if ((step & 15) == 13) fetch_ids(page0 + (step + 3) * kStepPages);
+    if ((step & 15) == 14) fetch_scales();
+    held = (uint32_t)(__ballot(my_page >= 0) >> l) & 15u;
+    v_page = __builtin_amdgcn_readlane(my_page, l + wave);
+    vs_next = lane_f(my_vs, l + wave);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int at = l + 2 * h + (wave >> 1);
@@ -370,12 +406,14 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
       kr[h] = block_load<0>(block_rsrc(a.k_cache, __builtin_amdgcn_readlane(my_page, at), Hkv, g),
                             (wave & 1) * 1024 + lane * 16);
     }
-    vs = lane_f(my_vs, l + wave);
-    const __amdgpu_buffer_rsrc_t rv = block_rsrc(a.v_cache, __builtin_amdgcn_readlane(my_page, l + wave), Hkv, g);
+  };
+  auto load_v = [&]() __attribute__((always_inline)) {  // of the step that K was last loaded for
+    const __amdgpu_buffer_rsrc_t rv = block_rsrc(a.v_cache, v_page, Hkv, g);
+    vs = vs_next;
 #pragma unroll
     for (int h = 0; h < 2; ++h) vr[h] = block_load<0>(rv, vj * 1024 + (vq + 2 * h) * 256 + vx * 16);
   };
-  auto store = [&](int buf, int page) __attribute__((always_inline)) {
+  auto store_k = [&](int buf) __attribute__((always_inline)) {
     const int c = 4 * (wave & 1) + (lane >> 4);  // dims 16 c .. +16 of token lane & 15
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -383,100 +421,139 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
       s_k[buf][2 * c][key] = __builtin_bit_cast(uint4, widen8(kr[h].x, kr[h].y, ks[h]));
       s_k[buf][2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
     }
-    if ((page + kStepPages) * kPage > pos + ntok) {  // codes behind the last key may be anything, a NaN too
+  };
+  auto mask_v = [&](int page) __attribute__((always_inline)) {  // codes behind the last key may be anything, a NaN too
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t mask = quad_mask(pos + ntok - ((page + wave) * kPage + 4 * (vq + 2 * h)));
-        vr[h].x &= mask;
-        vr[h].y &= mask;
-        vr[h].z &= mask;
-        vr[h].w &= mask;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t mask = quad_mask(pos + ntok - ((page + wave) * kPage + 4 * (vq + 2 * h)));
+      vr[h].x &= mask;
+      vr[h].y &= mask;
+      vr[h].z &= mask;
+      vr[h].w &= mask;
     }
+  };
+  auto store_v = [&](int buf) __attribute__((always_inline)) {
     const uint32_t v0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, v1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
 #pragma unroll
     for (int d = 0; d < 4; ++d)
       s_v[buf][wave][vq][64 * vj + 16 * d + vx] = __builtin_bit_cast(uint4, widen8(v0[d], v1[d], vs));
   };
+  auto scores = [&](v16f (&s)[2], int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_k[buf][2 * k + kg][32 * b + lr]), qop[k], s[b],
+                                                       0, 0, 0);
+  };
+  auto mask_scores = [&](v16f (&s)[2], int key0, uint32_t there) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = key0 + 32 * b + 8 * (i >> 2) + 4 * kg + (i & 3);
+        const bool ok = key < key_end && ((there >> (2 * b + (i >> 3))) & 1);
+        s[b][i] = ok ? s[b][i] : -INFINITY;
+      }
+  };
+  auto score_max = [&](const v16f (&s)[2]) __attribute__((always_inline)) {
+    float x = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) x = fmaxf(x, s[0][i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x = fmaxf(x, s[1][i]);
+    return x;
+  };
+  // 32 keys' probabilities, and their sum as the second product will see them
+  auto probabilities = [&](const v16f& s, v8bf (&pb)[2], float m) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const v2bf x = {(__bf16)__builtin_amdgcn_exp2f(fmaf(s[i], a.scale, -m)),
+                      (__bf16)__builtin_amdgcn_exp2f(fmaf(s[i + 1], a.scale, -m))};
+      pb[i >> 3][i & 7] = x[0];
+      pb[i >> 3][(i & 7) + 1] = x[1];
+      l_run = __builtin_amdgcn_fdot2_f32_bf16(x, (v2bf){(__bf16)1.f, (__bf16)1.f}, l_run, false);
+    }
+  };
+  auto output = [&](const v8bf (&pb)[2], int buf, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_v[buf][2 * half + h][kg][32 * d + lr]), pb[h],
+                                                       o[d], 0, 0, 0);
+  };
 
-  fetch(page0);
-  load(0);
-  store(0, page0);
-  __syncthreads();
-  int buf = 0;
-  for (int page = page0, l = 0; page < page1; page += kStepPages, buf ^= 1) {
-    const int here = l;  // this step's first page among the 64
-    uint64_t held = __ballot(my_page >= 0) >> here;  // which of its pages there are
-    const bool more = page + kStepPages < page1;
-    l += kStepPages;
-    if (more) {
-      if (l == 64) {
-        l = 0;
-        fetch(page + kStepPages);
-      }
-      load(l);
+  // Step n's scores are formed in the course of step n - 1, beside its softmax, so that the wave has MFMAs and vector
+  // work at the same time: K of step n + 2 and V of step n + 1 go into LDS during step n.
+  const int steps = (page1 - page0 + kStepPages - 1) / kStepPages;
+  v16f s0[2], s1[2];
+  float pm;
+  auto step = [&](v16f (&s)[2], v16f (&next)[2], int n, int buf) __attribute__((always_inline)) {
+    const int next_page0 = page0 + (n + 1) * kStepPages, next_key = next_page0 * kPage;
+    const uint32_t held_next = held;
+    load_v();  // step n + 1
+    load_k(n + 2);
+    // A row's reference need not be its maximum: only where a score passes it by more than 2^kSlack are the sums
+    // scaled down (exp stays below 2^kSlack, and bf16 and fp32 are as exact there as below 1)
+    pm = half_max(pm) * a.scale;
+    if (__any(pm > m_ref + kSlack)) {
+      const float m_new = fmaxf(m_ref, pm);
+      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+      m_ref = m_new;
+      l_run *= corr;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= corr;
     }
-    const int key0 = page * kPage;
-    if (key0 < any_end) {  // wave-uniform
-      v16f s[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_k[buf][2 * k + kg][32 * b + lr]), qop[k],
-                                                         s[b], 0, 0, 0);
-      if (key0 + kTileKeys > all_end || (held & 15) != 15) {  // wave-uniform
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = key0 + 32 * b + 8 * (i >> 2) + 4 * kg + (i & 3);
-            const bool ok = key < key_end && ((held >> (2 * b + (i >> 3))) & 1);
-            s[b][i] = ok ? s[b][i] : -INFINITY;
-          }
-      }
-      float pm = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[0][i]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pm = fmaxf(pm, s[1][i]);
-      pm = half_max(pm) * a.scale;
-      if (__any(pm > m_run)) {
-        const float m_new = fmaxf(m_run, pm);
-        const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= corr;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= corr;
-      }
-      const float m_ref = m_run == -INFINITY ? 0.f : m_run;
-      float ps = 0.f;
-      v8bf pb[4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -m_ref));
-          ps += x;
-          pb[2 * b + (i >> 3)][i & 7] = (__bf16)x;
-        }
-      l_run += ps;
-#pragma unroll
-      for (int g4 = 0; g4 < kStepPages; ++g4)
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_v[buf][g4][kg][32 * d + lr]), pb[g4],
-                                                         o[d], 0, 0, 0);
-    }
-    if (more) store(buf ^ 1, page + kStepPages);
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+    v8bf pa[2], pb[2];
+    scores(next, buf ^ 1);
+    probabilities(s[0], pa, m_use);
+    MIX(16, VA);
+    asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(l_run));  // not to be put off past the branches
+    if (next_key + kTileKeys > all_end || held_next != 15) mask_scores(next, next_key, held_next);
+    if (next_key + kTileKeys > pos + ntok) mask_v(next_page0);
+    output(pa, buf, 0);
+    probabilities(s[1], pb, m_use);
+    output(pb, buf, 1);
+    pm = score_max(next);
+    store_v(buf ^ 1);
+    store_k(buf);
+    MIX(16, VB);
+#ifdef PRIO
+    __builtin_amdgcn_s_setprio(0);
+#endif
     __syncthreads();
+#ifdef PRIO
+    __builtin_amdgcn_s_setprio(1);
+#endif
+  };
+  fetch_ids(page0);
+  fetch_scales();
+  load_k(0);
+  store_k(0);
+  load_v();
+  const uint32_t held0 = held;
+  if ((page0 + kStepPages) * kPage > pos + ntok) mask_v(page0);
+  store_v(0);
+  load_k(1);
+  store_k(1);
+  __syncthreads();
+  scores(s0, 0);
+  if (page0 * kPage + kTileKeys > all_end || held0 != 15) mask_scores(s0, page0 * kPage, held0);
+  pm = score_max(s0);
+  for (int n = 0; n < steps; n += 2) {
+    step(s0, s1, n, 0);
+    if (n + 1 == steps) break;
+    step(s1, s0, n + 1, 1);
   }
+  const float m_run = m_ref;
   l_run = half_sum(l_run);
   if (!live) return;
   if (parts == 1) {
@@ -505,34 +582,39 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order.  A workgroup takes one
-// (rows, kv head, row) at a time: 8 groups of 32 lanes share the items, a lane 4 dims; four items' loads are in
-// flight at once.
+// merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order, a lane of 32 with 4 dims.
+// Up to kMergeFew items: the 8 groups of 32 lanes take a row each.  More: they share a row's items.  Either way a
+// group has four items' loads in flight.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   __shared__ float s_m[8], s_l[8];
   __shared__ __attribute__((aligned(16))) v4f s_o[8][32];
-  const int shorts = a.plan[PH_SHORT_MERGES];
-  const int short_tasks = shorts * p.Hkv * kShortRows, tasks = short_tasks + a.plan[PH_TILE_MERGES] * p.Hkv * kTileRows;
-  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {  // workgroup-uniform
-    const bool tile = task >= short_tasks;
-    const int stride = tile ? kTileRows : kShortRows, i = tile ? task - short_tasks : task;
-    const int r = i % stride, g = i / stride % p.Hkv;
-    const int4 e = *(const int4*)(a.plan + p.merges + 4L * ((tile ? shorts : 0) + i / stride / p.Hkv));
-    if (r >= e.w * p.G) continue;
+  constexpr int kChunks = kTileRows / kShortRows;  // of a tile's rows
+  const int shorts = a.plan[PH_SHORT_MERGES], chunks = shorts + a.plan[PH_TILE_MERGES] * kChunks;
+  for (int x = blockIdx.x; x < chunks * p.Hkv; x += gridDim.x) {  // workgroup-uniform
+    const int chunk = x / p.Hkv, g = x % p.Hkv;
+    const bool tile = chunk >= shorts;
+    const int r0 = blockIdx.y + (tile ? (chunk - shorts) % kChunks * kShortRows : 0);
+    const int4 e = *(const int4*)(a.plan + p.merges + 4L * (tile ? shorts + (chunk - shorts) / kChunks : chunk));
     const int ns = e.x;
+    const bool few = ns <= kMergeFew;
+    if (r0 >= e.w * p.G || (few && r0 % 8 != 0)) continue;
+    const int r = few ? r0 + grp : r0;
+    const bool live = r < e.w * p.G;
     const float* part = tile ? a.tile_o : a.short_o;
     const float* ml = tile ? a.tile_ml : a.short_ml;
     float M = -INFINITY, L = 0.f;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = grp; s0 < ns; s0 += 32) {
+    const int by = few ? 1 : 8;
+    for (int s0 = few ? 0 : grp; s0 < ns; s0 += 4 * by) {
       float2 x[4];
       v4f v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const long base = ((long)(e.y + min(s0 + 8 * u, ns - 1)) * p.Hkv + g) * stride + r;
+        const int s = min(s0 + by * u, ns - 1);
+        const long base = ((long)(e.y + s) * p.Hkv + g) * (tile ? kTileRows : kShortRows) + (live ? r : r0);
         x[u] = *(const float2*)(ml + 2 * base);
         v[u] = *(const v4f*)(part + base * kHD + 4 * lane);
       }
@@ -546,18 +628,18 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
       acc *= old;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float w = s0 + 8 * u < ns ? __builtin_amdgcn_exp2f(x[u].x - M) : 0.f;
+        const float w = s0 + by * u < ns ? __builtin_amdgcn_exp2f(x[u].x - M) : 0.f;
         L += x[u].y * w;
         acc += v[u] * w;
       }
     }
-    s_o[grp][lane] = acc;
-    if (lane == 0) {
-      s_m[grp] = M;
-      s_l[grp] = L;
-    }
-    __syncthreads();
-    if (grp == 0) {
+    if (!few) {
+      s_o[grp][lane] = acc;
+      if (lane == 0) {
+        s_m[grp] = M;
+        s_l[grp] = L;
+      }
+      __syncthreads();
 #pragma unroll
       for (int k = 0; k < 8; ++k) M = fmaxf(M, s_m[k]);
       L = 0.f;
@@ -568,11 +650,13 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
         L += s_l[k] * w;
         acc += s_o[k][lane] * w;
       }
+      __syncthreads();  // the sums are read
+    }
+    if (few ? live : grp == 0) {
       const float inv = M == -INFINITY ? 0.f : 1.0f / L;
       uint16_t* dst = a.out + ((long)(e.z + r / p.G) * p.Hq + g * p.G + r % p.G) * kHD + 4 * lane;
       *(uint2*)dst = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
     }
-    __syncthreads();  // the sums are read
   }
 }
 
@@ -581,7 +665,7 @@ struct Parts {
   long shorts, tiles;  // rows
 };
 Parts attn_parts(const PlanLayout& p) {
-  return {p.max_pages > kShortStep ? (long)p.S * p.Hkv * kShortRows : 0,
+  return {p.short_whole ? 0 : (long)p.S * p.Hkv * kShortRows,
           (long)p.max_pages * kPage > kTileMinKeys ? (long)p.split_tiles * p.Hkv * kTileRows : 0};
 }
 
@@ -594,7 +678,7 @@ void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
 
 bool attn_grid_ok(const PlanLayout& p) {
   return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) &&
-         moe_grid_fits((long)p.M * p.Hkv * kTileRows);
+         moe_grid_fits((long)p.M * p.Hkv);
 }
 
 }  // namespace
@@ -639,12 +723,18 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
     hipLaunchKernelGGL(attn_fp8_tile_kernel, dim3((unsigned)(p.N * p.Hkv)), dim3(256), 0, s, a);
     MOE_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL(attn_fp8_short_kernel, dim3((unsigned)(p.S * p.Hkv + kPadBlocks)), dim3(256), 0, s, a);
+  const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));
+  // whole sequences of up to 128 pages, and no more of them than CUs: 16 waves each, four pairs of pages a wave
+  if (p.short_whole && p.S * p.Hkv <= kFewItems)
+    hipLaunchKernelGGL(attn_fp8_short_kernel<16>, grid, dim3(1024), 0, s, a);
+  else
+    hipLaunchKernelGGL(attn_fp8_short_kernel<4>, grid, dim3(256), 0, s, a);
   MOE_CHECK_LAUNCH();
   if (parts.shorts + parts.tiles > 0 && p.M > 0) {
-    const long tasks = (long)p.M * p.Hkv * (parts.tiles > 0 ? kTileRows : kShortRows);
-    hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3((unsigned)(tasks < kMergeBlocks ? tasks : kMergeBlocks)), dim3(256), 0, s,
-                       a);
+    // with tiles among them mostly nothing is split: fewer workgroups, that come back for more
+    const long x = (long)p.M * p.Hkv;
+    hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3(parts.tiles > 0 && x > kMergeBlocks ? kMergeBlocks : x, p.short_rows), dim3(256),
+                       0, s, a);
     MOE_CHECK_LAUNCH();
   }
   return MOE_OK;

@@ -73,10 +73,17 @@ __device__ __forceinline__ void norm_rope(float* x, const float* w, const float*
   }
 }
 
-// cos and sin of pos * inv_freq
+// cos and sin of pos * inv_freq.  What is left of the angle behind whole quarter turns is at most 1 / 8 turn, so
+// its rounding to 32 bits moves it by 2^-28 turns (2.3e-8 rad), below fp32's step for cos and sin.
 __device__ __forceinline__ void rope_angle(int pos, float inv_freq, float* c, float* s) {
-  const double turns = (double)pos * (double)inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
-  sincospif(2.0f * (float)(turns - rint(turns)), s, c);
+  const double quarters = (double)pos * (double)inv_freq * 0.63661977236758134308;  // 2 / pi
+  const double whole = rint(quarters);
+  float cr, sr;
+  sincospif(0.5f * (float)(quarters - whole), &sr, &cr);
+  const int q = (int)(long long)whole & 3;
+  const float a = q & 1 ? sr : cr, b = q & 1 ? cr : sr;
+  *c = q == 1 || q == 2 ? -a : a;
+  *s = q >= 2 ? -b : b;
 }
 
 template <bool FUSED>

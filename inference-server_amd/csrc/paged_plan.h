@@ -26,6 +26,9 @@ constexpr int kShortStep = 8;        // pages that a short item's workgroup take
 // Items that short sequences are split into, over all kv heads: the 1024 workgroups that the GPU
 // holds at once.
 constexpr int kShortTarget = 1024;
+// Tables of up to so many pages: a short sequence is one item and there is nothing to join, which saves the merge's
+// launch (3.5 us and a gap, of 13 us for one sequence of 1000 tokens).
+constexpr int kShortWhole = 128;
 // Workgroups that tiles are split for when there are fewer: two per CU, each with kTileMinKeys at least.
 constexpr int kTileTarget = 512;
 constexpr int kTileMinKeys = 512;
@@ -38,6 +41,8 @@ enum { PI_SEQ, PI_TOK, PI_NTOK, PI_POS, PI_PAGE0, PI_PAGE1, PI_PARTS, PI_INTS = 
 struct PlanLayout {
   int B, T, max_new, max_pages, Hq, Hkv, G;
   int tile_tok;               // tokens per tile
+  int short_rows;             // query rows that a short item may have
+  bool short_whole;           // short sequences are not split
   int W, S, N, M;             // list capacities
   int split_tiles;            // tiles, and items of tiles, that may hold partial results
   long cu, ctx, pos, slot, writes, shorts, tiles, merges, ints;  // offsets
@@ -60,7 +65,9 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   p.W = (int)(T < (T + 30 * B) / 16 ? T : (T + 30 * B) / 16);
   const long seqs = B < T ? B : T;  // with new tokens
   const long per = (s->max_pages + kShortStep - 1) / kShortStep;
-  const long by_target = seqs + (kShortTarget + p.Hkv - 1) / p.Hkv, by_pages = seqs * per;
+  p.short_rows = (long)p.max_new * p.G < kShortRows ? p.max_new * p.G : kShortRows;
+  p.short_whole = p.max_pages <= kShortWhole;
+  const long by_target = seqs + (kShortTarget + p.Hkv - 1) / p.Hkv, by_pages = p.short_whole ? seqs : seqs * per;
   p.S = (int)(by_target < by_pages ? by_target : by_pages);
   // no sequence is long enough for tiles: none
   const bool tiles = (long)p.max_new * p.G > kShortRows;

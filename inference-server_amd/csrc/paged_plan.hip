@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   // pages per short item
   long pps = ((long)s_pages * p.Hkv + kShortTarget - 1) / kShortTarget;
   pps = max(pps, 1L) + kShortStep - 1;
-  pps = pps / kShortStep * kShortStep;
+  pps = p.short_whole ? kShortWhole : pps / kShortStep * kShortStep;
   // keys per item of a tile; with enough tiles to fill the GPU they are not split
   long chunk = ((long)s_keys * p.Hkv + kTileTarget - 1) / kTileTarget;
   chunk = (max(chunk, (long)kTileMinKeys) + kTileKeys - 1) / kTileKeys * kTileKeys;
