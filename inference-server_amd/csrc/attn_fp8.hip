@@ -305,25 +305,19 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
 // ---------------------------------------------------------------------------
 constexpr int kStepPages = kTileKeys / kPage;
 
-// Scheduling of the block so far: N MFMAs with V vector instructions behind each, LDS reads kAhead MFMAs ahead
-#ifndef AHEAD
-#define AHEAD 2
-#endif
-#ifndef VA
-#define VA 3
-#endif
-#ifndef VB
-#define VB 5
-#endif
-#define MIX(N, V)                                              \
-  do {                                                         \
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);     \
-    _Pragma("unroll") for (int _i = 0; _i < (N); ++_i) {       \
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
-      if (_i + AHEAD < (N)) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       \
-      __builtin_amdgcn_sched_group_barrier(0x002, (V), 0);     \
-    }                                                          \
+// Schedules a step's half so far as 16 MFMAs with four vector instructions behind each, the LDS reads two MFMAs
+// ahead of their use.  (8192 tokens, 64 / 4 heads: the compiler's own order 1120 us, one read ahead 1100, two 1067,
+// four 1070, eight 1082; three to seven vector instructions within 1%.)
+#define MIX_MFMAS()                                                            \
+  do {                                                                         \
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                         \
+    _Pragma("unroll") for (int _i = 0; _i < 16; ++_i) {                        \
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                       \
+      if (_i + 2 < 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      \
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);                       \
+    }                                                                          \
   } while (0)
+
 __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 63;
@@ -515,7 +509,7 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
     v8bf pa[2], pb[2];
     scores(next, buf ^ 1);
     probabilities(s[0], pa, m_use);
-    MIX(16, VA);
+    MIX_MFMAS();
     asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(l_run));  // not to be put off past the branches
     if (next_key + kTileKeys > all_end || held_next != 15) mask_scores(next, next_key, held_next);
     if (next_key + kTileKeys > pos + ntok) mask_v(next_page0);
@@ -525,14 +519,8 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
     pm = score_max(next);
     store_v(buf ^ 1);
     store_k(buf);
-    MIX(16, VB);
-#ifdef PRIO
-    __builtin_amdgcn_s_setprio(0);
-#endif
+    MIX_MFMAS();
     __syncthreads();
-#ifdef PRIO
-    __builtin_amdgcn_s_setprio(1);
-#endif
   };
   fetch_ids(page0);
   fetch_scales();
@@ -597,7 +585,7 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
     const int chunk = x / p.Hkv, g = x % p.Hkv;
     const bool tile = chunk >= shorts;
     const int r0 = blockIdx.y + (tile ? (chunk - shorts) % kChunks * kShortRows : 0);
-    const int4 e = *(const int4*)(a.plan + p.merges + 4L * (tile ? shorts + (chunk - shorts) / kChunks : chunk));
+    const int4 e = *(const int4*)(a.plan + (tile ? p.tile_merges + 4L * ((chunk - shorts) / kChunks) : p.short_merges + 4L * chunk));
     const int ns = e.x;
     const bool few = ns <= kMergeFew;
     if (r0 >= e.w * p.G || (few && r0 % 8 != 0)) continue;
@@ -678,7 +666,7 @@ void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
 
 bool attn_grid_ok(const PlanLayout& p) {
   return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) &&
-         moe_grid_fits((long)p.M * p.Hkv);
+         moe_grid_fits((long)(p.SM + p.TM) * p.Hkv);
 }
 
 }  // namespace
@@ -730,9 +718,9 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   else
     hipLaunchKernelGGL(attn_fp8_short_kernel<4>, grid, dim3(256), 0, s, a);
   MOE_CHECK_LAUNCH();
-  if (parts.shorts + parts.tiles > 0 && p.M > 0) {
+  if (parts.shorts + parts.tiles > 0 && p.SM > 0) {
     // with tiles among them mostly nothing is split: fewer workgroups, that come back for more
-    const long x = (long)p.M * p.Hkv;
+    const long x = (long)(p.SM + p.TM) * p.Hkv;
     hipLaunchKernelGGL(attn_fp8_merge_kernel, dim3(parts.tiles > 0 && x > kMergeBlocks ? kMergeBlocks : x, p.short_rows), dim3(256),
                        0, s, a);
     MOE_CHECK_LAUNCH();

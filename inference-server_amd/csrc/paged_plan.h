@@ -9,8 +9,8 @@
 //   writes  [W][4]       pages that get tokens: {page or -1, first token, its slot, tokens}
 //   shorts  [S][8]       attention items of sequences with few query rows (PI_*)
 //   tiles   [N][8]       attention items of the others: kTileRows query rows (PI_*)
-//   merges  [M][4]       rows whose keys are split over items, the short ones' first: {items, first item, first
-//                        token, tokens}
+//   short_merges [..][4] sequences, resp. tiles, whose keys are split over items: {items, first item, first
+//   tile_merges  [..][4] token, tokens}
 #pragma once
 
 #include "common.h"
@@ -43,9 +43,9 @@ struct PlanLayout {
   int tile_tok;               // tokens per tile
   int short_rows;             // query rows that a short item may have
   bool short_whole;           // short sequences are not split
-  int W, S, N, M;             // list capacities
+  int W, S, N, SM, TM;        // list capacities
   int split_tiles;            // tiles, and items of tiles, that may hold partial results
-  long cu, ctx, pos, slot, writes, shorts, tiles, merges, ints;  // offsets
+  long cu, ctx, pos, slot, writes, shorts, tiles, short_merges, tile_merges, ints;  // offsets
 };
 
 static inline bool plan_shape_ok(const moe_mi355x_plan_shape* s) {
@@ -75,7 +75,8 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   const long target = (kTileTarget + p.Hkv - 1) / p.Hkv;
   p.split_tiles = (int)(tiles ? (nt < target ? nt : target) + target : 0);
   p.N = (int)(nt > p.split_tiles ? nt : p.split_tiles);
-  p.M = (int)(seqs + (nt < target ? nt : target));
+  p.SM = (int)seqs;
+  p.TM = (int)(nt < target ? nt : target);
   p.cu = PH_INTS;
   p.ctx = p.cu + B + 1;
   p.pos = p.ctx + B;
@@ -89,6 +90,7 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   p.writes = at(4L * p.W);
   p.shorts = at((long)PI_INTS * p.S);
   p.tiles = at((long)PI_INTS * p.N);
-  p.merges = at(4L * p.M);
+  p.short_merges = at(4L * p.SM);
+  p.tile_merges = at(4L * p.TM);
   return p;
 }
