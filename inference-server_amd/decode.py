@@ -22,6 +22,12 @@ faster than hipBLASLt in a graph replay (q/k/v + o_proj 1 / 16 / 24 rows: 19.7 /
 against 26.1 / 26.4 / 26.6 us), and on hipBLASLt through ``torch.nn.functional.linear`` above
 (32 rows: 24.5 against 23.6 us).
 ``DecodeModel.capture`` records a whole step as one HIP graph, so a step costs one launch.
+
+Over an 8-bit cache (``PagedKVCacheFp8``) ``DecodeModel.run`` takes prompts, chunks of them and single
+tokens in one call: ``DecodeModel.plan`` (``moe_mi355x_paged_plan``) builds the block tables, slots and positions
+on the GPU from the sequences' lengths, and each layer runs ``moe_mi355x_qk_norm_rope_append_fp8`` and
+``moe_mi355x_paged_attn_fp8`` in the place of the bf16 cache's pair.  ``DecodeModel.capture_run`` records plan and layers
+as one graph, which replays on lengths that change on the GPU.
 """
 
 from __future__ import annotations
@@ -83,6 +89,25 @@ class PagedKVCache:
         self.n_pages = n_pages
 
 
+class PagedKVCacheFp8:
+    """Per-layer paged K / V pools of e4m3 codes in the layout of ``moe_mi355x_kv_append_fp8``, with one power-of-two
+    scale per (page, kv head): half a ``PagedKVCache`` and 0.2%."""
+
+    def __init__(self, n_layers: int, n_pages: int, kv_heads: int, device):
+        def codes(block):
+            shape = (n_pages, kv_heads, *block)
+            return [torch.zeros(shape, dtype=torch.uint8, device=device).view(kernels.FP8) for _ in range(n_layers)]
+
+        self.k, self.v = codes(kernels.K_BLOCK_FP8), codes(kernels.V_BLOCK_FP8)
+        self.k_scale, self.v_scale = ([torch.ones((n_pages, kv_heads), dtype=torch.float32, device=device)
+                                       for _ in range(n_layers)] for _ in range(2))
+        self.n_pages = n_pages
+
+    def layer(self, i: int):
+        """Layer i's ``k_cache, v_cache, k_scale, v_scale``."""
+        return self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]
+
+
 class DecoderLayerWeights:
     """Weights of one decoder layer.  The q/k/v projections are stored as one fused
     [(Hq + 2 Hkv) * d, H] matrix (rows: q, then k, then v), so one GEMM serves all three."""
@@ -142,6 +167,18 @@ def attention_sublayer(w: DecoderLayerWeights, h, positions, context_lens, block
     return _linear(a.view(B, cfg.heads * cfg.head_dim), w.wo)
 
 
+def attention_sublayer_fp8(w: DecoderLayerWeights, h, plan: kernels.PagedPlan, inv_freq, k_cache, v_cache, k_scale,
+                           v_scale):
+    """``attention_sublayer`` over the 8-bit cache, for the rows of a plan: prompts and single tokens."""
+    cfg = w.cfg
+    x = kernels.rms_norm(h, w.ln1, cfg.rms_eps)
+    cache = (k_cache, v_cache, k_scale, v_scale)
+    q = kernels.qk_norm_rope_append_fp8(_linear(x, w.wqkv), w.q_norm, w.k_norm, inv_freq, cfg.heads, cfg.kv_heads,
+                                        cfg.rms_eps, *cache, plan)
+    a = kernels.paged_attention_fp8(q, *cache, plan, cfg.head_dim ** -0.5)
+    return _linear(a.view(h.shape[0], cfg.heads * cfg.head_dim), w.wo)
+
+
 def moe_sublayer(w: DecoderLayerWeights, h, attn_out=None):
     """``h' + moe_block(post_attention_layernorm(h'))`` with ``h' = h + attn_out``
     (modeling_qwen3_moe.py:341-347; ``attn_out`` None: ``h' = h``)."""
@@ -164,9 +201,12 @@ class DecodeModel:
     ``context_lens`` = positions + 1, ``block_tables`` int32 [B, max_pages]).  ``capture`` records
     one step as a HIP graph over static input buffers: copy a step's inputs into those buffers,
     then call the graph's ``replay()``.
+
+    With a ``PagedKVCacheFp8``, ``plan`` and ``run`` take the place of ``step``, and ``capture_run`` of ``capture``.
     """
 
-    def __init__(self, cfg: DecoderConfig, layers: list[DecoderLayerWeights], cache: PagedKVCache):
+    def __init__(self, cfg: DecoderConfig, layers: list[DecoderLayerWeights],
+                 cache: PagedKVCache | PagedKVCacheFp8):
         self.cfg = cfg
         self.layers = layers
         self.cache = cache
@@ -174,7 +214,52 @@ class DecodeModel:
         self.inv_freq = default_inv_freq(cfg, dev)
         self._graph = None
 
+    def _need_cache(self, kind) -> None:
+        if not isinstance(self.cache, kind):
+            raise TypeError(f"this call needs a {kind.__name__}, the model has a {type(self.cache).__name__}")
+
+    def plan(self, cached_lens, new_lens, block_tables, free_pages, num_tokens: int, max_new_tokens: int,
+             out: kernels.PagedPlan | None = None) -> kernels.PagedPlan:
+        """The plan of a step over the 8-bit cache (``kernels.paged_plan`` with this model's heads)."""
+        return kernels.paged_plan(cached_lens, new_lens, block_tables, free_pages, num_tokens, max_new_tokens,
+                                  self.cfg.heads, self.cfg.kv_heads, out=out)
+
+    def run(self, h, plan: kernels.PagedPlan):
+        """Every layer on the hidden states [T, hidden] of a plan's rows, over the 8-bit cache; returns theirs after
+        the last layer (padding rows: of no use)."""
+        self._need_cache(PagedKVCacheFp8)
+        for i, w in enumerate(self.layers):
+            h = moe_sublayer(w, h, attention_sublayer_fp8(w, h, plan, self.inv_freq, *self.cache.layer(i)))
+        return h
+
+    def capture_run(self, h, cached_lens, new_lens, block_tables, free_pages, max_new_tokens: int):
+        """Records a step's plan and ``run`` on copies of the given inputs; returns (graph, static inputs, static
+        output, plan).  ``block_tables`` is among the static inputs: a replay enters the new pages there."""
+        self._need_cache(PagedKVCacheFp8)
+        dev = h.device
+        statics = [t.clone() for t in (h, cached_lens, new_lens, block_tables, free_pages)]
+        lens = statics[2]
+        real = lens.clone()
+
+        def step():
+            plan = self.plan(*statics[1:], h.shape[0], max_new_tokens)
+            return self.run(statics[0], plan), plan
+
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):  # warm the allocator and the library, on no tokens: the cache stays as it is
+            lens.zero_()
+            step()
+            lens.copy_(real)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        torch.cuda.synchronize(dev)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, plan = step()
+        return graph, statics, out, plan
+
     def step(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True):
+        self._need_cache(PagedKVCache)
         for i, w in enumerate(self.layers):
             o = None
             if attention:
