@@ -2,14 +2,14 @@
 // single tokens (paged_plan.h): for token t of a sequence at position p, query head h and kv head h / G,
 //   o = sum_{j <= p} softmax_j(scale q . K_j) V_j
 // with K and V the values that the codes stand for, everything in fp32 but for two operands: the bf16 q, and
-// the probabilities exp(s - max), rounded to bf16 (half a step, 2^-9) for the second MFMA; their sum is
-// formed from the unrounded ones.  The codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8 with the
+// the probabilities, rounded to bf16 (by 2^-8 at most) for the second MFMA; the tiles sum them as rounded, so that
+// a row that one key dominates is exact, the short items before it.  The codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8 with the
 // page's power-of-two scale), so both products run on the bf16 MFMAs without a further error.
 //
 // Two kernels, by the rows (tokens x heads of the group) that a sequence has for one kv head:
 //   short: up to 16 rows (a decoding sequence), bound by the cache's bytes.  One workgroup per (sequence, kv
 //     head, run of pages); its 4 waves take pairs of pages round robin, straight from HBM to the MFMA.
-//   tile: more rows (prompts), bound by the MFMA and the softmax.  One workgroup per (128 rows, kv
+//   tile: more rows (prompts), bound by the MFMA and the softmax.  One workgroup per (128 or 256 rows, kv
 //     head); pages are widened to bf16 once per workgroup, in LDS.
 // Rows whose keys are split over several workgroups leave fp32 partial results that the merge kernel joins in key
 // order, so results do not depend on timing.
@@ -296,14 +296,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
 }
 
 // ---------------------------------------------------------------------------
-// tile: 128 rows, 32 a wave, 64 keys (4 pages) a step.  S^T [32 keys x 32 rows] = K Q^T (8 MFMAs 32x32x16
+// tile: 32 rows a wave, 4 or 8 waves, 64 keys (4 pages) a step.  S^T [32 keys x 32 rows] = K Q^T (8 MFMAs 32x32x16
 // per 32 keys), O^T [128 x 32 rows] += V^T [128 x 16 keys] P^T (4 MFMAs a page).  Lane l has row l & 31 and,
 // of a page's keys, 4 (l >> 5) + {0..3, 8..11}: again the 8 that the second MFMA wants from it.
 // In LDS, bf16: K [dim / 8][key 64][8 dims] and V [page][quad & 1][dim slot][8 keys], quads q and q + 2 together;
 // the slot 64 j + 16 d + x of dim 64 j + 4 x + d makes the writes contiguous.  Every read and write of 16
 // bytes is contiguous over the lanes that the LDS serves together.
 // ---------------------------------------------------------------------------
-constexpr int kStepPages = kTileKeys / kPage;
 
 // Schedules a step's half so far as 16 MFMAs with four vector instructions behind each, the LDS reads two MFMAs
 // ahead of their use.  (8192 tokens, 64 / 4 heads: the compiler's own order 1120 us, one read ahead 1100, two 1067,
@@ -318,7 +317,14 @@ constexpr int kStepPages = kTileKeys / kPage;
     }                                                                          \
   } while (0)
 
-__global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
+  constexpr int kTileRows = 32 * kWaves;
+  // Steps whose K and V are in LDS.  Two: a barrier after each step, and room for two workgroups in a CU.  Four, where
+  // the registers leave room for one only: a barrier after two steps.
+  constexpr int kRing = kWaves == 4 ? 2 : 4;
+  constexpr int kAheadK = kRing == 4 ? 3 : 2, kAheadV = kAheadK - 1;  // steps from storing to use
+  constexpr int kLoads = 8 / kWaves;  // 16-byte pieces of a step's K, and 8-byte ones of a quad of V, for each thread
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -334,8 +340,8 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
   const int parts = __builtin_amdgcn_readfirstlane(i1.z);
 
-  __shared__ __attribute__((aligned(16))) uint4 s_k[2][kHD / 8][kTileKeys];
-  __shared__ __attribute__((aligned(16))) uint4 s_v[2][kStepPages][2][kHD];
+  __shared__ __attribute__((aligned(16))) uint4 s_k[kRing][kHD / 8][kTileKeys];
+  __shared__ __attribute__((aligned(16))) uint4 s_v[kRing][kTilePages][2][kHD];
 
   const int r = 32 * wave + lr;
   const bool live = r < ntok * G;
@@ -374,44 +380,56 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));
   };
-  // This thread's codes of a step: K, 16 bytes (16 dims of a token) of pages wave / 2 and 2 + wave / 2; V, of page
-  // `wave` the quads vq and vq + 2 of 4 dims.  K runs a step ahead of V.
-  uint4 kr[2], vr[2];
-  float ks[2], vs = 1.f, vs_next = 1.f;
+  // This thread's codes of a step.  K: 16 bytes (16 dims of a token) of kLoads pages.  V: of one page the quads vq
+  // and vq + 2 of 2 kLoads dims.  K runs a step ahead of V.
+  uint4 kr[kLoads];
+  uint32_t vr[2][2 * kLoads];
+  float ks[kLoads], vs = 1.f, vs_next = 1.f;
   int v_page = -1;      // of the step that K was last loaded for
   uint32_t held = 0;    // which of that step's pages there are
-  const int vj = lane >> 5, vq = (lane >> 4) & 1, vx = lane & 15;
+  const int k_page = wave >> 1, k_part = wave & 1;  // the first of the K pages (2 apart), the half of a block
+  const int v_at = wave * kTilePages / kWaves;      // the V page
+  // four waves: a lane has dims 64 vj + 4 vx .. +4; eight: of those two, 2 vd .. +2
+  const int vj = kWaves == 4 ? lane >> 5 : wave & 1, vd = kWaves == 4 ? 0 : lane >> 5, vq = (lane >> 4) & 1, vx = lane & 15;
   auto load_k = [&](int step) __attribute__((always_inline)) {
-    const int l = (step & 15) * kStepPages;
+    const int l = (step & 15) * kTilePages;
     if (l == 0) {
       my_page = next_page;
       my_ks = next_ks;
       my_vs = next_vs;
     }
-    if ((step & 15) == 13) fetch_ids(page0 + (step + 3) * kStepPages);
+    if ((step & 15) == 13) fetch_ids(page0 + (step + 3) * kTilePages);
     if ((step & 15) == 14) fetch_scales();
     held = (uint32_t)(__ballot(my_page >= 0) >> l) & 15u;
-    v_page = __builtin_amdgcn_readlane(my_page, l + wave);
-    vs_next = lane_f(my_vs, l + wave);
+    v_page = __builtin_amdgcn_readlane(my_page, l + v_at);
+    vs_next = lane_f(my_vs, l + v_at);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = l + 2 * h + (wave >> 1);
+    for (int h = 0; h < kLoads; ++h) {
+      const int at = l + 2 * h + k_page;
       ks[h] = lane_f(my_ks, at);
-      kr[h] = block_load<0>(block_rsrc(a.k_cache, __builtin_amdgcn_readlane(my_page, at), Hkv, g),
-                            (wave & 1) * 1024 + lane * 16);
+      kr[h] = block_load<0>(block_rsrc(a.k_cache, __builtin_amdgcn_readlane(my_page, at), Hkv, g), k_part * 1024 + lane * 16);
     }
   };
   auto load_v = [&]() __attribute__((always_inline)) {  // of the step that K was last loaded for
     const __amdgpu_buffer_rsrc_t rv = block_rsrc(a.v_cache, v_page, Hkv, g);
     vs = vs_next;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) vr[h] = block_load<0>(rv, vj * 1024 + (vq + 2 * h) * 256 + vx * 16);
+    for (int h = 0; h < 2; ++h) {
+      const int at = vj * 1024 + (vq + 2 * h) * 256 + vx * 16 + vd * 8;
+      if constexpr (kWaves == 4) {
+        const uint4 x = block_load<0>(rv, at);
+        vr[h][0] = x.x, vr[h][1] = x.y, vr[h][2] = x.z, vr[h][3] = x.w;
+      } else {
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, at, 0, 0));
+        vr[h][0] = x.x, vr[h][1] = x.y;
+      }
+    }
   };
   auto store_k = [&](int buf) __attribute__((always_inline)) {
-    const int c = 4 * (wave & 1) + (lane >> 4);  // dims 16 c .. +16 of token lane & 15
+    const int c = 4 * k_part + (lane >> 4);  // dims 16 c .. +16 of token lane & 15
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = (2 * h + (wave >> 1)) * kPage + (lane & 15);
+    for (int h = 0; h < kLoads; ++h) {
+      const int key = (2 * h + k_page) * kPage + (lane & 15);
       s_k[buf][2 * c][key] = __builtin_bit_cast(uint4, widen8(kr[h].x, kr[h].y, ks[h]));
       s_k[buf][2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
     }
@@ -419,18 +437,15 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   auto mask_v = [&](int page) __attribute__((always_inline)) {  // codes behind the last key may be anything, a NaN too
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t mask = quad_mask(pos + ntok - ((page + wave) * kPage + 4 * (vq + 2 * h)));
-      vr[h].x &= mask;
-      vr[h].y &= mask;
-      vr[h].z &= mask;
-      vr[h].w &= mask;
+      const uint32_t mask = quad_mask(pos + ntok - ((page + v_at) * kPage + 4 * (vq + 2 * h)));
+#pragma unroll
+      for (int d = 0; d < 2 * kLoads; ++d) vr[h][d] &= mask;
     }
   };
   auto store_v = [&](int buf) __attribute__((always_inline)) {
-    const uint32_t v0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, v1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-      s_v[buf][wave][vq][64 * vj + 16 * d + vx] = __builtin_bit_cast(uint4, widen8(v0[d], v1[d], vs));
+    for (int d = 0; d < 2 * kLoads; ++d)
+      s_v[buf][v_at][vq][64 * vj + 16 * (2 * vd + d) + vx] = __builtin_bit_cast(uint4, widen8(vr[0][d], vr[1][d], vs));
   };
   auto scores = [&](v16f (&s)[2], int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -483,15 +498,17 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
   };
 
   // Step n's scores are formed in the course of step n - 1, beside its softmax, so that the wave has MFMAs and vector
-  // work at the same time: K of step n + 2 and V of step n + 1 go into LDS during step n.
-  const int steps = (page1 - page0 + kStepPages - 1) / kStepPages;
+  // work at the same time: K of step n + kAheadK and V of step n + kAheadV go into LDS during step n.
+  const int steps = (page1 - page0 + kTilePages - 1) / kTilePages;
   v16f s0[2], s1[2];
   float pm;
+  uint32_t queue = 0;  // the held pages of the steps from n + 1 to that which K was last loaded for, 4 bits each
   auto step = [&](v16f (&s)[2], v16f (&next)[2], int n, int buf) __attribute__((always_inline)) {
-    const int next_page0 = page0 + (n + 1) * kStepPages, next_key = next_page0 * kPage;
-    const uint32_t held_next = held;
-    load_v();  // step n + 1
-    load_k(n + 2);
+    const int next_key = (page0 + (n + 1) * kTilePages) * kPage;
+    const uint32_t held_next = queue & 15;
+    load_v();  // step n + kAheadV
+    load_k(n + kAheadK);
+    queue = (queue >> 4) | (held << (4 * (kAheadK - 2)));
     // A row's reference need not be its maximum: only where a score passes it by more than 2^kSlack are the sums
     // scaled down (exp stays below 2^kSlack, and bf16 and fp32 are as exact there as below 1)
     pm = half_max(pm) * a.scale;
@@ -507,39 +524,52 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
     }
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
     v8bf pa[2], pb[2];
-    scores(next, buf ^ 1);
+    scores(next, (buf + 1) % kRing);
     probabilities(s[0], pa, m_use);
     MIX_MFMAS();
     asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(l_run));  // not to be put off past the branches
     if (next_key + kTileKeys > all_end || held_next != 15) mask_scores(next, next_key, held_next);
-    if (next_key + kTileKeys > pos + ntok) mask_v(next_page0);
+    const int v_page0 = page0 + (n + kAheadV) * kTilePages;
+    if ((v_page0 + kTilePages) * kPage > pos + ntok) mask_v(v_page0);
     output(pa, buf, 0);
     probabilities(s[1], pb, m_use);
     output(pb, buf, 1);
     pm = score_max(next);
-    store_v(buf ^ 1);
-    store_k(buf);
+    store_v((buf + kAheadV) % kRing);
+    store_k((buf + kAheadK) % kRing);
     MIX_MFMAS();
-    __syncthreads();
+    if (kRing == 2 || buf % 2 == 1) __syncthreads();
   };
   fetch_ids(page0);
   fetch_scales();
-  load_k(0);
-  store_k(0);
-  load_v();
-  const uint32_t held0 = held;
-  if ((page0 + kStepPages) * kPage > pos + ntok) mask_v(page0);
-  store_v(0);
-  load_k(1);
-  store_k(1);
+  uint32_t held0 = 0;
+#pragma unroll
+  for (int n = 0; n < kAheadK; ++n) {
+    load_k(n);
+    store_k(n);
+    if (n == 0) held0 = held;
+    if (n > 0) queue |= held << (4 * (n - 1));
+    if (n < kAheadV) {
+      load_v();
+      const int v_page0 = page0 + n * kTilePages;
+      if ((v_page0 + kTilePages) * kPage > pos + ntok) mask_v(v_page0);
+      store_v(n);
+    }
+  }
   __syncthreads();
   scores(s0, 0);
   if (page0 * kPage + kTileKeys > all_end || held0 != 15) mask_scores(s0, page0 * kPage, held0);
   pm = score_max(s0);
-  for (int n = 0; n < steps; n += 2) {
+  for (int n = 0; n < steps; n += kRing) {
     step(s0, s1, n, 0);
-    if (n + 1 == steps) break;
+    if (n + 1 >= steps) break;
     step(s1, s0, n + 1, 1);
+    if constexpr (kRing == 4) {
+      if (n + 2 >= steps) break;
+      step(s0, s1, n + 2, 2);
+      if (n + 3 >= steps) break;
+      step(s1, s0, n + 3, 3);
+    }
   }
   const float m_run = m_ref;
   l_run = half_sum(l_run);
@@ -579,13 +609,13 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   __shared__ float s_m[8], s_l[8];
   __shared__ __attribute__((aligned(16))) v4f s_o[8][32];
-  constexpr int kChunks = kTileRows / kShortRows;  // of a tile's rows
-  const int shorts = a.plan[PH_SHORT_MERGES], chunks = shorts + a.plan[PH_TILE_MERGES] * kChunks;
+  const int tile_chunks = p.tile_rows / kShortRows;  // of a tile's rows
+  const int shorts = a.plan[PH_SHORT_MERGES], chunks = shorts + a.plan[PH_TILE_MERGES] * tile_chunks;
   for (int x = blockIdx.x; x < chunks * p.Hkv; x += gridDim.x) {  // workgroup-uniform
     const int chunk = x / p.Hkv, g = x % p.Hkv;
     const bool tile = chunk >= shorts;
-    const int r0 = blockIdx.y + (tile ? (chunk - shorts) % kChunks * kShortRows : 0);
-    const int4 e = *(const int4*)(a.plan + (tile ? p.tile_merges + 4L * ((chunk - shorts) / kChunks) : p.short_merges + 4L * chunk));
+    const int r0 = blockIdx.y + (tile ? (chunk - shorts) % tile_chunks * kShortRows : 0);
+    const int4 e = *(const int4*)(a.plan + (tile ? p.tile_merges + 4L * ((chunk - shorts) / tile_chunks) : p.short_merges + 4L * chunk));
     const int ns = e.x;
     const bool few = ns <= kMergeFew;
     if (r0 >= e.w * p.G || (few && r0 % 8 != 0)) continue;
@@ -602,7 +632,7 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int s = min(s0 + by * u, ns - 1);
-        const long base = ((long)(e.y + s) * p.Hkv + g) * (tile ? kTileRows : kShortRows) + (live ? r : r0);
+        const long base = ((long)(e.y + s) * p.Hkv + g) * (tile ? p.tile_rows : kShortRows) + (live ? r : r0);
         x[u] = *(const float2*)(ml + 2 * base);
         v[u] = *(const v4f*)(part + base * kHD + 4 * lane);
       }
@@ -654,7 +684,7 @@ struct Parts {
 };
 Parts attn_parts(const PlanLayout& p) {
   return {p.short_whole ? 0 : (long)p.S * p.Hkv * kShortRows,
-          (long)p.max_pages * kPage > kTileMinKeys ? (long)p.split_tiles * p.Hkv * kTileRows : 0};
+          (long)p.max_pages * kPage >= 2 * kTileMinKeys ? (long)p.split_tiles * p.Hkv * p.tile_rows : 0};
 }
 
 void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
@@ -708,7 +738,11 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   attn_carve(c, parts, &a);
   hipStream_t s = (hipStream_t)stream;
   if (p.N > 0) {
-    hipLaunchKernelGGL(attn_fp8_tile_kernel, dim3((unsigned)(p.N * p.Hkv)), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)(p.N * p.Hkv));
+    if (p.tile_rows == kTileRowsMany)
+      hipLaunchKernelGGL(attn_fp8_tile_kernel<8>, grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL(attn_fp8_tile_kernel<4>, grid, dim3(256), 0, s, a);
     MOE_CHECK_LAUNCH();
   }
   const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));

@@ -8,7 +8,7 @@
 //   slot    [T]          16 * page + slot of each token (-1: none)
 //   writes  [W][4]       pages that get tokens: {page or -1, first token, its slot, tokens}
 //   shorts  [S][8]       attention items of sequences with few query rows (PI_*)
-//   tiles   [N][8]       attention items of the others: kTileRows query rows (PI_*)
+//   tiles   [N][8]       attention items of the others: 128 or 256 query rows (PI_*)
 //   short_merges [..][4] sequences, resp. tiles, whose keys are split over items: {items, first item, first
 //   tile_merges  [..][4] token, tokens}
 #pragma once
@@ -21,7 +21,9 @@ constexpr int kPlanMaxTokens = 1 << 18;
 constexpr int kPlanMaxPages = 1 << 22;  // per sequence
 
 constexpr int kShortRows = 16;       // query rows (tokens x heads of the group) of a short item
-constexpr int kTileRows = 128;       // and of a tile
+constexpr int kTileRows = 128;       // and of a tile, or, where rows fill so many of them,
+constexpr int kTileRowsMany = 256;   // of these: the cache is widened and staged half as often (a prompt of 4096
+constexpr int kManyTiles = 512;      // tokens, 32 / 4 heads: 154 -> 139 us; at 2500, half as many: 73 -> 120)
 constexpr int kShortStep = 8;        // pages that a short item's workgroup takes at once
 // Items that short sequences are split into, over all kv heads: the 1024 workgroups that the GPU
 // holds at once.
@@ -29,10 +31,14 @@ constexpr int kShortTarget = 1024;
 // Tables of up to so many pages: a short sequence is one item and there is nothing to join, which saves the merge's
 // launch (3.5 us and a gap, of 13 us for one sequence of 1000 tokens).
 constexpr int kShortWhole = 128;
-// Workgroups that tiles are split for when there are fewer: two per CU, each with kTileMinKeys at least.
+// Fewer tiles than this, one per CU, are split along their keys, for twice as many workgroups in all and
+// kTileMinKeys at least.  (8000 cached tokens and n new ones, 32 / 4 heads, split against whole: n = 100 47 us / 61,
+// 200 79 / 86, 700 169 / 174; one more would not pay, n = 1024 228 / 180.)
+constexpr int kTileFew = 256;
 constexpr int kTileTarget = 512;
 constexpr int kTileMinKeys = 512;
-constexpr int kTileKeys = 64;        // keys per step of a tile
+constexpr int kTileKeys = 64;        // keys and pages per step of a tile
+constexpr int kTilePages = kTileKeys / kPlanPage;
 
 enum { PH_TOKENS, PH_WRITES, PH_SHORTS, PH_TILES, PH_SHORT_MERGES, PH_TILE_MERGES, PH_PAGES = 15, PH_INTS };
 // page_begin .. page_end: the item's keys; parts: items that share the rows (1: none other)
@@ -40,7 +46,7 @@ enum { PI_SEQ, PI_TOK, PI_NTOK, PI_POS, PI_PAGE0, PI_PAGE1, PI_PARTS, PI_INTS = 
 
 struct PlanLayout {
   int B, T, max_new, max_pages, Hq, Hkv, G;
-  int tile_tok;               // tokens per tile
+  int tile_rows, tile_tok;    // rows and tokens of a tile
   int short_rows;             // query rows that a short item may have
   bool short_whole;           // short sequences are not split
   int W, S, N, SM, TM;        // list capacities
@@ -59,7 +65,8 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   p.B = s->seqs, p.T = s->tokens, p.max_pages = s->max_pages, p.Hq = s->heads, p.Hkv = s->kv_heads;
   p.max_new = s->max_new < p.T ? s->max_new : p.T;
   p.G = p.Hq / p.Hkv;
-  p.tile_tok = kTileRows / p.G;
+  p.tile_rows = (long)p.T * p.Hq / kTileRowsMany >= kManyTiles ? kTileRowsMany : kTileRows;
+  p.tile_tok = p.tile_rows / p.G;
   const long B = p.B, T = p.T;
   // a sequence with n new tokens touches at most (n + 30) / 16 pages, and at most n
   p.W = (int)(T < (T + 30 * B) / 16 ? T : (T + 30 * B) / 16);
@@ -72,11 +79,11 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   // no sequence is long enough for tiles: none
   const bool tiles = (long)p.max_new * p.G > kShortRows;
   const long nt = tiles ? T / p.tile_tok + seqs : 0;
-  const long target = (kTileTarget + p.Hkv - 1) / p.Hkv;
-  p.split_tiles = (int)(tiles ? (nt < target ? nt : target) + target : 0);
+  const long few = (kTileFew + p.Hkv - 1) / p.Hkv, whole = nt < few ? nt : few;
+  p.split_tiles = (int)(tiles ? whole + (kTileTarget + p.Hkv - 1) / p.Hkv : 0);
   p.N = (int)(nt > p.split_tiles ? nt : p.split_tiles);
   p.SM = (int)seqs;
-  p.TM = (int)(nt < target ? nt : target);
+  p.TM = (int)whole;
   p.cu = PH_INTS;
   p.ctx = p.cu + B + 1;
   p.pos = p.ctx + B;

@@ -238,16 +238,15 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     if (new_of(b) * p.G > kShortRows) first[0] += (new_of(b) + p.tile_tok - 1) / p.tile_tok;
   }
   __syncthreads();
-  // keys per item; with enough tiles to fill the GPU they are not split
+  // keys that an item has at least
   long chunk = ((long)s_sum * p.Hkv + kTileTarget - 1) / kTileTarget;
-  chunk = (max(chunk, (long)kTileMinKeys) + kTileKeys - 1) / kTileKeys * kTileKeys;
-  if ((long)tiles[0] * p.Hkv >= kTileTarget) chunk = 1L << 40;
+  chunk = (long)tiles[0] * p.Hkv < kTileFew ? max(chunk, (long)kTileMinKeys) : 1L << 40;
 
   // Those with the most keys first, over all sequences: the launch drains on short ones (447 against 462 us for
   // seven prompts of 1 to 1500 tokens in sequence order).  A counting sort by 256 classes of keys; within a class the
   // order is the atomics', on which no result depends.
   struct Tile {
-    int b, tok, count, pos, keys, ns, cls;
+    int b, tok, count, pos, pages, step, ns, cls;  // step: pages per item
   };
   auto tile = [&](int k) __attribute__((always_inline)) {
     Tile x;
@@ -256,9 +255,12 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     x.tok = row0 + i * p.tile_tok;
     x.count = min(p.tile_tok, n - i * p.tile_tok);
     x.pos = s_cached[x.b] + i * p.tile_tok;
-    x.keys = min(x.pos + x.count, room);
-    x.ns = (int)((x.keys + chunk - 1) / chunk);
-    x.cls = kClasses - 1 - (int)((long)x.keys * kClasses / (s_most + 1));
+    const int keys = min(x.pos + x.count, room);
+    x.pages = pages_of(keys);
+    const int ns = max(1, (int)(keys / chunk));
+    x.step = (x.pages + kTilePages * ns - 1) / (kTilePages * ns) * kTilePages;
+    x.ns = (x.pages + x.step - 1) / x.step;
+    x.cls = kClasses - 1 - (int)((long)keys * kClasses / (s_most + 1));
     return x;
   };
   for (int k = tid; k < tiles[0]; k += kThreads) {
@@ -274,11 +276,10 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     const Tile x = tile(k);
     const int item = atomicAdd(&s_class[x.cls], x.ns);
     if (x.ns > 1) *(int4*)(plan + p.tile_merges + 4L * atomicAdd(&s_merged, 1)) = make_int4(x.ns, item, x.tok, x.count);
-    const int pages = pages_of(x.keys), step = x.ns > 1 ? (int)(chunk / kPlanPage) : pages;
     for (int s = 0; s < x.ns; ++s) {
       int4* dst = (int4*)(plan + p.tiles + (long)PI_INTS * (item + s));
       dst[0] = make_int4(x.b, x.tok, x.count, x.pos);
-      dst[1] = make_int4(s * step, min((s + 1) * step, pages), x.ns, 0);
+      dst[1] = make_int4(s * x.step, min((s + 1) * x.step, x.pages), x.ns, 0);
     }
   }
   __syncthreads();

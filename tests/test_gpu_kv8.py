@@ -2,9 +2,11 @@
 
 Tolerances, from the roundings alone.  A bf16 value is off by half a step, 2^-8 of it; an e4m3 code by 2^-4 of its
 value or, among the subnormals, 2^-10 scales.
-  attention: each probability is rounded to bf16 for the product with V and the result once more, so
-    |o - ref| <= 2^-8 (sum p |v| + |ref|); 5% more, 2e-4 of sum p |v|, covers the fp32 scores: 128 products and their
-    sum, each step off by 2^-24 of sum |q k|, with scale sum |q k| below 100 here, move exp by 100 * 2^-24 * 2 * 8 at most.
+  attention: with p the probabilities, each rounded to bf16 for the product with V, p' = p (1 + d), |d| <= 2^-8, and
+    the tiles' sum formed from the rounded ones, o' = sum p' v / sum p' differs from o = sum p v (sum p = 1) by
+    |sum p d (v - o)| / |sum p'| <= 2^-8 (sum p |v| + |o|) (1 + 2^-8); rounding the result adds 2^-8 |o|.  5% more
+    covers the (1 + 2^-8) and the fp32 scores: 128 products summed in fp32 are off by 128 * 2^-24 of their sum of
+    |q k| at most, with scale sum |q k| below 25 here 2e-4 of each p, which is 5% of 2^-8.
   norm and rotary: r, the weight, the angle (rounded to 2^-25 of a turn: 2^-22 radians), cos, sin and the two
     products in fp32 are each off by a few 2^-24: 2^-19 of |a| + |b| in all, beside the one rounding."""
 
@@ -101,7 +103,7 @@ class Step:
         ref, size = self.attention_ref(q)
         got = o.float().cpu().numpy()
         assert np.isfinite(got).all()
-        worst = np.abs(got - ref) - 2.0 ** -8 * (1.05 * size + np.abs(ref))
+        worst = np.abs(got - ref) - 2.0 ** -8 * (1.05 * (size + np.abs(ref)) + np.abs(ref))
         assert (worst <= 1e-30).all(), (worst.max(), np.argwhere(worst > 0)[:4])
 
 
