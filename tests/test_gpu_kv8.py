@@ -433,3 +433,96 @@ def test_refusals(pkg, dev):
     with pytest.raises(ValueError):
         pkg.qk_norm_rope_append_fp8(torch.zeros((3, 40 * D), dtype=torch.bfloat16, device=dev), x[0, 0], x[0, 0],
                                     torch.zeros(64, device=dev), 16, 4, 1e-6, k, v, ks, vs, p)
+
+
+def test_plan_at_its_limits(pkg, dev):
+    """2^18 rows: one prompt of them all, and 4096 sequences of 64."""
+    s = Step(pkg, dev, [5], [1 << 18], 16, 1, seed=20)
+    s.check_plan(s.plan())
+    s = Step(pkg, dev, [3] * 4096, [64] * 4096, 16, 1, seed=21)
+    s.check_plan(s.plan())
+
+
+def test_blocks_past_32_bits(pkg, dev):
+    """Pools of over 2^32 bytes: pages at both ends, written and read."""
+    Hkv, pages = 4, (1 << 32) // (4 * 2048) + 40
+    s = Step(pkg, dev, [40, 0, 700], [1, 70, 1], 32, Hkv, seed=22)
+    used = s.ref[4][s.ref[4] >= 0]
+    high = {int(p): (pages - 1 - i if i % 2 else i) for i, p in enumerate(sorted(set(used.tolist()) | set(s.free.tolist())))}
+    big = [torch.zeros((pages, Hkv, *shape), dtype=torch.uint8, device=dev) for shape in (K_SHAPE, V_SHAPE)]
+    scales = [torch.ones((pages, Hkv), device=dev) for _ in range(2)]
+    for p, q in high.items():
+        for dst, src in zip((*big, *scales), (s.k, s.v, s.ks, s.vs)):
+            dst[q] = torch.from_numpy(src[p]).to(dev) if src.ndim > 2 else torch.from_numpy(src[p]).to(dev)
+    move = lambda a: np.array([high.get(int(x), -1) for x in a.flat], np.int32).reshape(a.shape)  # noqa: E731
+    s.g_tables, s.g_free = i32(move(s.tables), dev), i32(move(s.free), dev)
+    p = s.plan()
+    cache = (big[0].view(FP8), big[1].view(FP8), *scales)
+    k, v = new_kv(s)
+    pkg.kv_append_fp8(to_bf16(k, dev), to_bf16(v, dev), *cache, p)
+    q = orc.round_bf16(s.rng.standard_normal((s.T, 32, D)).astype(np.float32))
+    o = pkg.paged_attention_fp8(to_bf16(q, dev), *cache, p, SCALE)
+    # the same step on the small pools
+    small = Step(pkg, dev, [40, 0, 700], [1, 70, 1], 32, Hkv, seed=22)
+    ps = small.plan()
+    pkg.kv_append_fp8(to_bf16(k, dev), to_bf16(v, dev), *small.cache, ps)
+    assert torch.equal(o, pkg.paged_attention_fp8(to_bf16(q, dev), *small.cache, ps, SCALE))
+    small.check_output(o, q)
+
+
+def test_calls_on_two_streams_share_nothing(pkg, dev):
+    """Two attentions of one plan at once, each split over many workgroups, on streams of their own."""
+    s = Step(pkg, dev, [9000, 8000], [1, 1], 32, 4, seed=23)
+    p = s.plan()
+    qs = [to_bf16(s.rng.standard_normal((2, 32, D)).astype(np.float32), dev) for _ in range(2)]
+    want = [pkg.paged_attention_fp8(q, *s.cache, p, SCALE) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for st, q in zip(streams, qs):
+            with torch.cuda.stream(st):
+                got.append(pkg.paged_attention_fp8(q, *s.cache, p, SCALE))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(got))
+
+
+def test_two_graphs_share_nothing(pkg, dev):
+    """Attentions of two plans captured into two graphs of one pool, replayed in turn with eager work between."""
+    steps = [Step(pkg, dev, [6000, 300], [1, 40], 32, 4, seed=24), Step(pkg, dev, [100, 9000], [50, 1], 32, 4, seed=25)]
+    graphs, outs, want = [], [], []
+    for s in steps:
+        p = s.plan()
+        q = to_bf16(s.rng.standard_normal((s.T, 32, D)).astype(np.float32), dev)
+        want.append(pkg.paged_attention_fp8(q, *s.cache, p, SCALE))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pkg.paged_attention_fp8(q, *s.cache, p, SCALE))
+        graphs.append((g, p, q))
+    for _ in range(3):
+        for (g, _, _), o, w in zip(graphs, outs, want):
+            o.zero_()
+            g.replay()
+            torch.randn((512, 512), device=dev).sum()
+            torch.cuda.synchronize()
+            assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(2100, 64, 4), (9000, 16, 1)])
+def test_attention_large_tiles(pkg, dev, T, Hq, Hkv):
+    """Enough rows for the tiles of 256 of them: every row against a few, computed apart, in 64 bits."""
+    s = Step(pkg, dev, [0, 77, 1000], [T - 301, 300, 1], Hq, Hkv, seed=26)
+    p = s.plan()
+    q = orc.round_bf16(s.rng.standard_normal((T, Hq, D)).astype(np.float32))
+    o = pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, p, SCALE).float().cpu().numpy()
+    assert np.isfinite(o).all()
+    k, v, ks, vs = s.got()
+    k, v = kv.unpack(k, ks, kv.k_index), kv.unpack(v, vs, kv.v_index)
+    cu, pos = s.ref[2], s.ref[0]
+    some = sorted({0, 1, 15, 16, 17, 63, 64, T - 302, T - 301, T - 2, T - 1, *s.rng.integers(0, T, 25).tolist()})
+    for t in some:
+        b = int(np.searchsorted(cu, t, side="right")) - 1
+        ref, size = kv.attention(q[t:t + 1], k, v, [0, 1], pos[t:t + 1], s.ref[4][b:b + 1], SCALE)
+        worst = np.abs(o[t] - ref[0]) - 2.0 ** -8 * (1.05 * (size[0] + np.abs(ref[0])) + np.abs(ref[0]))
+        assert (worst <= 1e-30).all(), (t, worst.max())
