@@ -25,9 +25,10 @@ constexpr int kTileRows = 128;       // and of a tile, or, where rows fill so ma
 constexpr int kTileRowsMany = 256;   // of these: the cache is widened and staged half as often (a prompt of 4096
 constexpr int kManyTiles = 512;      // tokens, 32 / 4 heads: 154 -> 139 us; at 2500, half as many: 73 -> 120)
 constexpr int kShortStep = 8;        // pages that a short item's workgroup takes at once
-// Items that short sequences are split into, over all kv heads: the 1024 workgroups that the GPU
-// holds at once.
-constexpr int kShortTarget = 1024;
+// Items that short sequences are split into, over all kv heads: three for each CU.  (128 sequences of 512 to 8192
+// tokens, 32 / 4 heads, in us, for 512 / 768 / 1024 / 2048: 95.7 / 94.8 / 98.2 / 101.7; two of 100000 and more:
+// 45.8 / 47.6 / 49.4 / 58.0; 64 of up to 8192, 32 / 8 heads: 90.7 / 89.0 / 89.1 / 92.4.)
+constexpr int kShortTarget = 768;
 // Tables of up to so many pages: a short sequence is one item and there is nothing to join, which saves the merge's
 // launch (3.5 us and a gap, of 13 us for one sequence of 1000 tokens).
 constexpr int kShortWhole = 128;

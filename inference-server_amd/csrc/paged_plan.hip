@@ -177,17 +177,33 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       const int n = new_of(b);
       return n > 0 && n * p.G <= kShortRows ? (int)((pages_of(min(s_cached[b] + n, room)) + pps - 1) / pps) : 0;
     };
+    // Equal shares of a sequence's pages, each a multiple of what a workgroup takes at once; the sequences with the
+    // largest ones first (94.8 against 98.5 us for 128 sequences of 512 to 8192 tokens in their own order).
+    auto share = [&](int pages_b, int ns) __attribute__((always_inline)) {
+      return (pages_b + ns * kShortStep - 1) / (ns * kShortStep) * kShortStep;
+    };
+    auto class_of = [&](int b, int ns) __attribute__((always_inline)) {
+      return kClasses - 1 - (int)((long)share(pages_of(min(s_cached[b] + new_of(b), room)), ns) * kClasses / (pps + 1));
+    };
     int at[2] = {0, 0}, all[2];  // items, sequences that are split
+    s_class[tid] = 0;
+    __syncthreads();
     for (int b = b0; b < b1; ++b) {
       const int ns = splits(b);
       at[0] += ns;
       at[1] += ns > 1;
+      if (ns > 0) atomicAdd(&s_class[class_of(b, ns)], ns);
     }
     block_scan(at, all, s_wave);
+    int items[1] = {s_class[tid]}, all_items[1];
+    block_scan(items, all_items, s_wave);
+    s_class[tid] = items[0];
+    __syncthreads();
     for (int b = b0; b < b1; ++b) {
       const int ns = splits(b);
       s_a[b] = at[0];
-      if (ns > 1) *(int4*)(plan + p.short_merges + 4L * at[1]) = make_int4(ns, at[0], s_cu[b], new_of(b));
+      s_b[b] = ns > 0 ? atomicAdd(&s_class[class_of(b, ns)], ns) : 0;
+      if (ns > 1) *(int4*)(plan + p.short_merges + 4L * at[1]) = make_int4(ns, s_b[b], s_cu[b], new_of(b));
       at[0] += ns;
       at[1] += ns > 1;
     }
@@ -202,12 +218,10 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       const int b = last_le(s_a, p.B, k);
       const int row0 = s_cu[b], n = s_cu[b + 1] - row0;
       const int pages_b = pages_of(min(s_cached[b] + n, room)), ns = s_a[b + 1] - s_a[b];
-      // equal shares, each a multiple of what a workgroup takes at once
-      const int share = (pages_b + ns * kShortStep - 1) / (ns * kShortStep) * kShortStep;
-      const int page0 = (k - s_a[b]) * share;
-      int4* dst = (int4*)(plan + p.shorts + (long)PI_INTS * k);
+      const int step = share(pages_b, ns), i = k - s_a[b], page0 = i * step;
+      int4* dst = (int4*)(plan + p.shorts + (long)PI_INTS * (s_b[b] + i));
       dst[0] = make_int4(b, row0, n, s_cached[b]);
-      dst[1] = make_int4(page0, min(page0 + share, pages_b), ns, 0);
+      dst[1] = make_int4(page0, min(page0 + step, pages_b), ns, 0);
     }
     return;
   }
