@@ -114,9 +114,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
     return;
   }
   const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
-  if (item >= a.plan[PH_SHORTS]) return;
   const int4* it = (const int4*)(a.plan + p.shorts + (long)PI_INTS * item);
-  const int4 i0 = it[0], i1 = it[1];
+  const int count = a.plan[PH_SHORTS];
+  int4 i0 = it[0], i1 = it[1];
+  asm volatile("" : "+v"(i0.x), "+v"(i1.x));  // one round trip: the item, in the list or behind its end, with the count
+  if (item >= count) return;
   const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
   const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
   const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
@@ -332,9 +334,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
   const int Hkv = p.Hkv, G = p.G;
   // neighbours in the launch go to different XCDs (8), so with 2, 4 or 8 kv heads an XCD's L2 holds few heads
   const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
-  if (item >= a.plan[PH_TILES]) return;
   const int4* it = (const int4*)(a.plan + p.tiles + (long)PI_INTS * item);
-  const int4 i0 = it[0], i1 = it[1];
+  const int count = a.plan[PH_TILES];
+  int4 i0 = it[0], i1 = it[1];
+  asm volatile("" : "+v"(i0.x), "+v"(i1.x));
+  if (item >= count) return;
   const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
   const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
   const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
@@ -746,9 +750,11 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
     MOE_CHECK_LAUNCH();
   }
   const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));
-  // whole sequences of up to 128 pages, and no more of them than CUs: 16 waves each, four pairs of pages a wave
+  // Whole sequences, and no more of them than CUs: 8 waves each, of up to eight pairs of pages.  (One sequence of 1000
+  // tokens, in a graph: 4 waves 9.1 us, 8 waves 7.5, 16 waves 8.3; two to four pairs in flight per wave 7.9 to 8.6,
+  // for the code that has to be fetched.)
   if (p.short_whole && p.S * p.Hkv <= kFewItems)
-    hipLaunchKernelGGL(attn_fp8_short_kernel<16>, grid, dim3(1024), 0, s, a);
+    hipLaunchKernelGGL(attn_fp8_short_kernel<8>, grid, dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL(attn_fp8_short_kernel<4>, grid, dim3(256), 0, s, a);
   MOE_CHECK_LAUNCH();

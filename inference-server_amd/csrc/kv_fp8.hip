@@ -29,7 +29,7 @@ struct KvArgs {
   float *k_scale, *v_scale;  // [num_pages][Hkv]
   const int32_t* plan;
   const int4* writes;
-  int Hkv, num_pages;
+  int Hkv, num_pages, max_writes;
   // fused form
   const uint16_t *q, *qw, *kw;  // q rows, q_stride values apart
   long q_stride;
@@ -262,8 +262,12 @@ __global__ __launch_bounds__(256) void kv_append_fp8_kernel(KvArgs a) {
   }
   const int item = (int)blockIdx.x * 4 + wave;
   const int part = item % (2 * a.Hkv), i = item / (2 * a.Hkv);
-  if (i >= a.plan[PH_WRITES]) return;
-  const int4 w = a.writes[i];
+  const int count = a.plan[PH_WRITES];
+  int4 w = a.writes[min(i, a.max_writes - 1)];
+  asm volatile("" : "+v"(w.x));  // one round trip: the record, in the list or behind its end, with the count
+  if (i >= count) return;
+  w = make_int4(__builtin_amdgcn_readfirstlane(w.x), __builtin_amdgcn_readfirstlane(w.y), __builtin_amdgcn_readfirstlane(w.z),
+                __builtin_amdgcn_readfirstlane(w.w));
   if (w.x < 0 || w.x >= a.num_pages) return;  // no page: the tokens are not kept
   if (part < a.Hkv)
     write_k<FUSED>(a, w, part, lane);
@@ -284,7 +288,7 @@ KvArgs kv_args(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int
   a.plan = (const int32_t*)plan;
   a.writes = (const int4*)(a.plan + p.writes);
   a.pos = a.plan + p.pos;
-  a.Hkv = p.Hkv, a.num_pages = num_pages, a.T = p.T, a.Hq = p.Hq;
+  a.Hkv = p.Hkv, a.num_pages = num_pages, a.max_writes = p.W, a.T = p.T, a.Hq = p.Hq;
   return a;
 }
 
@@ -305,6 +309,7 @@ extern "C" int moe_mi355x_kv_append_fp8(const void* k, const void* v, long long 
                     !moe_aligned16(v_cache) || !moe_aligned16(plan),
                 MOE_ERR_ALIGNMENT);
   MOE_RETURN_IF(!moe_grid_fits(write_blocks(p)), MOE_ERR_INVALID_ARG);
+  if (p.W == 0) return MOE_OK;
   KvArgs a = kv_args(k_cache, v_cache, k_scale, v_scale, num_pages, p, plan);
   a.k = (const uint16_t*)k, a.v = (const uint16_t*)v, a.k_stride = k_stride, a.v_stride = v_stride;
   hipLaunchKernelGGL(kv_append_fp8_kernel<false>, dim3((unsigned)write_blocks(p)), dim3(256), 0, (hipStream_t)stream, a);

@@ -29,9 +29,13 @@ constexpr int kShortStep = 8;        // pages that a short item's workgroup take
 // tokens, 32 / 4 heads, in us, for 512 / 768 / 1024 / 2048: 95.7 / 94.8 / 98.2 / 101.7; two of 100000 and more:
 // 45.8 / 47.6 / 49.4 / 58.0; 64 of up to 8192, 32 / 8 heads: 90.7 / 89.0 / 89.1 / 92.4.)
 constexpr int kShortTarget = 768;
-// Tables of up to so many pages: a short sequence is one item and there is nothing to join, which saves the merge's
-// launch (3.5 us and a gap, of 13 us for one sequence of 1000 tokens).
+// Tables of up to so many pages, for many (sequence, kv head) pairs and for few: a short sequence is one item and there
+// is nothing to join, which saves the merge's launch.  (us in a graph, whole against split: one sequence of 1000
+// tokens and 4 kv heads 7.5 / 7.4, of 1400 8.9 / 6.9; 16 of 700..1400 10.1 / 10.7, of 1000..2000 13.6 / 12.2; 100 of
+// 500..2000 27.0 / 29.9.  Without a graph a launch is 2.7 us of the host's time besides.)
 constexpr int kShortWhole = 128;
+constexpr int kShortWholeFew = 80;
+constexpr int kFewPairs = 64;
 // Fewer tiles than this, one per CU, are split along their keys, for twice as many workgroups in all and
 // kTileMinKeys at least.  (8000 cached tokens and n new ones, 32 / 4 heads, split against whole: n = 100 47 us / 61,
 // 200 79 / 86, 700 169 / 174; one more would not pay, n = 1024 228 / 180.)
@@ -74,7 +78,7 @@ static inline PlanLayout plan_layout(const moe_mi355x_plan_shape* s) {
   const long seqs = B < T ? B : T;  // with new tokens
   const long per = (s->max_pages + kShortStep - 1) / kShortStep;
   p.short_rows = (long)p.max_new * p.G < kShortRows ? p.max_new * p.G : kShortRows;
-  p.short_whole = p.max_pages <= kShortWhole;
+  p.short_whole = p.max_pages <= (seqs * p.Hkv <= kFewPairs ? kShortWholeFew : kShortWhole);
   const long by_target = seqs + (kShortTarget + p.Hkv - 1) / p.Hkv, by_pages = p.short_whole ? seqs : seqs * per;
   p.S = (int)(by_target < by_pages ? by_target : by_pages);
   // no sequence is long enough for tiles: none

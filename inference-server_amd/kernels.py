@@ -463,9 +463,10 @@ class PagedPlan:
 
     __slots__ = ("sizes", "buffer", "block_tables", "device", "_shape", "_ref", "_ws_bytes", "_sections", "_views")
 
-    def __init__(self, sizes: tuple, buffer: torch.Tensor, block_tables: torch.Tensor):
-        self.sizes, self.buffer, self.block_tables, self.device = sizes, buffer, block_tables, buffer.get_device()
-        self._shape, self._ref, _, self._sections, self._ws_bytes = _plan_sizes(*sizes)
+    def __init__(self, sizes: tuple, block_tables: torch.Tensor):
+        self.sizes, self.block_tables, self.device = sizes, block_tables, block_tables.get_device()
+        self._shape, self._ref, ints, self._sections, self._ws_bytes = _plan_sizes(*sizes)
+        self.buffer = block_tables.new_empty(ints)
         self._views = None
 
     def _section(self, name: str) -> torch.Tensor:
@@ -530,8 +531,7 @@ def paged_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: 
         raise ValueError("free_pages is too long")
     sizes = (B, num_tokens, max_new_tokens, max_pages, num_heads, num_kv_heads)
     if out is None:
-        ints = _plan_sizes(*sizes)[2]
-        out = PagedPlan(sizes, torch.empty(ints, dtype=torch.int32, device=block_tables.device), block_tables)
+        out = PagedPlan(sizes, block_tables)
     else:
         if out.sizes != sizes or out.device != dev:
             raise ValueError(f"out is a plan of sizes {out.sizes} on device {out.device}, not of {sizes} on {dev}")

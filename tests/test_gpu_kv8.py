@@ -161,6 +161,18 @@ def test_plan_without_tokens_or_sequences(pkg, dev):
     p = s.plan()
     assert p.cu_tokens.tolist() == [0] and p.positions.tolist() == [-1] * 5 and p.pages_used.item() == 0
     s.check_attention(p)
+    before = s.got()
+    x = torch.ones((5, 4, D), dtype=torch.bfloat16, device=dev)
+    pkg.kv_append_fp8(x, x, *s.cache, p)
+    q = pkg.qk_norm_rope_append_fp8(torch.ones((5, 40 * D), dtype=torch.bfloat16, device=dev), x[0, 0], x[0, 0],
+                                    torch.ones(64, device=dev), 32, 4, 1e-6, *s.cache, p)
+    assert (q == 0).all() and all(np.array_equal(a, b) for a, b in zip(before, s.got()))
+    s = Step(pkg, dev, [3, 16], [0, 0], 32, 4, T=0)
+    p = s.plan()
+    s.check_plan(p)
+    pkg.kv_append_fp8(x[:0], x[:0], *s.cache, p)
+    assert pkg.paged_attention_fp8(x[:0].reshape(0, 1, 4, D).expand(0, 8, 4, D).reshape(0, 32, D), *s.cache, p, SCALE).shape == \
+        (0, 32, D)
 
 
 def new_kv(s, outliers=True):
