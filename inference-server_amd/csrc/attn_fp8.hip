@@ -97,28 +97,20 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // of its scores keys 4 (l >> 4) + i of each page, which are the 8 keys that the second MFMA wants from it.
 // ---------------------------------------------------------------------------
 template <int kWaves>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))) void attn_fp8_short_kernel(AttnFp8Args a) {
+struct ShortLds {  // for joining the waves
+  float m[kWaves][kShortRows], l[kWaves][kShortRows], o[kWaves][kShortRows][kHD + 4];
+};
+
+template <int kWaves>
+__device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g, ShortLds<kWaves>& lds) {
   constexpr int kThreads = 64 * kWaves;
   const PlanLayout& p = a.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int Hkv = p.Hkv, G = p.G;
-  const int items = p.S * Hkv;
-  if ((int)blockIdx.x >= items) {  // rows behind the last sequence: zeros
-    const long row = (long)p.Hq * kHD / 8;  // 16-byte pieces of a token
-    const long end = p.T * row;
-    for (long i = a.plan[PH_TOKENS] * row + ((int)blockIdx.x - items) * kThreads + threadIdx.x; i < end;
-         i += kPadBlocks * kThreads)
-      ((uint4*)a.out)[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
   const int4* it = (const int4*)(a.plan + p.shorts + (long)PI_INTS * item);
-  const int count = a.plan[PH_SHORTS];
-  int4 i0 = it[0], i1 = it[1];
-  asm volatile("" : "+v"(i0.x), "+v"(i1.x));  // one round trip: the item, in the list or behind its end, with the count
-  if (item >= count) return;
+  const int4 i0 = it[0], i1 = it[1];
   const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
   const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
   const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
@@ -254,34 +246,32 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
   }
   l_run = rows_sum(l_run);
 
-  // join the 4 waves
-  __shared__ float s_m[kWaves][kShortRows], s_l[kWaves][kShortRows];
-  __shared__ __attribute__((aligned(16))) float s_o[kWaves][kShortRows][kHD + 4];
+  // join the waves
   if (lg == 0) {
-    s_m[wave][lr] = m_run;
-    s_l[wave][lr] = l_run;
+    lds.m[wave][lr] = m_run;
+    lds.l[wave][lr] = l_run;
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *(v4f*)&s_o[wave][lr][64 * j + 16 * lg + 4 * i] = (v4f){o[4 * j][i], o[4 * j + 1][i], o[4 * j + 2][i], o[4 * j + 3][i]};
+      *(v4f*)&lds.o[wave][lr][64 * j + 16 * lg + 4 * i] = (v4f){o[4 * j][i], o[4 * j + 1][i], o[4 * j + 2][i], o[4 * j + 3][i]};
   __syncthreads();
   constexpr int kDims = kShortRows * kHD / kThreads;  // of a row, a thread's
   const int r = threadIdx.x / (kHD / kDims), d0 = threadIdx.x % (kHD / kDims) * kDims;
   if (r >= rows) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, lds.m[w][r]);
   float acc[kDims], L = 0.f;
 #pragma unroll
   for (int d = 0; d < kDims; ++d) acc[d] = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const float wgt = s_m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][r] - M);
-    L += s_l[w][r] * wgt;
+    const float wgt = lds.m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lds.m[w][r] - M);
+    L += lds.l[w][r] * wgt;
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) acc[d] += s_o[w][r][d0 + d] * wgt;
+    for (int d = 0; d < kDims; ++d) acc[d] += lds.o[w][r][d0 + d] * wgt;
   }
   if (parts == 1) {
     const float inv = M == -INFINITY ? 0.f : 1.0f / L;  // no key at all: zeros
@@ -319,12 +309,21 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
     }                                                                          \
   } while (0)
 
+// Steps whose K and V are in LDS.  Two: a barrier after each step, and room for two workgroups in a CU.  Four, where
+// the registers leave room for one only: a barrier after two steps.
+constexpr int tile_ring(int waves) { return waves == 4 ? 2 : 4; }
+
 template <int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
+struct TileLds {
+  struct {
+    uint4 k[kHD / 8][kTileKeys], v[kTilePages][2][kHD];
+  } step[tile_ring(kWaves)];
+};
+
+template <int kWaves>
+__device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g, TileLds<kWaves>& lds) {
   constexpr int kTileRows = 32 * kWaves;
-  // Steps whose K and V are in LDS.  Two: a barrier after each step, and room for two workgroups in a CU.  Four, where
-  // the registers leave room for one only: a barrier after two steps.
-  constexpr int kRing = kWaves == 4 ? 2 : 4;
+  constexpr int kRing = tile_ring(kWaves);
   constexpr int kAheadK = kRing == 4 ? 3 : 2, kAheadV = kAheadK - 1;  // steps from storing to use
   constexpr int kLoads = 8 / kWaves;  // 16-byte pieces of a step's K, and 8-byte ones of a quad of V, for each thread
   const PlanLayout& p = a.p;
@@ -332,20 +331,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 31, kg = lane >> 5;
   const int Hkv = p.Hkv, G = p.G;
-  // neighbours in the launch go to different XCDs (8), so with 2, 4 or 8 kv heads an XCD's L2 holds few heads
-  const int item = blockIdx.x / Hkv, g = blockIdx.x % Hkv;
   const int4* it = (const int4*)(a.plan + p.tiles + (long)PI_INTS * item);
-  const int count = a.plan[PH_TILES];
-  int4 i0 = it[0], i1 = it[1];
-  asm volatile("" : "+v"(i0.x), "+v"(i1.x));
-  if (item >= count) return;
+  const int4 i0 = it[0], i1 = it[1];
   const int seq = __builtin_amdgcn_readfirstlane(i0.x), tok = __builtin_amdgcn_readfirstlane(i0.y);
   const int ntok = __builtin_amdgcn_readfirstlane(i0.z), pos = __builtin_amdgcn_readfirstlane(i0.w);
   const int page0 = __builtin_amdgcn_readfirstlane(i1.x), page1 = __builtin_amdgcn_readfirstlane(i1.y);
   const int parts = __builtin_amdgcn_readfirstlane(i1.z);
-
-  __shared__ __attribute__((aligned(16))) uint4 s_k[kRing][kHD / 8][kTileKeys];
-  __shared__ __attribute__((aligned(16))) uint4 s_v[kRing][kTilePages][2][kHD];
 
   const int r = 32 * wave + lr;
   const bool live = r < ntok * G;
@@ -434,8 +425,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
 #pragma unroll
     for (int h = 0; h < kLoads; ++h) {
       const int key = (2 * h + k_page) * kPage + (lane & 15);
-      s_k[buf][2 * c][key] = __builtin_bit_cast(uint4, widen8(kr[h].x, kr[h].y, ks[h]));
-      s_k[buf][2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
+      lds.step[buf].k[2 * c][key] = __builtin_bit_cast(uint4, widen8(kr[h].x, kr[h].y, ks[h]));
+      lds.step[buf].k[2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
     }
   };
   auto mask_v = [&](int page) __attribute__((always_inline)) {  // codes behind the last key may be anything, a NaN too
@@ -449,7 +440,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
   auto store_v = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < 2 * kLoads; ++d)
-      s_v[buf][v_at][vq][64 * vj + 16 * (2 * vd + d) + vx] = __builtin_bit_cast(uint4, widen8(vr[0][d], vr[1][d], vs));
+      lds.step[buf].v[v_at][vq][64 * vj + 16 * (2 * vd + d) + vx] = __builtin_bit_cast(uint4, widen8(vr[0][d], vr[1][d], vs));
   };
   auto scores = [&](v16f (&s)[2], int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -460,7 +451,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
     for (int k = 0; k < 8; ++k)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_k[buf][2 * k + kg][32 * b + lr]), qop[k], s[b],
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, lds.step[buf].k[2 * k + kg][32 * b + lr]), qop[k], s[b],
                                                        0, 0, 0);
   };
   auto mask_scores = [&](v16f (&s)[2], int key0, uint32_t there) __attribute__((always_inline)) {
@@ -497,7 +488,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int d = 0; d < 4; ++d)
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, s_v[buf][2 * half + h][kg][32 * d + lr]), pb[h],
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, lds.step[buf].v[2 * half + h][kg][32 * d + lr]), pb[h],
                                                        o[d], 0, 0, 0);
   };
 
@@ -604,6 +595,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_tile_kernel(AttnFp8Ar
 }
 
 // ---------------------------------------------------------------------------
+// The launches.  A step of short sequences alone is the short kernel's, many tiles the tile kernel's and then the short
+// kernel's.  In between the step kernel takes both, the tiles first, so that its short items fill the CUs that the last
+// tiles leave (2048 tokens of a prompt and 63 decoding sequences 172 -> 160 us, 64 and 64 84 -> 59, 100 tokens alone
+// 13.6 -> 11.2 against two launches; both kinds side by side from the start: 170, 71 and 10.7).  Workgroups that follow
+// each other go to different XCDs (8), so with 1, 2, 4 or 8 kv heads a tile's XCD sees few heads of the cache.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void clear_padding(const AttnFp8Args& a, int block) {  // rows behind the last sequence: zeros
+  const long row = (long)a.p.Hq * kHD / 8;  // 16-byte pieces of a token
+  const long end = a.p.T * row;
+  for (long i = a.plan[PH_TOKENS] * row + (long)block * blockDim.x + threadIdx.x; i < end; i += (long)kPadBlocks * blockDim.x)
+    ((uint4*)a.out)[i] = make_uint4(0, 0, 0, 0);
+}
+
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))) void attn_fp8_short_kernel(AttnFp8Args a) {
+  __shared__ __attribute__((aligned(16))) ShortLds<kWaves> lds;
+  const int items = a.p.S * a.p.Hkv;
+  if ((int)blockIdx.x >= items) return clear_padding(a, (int)blockIdx.x - items);
+  const int item = blockIdx.x / a.p.Hkv;
+  if (item < a.plan[PH_SHORTS]) short_item<kWaves>(a, item, blockIdx.x % a.p.Hkv, lds);
+}
+
+__global__ __launch_bounds__(256, 2) void attn_fp8_step_kernel(AttnFp8Args a) {
+  __shared__ __attribute__((aligned(16))) union {
+    ShortLds<4> s;
+    TileLds<4> t;
+  } lds;
+  const int Hkv = a.p.Hkv, items = (a.p.S + a.p.N) * Hkv, i = blockIdx.x;
+  if (i >= items) return clear_padding(a, i - items);
+  const int tiles = a.plan[PH_TILES] * Hkv, shorts = a.plan[PH_SHORTS] * Hkv;
+  if (i < tiles)
+    tile_item<4>(a, i / Hkv, i % Hkv, lds.t);
+  else if (i < tiles + shorts)
+    short_item<4>(a, (i - tiles) / Hkv, (i - tiles) % Hkv, lds.s);
+}
+
+__global__ __launch_bounds__(512, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
+  __shared__ __attribute__((aligned(16))) TileLds<8> lds;
+  const int item = blockIdx.x / a.p.Hkv;
+  if (item < a.plan[PH_TILES]) tile_item<8>(a, item, blockIdx.x % a.p.Hkv, lds);
+}
+
+// ---------------------------------------------------------------------------
 // merge: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's items, in key order, a lane of 32 with 4 dims.
 // Up to kMergeFew items: the 8 groups of 32 lanes take a row each.  More: they share a row's items.  Either way a
 // group has four items' loads in flight.
@@ -699,7 +733,7 @@ void attn_carve(WsCarver& c, const Parts& n, AttnFp8Args* a) {
 }
 
 bool attn_grid_ok(const PlanLayout& p) {
-  return moe_grid_fits((long)p.S * p.Hkv + kPadBlocks) && moe_grid_fits((long)p.N * p.Hkv) &&
+  return moe_grid_fits((long)(p.S + p.N) * p.Hkv + kPadBlocks) &&
          moe_grid_fits((long)(p.SM + p.TM) * p.Hkv);
 }
 
@@ -741,23 +775,26 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   WsCarver c(workspace);
   attn_carve(c, parts, &a);
   hipStream_t s = (hipStream_t)stream;
-  if (p.N > 0) {
-    const dim3 grid((unsigned)(p.N * p.Hkv));
-    if (p.tile_rows == kTileRowsMany)
-      hipLaunchKernelGGL(attn_fp8_tile_kernel<8>, grid, dim3(512), 0, s, a);
+  const bool many = p.N > 0 && p.tile_rows == kTileRowsMany;
+  if (p.N > 0 && !many) {
+    const dim3 grid((unsigned)((p.N + p.S) * p.Hkv + kPadBlocks));
+    hipLaunchKernelGGL(attn_fp8_step_kernel, grid, dim3(256), 0, s, a);
+    MOE_CHECK_LAUNCH();
+  } else {
+    if (many) {
+      hipLaunchKernelGGL(attn_fp8_tile_kernel, dim3((unsigned)(p.N * p.Hkv)), dim3(512), 0, s, a);
+      MOE_CHECK_LAUNCH();
+    }
+    const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));
+    // Whole sequences, and no more of them than CUs: 8 waves each, of up to eight pairs of pages.  (One sequence of 1000
+    // tokens, in a graph: 4 waves 9.1 us, 8 waves 7.5, 16 waves 8.3; two to four pairs in flight per wave 7.9 to 8.6,
+    // for the code that has to be fetched.)
+    if (p.short_whole && p.S * p.Hkv <= kFewItems)
+      hipLaunchKernelGGL(attn_fp8_short_kernel<8>, grid, dim3(512), 0, s, a);
     else
-      hipLaunchKernelGGL(attn_fp8_tile_kernel<4>, grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL(attn_fp8_short_kernel<4>, grid, dim3(256), 0, s, a);
     MOE_CHECK_LAUNCH();
   }
-  const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));
-  // Whole sequences, and no more of them than CUs: 8 waves each, of up to eight pairs of pages.  (One sequence of 1000
-  // tokens, in a graph: 4 waves 9.1 us, 8 waves 7.5, 16 waves 8.3; two to four pairs in flight per wave 7.9 to 8.6,
-  // for the code that has to be fetched.)
-  if (p.short_whole && p.S * p.Hkv <= kFewItems)
-    hipLaunchKernelGGL(attn_fp8_short_kernel<8>, grid, dim3(512), 0, s, a);
-  else
-    hipLaunchKernelGGL(attn_fp8_short_kernel<4>, grid, dim3(256), 0, s, a);
-  MOE_CHECK_LAUNCH();
   if (parts.shorts + parts.tiles > 0 && p.SM > 0) {
     // with tiles among them mostly nothing is split: fewer workgroups, that come back for more
     const long x = (long)(p.SM + p.TM) * p.Hkv;
