@@ -3,10 +3,11 @@
 //   o = sum_{j <= p} softmax_j(scale q . K_j) V_j
 // with K and V the values that the codes stand for, everything in fp32 but for two operands: the bf16 q, and
 // the probabilities, rounded to bf16 (by 2^-8 at most) for the second MFMA; the tiles sum them as rounded, so that
-// a row that one key dominates is exact, the short items before it.  The codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8 with the
-// page's power-of-two scale), so both products run on the bf16 MFMAs without a further error.
+// a row that one key dominates is exact, the short items before it.  The codes become bf16 exactly
+// (v_cvt_scalef32_pk_bf16_fp8 with the page's power-of-two scale), so both products run on the bf16 MFMAs without a
+// further error.
 //
-// Two kernels, by the rows (tokens x heads of the group) that a sequence has for one kv head:
+// Two forms, by the rows (tokens x heads of the group) that a sequence has for one kv head:
 //   short: up to 16 rows (a decoding sequence), bound by the cache's bytes.  One workgroup per (sequence, kv
 //     head, run of pages); its 4 waves take pairs of pages round robin, straight from HBM to the MFMA.
 //   tile: more rows (prompts), bound by the MFMA and the softmax.  One workgroup per (128 or 256 rows, kv
@@ -23,10 +24,10 @@ constexpr int kPage = kPlanPage;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCachePolicyNT = 2;  // the instruction's cache-policy field: nt (streaming)
 constexpr int kPadBlocks = 8;      // workgroups that clear the rows behind the last sequence
-constexpr int kMergeBlocks = 512;
-constexpr int kMergeFew = 8;
-constexpr int kFewItems = 256;
-constexpr float kSlack = 8.f;
+constexpr int kMergeBlocks = 512;  // of each row, where a step has tiles: mostly nothing is split then
+constexpr int kMergeFew = 8;       // items of a row that one group of the merge takes alone
+constexpr int kFewItems = 256;     // one per CU
+constexpr float kSlack = 8.f;      // log2 of what an unnormalised probability may reach
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -555,6 +556,7 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
   scores(s0, 0);
   if (page0 * kPage + kTileKeys > all_end || held0 != 15) mask_scores(s0, page0 * kPage, held0);
   pm = score_max(s0);
+  __syncthreads();  // every wave has read the first step's K, whose place a later step's K takes before the next barrier
   for (int n = 0; n < steps; n += kRing) {
     step(s0, s1, n, 0);
     if (n + 1 >= steps) break;
