@@ -597,11 +597,11 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
 }
 
 // ---------------------------------------------------------------------------
-// The launches.  A step of short sequences alone is the short kernel's, many tiles the tile kernel's and then the short
-// kernel's.  In between the step kernel takes both, the tiles first, so that its short items fill the CUs that the last
-// tiles leave (2048 tokens of a prompt and 63 decoding sequences 172 -> 160 us, 64 and 64 84 -> 59, 100 tokens alone
-// 13.6 -> 11.2 against two launches; both kinds side by side from the start: 170, 71 and 10.7).  Workgroups that follow
-// each other go to different XCDs (8), so with 1, 2, 4 or 8 kv heads a tile's XCD sees few heads of the cache.
+// The launches.  A step of short sequences alone is the short kernel's.  Any other is the step kernel's, which takes
+// both kinds, the tiles first, so that its short items fill the CUs that the last tiles leave (2048 tokens of a prompt
+// and 63 decoding sequences 172 -> 160 us, 64 and 64 84 -> 59, 100 tokens alone 13.6 -> 11.2 against two launches; both
+// kinds side by side from the start: 170, 71 and 10.7).  Workgroups that follow each other go to different XCDs (8), so
+// with 1, 2, 4 or 8 kv heads a tile's XCD sees few heads of the cache.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void clear_padding(const AttnFp8Args& a, int block) {  // rows behind the last sequence: zeros
   const long row = (long)a.p.Hq * kHD / 8;  // 16-byte pieces of a token
@@ -619,24 +619,19 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
   if (item < a.plan[PH_SHORTS]) short_item<kWaves>(a, item, blockIdx.x % a.p.Hkv, lds);
 }
 
-__global__ __launch_bounds__(256, 2) void attn_fp8_step_kernel(AttnFp8Args a) {
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_fp8_step_kernel(AttnFp8Args a) {
   __shared__ __attribute__((aligned(16))) union {
-    ShortLds<4> s;
-    TileLds<4> t;
+    ShortLds<kWaves> s;
+    TileLds<kWaves> t;
   } lds;
   const int Hkv = a.p.Hkv, items = (a.p.S + a.p.N) * Hkv, i = blockIdx.x;
   if (i >= items) return clear_padding(a, i - items);
   const int tiles = a.plan[PH_TILES] * Hkv, shorts = a.plan[PH_SHORTS] * Hkv;
   if (i < tiles)
-    tile_item<4>(a, i / Hkv, i % Hkv, lds.t);
+    tile_item<kWaves>(a, i / Hkv, i % Hkv, lds.t);
   else if (i < tiles + shorts)
-    short_item<4>(a, (i - tiles) / Hkv, (i - tiles) % Hkv, lds.s);
-}
-
-__global__ __launch_bounds__(512, 2) void attn_fp8_tile_kernel(AttnFp8Args a) {
-  __shared__ __attribute__((aligned(16))) TileLds<8> lds;
-  const int item = blockIdx.x / a.p.Hkv;
-  if (item < a.plan[PH_TILES]) tile_item<8>(a, item, blockIdx.x % a.p.Hkv, lds);
+    short_item<kWaves>(a, (i - tiles) / Hkv, (i - tiles) % Hkv, lds.s);
 }
 
 // ---------------------------------------------------------------------------
@@ -777,16 +772,14 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
   WsCarver c(workspace);
   attn_carve(c, parts, &a);
   hipStream_t s = (hipStream_t)stream;
-  const bool many = p.N > 0 && p.tile_rows == kTileRowsMany;
-  if (p.N > 0 && !many) {
+  if (p.N > 0) {
     const dim3 grid((unsigned)((p.N + p.S) * p.Hkv + kPadBlocks));
-    hipLaunchKernelGGL(attn_fp8_step_kernel, grid, dim3(256), 0, s, a);
+    if (p.tile_rows == kTileRowsMany)
+      hipLaunchKernelGGL(attn_fp8_step_kernel<8>, grid, dim3(512), 0, s, a);
+    else
+      hipLaunchKernelGGL(attn_fp8_step_kernel<4>, grid, dim3(256), 0, s, a);
     MOE_CHECK_LAUNCH();
   } else {
-    if (many) {
-      hipLaunchKernelGGL(attn_fp8_tile_kernel, dim3((unsigned)(p.N * p.Hkv)), dim3(512), 0, s, a);
-      MOE_CHECK_LAUNCH();
-    }
     const dim3 grid((unsigned)(p.S * p.Hkv + kPadBlocks));
     // Whole sequences, and no more of them than CUs: 8 waves each, of up to eight pairs of pages.  (One sequence of 1000
     // tokens, in a graph: 4 waves 9.1 us, 8 waves 7.5, 16 waves 8.3; two to four pairs in flight per wave 7.9 to 8.6,
