@@ -333,8 +333,9 @@ int moe_mi355x_kv_append_fp8(const void* k, const void* v, long long k_stride, l
 
 /*
  * moe_mi355x_kv_append_fp8 from the fused q/k/v projections, with q_norm / k_norm and the rotary embedding at each
- * row's position (TF/models/qwen3_moe/modeling_qwen3_moe.py:162-171), for prompts and single tokens.  fp32
- * throughout (the angle position * inv_freq in 64 bits) and one rounding: q to bf16, k and v to their codes.
+ * row's position (TF/models/qwen3_moe/modeling_qwen3_moe.py:162-171), for prompts and single tokens.  q in
+ * fp32 (the angle position * inv_freq in 64 bits) and rounded once to bf16; k in 64 bits throughout, so that its codes
+ * and scales are those of the formula.
  *   qkv      bf16 [tokens, (heads + 2 kv_heads) * 128]  (q heads, then k heads, then v heads)
  *   q_norm_w, k_norm_w bf16 [128]   inv_freq fp32 [64]   q_out bf16 [tokens, heads, 128] (padding rows: 0)
  */

@@ -10,9 +10,11 @@
 // A page that begins is written whole (zeros behind its tokens), so nothing stale is ever read from it.
 //
 // One wave per (page that gets tokens, kv head, K or V), from the plan's list: it alone writes the block, so
-// there are no atomics and no second pass, and the maximum is a wave's.  norm and rotary stay in fp32 from the bf16
-// projections to the one rounding (bf16 for q, e4m3 for k).  The angle is position * inv_freq in 64 bits,
-// reduced to a turn before it is rounded to 32: at position 10^5 a 32-bit product is off by up to 0.004.
+// there are no atomics and no second pass, and the maximum is a wave's.  norm and rotary of q stay in fp32 from the bf16
+// projection to the one rounding to bf16.  Its angle is position * inv_freq in 64 bits, reduced to a turn before
+// it is rounded to 32: at position 10^5 a 32-bit product is off by up to 0.004.  Those of k, of which there are few
+// rows, are in 64 bits throughout: in 32, two to eight codes of 4 million fell on the other side of a tie, each 2^-4 of
+// its value away (8178 tokens, 64 / 4 heads: 54.4 -> 56.1 us; 16 tokens alike, 4.6).
 // Memory bound for prompts (512 B read and 256 B written per token and kv head, 512 B per token and q head).
 #include "kv_fp8.h"
 #include "paged_plan.h"
@@ -40,7 +42,7 @@ struct KvArgs {
   float eps;
 };
 
-// 8 values that are read once: past the caches (3% at 8178 tokens and 64 / 4 heads, 56.9 -> 55.0 us)
+// 8 values that are read once: past the caches (3% at 8178 tokens and 64 / 4 heads)
 __device__ __forceinline__ uint4 load_once(const uint16_t* p) {
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u4*)p));
@@ -92,6 +94,45 @@ __device__ __forceinline__ void rope_angle(int pos, float inv_freq, float* c, fl
   *s = q >= 2 ? -b : b;
 }
 
+// x in 32 bits, an inexact one with its last bit set: rounding that to e4m3 is rounding x to e4m3.
+__device__ __forceinline__ float round_to_odd(double x) {
+  const float f = (float)x;
+  uint32_t b = __float_as_uint(f);
+  if (fabs((double)f) > fabs(x)) b -= 1;
+  if ((double)f < x || (double)f > x) b |= 1;
+  return __uint_as_float(b);
+}
+
+// The same for a k row, angles included, in 64 bits.  Four pairs at a time are enough to fill the lanes' pipeline; all
+// eight take registers that other waves miss (56.9 us against 56.1).
+__device__ __forceinline__ void norm_rope_k(float* x, const float* w, const float* inv_freq, int pos, float eps) {
+  double ss = 0.;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) ss = fma((double)x[i], (double)x[i], ss);
+  ss += __shfl_xor(ss, 1);
+  ss += __shfl_xor(ss, 2);
+  ss += __shfl_xor(ss, 4);
+  const double r = 1.0 / sqrt(ss * (1.0 / kHD) + (double)eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double quarters = (double)pos * (double)inv_freq[i] * 0.63661977236758134308;  // 2 / pi
+    const double whole = rint(quarters);
+    // Taylor's series on |angle| <= pi / 4, off by 4e-13 at most
+    const double t = (quarters - whole) * 1.57079632679489661923, z = t * t;
+    const double sr = t * fma(z, fma(z, fma(z, fma(z, fma(z, fma(z, 1. / 6227020800., -1. / 39916800.), 1. / 362880.), -1. / 5040.),
+                                            1. / 120.), -1. / 6.), 1.);
+    const double cr = fma(z, fma(z, fma(z, fma(z, fma(z, fma(z, 1. / 479001600., -1. / 3628800.), 1. / 40320.), -1. / 720.), 1. / 24.),
+                                 -.5), 1.);
+    const int q = (int)(long long)whole & 3;
+    const double u = q & 1 ? sr : cr, v = q & 1 ? cr : sr;
+    const double c = q == 1 || q == 2 ? -u : u, s = q >= 2 ? -v : v;
+    const double a = x[i] * r * w[i], b = x[8 + i] * r * w[8 + i];
+    x[i] = round_to_odd(a * c - b * s);
+    x[8 + i] = round_to_odd(b * c + a * s);
+    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 template <bool FUSED>
 __device__ __forceinline__ void write_k(const KvArgs& a, int4 w, int g, int lane) {
   const int tl = lane >> 3, j = lane & 7;  // rounds r = 0, 1: token tl + 8 r
@@ -130,10 +171,7 @@ __device__ __forceinline__ void write_k(const KvArgs& a, int4 w, int g, int lane
     if constexpr (FUSED) {
       if (8 * r < w.z + w.w && 8 * r + 8 > w.z) {  // wave-uniform: a round with tokens
         const int pos = a.pos[w.y - w.z + (live ? t : w.z)];
-        float c[8], s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rope_angle(pos, a.inv_freq[8 * j + i], &c[i], &s[i]);
-        norm_rope(x[r], wt, c, s, a.eps);
+        norm_rope_k(x[r], wt, a.inv_freq + 8 * j, pos, a.eps);
       }
     }
 #pragma unroll

@@ -620,7 +620,8 @@ def qk_norm_rope_append_fp8(qkv: torch.Tensor, q_norm_weight: torch.Tensor, k_no
                             v_scale: torch.Tensor, plan: PagedPlan) -> torch.Tensor:
     """q/k RMSNorm, rotary embedding at the plan's positions and ``kv_append_fp8`` in one launch, for a step's prompts
     and single tokens (modeling_qwen3_moe.py:162-171).  ``qkv`` bf16 [T, (Hq + 2 Hkv) * 128]; returns q bf16
-    [T, Hq, 128] (padding rows: zeros).  fp32 from the projections to the one rounding of each result."""
+    [T, Hq, 128] (padding rows: zeros).  q in fp32 and k in 64 bits, from the projections to the one
+    rounding of each result."""
     pages = _check_fp8_cache(k_cache, v_cache, k_scale, v_scale, plan)
     _, tokens, _, _, heads, kv_heads = plan.sizes
     if num_heads != heads or num_kv_heads != kv_heads:

@@ -280,6 +280,23 @@ def test_qk_norm_rope_append_matches_oracle(pkg, dev, cached, new, Hq, Hkv):
     assert ((gks == eks) | (np.abs(np.log2(gks / eks)) == 1)).all() and (gks != eks).mean() < 0.02
 
 
+def test_qk_norm_rope_append_codes_are_those_of_64_bits(pkg, dev):
+    """Scales and codes of 3 million keys to the bit: the 64-bit forms differ by 1e-12 of a value, and a code's tie lies
+    that near for one value in 10^10.  (In fp32 a tie lies within the error for one in 10^6.)"""
+    s = Step(pkg, dev, [0, 70000, 21], [3500, 2000, 900], 8, 4, seed=31)
+    x = orc.round_bf16(s.rng.standard_normal((s.T, 16, D)).astype(np.float32))
+    qw, kw = (orc.round_bf16((1 + 0.3 * s.rng.standard_normal(D)).astype(np.float32)) for _ in range(2))
+    inv_freq = (1e6 ** (-np.arange(0, D, 2) / D)).astype(np.float32)
+    pkg.qk_norm_rope_append_fp8(to_bf16(x.reshape(s.T, -1), dev), to_bf16(qw, dev), to_bf16(kw, dev),
+                                torch.from_numpy(inv_freq).to(dev), 8, 4, 1e-6, *s.cache, s.plan())
+    k, _ = kv.norm_rope(x[:, 8:12], kw, inv_freq, s.ref[0], float(np.float32(1e-6)))
+    ek, eks = s.k.copy(), s.ks.copy()
+    kv.append(k, s.ref[1], s.ref[0], ek, eks, kv.k_index)
+    gk, _, gks, _ = s.got()
+    assert np.array_equal(gks, eks)
+    assert np.array_equal(gk, ek), int((gk != ek).sum())
+
+
 ATTENTION = [
     ([0], [1]),
     ([0, 15, 16, 17, 31], [1, 1, 1, 1, 1]),           # single tokens around a page's edges
