@@ -674,14 +674,16 @@ __global__ __launch_bounds__(256) void attn_fp8_merge_kernel(AttnFp8Args a) {
       float m_new = M;
 #pragma unroll
       for (int u = 0; u < 4; ++u) m_new = fmaxf(m_new, x[u].x);  // the last item again changes nothing
-      if (m_new == -INFINITY) continue;                          // only empty pages so far
-      const float old = __builtin_amdgcn_exp2f(M - m_new);
+      // Without a maximum, an item has only empty pages and zeros, or only NaN: either is added with weight 0, which
+      // leaves the one nothing and the other NaN.
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float old = __builtin_amdgcn_exp2f(M - m_use);
       M = m_new;
       L *= old;
       acc *= old;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float w = s0 + by * u < ns ? __builtin_amdgcn_exp2f(x[u].x - M) : 0.f;
+        const float w = s0 + by * u < ns ? __builtin_amdgcn_exp2f(x[u].x - m_use) : 0.f;
         L += x[u].y * w;
         acc += v[u] * w;
       }

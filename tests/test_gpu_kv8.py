@@ -555,3 +555,40 @@ def test_attention_large_tiles(pkg, dev, T, Hq, Hkv):
         ref, size = kv.attention(q[t:t + 1], k, v, [0, 1], pos[t:t + 1], s.ref[4][b:b + 1], SCALE)
         worst = np.abs(o[t] - ref[0]) - 2.0 ** -8 * (1.05 * (size[0] + np.abs(ref[0])) + np.abs(ref[0]))
         assert (worst <= 1e-30).all(), (t, worst.max())
+
+
+def check_but(o, ref, size, lost):
+    """``o`` is not finite where ``lost`` says so (broadcast to [T, Hq, 128]) and within the module's tolerance elsewhere."""
+    got, lost = o.float().cpu().numpy(), np.broadcast_to(lost, o.shape)
+    assert not np.isfinite(got[lost]).any(), np.argwhere(np.isfinite(got) & lost)[:4]
+    worst = np.abs(got - ref) - 2.0 ** -8 * (1.05 * (size + np.abs(ref)) + np.abs(ref))
+    assert (worst[~lost] <= 1e-30).all(), np.argwhere(~(worst <= 1e-30) & ~lost)[:4]
+
+
+@pytest.mark.parametrize("cached,new", [
+    ([300], [1]),                # whole
+    ([2000] * 16, [1] * 16),     # split over 8 items
+    ([8191], [1]),               # over 64
+    ([0], [130]),                # tiles, whole
+    ([3000], [40]),              # tiles, split
+])
+def test_attention_nan_query_gives_nan_whatever_the_split(pkg, dev, cached, new):
+    s = Step(pkg, dev, cached, new, 32, 4, seed=40)
+    q = orc.round_bf16(s.rng.standard_normal((s.T, 32, D)).astype(np.float32))
+    ref, size = s.attention_ref(q)
+    lost = np.zeros((s.T, 32, 1), bool)
+    lost[s.T // 2, 5] = lost[-1, 31] = True
+    o = pkg.paged_attention_fp8(to_bf16(np.where(lost, np.float32(np.nan), q), dev), *s.cache, s.plan(), SCALE)
+    check_but(o, ref, size, lost)
+
+
+def test_attention_nan_keys_of_whole_items_reach_the_result(pkg, dev):
+    """The keys of a sequence's first four items out of eight, which a lane of the merge loads at once, are NaN."""
+    s = Step(pkg, dev, [2000] * 16, [1] * 16, 32, 4, seed=41)
+    s.k[s.ref[4][3, :64]] = 0x7F
+    s.cache = (torch.from_numpy(s.k).to(dev).view(FP8), *s.cache[1:])
+    q = orc.round_bf16(s.rng.standard_normal((s.T, 32, D)).astype(np.float32))
+    ref, size = s.attention_ref(q)
+    lost = np.zeros((s.T, 32, 1), bool)
+    lost[3] = True
+    check_but(pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, s.plan(), SCALE), ref, size, lost)
