@@ -145,7 +145,8 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
     int my_page = mine < page1 ? table[mine] : -1;
     if (my_page >= a.num_pages || my_page < 0) my_page = -1;  // a pad or a stale id: an empty page
     const long my_blk = my_page < 0 ? 0 : (long)my_page * Hkv + g;
-    const float my_ks = a.num_pages > 0 ? a.k_scale[my_blk] : 1.f, my_vs = a.num_pages > 0 ? a.v_scale[my_blk] : 1.f;
+    float my_ks = a.num_pages > 0 ? a.k_scale[my_blk] : 1.f, my_vs = a.num_pages > 0 ? a.v_scale[my_blk] : 1.f;
+    if (my_page < 0) my_ks = my_vs = 1.f;  // zeros under page 0's scale, which may never have been written, could be NaN
     const int pairs = (min(page1 - first, 64 * kWaves) + 1) / 2;  // of all waves
     const int n = pairs > wave ? (pairs - wave + kWaves - 1) / kWaves : 0;
 
@@ -372,6 +373,7 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
     const long blk = next_page < 0 ? 0 : (long)next_page * Hkv + g;
     next_ks = a.num_pages > 0 ? a.k_scale[blk] : 1.f;
     next_vs = a.num_pages > 0 ? a.v_scale[blk] : 1.f;
+    if (next_page < 0) next_ks = next_vs = 1.f;  // not page 0's, which may never have been written
   };
   auto lane_f = [&](float x, int l) __attribute__((always_inline)) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), l));

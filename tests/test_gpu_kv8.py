@@ -592,3 +592,22 @@ def test_attention_nan_keys_of_whole_items_reach_the_result(pkg, dev):
     lost = np.zeros((s.T, 32, 1), bool)
     lost[3] = True
     check_but(pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, s.plan(), SCALE), ref, size, lost)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -3.0])
+@pytest.mark.parametrize("cached,new", [([40, 700], [1, 1]), ([20, 100], [1, 30]), ([9000, 64], [1, 1])])
+def test_attention_takes_no_scale_of_a_page_that_no_sequence_has(pkg, dev, bad, cached, new):
+    """A pool whose scales were never filled: those of pages without an owner, page 0 among them, may be anything, and
+    an odd number of pages leaves half a pair and a part of a tile's step without one."""
+    s = Step(pkg, dev, cached, new, 32, 4, seed=42)
+    up = lambda a: np.where(a >= 0, a + 1, a).astype(np.int32)  # noqa: E731
+    s.tables, s.free = up(s.tables), up(s.free)
+    s.ref = kv.plan(s.cached, s.new, s.tables, s.free, s.T, s.max_new)
+    s.g_tables, s.g_free = i32(s.tables, dev), i32(s.free, dev)
+    own = np.unique(s.ref[4][s.ref[4] >= 0])
+    pools = [np.concatenate([a[:1], a]) for a in (s.k, s.v, s.ks, s.vs)]
+    for a in pools[2:]:
+        a[~np.isin(np.arange(len(a)), own)] = bad
+    s.cache = tuple(torch.from_numpy(a).to(dev) for a in pools)
+    s.cache = (s.cache[0].view(FP8), s.cache[1].view(FP8), *s.cache[2:])
+    s.check_attention(s.plan())
