@@ -350,8 +350,8 @@ int moe_mi355x_qk_norm_rope_append_fp8(const void* qkv, const void* q_norm_w, co
  *   out = bf16( softmax(scale * q . K) . V )
  * with fp32 scores, softmax and sums, and bf16 probabilities in the product with V.  Keys of a page that the table
  * does not hold (an entry outside [0, num_pages)) are left out; a row without keys and a padding row are 0.  What lies
- * behind a sequence's last token, a NaN code too, reaches no result; a NaN among its own values reaches the later rows
- * and may reach earlier ones of the same step.
+ * behind a sequence's last token, a NaN code too, reaches no result; a NaN among its own values reaches the rows from
+ * its token on (one of V in its dim alone) and none before it.
  *   q   bf16 [tokens, heads, 128], rows of a token q_stride values apart (a multiple of 8)
  *   out bf16 [tokens, heads, 128]      block_tables as the plan left them      scale finite, > 0
  */

@@ -88,6 +88,14 @@ __device__ __forceinline__ uint32_t quad_mask(int live) {
   return live >= 4 ? 0xffffffffu : live <= 0 ? 0u : (1u << (8 * live)) - 1u;
 }
 
+// 0xff in the bytes of 4 codes that are no finite value under the scale: NaN, and 2^128 or more.  With e the scale's
+// exponent a code of exponent field f is below 2^(f - 6 + e), so the latter are those with f >= 135 - e.
+__device__ __forceinline__ uint32_t not_finite4(uint32_t codes, float scale) {
+  const int least = min(127, 8 * (262 - (int)((__float_as_uint(scale) >> 23) & 255)));
+  const uint32_t high = ((codes & 0x7f7f7f7fu) + 0x01010101u * (uint32_t)(128 - least)) & 0x80808080u;
+  return high | (high - (high >> 7));
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
 }
@@ -100,6 +108,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 template <int kWaves>
 struct ShortLds {  // for joining the waves
   float m[kWaves][kShortRows], l[kWaves][kShortRows], o[kWaves][kShortRows][kHD + 4];
+  int late[kWaves];
 };
 
 template <int kWaves>
@@ -137,6 +146,7 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
 #pragma unroll
   for (int n = 0; n < 8; ++n) o[n] = (v4f){0.f, 0.f, 0.f, 0.f};
 
+  bool late = false;  // this wave has met values that are not finite and that not every row sees
   const int32_t* table = a.tables + (long)seq * p.max_pages;
   // 32 pairs of pages at a time: lane l holds the id and the scales of page l & 1 of this wave's pair l >> 1, so
   // that a page's loads wait for no other
@@ -194,15 +204,23 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
           const int end = page_at(i, h) < 0 ? 0 : key_end;
 #pragma unroll
           for (int e = 0; e < 4; ++e) sv[h][e] = key0 + kPage * h + 4 * lg + e < end ? sv[h][e] : -INFINITY;
-          // codes behind the last key may be anything, a NaN too: zero them rather than multiply them by zero
-          const uint32_t mask = quad_mask(pos + ntok - (key0 + kPage * h + 4 * lg));
+          // Codes behind the last key may be anything, a NaN too: zero them rather than multiply them by zero.  So
+          // with what is not finite among the keys that not every row sees: the rows that do get it at the end.
+          const int key = key0 + kPage * h + 4 * lg;
+          const uint32_t mask = quad_mask(pos + ntok - key), some = ~quad_mask(pos + 1 - key);
+          const float vs = scale_at(my_vs, i, h);
+          uint32_t drop = 0;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            vr[h][j].x &= mask;
-            vr[h][j].y &= mask;
-            vr[h][j].z &= mask;
-            vr[h][j].w &= mask;
-          }
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              uint32_t& v = (&vr[h][j].x)[d];
+              v &= mask;
+              const uint32_t x = not_finite4(v, vs) & some;
+              v &= ~x;
+              drop |= x;
+            }
+          late |= __any(drop != 0);
         }
       }
       float pm = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
@@ -253,6 +271,7 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
     lds.m[wave][lr] = m_run;
     lds.l[wave][lr] = l_run;
   }
+  if (lane == 0) lds.late[wave] = late;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -275,6 +294,22 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
 #pragma unroll
     for (int d = 0; d < kDims; ++d) acc[d] += lds.o[w][r][d0 + d] * wgt;
   }
+  int any_late = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) any_late |= lds.late[w];
+  if (any_late)
+    for (int key = max(pos + 1, page0 * kPage); key < min(pos + r / G + 1, page1 * kPage); ++key) {
+      const int page = table[key / kPage];
+      if (page < 0 || page >= a.num_pages) continue;
+      const long blk = (long)page * Hkv + g;
+      const float vs = a.v_scale[blk];
+      const uint8_t* src = a.v_cache + blk * kKvBlock + (d0 >> 6) * 1024 + key % kPage / 4 * 256 + key % 4;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        const uint32_t c = src[(d0 % 64 + d) * 4];
+        if (not_finite4(c, vs) & 1) acc[d] += __builtin_amdgcn_cvt_f32_fp8(c, 0) * vs;
+      }
+    }
   if (parts == 1) {
     const float inv = M == -INFINITY ? 0.f : 1.0f / L;  // no key at all: zeros
     uint16_t* dst = a.out + ((long)(tok + r / G) * p.Hq + g * G + r % G) * kHD + d0;
@@ -320,6 +355,7 @@ struct TileLds {
   struct {
     uint4 k[kHD / 8][kTileKeys], v[kTilePages][2][kHD];
   } step[tile_ring(kWaves)];
+  int late[kWaves];
 };
 
 template <int kWaves>
@@ -432,13 +468,25 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
       lds.step[buf].k[2 * c + 1][key] = __builtin_bit_cast(uint4, widen8(kr[h].z, kr[h].w, ks[h]));
     }
   };
-  auto mask_v = [&](int page) __attribute__((always_inline)) {  // codes behind the last key may be anything, a NaN too
+  // Codes behind the last key may be anything, a NaN too: zeros.  So with what is not finite among the keys that not
+  // every row sees, for a zero probability times it is no zero: the rows that do see it get it at the end.  A barrier
+  // lies between a step's staging and its use, so also between this wave's note and the end.
+  if (lane == 0) lds.late[wave] = 0;
+  auto mask_v = [&](int page) __attribute__((always_inline)) {
+    uint32_t drop = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t mask = quad_mask(pos + ntok - ((page + v_at) * kPage + 4 * (vq + 2 * h)));
+      const int key = (page + v_at) * kPage + 4 * (vq + 2 * h);
+      const uint32_t mask = quad_mask(pos + ntok - key), some = ~quad_mask(pos + 1 - key);
 #pragma unroll
-      for (int d = 0; d < 2 * kLoads; ++d) vr[h][d] &= mask;
+      for (int d = 0; d < 2 * kLoads; ++d) {
+        vr[h][d] &= mask;
+        const uint32_t x = not_finite4(vr[h][d], vs) & some;
+        vr[h][d] &= ~x;
+        drop |= x;
+      }
     }
+    if (__any(drop != 0) && lane == 0) lds.late[wave] = 1;
   };
   auto store_v = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -528,7 +576,7 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
     asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(l_run));  // not to be put off past the branches
     if (next_key + kTileKeys > all_end || held_next != 15) mask_scores(next, next_key, held_next);
     const int v_page0 = page0 + (n + kAheadV) * kTilePages;
-    if ((v_page0 + kTilePages) * kPage > pos + ntok) mask_v(v_page0);
+    if ((v_page0 + kTilePages) * kPage > pos + 1) mask_v(v_page0);
     output(pa, buf, 0);
     probabilities(s[1], pb, m_use);
     output(pb, buf, 1);
@@ -550,7 +598,7 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
     if (n < kAheadV) {
       load_v();
       const int v_page0 = page0 + n * kTilePages;
-      if ((v_page0 + kTilePages) * kPage > pos + ntok) mask_v(v_page0);
+      if ((v_page0 + kTilePages) * kPage > pos + 1) mask_v(v_page0);
       store_v(n);
     }
   }
@@ -572,6 +620,34 @@ __device__ __forceinline__ void tile_item(const AttnFp8Args& a, int item, int g,
   }
   const float m_run = m_ref;
   l_run = half_sum(l_run);
+  if (page1 * kPage > pos + 1) {  // some of the item's keys are not every row's
+    int any_late = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) any_late |= lds.late[w];
+    const int end = any_late ? min(key_end, page1 * kPage) : 0;
+#pragma unroll 1
+    for (int key = max(pos + 1, page0 * kPage); key < end; ++key) {
+      const int page = table[key / kPage];
+      if (page < 0 || page >= a.num_pages) continue;
+      const long blk = (long)page * Hkv + g;
+      const float scale = a.v_scale[blk];
+      const uint8_t* src = a.v_cache + blk * kKvBlock + key % kPage / 4 * 256 + 16 * 4 * kg;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = 8 * (i >> 2) + (i & 3);  // dims 64 j + 4 (x + 4 kg) .. +4
+          const uint4 c = *(const uint4*)(src + j * 1024 + 16 * x);
+          const uint32_t code[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t u = code[d] >> 8 * (key % 4);
+            const float add = not_finite4(u, scale) & 1 ? __builtin_amdgcn_cvt_f32_fp8(u, 0) * scale : 0.f;
+            o[2 * j + (d >> 1)][i + 8 * (d & 1)] += add;
+          }
+        }
+    }
+  }
   if (!live) return;
   if (parts == 1) {
     const float inv = m_run == -INFINITY ? 0.f : 1.0f / l_run;  // no key at all: zeros

@@ -611,3 +611,54 @@ def test_attention_takes_no_scale_of_a_page_that_no_sequence_has(pkg, dev, bad, 
     s.cache = tuple(torch.from_numpy(a).to(dev) for a in pools)
     s.cache = (s.cache[0].view(FP8), s.cache[1].view(FP8), *s.cache[2:])
     s.check_attention(s.plan())
+
+
+LATE = [
+    ([70], [5], 8, 4, None),             # 10 rows
+    ([9000, 30], [4, 2], 8, 2, None),    # 16 rows, split
+    ([40, 0], [150, 33], 32, 4, None),   # tiles
+    ([3000], [40], 32, 4, None),         # tiles, split
+    ([100], [300], 64, 4, 2100),         # tiles of 256 rows
+]
+
+
+@pytest.mark.parametrize("cached,new,Hq,Hkv,T", LATE)
+def test_attention_nan_reaches_no_earlier_token(pkg, dev, cached, new, Hq, Hkv, T):
+    """A NaN in K or V of a step's own token: in the rows from that token on, of V in its dim alone."""
+    s = Step(pkg, dev, cached, new, Hq, Hkv, seed=43, T=T)
+    q = orc.round_bf16(s.rng.standard_normal((s.T, Hq, D)).astype(np.float32))
+    ref, size = s.attention_ref(q)
+    k, v, lost, G = s.k.copy(), s.v.copy(), np.zeros((s.T, Hq, D), bool), Hq // Hkv
+    for i, n in ((0, new[0] // 2), (len(new) - 1, new[-1] - 1)):
+        t = int(s.ref[2][i]) + n
+        page, slot = divmod(int(s.ref[1][t]), PAGE)
+        v[(page, 0, *kv.v_index(slot, np.array([3, 77])))] = 0x7F, 0xFF
+        k[(page, 1, *kv.k_index(slot, np.array([100])))] = 0x7F
+        rows = slice(t, int(s.ref[2][i + 1]))
+        lost[rows, :G, [[3], [77]]] = True
+        lost[rows, G:2 * G] = True
+    s.cache = (torch.from_numpy(k).to(dev).view(FP8), torch.from_numpy(v).to(dev).view(FP8), *s.cache[2:])
+    check_but(pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, s.plan(), SCALE), ref, size, lost)
+
+
+@pytest.mark.parametrize("cached,new,Hq,Hkv,T", LATE)
+def test_attention_values_past_the_largest_reach_no_earlier_token(pkg, dev, cached, new, Hq, Hkv, T):
+    """A value within half a code of 2^128 is coded as 2^128, which is infinite in 32 bits, and so is an infinity
+    beside it: not to be multiplied by the zero probabilities of the rows before it."""
+    s = Step(pkg, dev, cached, new, Hq, Hkv, seed=44, T=T)
+    t = new[0] // 2
+    k, v = new_kv(s)
+    v[t, 1, 5], v[t, 1, 9] = 3.38e38, -np.inf
+    p = s.plan()
+    pkg.kv_append_fp8(to_bf16(k, dev), to_bf16(v, dev), *s.cache, p)
+    q = orc.round_bf16(s.rng.standard_normal((s.T, Hq, D)).astype(np.float32))
+    with np.errstate(all="ignore"):
+        gk, gv, ks, vs = s.got()
+        clean = kv.unpack(gv, vs, kv.v_index)
+        past = np.abs(clean) >= 2.0 ** 128
+        assert past.sum() == 2
+        ref, size = kv.attention(q, kv.unpack(gk, ks, kv.k_index), np.where(past, 0, clean), s.ref[2], s.ref[0], s.ref[4],
+                                 SCALE)
+    lost, G = np.zeros((s.T, Hq, D), bool), Hq // Hkv
+    lost[t:new[0], G:2 * G, [[5], [9]]] = True
+    check_but(pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, p, SCALE), ref, size, lost)
