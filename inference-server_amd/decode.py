@@ -214,9 +214,9 @@ class DecodeModel:
         self.inv_freq = default_inv_freq(cfg, dev)
         self._graph = None
 
-    def _need_cache(self, kind) -> None:
-        if not isinstance(self.cache, kind):
-            raise TypeError(f"this call needs a {kind.__name__}, the model has a {type(self.cache).__name__}")
+    def _need_fp8_cache(self) -> None:
+        if not isinstance(self.cache, PagedKVCacheFp8):
+            raise TypeError(f"this call needs a PagedKVCacheFp8, the model has a {type(self.cache).__name__}")
 
     def plan(self, cached_lens, new_lens, block_tables, free_pages, num_tokens: int, max_new_tokens: int,
              out: kernels.PagedPlan | None = None) -> kernels.PagedPlan:
@@ -227,7 +227,7 @@ class DecodeModel:
     def run(self, h, plan: kernels.PagedPlan):
         """Every layer on the hidden states [T, hidden] of a plan's rows, over the 8-bit cache; returns theirs after
         the last layer (padding rows: of no use)."""
-        self._need_cache(PagedKVCacheFp8)
+        self._need_fp8_cache()
         for i, w in enumerate(self.layers):
             h = moe_sublayer(w, h, attention_sublayer_fp8(w, h, plan, self.inv_freq, *self.cache.layer(i)))
         return h
@@ -235,7 +235,7 @@ class DecodeModel:
     def capture_run(self, h, cached_lens, new_lens, block_tables, free_pages, max_new_tokens: int):
         """Records a step's plan and ``run`` on copies of the given inputs; returns (graph, static inputs, static
         output, plan).  ``block_tables`` is among the static inputs: a replay enters the new pages there."""
-        self._need_cache(PagedKVCacheFp8)
+        self._need_fp8_cache()
         dev = h.device
         statics = [t.clone() for t in (h, cached_lens, new_lens, block_tables, free_pages)]
         lens = statics[2]
@@ -259,7 +259,8 @@ class DecodeModel:
         return graph, statics, out, plan
 
     def step(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True):
-        self._need_cache(PagedKVCache)
+        if attention and isinstance(self.cache, PagedKVCacheFp8):
+            raise TypeError("step's attention reads a bf16 cache (PagedKVCache), the model has a PagedKVCacheFp8")
         for i, w in enumerate(self.layers):
             o = None
             if attention:
