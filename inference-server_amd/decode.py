@@ -254,7 +254,7 @@ class DecodeModel:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, stream=side):  # a stream of dev, whichever device is the current one
             out, plan = step()
         return graph, statics, out, plan
 
@@ -284,6 +284,6 @@ class DecodeModel:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, stream=side):  # a stream of dev, whichever device is the current one
             out = self.step(*statics, moe=moe, attention=attention)
         return graph, statics, out
