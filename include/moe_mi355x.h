@@ -353,7 +353,7 @@ int moe_mi355x_qk_norm_rope_append_fp8(const void* qkv, const void* q_norm_w, co
  * behind a sequence's last token, a NaN code too, reaches no result; a NaN among its own values reaches the rows from
  * its token on (one of V in its dim alone) and none before it.
  *   q   bf16 [tokens, heads, 128], rows of a token q_stride values apart (a multiple of 8)
- *   out bf16 [tokens, heads, 128]      block_tables as the plan left them      scale finite, > 0
+ *   out bf16 [tokens, heads, 128]      block_tables as the plan left them      scale > 0, scale * log2(e) finite in fp32
  */
 size_t moe_mi355x_paged_attn_fp8_workspace_bytes(const moe_mi355x_plan_shape* shape);
 int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache,

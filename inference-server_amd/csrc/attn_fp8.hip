@@ -832,7 +832,7 @@ extern "C" int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, cons
                                          const moe_mi355x_plan_shape* shape, const void* plan, void* out,
                                          void* workspace, size_t workspace_bytes, void* stream) {
   MOE_RETURN_IF(!plan_shape_ok(shape) || head_dim != kHD || page_size != kPage || num_pages < 0, MOE_ERR_INVALID_ARG);
-  MOE_RETURN_IF(!(scale > 0.f) || !(scale < INFINITY), MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(!(scale > 0.f) || !(scale * kLog2e < INFINITY), MOE_ERR_INVALID_ARG);
   if (shape->tokens == 0) return MOE_OK;
   MOE_RETURN_IF(!q || !k_cache || !v_cache || !k_scale || !v_scale || !plan || !out, MOE_ERR_INVALID_ARG);
   MOE_RETURN_IF(shape->seqs > 0 && !block_tables, MOE_ERR_INVALID_ARG);

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -420,6 +421,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
 K_BLOCK_FP8 = (HEAD_DIM // 16, PAGE_SIZE, 16)                # dim / 16, token, dim % 16
 V_BLOCK_FP8 = (2, PAGE_SIZE // 4, HEAD_DIM // 2, 4)          # dim / 64, token / 4, dim % 64, token % 4
 PLAN_MAX_SEQS, PLAN_MAX_TOKENS, PLAN_MAX_PAGES = 4096, 1 << 18, 1 << 22
+MAX_SCALE = torch.finfo(torch.float32).max / math.log2(math.e)  # of the attention: the kernels take it times log2(e)
 
 
 def _launch(what: str, device: int, entry, *args) -> None:
@@ -658,8 +660,8 @@ def paged_attention_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     heads = plan.sizes[4]
     q_stride = _need_rows(q, "q", plan, heads)
     scale = float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= MAX_SCALE:
+        raise ValueError(f"scale must be positive and at most {MAX_SCALE}, got {scale}")
     out = q.new_empty((plan.sizes[1], heads, HEAD_DIM))
     nws = plan._ws_bytes
     ws = plan.buffer.new_empty(nws // 4) if nws else None

@@ -129,3 +129,18 @@ def test_unpack_tells_the_pools_apart(pkg):
         pkg.unpack_kv_fp8(k, s[:1])
     with pytest.raises(ValueError):
         pkg.unpack_kv_fp8(k.float(), s)
+
+
+def test_attention_refuses_a_scale_past_fp32(pkg, lib):
+    """The kernels work with scale * log2(e): infinite, it would make NaN of a score of 0."""
+    good = (128, 128, 1, 512, 32, 4)
+    n = lib.moe_mi355x_paged_attn_fp8_workspace_bytes(shape(pkg, *good))
+
+    def call(scale, ws):
+        return lib.moe_mi355x_paged_attn_fp8(FAKE, 4096, FAKE, FAKE, FAKE, FAKE, FAKE, 128, 16, 9, scale, shape(pkg, *good),
+                                             FAKE, FAKE, ws, n, None)
+
+    for scale in (2.4e38, 3.4e38):
+        assert call(scale, None) == -1
+    for scale in (2.3e38, 1e-38):  # taken, so the next check answers
+        assert call(scale, None) == -2
