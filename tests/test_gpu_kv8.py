@@ -662,3 +662,53 @@ def test_attention_values_past_the_largest_reach_no_earlier_token(pkg, dev, cach
     lost, G = np.zeros((s.T, Hq, D), bool), Hq // Hkv
     lost[t:new[0], G:2 * G, [[5], [9]]] = True
     check_but(pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, p, SCALE), ref, size, lost)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(9000, 16, 1), (2100, 64, 4), (11000, 12, 4), (9400, 14, 2)])
+def test_attention_large_step_mostly_padding(pkg, dev, T, Hq, Hkv):
+    """A step of a large capacity that holds a chunk and a few single tokens: tiles of 256 rows (of 255 and 252, where
+    the group does not divide them), few enough to be split along their keys."""
+    s = Step(pkg, dev, [3000, 700, 0, 5], [300, 1, 2, 0], Hq, Hkv, seed=45, T=T, max_new=2000)
+    s.check_attention(s.plan())
+
+
+@pytest.mark.parametrize("T,Hq,Hkv", [(600, 32, 4), (2100, 64, 4)])
+def test_attention_decode_steps_under_a_chunks_capacity(pkg, dev, T, Hq, Hkv):
+    """A graph captured for chunks, replayed on 120 decoding sequences alone, then on a chunk with 40 of them, then on
+    nothing: the short items run beside no tiles, beside some, and not at all."""
+    rng = np.random.default_rng(46)
+    B = 120
+    cached = [int(c) for c in rng.integers(1, 1500, B)]
+    s = Step(pkg, dev, cached, [1] * B, Hq, Hkv, seed=46, T=T, max_new=400, width=300, spare=40)
+    held = {}
+
+    def step():
+        held["plan"] = s.plan()
+        held["o"] = pkg.paged_attention_fp8(held["q"], *s.cache, held["plan"], SCALE)
+
+    q = orc.round_bf16(rng.standard_normal((T, Hq, D)).astype(np.float32))
+    held["q"] = to_bf16(q, dev)
+    g_tables = s.g_tables.clone()
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    plan, o = held["plan"], held["o"]
+    for new in ([1] * B, [400] + [1] * 40 + [0] * (B - 41), [0] * B):
+        s.new = new
+        s.ref = kv.plan(s.cached, new, s.tables, s.free, T, s.max_new)
+        s.g_new.copy_(i32(new, dev))
+        s.g_tables.copy_(g_tables)
+        o.fill_(7)
+        graph.replay()
+        s.check_plan(plan)
+        s.check_output(o, q)
+        again = s.plan()
+        assert torch.equal(o, pkg.paged_attention_fp8(held["q"], *s.cache, again, SCALE))
+
+
+@pytest.mark.parametrize("cached,new", [([131000, 100001], [1, 3]), ([100000], [40]), ([120000, 60], [33, 1])])
+def test_attention_far_contexts(pkg, dev, cached, new):
+    s = Step(pkg, dev, cached, new, 16, 1, seed=47)
+    s.check_attention(s.plan())
