@@ -712,3 +712,21 @@ def test_attention_decode_steps_under_a_chunks_capacity(pkg, dev, T, Hq, Hkv):
 def test_attention_far_contexts(pkg, dev, cached, new):
     s = Step(pkg, dev, cached, new, 16, 1, seed=47)
     s.check_attention(s.plan())
+
+
+@pytest.mark.parametrize("cached,new", [*LENS, ([100000, 131000], [3, 1]), ([0, 60000], [700, 500])])
+@pytest.mark.parametrize("Hq,Hkv", [(32, 4), (14, 2), (5, 5)])
+def test_qk_norm_rope_append_keys_to_the_bit(pkg, dev, cached, new, Hq, Hkv):
+    """Codes and scales of K where pages begin and go on, for group sizes and positions other than the above."""
+    s = Step(pkg, dev, cached, new, Hq, Hkv, seed=48, T=sum(new) + 2)
+    x = orc.round_bf16(s.rng.standard_normal((s.T, Hq + 2 * Hkv, D)).astype(np.float32))
+    qw, kw = (orc.round_bf16((1 + 0.3 * s.rng.standard_normal(D)).astype(np.float32)) for _ in range(2))
+    inv_freq = (1e6 ** (-np.arange(0, D, 2) / D)).astype(np.float32)
+    pkg.qk_norm_rope_append_fp8(to_bf16(x.reshape(s.T, -1), dev), to_bf16(qw, dev), to_bf16(kw, dev),
+                                torch.from_numpy(inv_freq).to(dev), Hq, Hkv, 1e-6, *s.cache, s.plan())
+    k, _ = kv.norm_rope(x[:, Hq:Hq + Hkv], kw, inv_freq, s.ref[0], float(np.float32(1e-6)))
+    ek, eks = s.k.copy(), s.ks.copy()
+    kv.append(k, s.ref[1], s.ref[0], ek, eks, kv.k_index)
+    gk, _, gks, _ = s.got()
+    assert np.array_equal(gks, eks)
+    assert np.array_equal(gk & 127, ek & 127) and np.array_equal(gk[(ek & 127) != 0], ek[(ek & 127) != 0])
