@@ -610,7 +610,8 @@ def test_attention_takes_no_scale_of_a_page_that_no_sequence_has(pkg, dev, bad, 
         a[~np.isin(np.arange(len(a)), own)] = bad
     s.cache = tuple(torch.from_numpy(a).to(dev) for a in pools)
     s.cache = (s.cache[0].view(FP8), s.cache[1].view(FP8), *s.cache[2:])
-    s.check_attention(s.plan())
+    with np.errstate(invalid="ignore"):  # the oracle unpacks these pages, too
+        s.check_attention(s.plan())
 
 
 LATE = [
