@@ -24,7 +24,8 @@ constexpr int kPage = kPlanPage;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCachePolicyNT = 2;  // the instruction's cache-policy field: nt (streaming)
 constexpr int kPadBlocks = 8;      // workgroups that clear the rows behind the last sequence
-constexpr int kMergeBlocks = 512;  // of each row, where a step has tiles: mostly nothing is split then
+constexpr int kMergeBlocks = 512;  // for each of 16 rows, where a step has tiles.  Mostly nothing is split then: 4.6 us
+                                   // for the 8192 workgroups to find that
 constexpr int kMergeFew = 8;       // items of a row that one group of the merge takes alone
 constexpr int kFewItems = 256;     // one per CU
 constexpr float kSlack = 8.f;      // log2 of what an unnormalised probability may reach

@@ -15,7 +15,9 @@
 // it is rounded to 32: at position 10^5 a 32-bit product is off by up to 0.004.  Those of k, of which there are few
 // rows, are in 64 bits throughout: in 32, two to eight codes of 4 million fell on the other side of a tie, each 2^-4 of
 // its value away (8178 tokens, 64 / 4 heads: 54.4 -> 56.1 us; 16 tokens alike, 4.6).
-// Memory bound for prompts (512 B read and 256 B written per token and kv head, 512 B per token and q head).
+// HBM bound for long prompts with q (512 B read and 256 B written per token and kv head, 512 B per token and q head:
+// 5.2 TB/s for 8178 tokens, 64 / 4 heads).  K and V alone are too few bytes for that: 4499 tokens, 4 kv heads, take
+// 5.8 us at 2.4 TB/s, for a wave's one chain of record, rows, maximum and stores.
 #include "kv_fp8.h"
 #include "paged_plan.h"
 
