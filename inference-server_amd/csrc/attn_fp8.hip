@@ -2,10 +2,9 @@
 // single tokens (paged_plan.h): for token t of a sequence at position p, query head h and kv head h / G,
 //   o = sum_{j <= p} softmax_j(scale q . K_j) V_j
 // with K and V the values that the codes stand for, everything in fp32 but for two operands: the bf16 q, and
-// the probabilities, rounded to bf16 (by 2^-8 at most) for the second MFMA; the tiles sum them as rounded, so that
-// a row that one key dominates is exact, the short items before it.  The codes become bf16 exactly
-// (v_cvt_scalef32_pk_bf16_fp8 with the page's power-of-two scale), so both products run on the bf16 MFMAs without a
-// further error.
+// the probabilities, rounded to bf16 (by 2^-8 at most) for the second MFMA and summed as rounded, so that the value of
+// a key that dominates its row comes out exact.  The codes become bf16 exactly (v_cvt_scalef32_pk_bf16_fp8 with the
+// page's power-of-two scale), so both products run on the bf16 MFMAs without a further error.
 //
 // Two forms, by the rows (tokens x heads of the group) that a sequence has for one kv head:
 //   short: up to 16 rows (a decoding sequence), bound by the cache's bytes.  One workgroup per (sequence, kv
@@ -245,17 +244,17 @@ __device__ __forceinline__ void short_item(const AttnFp8Args& a, int item, int g
         for (int d = 0; d < 8; ++d) o[d] *= corr;
       }
       const float m_ref = m_run == -INFINITY ? 0.f : m_run;
-      float ps = 0.f;
       v8bf pb;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(sv[h][e] - m_ref);
-          ps += x;
-          pb[4 * h + e] = (__bf16)x;
+        for (int e = 0; e < 4; e += 2) {
+          const v2bf x = {(__bf16)__builtin_amdgcn_exp2f(sv[h][e] - m_ref), (__bf16)__builtin_amdgcn_exp2f(sv[h][e + 1] - m_ref)};
+          pb[4 * h + e] = x[0];
+          pb[4 * h + e + 1] = x[1];
+          // this lane's keys, as the second product sees them; the row's lanes are summed at the end
+          l_run = __builtin_amdgcn_fdot2_f32_bf16(x, (v2bf){(__bf16)1.f, (__bf16)1.f}, l_run, false);
         }
-      l_run += ps;  // this lane's keys; the row's lanes are summed at the end
       const float vs0 = scale_at(my_vs, i, 0), vs1 = scale_at(my_vs, i, 1);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

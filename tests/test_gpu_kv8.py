@@ -731,3 +731,33 @@ def test_qk_norm_rope_append_keys_to_the_bit(pkg, dev, cached, new, Hq, Hkv):
     gk, _, gks, _ = s.got()
     assert np.array_equal(gks, eks)
     assert np.array_equal(gk & 127, ek & 127) and np.array_equal(gk[(ek & 127) != 0], ek[(ek & 127) != 0])
+
+
+@pytest.mark.parametrize("cached,new", [([300, 420, 900], [1, 1, 2]), ([6000, 2000], [1, 1]), ([300], [40])])
+def test_attention_of_one_key_is_its_value(pkg, dev, cached, new):
+    """Rows of which one key has almost all the weight, a probability that bf16 does not hold: the sum has to be of the
+    probabilities as they are multiplied, so that the rounding cancels.  |sum p d (v - o)| <= 2^-8 sum p |v - o|, the mean
+    distance, which is at most the standard deviation of V under p (5% more as in the module's bound), and the output's
+    rounding; no 2^-8 of the value itself for p."""
+    H = 8
+    s = Step(pkg, dev, cached, new, H, H, seed=49)
+    sign = np.where(s.rng.integers(0, 2, (H, D)) > 0, 1.0, -1.0)
+    steps = np.array([0.28125, 0.3125, 0.34375, 0.375, 0.40625, 0.4375, 0.46875, 0.25])  # 4 to 7.7 in the power of 2
+    s.ks[:] = 1
+    for b in range(len(cached)):
+        c = np.full((s.width * PAGE, H), -2.0)
+        c[0], c[256 + 3] = 0, steps  # of one wave, the second after the first has set what the others are measured by
+        for j, page in enumerate(s.ref[4][b]):
+            for slot in range(PAGE if page >= 0 else 0):
+                row = kv.to_e4m3(c[j * PAGE + slot][:, None] * sign).T
+                s.k[(page, slice(None), *kv.k_index(slot, np.arange(D)))] = row
+    s.cache = (torch.from_numpy(s.k).to(dev).view(FP8), s.cache[1], torch.from_numpy(s.ks).to(dev), s.cache[3])
+    q = np.broadcast_to(sign, (s.T, H, D)).astype(np.float32)
+    k, v, ks, vs = s.got()
+    k, v = kv.unpack(k, ks, kv.k_index), kv.unpack(v, vs, kv.v_index)
+    ref, size = kv.attention(q, k, v, s.ref[2], s.ref[0], s.ref[4], SCALE)
+    square, _ = kv.attention(q, k, v * v, s.ref[2], s.ref[0], s.ref[4], SCALE)
+    apart = np.sqrt(np.maximum(square - ref * ref, 0))
+    got = pkg.paged_attention_fp8(to_bf16(q, dev), *s.cache, s.plan(), SCALE).float().cpu().numpy()
+    worst = np.abs(got - ref) - 2.0 ** -8 * (1.05 * apart + np.abs(ref)) - 2.0 ** -16 * (size + np.abs(ref))
+    assert (worst <= 1e-30).all(), (worst.max(), np.argwhere(worst > 0)[:4])
