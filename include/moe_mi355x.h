@@ -362,6 +362,52 @@ int moe_mi355x_paged_attn_fp8(const void* q, long long q_stride, const void* k_c
                               const void* plan, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Low-rank adapters of many requests at once.  The plan of a step's rows by adapter, built on the GPU from the
+ * adapters' numbers: a stable sort of the T rows, those without an adapter (a number outside [0, L)) last.  No
+ * counterpart in the reference.
+ *   adapter_ids  int32 [T], a number for each row; with cu_rows, [seqs], for each sequence
+ *   cu_rows      int32 [seqs + 1] or NULL: sequence b has the rows cu_rows[b] .. cu_rows[b + 1] (ascending; the cu of a
+ *                moe_mi355x_paged_plan serves); rows of no sequence have no adapter
+ *   plan         lora_plan_bytes(T, L) bytes, 16-byte aligned; read by moe_mi355x_lora_add for the same T and L
+ * lora_plan_bytes returns 0 for unsupported sizes, and puts (offsets not null) the positions, in int32 from the plan's
+ * start, of: the first entry of each adapter, of the rows without one, and T [L + 2]; the sorted rows [T].
+ * 0 <= T <= 262144, 1 <= L <= 256, seqs <= 4096.
+ */
+size_t moe_mi355x_lora_plan_bytes(int T, int L, int32_t* offsets);
+int moe_mi355x_lora_plan(const int32_t* adapter_ids, const int32_t* cu_rows, int seqs, int T, int L, void* plan,
+                         size_t plan_bytes, void* stream);
+
+/*
+ * What the rows' adapters add to a shared projection, in place: for row t with adapter l, column n in part p of the
+ * projection (the q, k and v of a fused one are its parts; columns[p] columns each), r < min(ranks[l], R):
+ *   u = sum_k x[t, k] a[l, p R + r, k]      y[t, n] = bf16( y[t, n] + scales[l] sum_r u[t, p, r] b[l, n, r] )
+ * with fp32 sums, u kept to 2^-17 of its value, one rounding.  Rows without an adapter, and with one of rank 0 or less,
+ * are left as they are; what a and b hold past an adapter's rank reaches nothing.
+ *   y bf16 [T, N], N = sum of columns, and x bf16 [T, K]; rows y_stride and x_stride values apart (multiples of 8)
+ *   a bf16 [L, parts R, K]    b bf16 [L, N, R]    ranks int32 [L]    scales fp32 [L]    columns: host array [parts]
+ * K % 32 == 0, R % 16 == 0, R <= 128, 1 <= parts <= 4, columns[p] % 32 == 0; x and y must not overlap.
+ */
+int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, long long x_stride, const void* a, const void* b,
+                        const int32_t* ranks, const float* scales, const void* plan, int T, int L, int K, int R, int parts,
+                        const int* columns, void* stream);
+
+/*
+ * Log probabilities of given tokens, with entropy and the k most likely tokens, of T rows of logits:
+ *   logprobs[t] = log softmax(logits[t])[tokens[t]]     entropy[t] = -sum p log p     (0 log 0 = 0)
+ *   top_ids, top_logprobs [t, k]: the k largest logits' indices and logprobs, descending, lower index first among
+ *   equals, a NaN above everything
+ * A negative token asks for nothing: 0; one of V or more gives NaN.  A row with a NaN or a +inf, or with nothing but -inf,
+ * has NaN for logprobs and entropy.  fp32 sums.  No counterpart in the reference.
+ *   logits  bf16 (dtype 0) or fp32 (1) [T, V], rows `stride` values apart    tokens [T] (id_bytes 4 or 8) or NULL, then
+ *   logprobs may be NULL    entropy fp32 [T]    top_ids int64, top_logprobs fp32 [T, k] (k 0: may be NULL)
+ * 1 <= V, 0 <= k <= min(V, 64), T < 2^24.
+ */
+size_t moe_mi355x_token_logprobs_workspace_bytes(int T, int V, int k);
+int moe_mi355x_token_logprobs(const void* logits, int dtype, long long stride, const void* tokens, int id_bytes, int T,
+                              int V, int k, float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing (instrumentation; no counterpart in the reference).  While enabled, each
  * kernel launch of this library is bracketed by hipEvents on its stream; profile_read
  * waits for them and returns the launch count and summed duration (ms) of one slot:

@@ -28,12 +28,17 @@ from .experts import (  # noqa: F401
     swap_moe_blocks,
 )
 from .kernels import (  # noqa: F401
+    LoraPlan,
+    LoraPool,
     PagedPlan,
+    TokenLogprobs,
     align,
     experts_bf16,
     experts_fp8,
     kv_append,
     kv_append_fp8,
+    lora_add,
+    lora_plan,
     moe_block_bf16,
     moe_block_fp8,
     moe_sublayer_fp8,
@@ -47,6 +52,7 @@ from .kernels import (  # noqa: F401
     quantize_act_fp8,
     quantize_weight_fp8,
     route,
+    token_logprobs,
     topk_softmax,
     unpack_kv_fp8,
 )

@@ -82,6 +82,13 @@ SIGNATURES = {
     "moe_mi355x_paged_attn_fp8_workspace_bytes": (_c_size, [_shape]),
     "moe_mi355x_paged_attn_fp8": (_c_int, [_vp, _c_ll, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int,
                                            ctypes.c_float, _shape, _vp, _vp, _vp, _c_size, _vp]),
+    "moe_mi355x_lora_plan_bytes": (_c_size, [_c_int, _c_int, _vp]),
+    "moe_mi355x_lora_plan": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
+    "moe_mi355x_lora_add": (_c_int, [_vp, _c_ll, _vp, _c_ll, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
+                                     _c_int, _vp, _vp]),
+    "moe_mi355x_token_logprobs_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "moe_mi355x_token_logprobs": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp,
+                                           _vp, _c_size, _vp]),
     "moe_mi355x_profile_enable": (_c_int, [_c_int]),
     "moe_mi355x_profile_read": (_c_int, [_c_int, ctypes.POINTER(_c_int), ctypes.POINTER(ctypes.c_double)]),
     "moe_mi355x_profile_slot_name": (ctypes.c_char_p, [_c_int]),

@@ -1,0 +1,470 @@
+// Log probabilities of given tokens, entropy and the most likely tokens of rows of logits (the softmax that ends a
+// step, beside the router's in route.hip): for row x[0 .. V) and token g,
+//   m = max x, Z = sum e^(x - m)      logprob = x[g] - m - ln Z      entropy = ln Z - (1 / Z) sum e^(x - m) (x - m)
+// and the k largest by (value, lower index first) with their logprobs.
+//
+// One pass over the logits, bound by their bytes and, for bf16, nearly by the vector unit (an exponential takes four
+// of the about nine issue slots that a value costs).  A wave keeps a reference near its maximum instead of the
+// maximum: the sums are scaled only where a value passes it by 2^8, which after the first values happens rarely.
+//
+// The largest are found on the way.  Each lane's running maximum gives a bound: where j lanes of each of the four waves
+// have seen a value of at least b, with 4 j >= k, the k largest are all >= b.  The bound is renewed at doubling
+// distances, so that a few hundred values of a row pass it; those are kept in LDS, cut down to the k largest if they get
+// many, and sorted at the end by counting.
+//
+// Few rows are split over workgroups, whose sums and lists a second kernel joins.  Rows with NaN, +inf or with
+// nothing but values near the type's lowest are gone over again by a plainer scan.
+#include "common.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / MOE_WAVE;
+constexpr int kMaxTop = 64;
+constexpr int kBuf = 1024;     // candidates that a wave keeps
+constexpr int kKeep = 256;     // ... after they are cut down, at most
+constexpr int kMaxSplits = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 5.5f;  // 8 ln 2: what a value may be above the reference
+constexpr float kNoTerm = -200.f;  // log2 of a term that is zero in fp32, in the place of -inf times zero
+
+struct LpArgs {
+  const void* x;  // [T][V], rows `stride` values apart
+  long stride;
+  const void* tokens;  // [T] or null
+  int id_bytes;
+  int T, V, k, splits;
+  float *logprobs, *entropy;  // [T]
+  int64_t* top_ids;           // [T][k]
+  float* top_logprobs;        // [T][k]
+  float4* sums;               // [T][splits] {m, s, t, -}
+  uint64_t* keys;             // [T][splits][k]
+};
+
+// Values as whole numbers of the same order; -0 as 0, NaN above all.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = x != x ? 0x7fc00000u : __float_as_uint(x + 0.f);
+  return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  return __uint_as_float(o ^ ((uint32_t)((int)~o >> 31) | 0x80000000u));
+}
+// The larger the better: the value, then the lower index.  No key of a value is 0.
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+  return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)index);
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
+__device__ __forceinline__ float value_of(uint64_t key) { return from_ordered((uint32_t)(key >> 32)); }
+
+__device__ __forceinline__ void unpack(uint4 r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(uint4 r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ float value_at(const uint16_t* x, long i) { return bf16_to_f32(x[i]); }
+__device__ __forceinline__ float value_at(const float* x, long i) { return x[i]; }
+
+// s = sum 2^((x - m) log2 e), t = sum of each times its exponent, for one reference m
+struct Sums {
+  float m, s, t;
+};
+// b's sums added to a's, under the larger reference (-inf: no value yet)
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  auto under = [&](Sums v) {
+    const float d = v.m == m ? 0.f : fmaxf((v.m - m) * kLog2e, kNoTerm);
+    const float c = v.m == m ? 1.f : __builtin_amdgcn_exp2f((v.m - m) * kLog2e);
+    return Sums{m, v.s * c, fmaf(v.s, d, v.t) * c};
+  };
+  const Sums x = under(a), y = under(b);
+  return Sums{m, x.s + y.s, x.t + y.t};
+}
+__device__ __forceinline__ Sums join_wave(Sums v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.t, d)});
+  return v;
+}
+
+// From a row's sums to its results
+struct Row {
+  double m, ln_z;
+  float entropy;
+};
+__device__ __forceinline__ Row row_of(Sums v) {
+  const float m = v.m == -INFINITY ? 0.f : v.m;
+  const double ln_z = log((double)v.s);
+  return Row{(double)m, ln_z, (float)(ln_z - 0.69314718055994530942 * ((double)v.t / (double)v.s))};
+}
+__device__ __forceinline__ float logprob(const Row& r, float x) { return (float)((double)x - r.m - r.ln_z); }
+
+// Entropy and the given token's logprob, by one thread
+template <typename E>
+__device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r) {
+  a.entropy[row] = r.entropy;
+  if (!a.tokens) return;
+  const int64_t g = a.id_bytes == 8 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
+  a.logprobs[row] = g < 0 ? 0.f : g < a.V ? logprob(r, value_at((const E*)a.x + row * a.stride, g)) : NAN;
+}
+
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return ~wave_max_u32_uniform(~v); }
+
+// A bound that at least n of the wave's 64 values reach, close to the n-th largest
+__device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
+  uint32_t lo = wave_min_u32(mine), hi = wave_max_u32_uniform(mine);
+#pragma unroll 1
+  for (int i = 0; i < 14 && lo < hi; ++i) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    if (__popcll(__ballot(mine >= mid)) >= n) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+struct TopLds {
+  uint64_t buf[kWaves][kBuf];
+  uint32_t bound[kWaves];
+  int count;
+};
+
+// A wave's candidates
+struct Top {
+  uint64_t* buf;
+  int count;          // wave-uniform
+  uint64_t least;     // keys below are not among the k largest; wave-uniform
+  float least_value;
+  uint32_t lane_max;  // ordered
+};
+
+__device__ __forceinline__ void raise(Top& t, uint64_t least) {
+  if (least > t.least) {
+    t.least = least;
+    t.least_value = value_of(least);
+  }
+}
+
+// Cuts the candidates down to between k and kKeep (all k of them where they are fewer).
+__device__ __forceinline__ void cut(Top& t, int k, int lane) {
+  constexpr int kPer = kBuf / MOE_WAVE;
+  uint64_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = i * MOE_WAVE + lane;
+    key[i] = at < t.count ? t.buf[at] : 0;
+  }
+  uint64_t lo = t.least, hi = ~0ull;  // at least k keys are >= lo, fewer than k are > hi
+#pragma unroll 1
+  while (lo < hi) {
+    const uint64_t mid = lo + (hi - lo) / 2 + 1;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) n += __popcll(__ballot(key[i] >= mid));
+    if (n >= k) {
+      lo = mid;
+      if (n <= kKeep) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  raise(t, lo);
+  t.count = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool keep = key[i] >= lo && key[i] != 0;
+    const uint64_t mask = __ballot(keep);
+    if (keep) t.buf[t.count + __popcll(mask & lanemask_lt())] = key[i];
+    t.count += __popcll(mask);
+  }
+}
+
+__device__ __forceinline__ void offer(Top& t, float x, int index, bool valid, int lane) {
+  const uint64_t key = key_of(x, index);
+  const bool pass = valid && key >= t.least;
+  const uint64_t mask = __ballot(pass);
+  if (mask == 0) return;
+  if (pass) t.buf[t.count + __popcll(mask & lanemask_lt())] = key;
+  t.count += __popcll(mask);
+}
+
+template <typename E, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
+  constexpr int kVec = 16 / sizeof(E);
+  constexpr int kRoom = kBuf - MOE_WAVE * kVec;  // more candidates than this are cut down before the next values
+  __shared__ TopLds lds;
+  __shared__ Sums s_sums[kWaves];
+  __shared__ float s_max[kWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const E* x = (const E*)a.x + row * a.stride;
+  // values in front of the first 16-byte boundary, vectors, values behind the last
+  const int head = min(a.V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(E));
+  const int vecs = (a.V - head) / kVec;
+  const int per = (vecs + a.splits - 1) / a.splits;
+  const int v0 = min(split * per, vecs), v1 = min(v0 + per, vecs);
+  const uint4* xv = (const uint4*)(x + head);
+  // the first and the last workgroup of a row take its edges too, their first wave a lane each
+  const int tail0 = head + vecs * kVec;
+  const int n_head = split == 0 ? head : 0, n_edge = wave == 0 ? n_head + (split == a.splits - 1 ? a.V - tail0 : 0) : 0;
+  const int edge = lane < n_head ? lane : tail0 + lane - n_head;
+  const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
+  const int per_wave = (a.k + kWaves - 1) / kWaves;
+
+  Top top{lds.buf[wave], 0, 0, -INFINITY, 0};
+  float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
+  auto reference = [&](float pm) __attribute__((always_inline)) {
+    if (__any(pm > limit)) {
+      const float old = m2;
+      const bool first = m == -INFINITY;
+      m = wave_max_uniform(fmaxf(m, pm));
+      m2 = m * kLog2e;
+      limit = m + kSlack;
+      const float d = old - m2, c = __builtin_amdgcn_exp2f(d);
+      t = first ? 0.f : fmaf(s, d, t) * c;
+      s = first ? 0.f : s * c;
+    }
+  };
+  auto add = [&](float v) __attribute__((always_inline)) {
+    const float d = fmaf(v, kLog2e, -m2), e = __builtin_amdgcn_exp2f(d);
+    s += e;
+    t = fmaf(e, fmaxf(d, kNoTerm), t);
+  };
+  auto renew = [&]() __attribute__((always_inline)) {
+    const uint32_t b = bound_of(top.lane_max, per_wave);
+    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = b;
+  };
+  auto take_bound = [&]() __attribute__((always_inline)) {
+    uint32_t b = ~0u;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
+    raise(top, (uint64_t)__builtin_amdgcn_readfirstlane(b) << 32);
+  };
+
+  // the edges, then a first vector to have a bound to go by
+  if (TOP) top.lane_max = lane < n_edge ? ordered(edge_value) : 0;
+  reference(edge_value);
+  add(edge_value);
+  int i = v0 + wave * MOE_WAVE + lane, turn = 0;
+  for (int i0 = v0 + wave * MOE_WAVE; i0 < v1 || turn == 0; i0 += kThreads, i += kThreads, ++turn) {
+    float v[kVec];
+    if (i < v1) {
+      unpack(xv[i], v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
+    }
+    float pm = v[0];
+#pragma unroll
+    for (int e = 1; e < kVec; ++e) pm = fmaxf(pm, v[e]);
+    reference(pm);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) add(v[e]);
+    if (TOP) {
+      if (i < v1) top.lane_max = max(top.lane_max, ordered(pm));
+      if ((turn & (turn + 1)) == 0) {
+        renew();
+        if (turn == 0) {
+          __syncthreads();
+          take_bound();
+          offer(top, edge_value, edge, lane < n_edge, lane);
+        } else {
+          take_bound();
+        }
+      }
+      if (__any(!(pm < top.least_value))) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) offer(top, v[e], head + i * kVec + e, i < v1, lane);
+        if (top.count > kRoom) cut(top, a.k, lane);
+      }
+    }
+  }
+  // from the reference as the sums used it, m log2(e) rounded, to m itself
+  const float off = m == -INFINITY ? 0.f : fmaf(m, kLog2e, -m2), undo = __builtin_amdgcn_exp2f(-off);
+  Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
+
+  // NaN, +inf, or a reference so far out that its product with log2(e) is infinite: again, from the maximum
+  if (lane == 0) s_max[wave] = m;
+  const bool odd = __any(!(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < INFINITY));
+  if (__syncthreads_or(odd)) {
+    m = s_max[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_max[w]);
+    s = t = 0.f;
+    const float ref = m == -INFINITY ? 0.f : m;
+    top.count = 0, top.least = 0, top.least_value = -INFINITY;
+    auto again = [&](float v) __attribute__((always_inline)) {
+      const float d = (v - ref) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+      s += e;
+      t = fmaf(e, fmaxf(d, kNoTerm), t);
+    };
+    again(edge_value);
+    if (TOP) offer(top, edge_value, edge, lane < n_edge, lane);
+    for (int i0 = v0 + wave * MOE_WAVE; i0 < v1; i0 += kThreads) {
+      const int j = i0 + lane;
+#pragma unroll 1
+      for (int e = 0; e < kVec; ++e) {
+        const float v = j < v1 ? value_at(x, head + (long)j * kVec + e) : -INFINITY;
+        again(v);
+        if (TOP) offer(top, v, head + j * kVec + e, j < v1, lane);
+      }
+      if (TOP && top.count > kRoom) cut(top, a.k, lane);
+    }
+    sum = Sums{m, s, t};
+    if (TOP) {
+      top.lane_max = 0;  // the bound of the first scan is not one of NaN's order
+      if (lane == 0) lds.bound[wave] = 0;
+    }
+  } else if (TOP) {
+    renew();
+  }
+  sum = join_wave(sum);
+  if (lane == 0) s_sums[wave] = sum;
+  if (TOP && top.count > kKeep) cut(top, a.k, lane);
+  if (threadIdx.x == 0) lds.count = 0;
+  __syncthreads();
+  sum = s_sums[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) sum = join(sum, s_sums[w]);
+  Row r{};
+  if (a.splits == 1) r = row_of(sum);
+
+  if (TOP) {  // the waves' candidates in one list, in registers meanwhile: it takes the place of their buffers
+    take_bound();
+    constexpr int kPer = kKeep / MOE_WAVE;
+    uint64_t key[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int at = j * MOE_WAVE + lane;
+      key[j] = at < top.count ? top.buf[at] : 0;
+    }
+    __syncthreads();
+    uint64_t* list = lds.buf[0];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (key[j] >= top.least && key[j] != 0) list[atomicAdd(&lds.count, 1)] = key[j];
+    __syncthreads();
+    const int n = lds.count;
+    uint64_t* out = a.splits > 1 ? a.keys + (long)blockIdx.x * a.k : nullptr;
+    if (out)  // a short split has fewer
+      for (int j = n + threadIdx.x; j < a.k; j += kThreads) out[j] = 0;
+    for (int j = threadIdx.x; j < n; j += kThreads) {
+      const uint64_t mine = list[j];
+      int rank = 0;
+      for (int o = 0; o < n; ++o) rank += list[o] > mine;
+      if (rank >= a.k) continue;
+      if (out) {
+        out[rank] = mine;
+      } else {
+        a.top_ids[(long)row * a.k + rank] = index_of(mine);
+        a.top_logprobs[(long)row * a.k + rank] = logprob(r, value_of(mine));
+      }
+    }
+  }
+  if (threadIdx.x != 0) return;
+  if (a.splits > 1) {
+    a.sums[blockIdx.x] = make_float4(sum.m, sum.s, sum.t, 0.f);
+    return;
+  }
+  finish<E>(a, row, r);
+}
+
+// Joins a row's splits: their sums, and the k largest of their lists
+template <typename E>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
+  __shared__ uint64_t list[kMaxSplits * kMaxTop];
+  __shared__ int s_count;
+  const int row = blockIdx.x, lane = threadIdx.x & 63;
+  const float4* parts = a.sums + (long)row * a.splits;
+  const uint64_t* keys = a.keys + (long)row * a.splits * a.k;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  const float4 v = lane < a.splits ? parts[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  const Row r = row_of(join_wave(Sums{v.x, v.y, v.z}));
+  if (a.k > 0) {
+    uint64_t least = lane < a.splits ? keys[(long)lane * a.k + a.k - 1] : 0;  // some split has k keys from here on
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      const uint64_t o = (uint64_t)__shfl_xor((long long)least, d);
+      least = o > least ? o : least;
+    }
+    for (int i = threadIdx.x; i < a.splits * a.k; i += kThreads) {
+      const uint64_t key = keys[i];
+      if (key >= least && key != 0) list[atomicAdd(&s_count, 1)] = key;
+    }
+    __syncthreads();
+    const int n = s_count;
+    for (int j = threadIdx.x; j < n; j += kThreads) {
+      const uint64_t mine = list[j];
+      int rank = 0;
+      for (int o = 0; o < n; ++o) rank += list[o] > mine;
+      if (rank >= a.k) continue;
+      a.top_ids[(long)row * a.k + rank] = index_of(mine);
+      a.top_logprobs[(long)row * a.k + rank] = logprob(r, value_of(mine));
+    }
+  }
+  if (threadIdx.x != 0) return;
+  finish<E>(a, row, r);
+}
+
+bool lp_ok(int T, int V, int k) { return T >= 0 && V >= 1 && k >= 0 && k <= kMaxTop && k <= V && T < (1 << 24); }
+
+// Workgroups of a row
+int lp_splits(int T, int V) {
+  const int most = (V + 4095) / 4096, want = (1024 + T - 1) / (T > 0 ? T : 1);
+  const int n = want < most ? want : most;
+  return n < 1 ? 1 : n < kMaxSplits ? n : kMaxSplits;
+}
+
+size_t lp_carve(WsCarver& c, int T, int k, int splits, LpArgs* a) {
+  if (splits > 1) {
+    a->sums = c.take<float4>((size_t)T * splits);
+    a->keys = c.take<uint64_t>((size_t)T * splits * k);
+  }
+  return moe_align_up(c.off, 256);
+}
+
+template <typename E>
+int lp_launch(const LpArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((long)a.T * a.splits));
+  if (a.k > 0)
+    hipLaunchKernelGGL((logprobs_kernel<E, true>), grid, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((logprobs_kernel<E, false>), grid, dim3(kThreads), 0, s, a);
+  MOE_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((logprobs_join_kernel<E>), dim3((unsigned)a.T), dim3(kThreads), 0, s, a);
+    MOE_CHECK_LAUNCH();
+  }
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" size_t moe_mi355x_token_logprobs_workspace_bytes(int T, int V, int k) {
+  if (!lp_ok(T, V, k)) return 0;
+  WsCarver c(nullptr);
+  LpArgs a{};
+  return lp_carve(c, T, k, lp_splits(T, V), &a);
+}
+
+extern "C" int moe_mi355x_token_logprobs(const void* logits, int dtype, long long stride, const void* tokens, int id_bytes,
+                                         int T, int V, int k, float* logprobs, float* entropy, int64_t* top_ids,
+                                         float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream) {
+  MOE_RETURN_IF(!lp_ok(T, V, k) || (dtype != 0 && dtype != 1) || stride < V || (id_bytes != 4 && id_bytes != 8), MOE_ERR_INVALID_ARG);
+  if (T == 0) return MOE_OK;
+  MOE_RETURN_IF(!logits || !entropy || (tokens && !logprobs) || (k > 0 && (!top_ids || !top_logprobs)), MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF((uintptr_t)logits % (dtype == 0 ? 2 : 4), MOE_ERR_ALIGNMENT);
+  const size_t need = moe_mi355x_token_logprobs_workspace_bytes(T, V, k);
+  MOE_RETURN_IF(need > 0 && (!workspace || workspace_bytes < need), MOE_ERR_WORKSPACE);
+  MOE_RETURN_IF(need > 0 && !moe_aligned16(workspace), MOE_ERR_ALIGNMENT);
+  LpArgs a{};
+  a.x = logits, a.stride = stride, a.tokens = tokens, a.id_bytes = id_bytes, a.T = T, a.V = V, a.k = k, a.splits = lp_splits(T, V);
+  a.logprobs = logprobs, a.entropy = entropy, a.top_ids = top_ids, a.top_logprobs = top_logprobs;
+  WsCarver c(workspace);
+  lp_carve(c, T, k, a.splits, &a);
+  return dtype == 0 ? lp_launch<uint16_t>(a, (hipStream_t)stream) : lp_launch<float>(a, (hipStream_t)stream);
+}

@@ -1,0 +1,158 @@
+// moe_mi355x_lora_plan: a step's rows sorted by their adapter, stably, and cut into tiles (lora.h), on the GPU from
+// the adapters' numbers alone.
+//
+// A counting sort in one launch.  Each workgroup places 1024 rows; where they go it works out by itself, from
+// counts over all rows (by sequence, where the numbers are the sequences'), which costs less than a second launch.
+// Within a wave the rows of one adapter find each other by the bits of its number (9 ballots), so that neither the
+// order nor the time depends on atomics or on how many adapters meet.
+#include "lora.h"
+
+namespace {
+
+constexpr int kThreads = 1024, kWaves = kThreads / MOE_WAVE;
+constexpr int kBins = kLoraMaxAdapters + 1;  // the last one used: rows without an adapter
+constexpr int kPerLane = (kBins + MOE_WAVE - 1) / MOE_WAVE;
+
+struct LoraPlanArgs {
+  const int32_t *ids, *cu;  // ids [seqs] with cu [seqs + 1], else [T]
+  int seqs;
+  int32_t* plan;
+  LoraLayout p;
+};
+
+// The lanes whose bin is this one's, among those with `live`.
+__device__ __forceinline__ uint64_t same_bin(int bin, bool live) {
+  uint64_t same = __ballot(live);
+#pragma unroll
+  for (int bit = 0; bit < 9; ++bit) {
+    const bool one = (bin >> bit) & 1;
+    const uint64_t with = __ballot(one);
+    same &= one ? with : ~with;
+  }
+  return same;
+}
+
+__global__ __launch_bounds__(kThreads) void lora_plan_kernel(LoraPlanArgs a) {
+  __shared__ int s_cu[kLoraMaxSeqs + 1];
+  __shared__ int s_total[kBins], s_before[kBins];  // rows of each adapter: all, and those in front of this workgroup's
+  __shared__ int s_wave[kWaves][kBins];
+  __shared__ int s_first[kBins + 1], s_tile[kBins + 1];
+  const LoraLayout& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int T = p.T, L = p.L, bins = L + 1;
+  const int row0 = blockIdx.x * kThreads, row = row0 + tid;
+  auto bin_of = [&](int id) { return id >= 0 && id < L ? id : L; };
+
+  for (int i = tid; i < bins; i += kThreads) s_total[i] = s_before[i] = 0;
+  for (int i = tid; i < kWaves * kBins; i += kThreads) (&s_wave[0][0])[i] = 0;
+  int bin = L;
+  if (a.cu) {
+    for (int i = tid; i <= a.seqs; i += kThreads) s_cu[i] = min(max(a.cu[i], 0), T);
+    __syncthreads();
+    for (int b = tid; b < a.seqs; b += kThreads) {
+      const int lo = s_cu[b], n = s_cu[b + 1] - lo, front = min(s_cu[b + 1], row0) - lo;
+      const int id = bin_of(a.ids[b]);
+      if (n > 0) atomicAdd(&s_total[id], n);
+      if (front > 0) atomicAdd(&s_before[id], front);
+    }
+    const int first = s_cu[0], end = s_cu[a.seqs];
+    if (tid == 0) {  // in front of the first sequence and behind the last
+      atomicAdd(&s_total[L], first + max(T - max(first, end), 0));
+      atomicAdd(&s_before[L], min(row0, first) + max(row0 - max(first, end), 0));
+    }
+    if (row >= first && row < end) {
+      int lo = 0, hi = a.seqs - 1;  // the first sequence that ends behind the row
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (s_cu[mid + 1] > row) hi = mid;
+        else lo = mid + 1;
+      }
+      bin = bin_of(a.ids[lo]);
+    }
+  } else {
+    __syncthreads();
+    for (int i0 = 0; i0 < T; i0 += kThreads) {
+      const int i = i0 + tid;
+      const bool live = i < T;
+      const int id = live ? bin_of(a.ids[i]) : L;
+      if (i0 == row0) bin = id;
+      const uint64_t same = same_bin(id, live);
+      if (live && (same & lanemask_lt()) == 0) {
+        atomicAdd(&s_total[id], __popcll(same));
+        if (i0 < row0) atomicAdd(&s_before[id], __popcll(same));
+      }
+    }
+  }
+  const bool live = row < T;
+  const uint64_t same = same_bin(bin, live);
+  const int in_wave = __popcll(same & lanemask_lt());
+  if (live && in_wave == 0) s_wave[wave][bin] = __popcll(same);
+  __syncthreads();
+
+  if (wave == 0) {  // where each adapter's rows and tiles begin
+    int n[kPerLane], t[kPerLane], rows = 0, tiles = 0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int b = lane * kPerLane + i;
+      n[i] = b < bins ? s_total[b] : 0;
+      t[i] = b < L ? (n[i] + p.tile_rows - 1) / p.tile_rows : 0;
+      rows += n[i], tiles += t[i];
+    }
+    int rows_to = rows, tiles_to = tiles;
+#pragma unroll
+    for (int d = 1; d < MOE_WAVE; d *= 2) {
+      const int r = __shfl_up(rows_to, d), s = __shfl_up(tiles_to, d);
+      if (lane >= d) rows_to += r, tiles_to += s;
+    }
+    rows_to -= rows, tiles_to -= tiles;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int b = lane * kPerLane + i;
+      if (b <= bins) s_first[b] = rows_to, s_tile[b] = tiles_to;
+      rows_to += n[i], tiles_to += t[i];
+    }
+  }
+  __syncthreads();
+  if (live) {
+    int to = s_first[bin] + s_before[bin] + in_wave;
+    for (int w = 0; w < wave; ++w) to += s_wave[w][bin];
+    if (to < T) a.plan[p.rows + to] = row;
+  }
+  if (blockIdx.x == 0) {
+    for (int i = tid; i <= bins; i += kThreads) a.plan[p.offsets + i] = s_first[i];
+    if (tid == 0) a.plan[LH_TILES] = s_tile[L];
+  }
+  for (int t = blockIdx.x * kThreads + tid; t < min(s_tile[L], p.N); t += gridDim.x * kThreads) {
+    int lo = 0, hi = L - 1;  // the last adapter whose tiles begin at t or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (s_tile[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    const int at = (t - s_tile[lo]) * p.tile_rows;
+    *(int4*)(a.plan + p.tiles + 4L * t) = make_int4(lo, s_first[lo] + at, min(s_total[lo] - at, p.tile_rows), 0);
+  }
+}
+
+}  // namespace
+
+extern "C" size_t moe_mi355x_lora_plan_bytes(int T, int L, int32_t* offsets) {
+  if (!lora_plan_ok(T, L)) return 0;
+  const LoraLayout p = lora_layout(T, L);
+  if (offsets) offsets[0] = (int32_t)p.offsets, offsets[1] = (int32_t)p.rows;
+  return (size_t)p.ints * 4;
+}
+
+extern "C" int moe_mi355x_lora_plan(const int32_t* adapter_ids, const int32_t* cu_rows, int seqs, int T, int L,
+                                    void* plan, size_t plan_bytes, void* stream) {
+  MOE_RETURN_IF(!lora_plan_ok(T, L), MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(cu_rows && (seqs < 0 || seqs > kLoraMaxSeqs), MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(!adapter_ids && (cu_rows ? seqs : T) > 0, MOE_ERR_INVALID_ARG);
+  LoraPlanArgs a{adapter_ids, cu_rows, seqs, (int32_t*)plan, lora_layout(T, L)};
+  MOE_RETURN_IF(!plan || plan_bytes < (size_t)a.p.ints * 4, MOE_ERR_WORKSPACE);
+  MOE_RETURN_IF(!moe_aligned16(plan), MOE_ERR_ALIGNMENT);
+  hipLaunchKernelGGL(lora_plan_kernel, dim3(T > kThreads ? (T + kThreads - 1) / kThreads : 1), dim3(kThreads), 0,
+                     (hipStream_t)stream, a);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -782,3 +783,256 @@ def moe_sublayer_fp8(hidden_states, ln_weight, eps, router_weight, top_k, gate_u
         gate_up_proj_scale_inv.data_ptr(), down_proj.data_ptr(), down_proj_scale_inv.data_ptr(), out.data_ptr(),
         ws.data_ptr(), ws.numel(), _stream(hidden_states)), "moe_sublayer_fp8")
     return out
+
+
+# ---------------------------------------------------------------------------
+# low-rank adapters of many requests beside a shared projection
+# ---------------------------------------------------------------------------
+
+LORA_MAX_ROWS, LORA_MAX_ADAPTERS, LORA_MAX_SEQS, LORA_MAX_RANK, LORA_MAX_PARTS = 1 << 18, 256, 4096, 128, 4
+
+
+class LoraPool:
+    """The adapters of one projection, all of one width: adapter l adds ``scales[l] * B_l A_l`` to the weight.
+
+    ``a`` bf16 [L, P * R, K] and ``b`` bf16 [L, N, R] for a projection of P parts (the q, k and v of a fused one), each
+    with its own ``A`` of up to R ranks: part p's are the rows p R .. of ``a``, its columns those of ``b`` in turn,
+    ``columns[p]`` of them.  ``ranks`` int32 [L] (how many of the R adapter l has; 0: nothing is added) and ``scales`` fp32
+    [L] (alpha / rank, mostly) are read on the GPU: what the four tensors hold may change between calls.
+    """
+
+    __slots__ = ("a", "b", "ranks", "scales", "columns", "in_features", "out_features", "max_rank", "num_adapters",
+                 "device", "_columns")
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, ranks: torch.Tensor, scales: torch.Tensor, columns):
+        _need(a, "a", torch.bfloat16, 3)
+        _need(b, "b", torch.bfloat16, 3)
+        _need(ranks, "ranks", torch.int32, 1)
+        _need(scales, "scales", torch.float32, 1)
+        _same_device(a, b=b, ranks=ranks, scales=scales)
+        columns = tuple(int(n) for n in columns)
+        L, PR, K = a.shape
+        R = b.shape[2]
+        if not 1 <= L <= LORA_MAX_ADAPTERS or not 1 <= len(columns) <= LORA_MAX_PARTS:
+            raise ValueError(f"a pool has 1 to {LORA_MAX_ADAPTERS} adapters of 1 to {LORA_MAX_PARTS} parts, got {L} of "
+                             f"{len(columns)}")
+        if R % 16 or not 16 <= R <= LORA_MAX_RANK:
+            raise ValueError(f"the pool's rank must be a multiple of 16 up to {LORA_MAX_RANK}, got {R}")
+        if PR != len(columns) * R or K == 0 or K % 32:
+            raise ValueError(f"a must be [L, {len(columns)} * {R}, K] with K % 32 == 0, got {tuple(a.shape)}")
+        if any(n <= 0 or n % 32 for n in columns) or b.shape[:2] != (L, sum(columns)):
+            raise ValueError(f"b must be [{L}, {sum(columns)}, R] with parts of multiples of 32 columns, got {tuple(b.shape)} "
+                             f"for {columns}")
+        if ranks.shape[0] != L or scales.shape[0] != L:
+            raise ValueError(f"ranks and scales must be [{L}]")
+        if K > 1 << 24 or sum(columns) > 1 << 24:
+            raise ValueError("at most 2^24 features")
+        self.a, self.b, self.ranks, self.scales, self.columns = a, b, ranks, scales, columns
+        self.in_features, self.out_features, self.max_rank, self.num_adapters = K, sum(columns), R, L
+        self.device = a.get_device()
+        self._columns = (ctypes.c_int * len(columns))(*columns)
+
+    @classmethod
+    def empty(cls, num_adapters: int, in_features: int, columns, max_rank: int, device) -> LoraPool:
+        """A pool without adapters (every rank 0), to ``load`` into."""
+        columns = tuple(int(n) for n in columns)
+        bf = {"dtype": torch.bfloat16, "device": device}
+        return cls(torch.zeros((num_adapters, len(columns) * max_rank, in_features), **bf),
+                   torch.zeros((num_adapters, sum(columns), max_rank), **bf),
+                   torch.zeros(num_adapters, dtype=torch.int32, device=device),
+                   torch.zeros(num_adapters, dtype=torch.float32, device=device), columns)
+
+    def load(self, index: int, parts, scale: float) -> None:
+        """Adapter ``index`` from ``parts``: an ``(A [r, K], B [columns, r])`` for each part, of one rank r, or None for a
+        part that it leaves alone.  Copied, on the current stream."""
+        if not 0 <= index < self.num_adapters:
+            raise ValueError(f"index must be in [0, {self.num_adapters}), got {index}")
+        if len(parts) != len(self.columns):
+            raise ValueError(f"the projection has {len(self.columns)} parts, got {len(parts)}")
+        ranks = {p[0].shape[0] for p in parts if p is not None}
+        if len(ranks) > 1 or any(not 1 <= r <= self.max_rank for r in ranks):
+            raise ValueError(f"an adapter has one rank of 1 to {self.max_rank}, got {sorted(ranks)}")
+        rank = max(ranks, default=0)
+        for p, n in zip(parts, self.columns):
+            if p is not None and (tuple(p[0].shape) != (rank, self.in_features) or tuple(p[1].shape) != (n, rank)):
+                raise ValueError(f"a part of rank {rank} must be [{rank}, {self.in_features}] and [{n}, {rank}], got "
+                                 f"{tuple(p[0].shape)} and {tuple(p[1].shape)}")
+        self.a[index].zero_()
+        self.b[index].zero_()
+        at = 0
+        for i, (p, n) in enumerate(zip(parts, self.columns)):
+            if p is not None:
+                self.a[index, i * self.max_rank:i * self.max_rank + rank].copy_(p[0])
+                self.b[index, at:at + n, :rank].copy_(p[1])
+            at += n
+        self.ranks[index] = rank
+        self.scales[index] = float(scale)
+
+
+class LoraPlan:
+    """A step's rows by adapter, as ``lora_plan`` left them on the GPU; built once a step, used by every projection.
+
+    ``rows`` int32 [T]: the step's rows in the order of their adapter, those without one last; ``offsets`` int32 [L + 2]:
+    the first of each adapter's, of those without one, and T.  Views of what the GPU holds.
+    """
+
+    __slots__ = ("num_rows", "num_adapters", "buffer", "device", "_at")
+
+    def __init__(self, num_rows: int, num_adapters: int, like: torch.Tensor):
+        self.num_rows, self.num_adapters, self.device = num_rows, num_adapters, like.get_device()
+        ints, self._at = _lora_sizes(num_rows, num_adapters)
+        self.buffer = like.new_empty(ints)
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self.buffer[self._at[0]:self._at[0] + self.num_adapters + 2]
+
+    @property
+    def rows(self) -> torch.Tensor:
+        return self.buffer[self._at[1]:self._at[1] + self.num_rows]
+
+
+@functools.lru_cache(maxsize=1024)
+def _lora_sizes(num_rows: int, num_adapters: int):
+    """(int32 of the plan, positions of its offsets and rows)"""
+    at = (ctypes.c_int32 * 2)()
+    return _lib.load().moe_mi355x_lora_plan_bytes(num_rows, num_adapters, at) // 4, tuple(at)
+
+
+def lora_plan(adapter_ids: torch.Tensor, num_adapters: int, cu_rows: torch.Tensor | None = None,
+              num_rows: int | None = None, out: LoraPlan | None = None) -> LoraPlan:
+    """Sorts a step's rows by their adapter, on the GPU.
+
+    ``adapter_ids`` int32: the adapter of each row [T], or, with ``cu_rows`` int32 [B + 1] (ascending; a ``PagedPlan``'s
+    ``cu_tokens`` serves), of each sequence [B] whose rows are ``cu_rows[b] .. cu_rows[b + 1]``; the step then has
+    ``num_rows`` rows.  A number outside [0, num_adapters) means none, and so do rows of no sequence.
+
+    With ``out``, an earlier plan of the same sizes, that plan's memory is filled again: a captured step keeps one.
+    """
+    dev = adapter_ids.get_device() if isinstance(adapter_ids, torch.Tensor) else -1
+    if not _fits(adapter_ids, torch.int32, dev, 1) or (cu_rows is not None and not _fits(cu_rows, torch.int32, dev, 1)):
+        _need(adapter_ids, "adapter_ids", torch.int32, 1)
+        _need(cu_rows, "cu_rows", torch.int32, 1)
+        _same_device(adapter_ids, cu_rows=cu_rows)
+    n = adapter_ids.shape[0]
+    if cu_rows is None:
+        if num_rows is not None and num_rows != n:
+            raise ValueError(f"without cu_rows there are as many rows as adapter_ids, {n}, not {num_rows}")
+        num_rows = n
+    else:
+        if cu_rows.shape[0] != n + 1:
+            raise ValueError(f"cu_rows needs one entry more than adapter_ids, {n + 1}, got {cu_rows.shape[0]}")
+        if num_rows is None:
+            raise ValueError("cu_rows needs num_rows")
+        if n > LORA_MAX_SEQS:
+            raise ValueError(f"a step has at most {LORA_MAX_SEQS} sequences, got {n}")
+    if not 0 <= num_rows <= LORA_MAX_ROWS or not 1 <= num_adapters <= LORA_MAX_ADAPTERS:
+        raise ValueError(f"a plan has at most {LORA_MAX_ROWS} rows and 1 to {LORA_MAX_ADAPTERS} adapters, got {num_rows} and "
+                         f"{num_adapters}")
+    if out is None:
+        out = LoraPlan(num_rows, num_adapters, adapter_ids)
+    elif (out.num_rows, out.num_adapters, out.device) != (num_rows, num_adapters, dev):
+        raise ValueError(f"out is a plan of {out.num_rows} rows and {out.num_adapters} adapters on device {out.device}, not of "
+                         f"{num_rows} and {num_adapters} on {dev}")
+    _launch("lora_plan", dev, _lib.load().moe_mi355x_lora_plan, adapter_ids.data_ptr(),
+            None if cu_rows is None else cu_rows.data_ptr(), n, num_rows, num_adapters, out.buffer.data_ptr(),
+            out.buffer.shape[0] * 4, _stream(adapter_ids))
+    return out
+
+
+def _rows_apart(t: torch.Tensor, name: str, rows: int, columns: int, device: int) -> int:
+    """Checks a bf16 [rows, columns] tensor whose rows may lie apart (a slice of a wider one); returns the values from
+    one row to the next."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must have dtype torch.bfloat16, got {t.dtype}")
+    if t.shape != (rows, columns):
+        raise ValueError(f"{name} must be {(rows, columns)}, got {tuple(t.shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on the plan's device, cuda:{device}, got {t.device}")
+    if t.is_contiguous():
+        return columns
+    apart, one = t.stride()
+    if one != 1 or apart < columns or apart % 8:
+        raise ValueError(f"{name}: rows must be contiguous, a multiple of 8 values apart and not overlap, got strides "
+                         f"{t.stride()}")
+    return apart
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, pool: LoraPool, plan: LoraPlan) -> torch.Tensor:
+    """Adds to ``y``, the shared projection of ``x``, in place what each row's adapter contributes:
+    ``y[t] += scale_l * B_l (A_l x[t])``, part by part.  Prompts and single tokens of any number of requests in
+    one call; rows without an adapter are left as they are.  ``y`` bf16 [T, N], ``x`` bf16 [T, K] (rows may lie
+    apart); returns ``y``.  fp32 sums, one rounding of the result; ``A x`` is kept to 2^-17 of its value."""
+    if not isinstance(pool, LoraPool) or not isinstance(plan, LoraPlan):
+        raise TypeError("pool must be a LoraPool and plan a LoraPlan (lora_plan)")
+    if pool.num_adapters != plan.num_adapters:
+        raise ValueError(f"the plan is for {plan.num_adapters} adapters, the pool has {pool.num_adapters}")
+    dev = plan.device
+    if pool.device != dev:
+        raise ValueError(f"the pool is on cuda:{pool.device}, the plan on cuda:{dev}")
+    y_stride = _rows_apart(y, "y", plan.num_rows, pool.out_features, dev)
+    x_stride = _rows_apart(x, "x", plan.num_rows, pool.in_features, dev)
+    _launch("lora_add", dev, _lib.load().moe_mi355x_lora_add, y.data_ptr(), y_stride, x.data_ptr(), x_stride,
+            pool.a.data_ptr(), pool.b.data_ptr(), pool.ranks.data_ptr(), pool.scales.data_ptr(), plan.buffer.data_ptr(),
+            plan.num_rows, plan.num_adapters, pool.in_features, pool.max_rank, len(pool.columns), pool._columns, _stream(y))
+    return y
+
+
+# ---------------------------------------------------------------------------
+# what a step answers with
+# ---------------------------------------------------------------------------
+
+TOP_MAX = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """``token_logprobs``' results: fp32 [T] (None without tokens), fp32 [T], int64 [T, k], fp32 [T, k]."""
+
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int32 or int64 [T]) under ``logits`` (bf16 or fp32 [T, V], rows may lie
+    apart), the entropy of each row and its ``top_k`` most likely tokens with their log probabilities, descending, the
+    lower id first among equals.  One pass over the logits, fp32 sums.
+
+    A negative token asks for nothing (0), one of V or more gives NaN.  A row with a NaN or +inf, or with nothing but
+    -inf, has NaN for log probabilities and entropy; among the most likely a NaN comes first."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"logits must have dtype torch.bfloat16 or torch.float32, got {logits.dtype}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [T, V], got shape {tuple(logits.shape)}")
+    dev = logits.get_device()
+    if dev < 0:
+        raise ValueError(f"logits must be on a ROCm GPU device, got {logits.device}")
+    T, V = logits.shape
+    stride = logits.stride(0) if T > 1 else V
+    if V < 1 or T >= 1 << 24:
+        raise ValueError(f"logits must have at least one column and fewer than 2^24 rows, got {tuple(logits.shape)}")
+    if (V > 1 and logits.stride(1) != 1) or stride < V:
+        raise ValueError(f"logits: rows must be contiguous and not overlap, got strides {logits.stride()}")
+    if not 0 <= top_k <= min(V, TOP_MAX):
+        raise ValueError(f"top_k must be in [0, min(V, {TOP_MAX})], got {top_k}")
+    if tokens is not None:
+        _need(tokens, "tokens", (torch.int32, torch.int64), 1)
+        _same_device(logits, tokens=tokens)
+        if tokens.shape[0] != T:
+            raise ValueError(f"tokens must be [{T}], got {tuple(tokens.shape)}")
+    lib = _lib.load()
+    f32 = logits.new_empty((T * (2 + top_k),), dtype=torch.float32)
+    entropy, logprobs, top = f32.split_with_sizes([T, T, T * top_k])
+    ids = logits.new_empty((T, top_k), dtype=torch.int64)
+    nws = lib.moe_mi355x_token_logprobs_workspace_bytes(T, V, top_k)
+    ws = logits.new_empty(nws, dtype=torch.uint8) if nws else None
+    _launch("token_logprobs", dev, lib.moe_mi355x_token_logprobs, logits.data_ptr(),
+            0 if logits.dtype == torch.bfloat16 else 1, stride, None if tokens is None else tokens.data_ptr(),
+            8 if tokens is None else _id_bytes(tokens), T, V, top_k, logprobs.data_ptr(), entropy.data_ptr(),
+            ids.data_ptr(), top.data_ptr(), ws.data_ptr() if nws else None, nws, _stream(logits))
+    return TokenLogprobs(None if tokens is None else logprobs, entropy, ids, top.view(T, top_k))
