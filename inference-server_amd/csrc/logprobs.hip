@@ -25,6 +25,7 @@ constexpr int kKeep = 256;     // ... after they are cut down, at most
 constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 5.5f;  // 8 ln 2: what a value may be above the reference
+constexpr float kFar = 1 << 20;  // a reference up to here, times log2(e), is off by 2^-5 at most, which is undone exactly
 constexpr float kNoTerm = -200.f;  // log2 of a term that is zero in fp32, in the place of -inf times zero
 
 struct LpArgs {
@@ -84,10 +85,12 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   const Sums x = under(a), y = under(b);
   return Sums{m, x.s + y.s, x.t + y.t};
 }
+// ... over a wave, as its first lane has it (lanes differ in which of two sums the compiler's fused product takes)
 __device__ __forceinline__ Sums join_wave(Sums v) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v = join(v, Sums{__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.t, d)});
-  return v;
+  auto first = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
+  return Sums{first(v.m), first(v.s), first(v.t)};
 }
 
 // From a row's sums to its results
@@ -97,8 +100,8 @@ struct Row {
 };
 __device__ __forceinline__ Row row_of(Sums v) {
   const float m = v.m == -INFINITY ? 0.f : v.m;
-  const double ln_z = log((double)v.s);
-  return Row{(double)m, ln_z, (float)(ln_z - 0.69314718055994530942 * ((double)v.t / (double)v.s))};
+  const double ln_z = log((double)v.s), entropy = ln_z - 0.69314718055994530942 * ((double)v.t / (double)v.s);
+  return Row{(double)m, ln_z, entropy < 0. ? 0.f : (float)entropy};
 }
 __device__ __forceinline__ float logprob(const Row& r, float x) { return (float)((double)x - r.m - r.ln_z); }
 
@@ -222,10 +225,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       const bool first = m == -INFINITY;
       m = wave_max_uniform(fmaxf(m, pm));
       m2 = m * kLog2e;
+      asm("" : "+v"(m2));  // rounded: as an operand of a fused difference it would not be what the terms were formed with
       limit = m + kSlack;
-      const float d = old - m2, c = __builtin_amdgcn_exp2f(d);
-      t = first ? 0.f : fmaf(s, d, t) * c;
-      s = first ? 0.f : s * c;
+      if (!first) {  // before the first value that is not -inf the sums are 0, or NaN
+        const float d = old - m2, c = __builtin_amdgcn_exp2f(d);
+        t = fmaf(s, d, t) * c;
+        s *= c;
+      }
     }
   };
   auto add = [&](float v) __attribute__((always_inline)) {
@@ -286,9 +292,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const float off = m == -INFINITY ? 0.f : fmaf(m, kLog2e, -m2), undo = __builtin_amdgcn_exp2f(-off);
   Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
 
-  // NaN, +inf, or a reference so far out that its product with log2(e) is infinite: again, from the maximum
+  // NaN, +inf, or a reference so far out that its product with log2(e) is rounded by much: again, from the maximum
   if (lane == 0) s_max[wave] = m;
-  const bool odd = __any(!(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < INFINITY));
+  const bool odd = __any(!(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar));
   if (__syncthreads_or(odd)) {
     m = s_max[0];
 #pragma unroll
