@@ -8,21 +8,28 @@
 // maximum: the sums are scaled only where a value passes it by 2^8, which after the first values happens rarely.
 //
 // The largest are found on the way.  Each lane's running maximum gives a bound: where j lanes of each of the four waves
-// have seen a value of at least b, with 4 j >= k, the k largest are all >= b.  The bound is renewed at doubling
-// distances, so that a few hundred values of a row pass it; those are kept in LDS, cut down to the k largest if they get
-// many, and sorted at the end by counting.
+// have seen a value of at least b, with 4 j >= k, the k largest are all >= b.  The bound is renewed at growing
+// distances.  Of a 16-byte vector with a value that passes it the maximum and the place are kept in LDS; those that pass
+// the bound at the end are read again, and their values that do sorted by counting.
 //
-// Few rows are split over workgroups, whose sums and lists a second kernel joins.  Rows with NaN, +inf or with
-// nothing but values near the type's lowest are gone over again by a plainer scan.
+// Few rows are split over workgroups, whose sums and lists a second kernel joins.  Rows with NaN or +inf, with a maximum
+// of a size past 7 * 10^5 (the type's lowest everywhere, say) or with more candidates than there is room for (values
+// that rise along the row, or nearly all equal) are gone over again by a plainer scan.
 #include "common.h"
 
+#ifndef LP_OCC
+#define LP_OCC 6
+#endif
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / MOE_WAVE;
 constexpr int kMaxTop = 64;
-constexpr int kBuf = 1024;     // candidates that a wave keeps
-constexpr int kKeep = 256;     // ... after they are cut down, at most
+constexpr int kBuf = 512;      // candidates that a wave keeps
+constexpr int kKeep = 128;     // ... after they are cut down, at most
+constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
+constexpr int kVecs = 256;             // vectors whose values a workgroup looks at at the end
 constexpr int kMaxSplits = 64;
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 5.5f;  // 8 ln 2: what a value may be above the reference
 constexpr float kFar = 1 << 20;  // a reference up to here, times log2(e), is off by 2^-5 at most, which is undone exactly
@@ -116,22 +123,32 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r) {
 
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return ~wave_max_u32_uniform(~v); }
 
-// A bound that at least n of the wave's 64 values reach, close to the n-th largest
+// A bound that at least n of the wave's 64 values reach, close to the n-th largest: down from the largest by growing
+// steps, of 1/32 of a binade at first, then back by three halvings of the last one.
 __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
-  uint32_t lo = wave_min_u32(mine), hi = wave_max_u32_uniform(mine);
+  const uint32_t most = wave_max_u32_uniform(mine);
+  auto reached = [&](uint32_t b) __attribute__((always_inline)) { return __popcll(__ballot(mine >= b)) >= n; };
+  uint32_t step = 1u << 18, lo = most, down = 0;
 #pragma unroll 1
-  for (int i = 0; i < 14 && lo < hi; ++i) {
-    const uint32_t mid = lo + (hi - lo + 1) / 2;
-    if (__popcll(__ballot(mine >= mid)) >= n) lo = mid;
-    else hi = mid - 1;
+  while (!reached(lo)) {  // 0 is reached by all
+    down = down + step;
+    lo = most > down ? most - down : 0;
+    step *= 2;
+  }
+#pragma unroll 1
+  for (int i = 0; i < 3 && down != 0; ++i) {
+    step = max(step / 2, 2u);
+    const uint32_t mid = lo + step / 2;
+    if (mid > lo && reached(mid)) lo = mid;
   }
   return lo;
 }
 
 struct TopLds {
-  uint64_t buf[kWaves][kBuf];
+  uint64_t buf[kWaves][kBuf];  // at the end the list of all waves, kList + 3 at most
+  int vecs[kVecs];
   uint32_t bound[kWaves];
-  int count;
+  int n_vecs, n_list;
 };
 
 // A wave's candidates
@@ -140,7 +157,8 @@ struct Top {
   int count;          // wave-uniform
   uint64_t least;     // keys below are not among the k largest; wave-uniform
   float least_value;
-  uint32_t lane_max;  // ordered
+  float lane_max;
+  uint32_t bound;  // of the wave's lanes
 };
 
 __device__ __forceinline__ void raise(Top& t, uint64_t least) {
@@ -150,7 +168,16 @@ __device__ __forceinline__ void raise(Top& t, uint64_t least) {
   }
 }
 
-// Cuts the candidates down to between k and kKeep (all k of them where they are fewer).
+// There is room for 64 more.
+__device__ __forceinline__ void offer(Top& t, float x, int index, bool valid) {
+  const uint64_t key = key_of(x, index);
+  const bool pass = valid && key >= t.least;
+  const uint64_t mask = __ballot(pass);
+  if (pass) t.buf[t.count + __popcll(mask & lanemask_lt())] = key;
+  t.count += __popcll(mask);
+}
+
+// Cuts the candidates down to between k and kKeep (all k of those from `least` on where they are fewer).
 __device__ __forceinline__ void cut(Top& t, int k, int lane) {
   constexpr int kPer = kBuf / MOE_WAVE;
   uint64_t key[kPer];
@@ -159,7 +186,7 @@ __device__ __forceinline__ void cut(Top& t, int k, int lane) {
     const int at = i * MOE_WAVE + lane;
     key[i] = at < t.count ? t.buf[at] : 0;
   }
-  uint64_t lo = t.least, hi = ~0ull;  // at least k keys are >= lo, fewer than k are > hi
+  uint64_t lo = t.least, hi = ~0ull;  // fewer than k are > hi; at least k are >= lo, or lo is `least`
 #pragma unroll 1
   while (lo < hi) {
     const uint64_t mid = lo + (hi - lo) / 2 + 1;
@@ -184,20 +211,26 @@ __device__ __forceinline__ void cut(Top& t, int k, int lane) {
   }
 }
 
-__device__ __forceinline__ void offer(Top& t, float x, int index, bool valid, int lane) {
-  const uint64_t key = key_of(x, index);
-  const bool pass = valid && key >= t.least;
-  const uint64_t mask = __ballot(pass);
-  if (mask == 0) return;
-  if (pass) t.buf[t.count + __popcll(mask & lanemask_lt())] = key;
-  t.count += __popcll(mask);
+// Writes the k largest of list[0 .. n), in order, as fn(place, key).  list has room to n + 3 and is 16-byte aligned.
+template <typename F>
+__device__ __forceinline__ void write_top(uint64_t* list, int n, int k, F fn) {
+  if (threadIdx.x < 3) list[n + threadIdx.x] = 0;
+  __syncthreads();
+  for (int j = threadIdx.x; j < n; j += kThreads) {
+    const uint64_t mine = list[j];
+    int rank = 0;
+    for (int o = 0; o < n; o += 4) {
+      const ulonglong2 a = *(const ulonglong2*)(list + o), b = *(const ulonglong2*)(list + o + 2);
+      rank += (a.x > mine) + (a.y > mine) + (b.x > mine) + (b.y > mine);
+    }
+    if (rank < k) fn(rank, mine);
+  }
 }
 
 template <typename E, bool TOP>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
+__global__ __launch_bounds__(kThreads, LP_OCC) void logprobs_kernel(LpArgs a) {
   constexpr int kVec = 16 / sizeof(E);
-  constexpr int kRoom = kBuf - MOE_WAVE * kVec;  // more candidates than this are cut down before the next values
-  __shared__ TopLds lds;
+  __shared__ __attribute__((aligned(16))) TopLds lds;
   __shared__ Sums s_sums[kWaves];
   __shared__ float s_max[kWaves];
   const int lane = threadIdx.x & 63;
@@ -217,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
   const int per_wave = (a.k + kWaves - 1) / kWaves;
 
-  Top top{lds.buf[wave], 0, 0, -INFINITY, 0};
+  Top top{lds.buf[wave], 0, 0, -INFINITY, -INFINITY, 0};
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
   auto reference = [&](float pm) __attribute__((always_inline)) {
     if (__any(pm > limit)) {
@@ -240,135 +273,186 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     t = fmaf(e, fmaxf(d, kNoTerm), t);
   };
   auto renew = [&]() __attribute__((always_inline)) {
-    const uint32_t b = bound_of(top.lane_max, per_wave);
-    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = b;
+    top.bound = max(bound_of(ordered(top.lane_max), per_wave), top.bound);
+    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = top.bound;
   };
   auto take_bound = [&]() __attribute__((always_inline)) {
     uint32_t b = ~0u;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
-    raise(top, (uint64_t)__builtin_amdgcn_readfirstlane(b) << 32);
+    raise(top, (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(b) << 32);
   };
 
-  // the edges, then a first vector to have a bound to go by
-  if (TOP) top.lane_max = lane < n_edge ? ordered(edge_value) : 0;
+  // the edges, then two vectors a turn, those of the next one on their way; the first gives a bound to go by
+  if (TOP) top.lane_max = edge_value;
   reference(edge_value);
   add(edge_value);
-  int i = v0 + wave * MOE_WAVE + lane, turn = 0;
-  for (int i0 = v0 + wave * MOE_WAVE; i0 < v1 || turn == 0; i0 += kThreads, i += kThreads, ++turn) {
-    float v[kVec];
-    if (i < v1) {
-      unpack(xv[i], v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
+  const int first = v0 + wave * MOE_WAVE;
+  auto load = [&](int i) __attribute__((always_inline)) { return xv[min(i, max(v1, 1) - 1)]; };
+  uint4 now[2], next[2];
+  if (vecs > 0) {
+    now[0] = load(first + lane);
+    now[1] = load(first + kThreads + lane);
+  }
+  int turn = 0, renewal = 2;
+  bool full = false;  // more candidates than there is room for
+  const bool brief = v1 - v0 <= 2 * kThreads;  // all in the first turn's registers
+  float v[2][kVec], pm[2];
+#pragma unroll 1
+  for (int i0 = first; i0 < v1 || turn == 0; i0 += 2 * kThreads, ++turn) {
+    const int i = i0 + lane;
+    if (i0 + 2 * kThreads < v1) {
+      next[0] = load(i + 2 * kThreads);
+      next[1] = load(i + 3 * kThreads);
     }
-    float pm = v[0];
 #pragma unroll
-    for (int e = 1; e < kVec; ++e) pm = fmaxf(pm, v[e]);
-    reference(pm);
+    for (int h = 0; h < 2; ++h) {
+      unpack(now[h], v[h]);
+      if (i0 + h * kThreads + MOE_WAVE > v1) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) add(v[e]);
+        for (int e = 0; e < kVec; ++e) v[h][e] = i + h * kThreads < v1 ? v[h][e] : -INFINITY;
+      }
+      pm[h] = v[h][0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) pm[h] = fmaxf(pm[h], v[h][e]);
+    }
+    const float most = fmaxf(pm[0], pm[1]);
+    reference(most);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) add(v[h][e]);
     if (TOP) {
-      if (i < v1) top.lane_max = max(top.lane_max, ordered(pm));
-      if ((turn & (turn + 1)) == 0) {
+      top.lane_max = fmaxf(top.lane_max, most);
+      if (brief) break;
+      if (turn == 0 || turn == renewal) {
         renew();
-        if (turn == 0) {
-          __syncthreads();
-          take_bound();
-          offer(top, edge_value, edge, lane < n_edge, lane);
-        } else {
-          take_bound();
-        }
+        if (turn == 0) __syncthreads();
+        else renewal = 4 * renewal + 3;
+        take_bound();
       }
-      if (__any(!(pm < top.least_value))) {
+      if (__any(!(most < top.least_value))) {
+        take_bound();  // the other waves may have renewed theirs
+        full |= top.count > kBuf - 2 * MOE_WAVE;
+        if (full) top.count = 0;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) offer(top, v[e], head + i * kVec + e, i < v1, lane);
-        if (top.count > kRoom) cut(top, a.k, lane);
+        for (int h = 0; h < 2; ++h) offer(top, pm[h], i + h * kThreads, i + h * kThreads < v1);
       }
     }
+    now[0] = next[0];
+    now[1] = next[1];
   }
   // from the reference as the sums used it, m log2(e) rounded, to m itself
   const float off = m == -INFINITY ? 0.f : fmaf(m, kLog2e, -m2), undo = __builtin_amdgcn_exp2f(-off);
   Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
 
-  // NaN, +inf, or a reference so far out that its product with log2(e) is rounded by much: again, from the maximum
   if (lane == 0) s_max[wave] = m;
-  const bool odd = __any(!(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar));
-  if (__syncthreads_or(odd)) {
+  if (TOP && threadIdx.x == 0) lds.n_vecs = lds.n_list = 0;
+  if (TOP) renew();
+  uint64_t* list = lds.buf[0];
+  bool again = __syncthreads_or(full || !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar));
+  if (TOP && !again) {
+    take_bound();
+    auto keep = [&](float v, int index) __attribute__((always_inline)) {
+      const uint64_t key = key_of(v, index);
+      if (key < top.least) return;
+      const int at = atomicAdd(&lds.n_list, 1);
+      if (at < kList) list[at] = key;
+    };
+    if (!brief) {
+      for (int j = lane; j < top.count; j += MOE_WAVE) {
+        const uint64_t key = top.buf[j];
+        if (key < top.least) continue;
+        const int at = atomicAdd(&lds.n_vecs, 1);
+        if (at < kVecs) lds.vecs[at] = index_of(key);
+      }
+      __syncthreads();
+      const int n = lds.n_vecs;
+      again = n > kVecs;
+      if ((int)threadIdx.x < min(n, kVecs)) {
+        const int at = lds.vecs[threadIdx.x];
+        unpack(xv[at], v[0]);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) keep(v[0][e], head + at * kVec + e);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = first + lane + h * kThreads;
+        if (at < v1 && !(pm[h] < top.least_value))
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) keep(v[h][e], head + at * kVec + e);
+      }
+    }
+    if (lane < n_edge) keep(edge_value, edge);
+    __syncthreads();
+    again |= lds.n_list > kList;
+  }
+
+  // NaN, +inf, a reference so far out that its product with log2(e) is rounded by much, more candidates than there is
+  // room for (values that rise along the row, or nearly all equal): again, from the maximum and value by value.
+  if (again) {
+    __syncthreads();  // the counts are read
     m = s_max[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_max[w]);
     s = t = 0.f;
     const float ref = m == -INFINITY ? 0.f : m;
-    top.count = 0, top.least = 0, top.least_value = -INFINITY;
-    auto again = [&](float v) __attribute__((always_inline)) {
+    auto term = [&](float v) __attribute__((always_inline)) {
       const float d = (v - ref) * kLog2e, e = __builtin_amdgcn_exp2f(d);
       s += e;
       t = fmaf(e, fmaxf(d, kNoTerm), t);
     };
-    again(edge_value);
-    if (TOP) offer(top, edge_value, edge, lane < n_edge, lane);
-    for (int i0 = v0 + wave * MOE_WAVE; i0 < v1; i0 += kThreads) {
+    term(edge_value);
+    if (TOP) {
+      if (threadIdx.x == 0) lds.n_list = 0;
+      top.count = 0, top.least = 0;
+      offer(top, edge_value, edge, lane < n_edge);
+    }
+    for (int i0 = first; i0 < v1; i0 += kThreads) {
       const int j = i0 + lane;
 #pragma unroll 1
       for (int e = 0; e < kVec; ++e) {
         const float v = j < v1 ? value_at(x, head + (long)j * kVec + e) : -INFINITY;
-        again(v);
-        if (TOP) offer(top, v, head + j * kVec + e, j < v1, lane);
+        term(v);
+        if (TOP) {
+          offer(top, v, head + j * kVec + e, j < v1);
+          if (top.count > (i0 + kThreads < v1 || e + 1 < kVec ? kBuf - MOE_WAVE : kKeep)) cut(top, a.k, lane);
+        }
       }
-      if (TOP && top.count > kRoom) cut(top, a.k, lane);
     }
     sum = Sums{m, s, t};
-    if (TOP) {
-      top.lane_max = 0;  // the bound of the first scan is not one of NaN's order
-      if (lane == 0) lds.bound[wave] = 0;
+    if (TOP) {  // the waves' candidates in one list, which takes the place of their buffers
+      uint64_t key[kKeep / MOE_WAVE];
+#pragma unroll
+      for (int j = 0; j < kKeep / MOE_WAVE; ++j) key[j] = j * MOE_WAVE + lane < top.count ? top.buf[j * MOE_WAVE + lane] : 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kKeep / MOE_WAVE; ++j)
+        if (key[j] != 0) list[atomicAdd(&lds.n_list, 1)] = key[j];
     }
-  } else if (TOP) {
-    renew();
   }
   sum = join_wave(sum);
   if (lane == 0) s_sums[wave] = sum;
-  if (TOP && top.count > kKeep) cut(top, a.k, lane);
-  if (threadIdx.x == 0) lds.count = 0;
   __syncthreads();
   sum = s_sums[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) sum = join(sum, s_sums[w]);
   Row r{};
   if (a.splits == 1) r = row_of(sum);
-
-  if (TOP) {  // the waves' candidates in one list, in registers meanwhile: it takes the place of their buffers
-    take_bound();
-    constexpr int kPer = kKeep / MOE_WAVE;
-    uint64_t key[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int at = j * MOE_WAVE + lane;
-      key[j] = at < top.count ? top.buf[at] : 0;
-    }
-    __syncthreads();
-    uint64_t* list = lds.buf[0];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (key[j] >= top.least && key[j] != 0) list[atomicAdd(&lds.count, 1)] = key[j];
-    __syncthreads();
-    const int n = lds.count;
+  if (TOP) {
+    const int n = lds.n_list;
     uint64_t* out = a.splits > 1 ? a.keys + (long)blockIdx.x * a.k : nullptr;
     if (out)  // a short split has fewer
       for (int j = n + threadIdx.x; j < a.k; j += kThreads) out[j] = 0;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-      const uint64_t mine = list[j];
-      int rank = 0;
-      for (int o = 0; o < n; ++o) rank += list[o] > mine;
-      if (rank >= a.k) continue;
+    write_top(list, n, a.k, [&](int place, uint64_t key) __attribute__((always_inline)) {
       if (out) {
-        out[rank] = mine;
+        out[place] = key;
       } else {
-        a.top_ids[(long)row * a.k + rank] = index_of(mine);
-        a.top_logprobs[(long)row * a.k + rank] = logprob(r, value_of(mine));
+        a.top_ids[(long)row * a.k + place] = index_of(key);
+        a.top_logprobs[(long)row * a.k + place] = logprob(r, value_of(key));
       }
-    }
+    });
   }
   if (threadIdx.x != 0) return;
   if (a.splits > 1) {
@@ -381,8 +465,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 // Joins a row's splits: their sums, and the k largest of their lists
 template <typename E>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
-  __shared__ uint64_t list[kMaxSplits * kMaxTop];
+  __shared__ __attribute__((aligned(16))) uint64_t list[kMaxSplits * kMaxTop + 4];
   __shared__ int s_count;
+  __shared__ uint32_t s_bound[kWaves];
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const float4* parts = a.sums + (long)row * a.splits;
   const uint64_t* keys = a.keys + (long)row * a.splits * a.k;
@@ -391,26 +476,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   const float4 v = lane < a.splits ? parts[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
   const Row r = row_of(join_wave(Sums{v.x, v.y, v.z}));
   if (a.k > 0) {
-    uint64_t least = lane < a.splits ? keys[(long)lane * a.k + a.k - 1] : 0;  // some split has k keys from here on
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const uint64_t o = (uint64_t)__shfl_xor((long long)least, d);
-      least = o > least ? o : least;
-    }
+    // Where c splits have j values of at least b each, with c j >= k, the k largest are all >= b: wave w looks at j = 1, 2, 4, 8.
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = min(1 << wave, a.k), c = (a.k + j - 1) / j;
+    const uint32_t mine = lane < a.splits ? (uint32_t)(keys[(long)lane * a.k + j - 1] >> 32) : 0;
+    const uint32_t b = c <= a.splits ? bound_of(mine, c) : 0;
+    if (lane == 0) s_bound[wave] = b;
+    __syncthreads();
+    const uint64_t least = (uint64_t)max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])) << 32;
     for (int i = threadIdx.x; i < a.splits * a.k; i += kThreads) {
       const uint64_t key = keys[i];
       if (key >= least && key != 0) list[atomicAdd(&s_count, 1)] = key;
     }
     __syncthreads();
-    const int n = s_count;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-      const uint64_t mine = list[j];
-      int rank = 0;
-      for (int o = 0; o < n; ++o) rank += list[o] > mine;
-      if (rank >= a.k) continue;
-      a.top_ids[(long)row * a.k + rank] = index_of(mine);
-      a.top_logprobs[(long)row * a.k + rank] = logprob(r, value_of(mine));
-    }
+    write_top(list, s_count, a.k, [&](int place, uint64_t key) __attribute__((always_inline)) {
+      a.top_ids[(long)row * a.k + place] = index_of(key);
+      a.top_logprobs[(long)row * a.k + place] = logprob(r, value_of(key));
+    });
   }
   if (threadIdx.x != 0) return;
   finish<E>(a, row, r);
@@ -419,8 +500,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
 bool lp_ok(int T, int V, int k) { return T >= 0 && V >= 1 && k >= 0 && k <= kMaxTop && k <= V && T < (1 << 24); }
 
 // Workgroups of a row
+#ifndef LP_WANT
+#define LP_WANT 1024
+#endif
+#ifndef LP_MIN
+#define LP_MIN 4096
+#endif
 int lp_splits(int T, int V) {
-  const int most = (V + 4095) / 4096, want = (1024 + T - 1) / (T > 0 ? T : 1);
+  const int most = (V + LP_MIN - 1) / LP_MIN, want = (LP_WANT + T - 1) / (T > 0 ? T : 1);
   const int n = want < most ? want : most;
   return n < 1 ? 1 : n < kMaxSplits ? n : kMaxSplits;
 }
