@@ -387,9 +387,10 @@ int moe_mi355x_lora_plan(const int32_t* adapter_ids, const int32_t* cu_rows, int
  *   a bf16 [L, parts R, K]    b bf16 [L, N, R]    ranks int32 [L]    scales fp32 [L]    columns: host array [parts]
  * K % 32 == 0, R % 16 == 0, R <= 128, 1 <= parts <= 4, columns[p] % 32 == 0; x and y must not overlap.
  */
+size_t moe_mi355x_lora_add_workspace_bytes(int T, int L, int K, int R, int parts, const int* columns);
 int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, long long x_stride, const void* a, const void* b,
                         const int32_t* ranks, const float* scales, const void* plan, int T, int L, int K, int R, int parts,
-                        const int* columns, void* stream);
+                        const int* columns, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Log probabilities of given tokens, with entropy and the k most likely tokens, of T rows of logits:

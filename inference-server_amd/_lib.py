@@ -84,8 +84,9 @@ SIGNATURES = {
                                            ctypes.c_float, _shape, _vp, _vp, _vp, _c_size, _vp]),
     "moe_mi355x_lora_plan_bytes": (_c_size, [_c_int, _c_int, _vp]),
     "moe_mi355x_lora_plan": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
+    "moe_mi355x_lora_add_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
     "moe_mi355x_lora_add": (_c_int, [_vp, _c_ll, _vp, _c_ll, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
-                                     _c_int, _vp, _vp]),
+                                     _c_int, _vp, _vp, _c_size, _vp]),
     "moe_mi355x_token_logprobs_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "moe_mi355x_token_logprobs": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp,
                                            _vp, _c_size, _vp]),

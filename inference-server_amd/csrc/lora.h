@@ -25,7 +25,7 @@ static inline bool lora_plan_ok(int T, int L) { return T >= 0 && T <= kLoraMaxRo
 
 // Rows of a tile: 16, an MFMA's, where there are few rows and each may have an adapter of its own; more where tiles
 // share their adapter with others, so that it is read less often.
-static inline int lora_tile_rows(int T) { return T <= 1024 ? 16 : 32; }
+static inline int lora_tile_rows(int T) { return T <= 1024 ? 16 : 64; }
 
 static inline LoraLayout lora_layout(int T, int L) {
   LoraLayout p{};

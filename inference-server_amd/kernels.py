@@ -832,6 +832,9 @@ class LoraPool:
         self.device = a.get_device()
         self._columns = (ctypes.c_int * len(columns))(*columns)
 
+    def _workspace_bytes(self, num_rows: int) -> int:
+        return _lora_workspace_bytes(num_rows, self.num_adapters, self.in_features, self.max_rank, self.columns)
+
     @classmethod
     def empty(cls, num_adapters: int, in_features: int, columns, max_rank: int, device) -> LoraPool:
         """A pool without adapters (every rank 0), to ``load`` into."""
@@ -890,6 +893,12 @@ class LoraPlan:
     @property
     def rows(self) -> torch.Tensor:
         return self.buffer[self._at[1]:self._at[1] + self.num_rows]
+
+
+@functools.lru_cache(maxsize=1024)
+def _lora_workspace_bytes(num_rows: int, num_adapters: int, in_features: int, max_rank: int, columns: tuple) -> int:
+    return _lib.load().moe_mi355x_lora_add_workspace_bytes(num_rows, num_adapters, in_features, max_rank, len(columns),
+                                                           (ctypes.c_int * len(columns))(*columns))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -974,9 +983,12 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, pool: LoraPool, plan: LoraPlan) -
         raise ValueError(f"the pool is on cuda:{pool.device}, the plan on cuda:{dev}")
     y_stride = _rows_apart(y, "y", plan.num_rows, pool.out_features, dev)
     x_stride = _rows_apart(x, "x", plan.num_rows, pool.in_features, dev)
+    nws = pool._workspace_bytes(plan.num_rows)
+    ws = y.new_empty(nws // 2) if nws else None
     _launch("lora_add", dev, _lib.load().moe_mi355x_lora_add, y.data_ptr(), y_stride, x.data_ptr(), x_stride,
             pool.a.data_ptr(), pool.b.data_ptr(), pool.ranks.data_ptr(), pool.scales.data_ptr(), plan.buffer.data_ptr(),
-            plan.num_rows, plan.num_adapters, pool.in_features, pool.max_rank, len(pool.columns), pool._columns, _stream(y))
+            plan.num_rows, plan.num_adapters, pool.in_features, pool.max_rank, len(pool.columns), pool._columns,
+            ws.data_ptr() if nws else None, nws, _stream(y))
     return y
 
 
