@@ -1,13 +1,15 @@
 // What the adapters of a step's rows add to a shared projection: for row t with adapter l, column n in part p of the
 // projection (q, k and v are parts of one), r < rank_l,
 //   u[t, p, r] = sum_k x[t, k] A_l[p R + r, k]          y[t, n] = bf16( y[t, n] + scale_l sum_r u[t, p, r] B_l[n, r] )
-// Both products on the bf16 MFMAs with fp32 sums.  u is split in two bf16 values for the second, u = hi + lo to 2^-17 of
-// it: the 16 ranks of a group times {hi, lo} fill the 32 of an MFMA, so this costs B's operand read twice and no MFMA
-// more than a group of 16 ranks takes anyway.  y enters as the accumulator and is rounded once.
+// with fp32 sums and one rounding, of y.  Bound by bytes: x, y and the adapters in use once each, if a load takes whole
+// lines.  An MFMA operand taken from memory as it lies (a lane a row) makes every lane of a load a request of its own,
+// 16 bytes a clock for each CU; so here consecutive lanes read consecutive bytes everywhere, and operands go through LDS.
 //
-// Two forms over the plan's tiles (up to tile_rows rows of one adapter):
-//   one launch: a workgroup per (tile, run of columns) forms the u of its part by itself;
-//   two: u of every (tile, part, share of K) to the workspace, in fp32, then the columns.
+// Two forms over the plan's tiles (rows of one adapter, lora.h):
+//   few rows (tiles of 4): one launch, a workgroup per (tile, run of columns), which forms the u of its part by
+//     itself; dot products over the lanes, no MFMA;
+//   many (tiles of 64): u of every (tile, part, share of K) to the workspace in fp32, then the columns, both on MFMAs.
+//     For the second product u is split in two bf16 values, u = hi + lo to 2^-17 of it.
 #include "lora.h"
 
 namespace {
@@ -15,7 +17,6 @@ namespace {
 constexpr int kGroup = 16;     // ranks of an MFMA operand
 constexpr int kMaxRank = 128;
 constexpr int kMaxParts = 4;
-constexpr int kCols = 32;      // columns that a wave takes at once
 
 struct LoraArgs {
   uint16_t* y;        // [T][N], rows y_stride values apart
@@ -37,7 +38,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ float lo_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// The first `live` of a lane's 8 values: ranks that the adapter has
+// The first `live` of 8 values: ranks that the adapter has
 __device__ __forceinline__ uint4 mask8(uint4 v, int live) {
   auto keep = [&](uint32_t w, int i) __attribute__((always_inline)) {
     return live >= i + 2 ? w : live == i + 1 ? w & 0xffffu : 0u;
@@ -45,131 +46,24 @@ __device__ __forceinline__ uint4 mask8(uint4 v, int live) {
   return make_uint4(keep(v.x, 0), keep(v.y, 2), keep(v.z, 4), keep(v.w, 6));
 }
 
-// A workgroup's rows: up to 16 MT of a tile
-template <int MT>
-struct Rows {
+// A workgroup's tile.  What the plan says is kept within the step and the pool, whatever it holds.
+struct Tile {
   int l, first, n, rank;  // adapter, first entry of the sorted rows, rows (0: nothing to do), rank
-  int row[MT];            // this lane's, of each 16: l & 15
 
-  __device__ __forceinline__ Rows(const LoraArgs& a, int block, int lane) {
-    const int sub = a.p.tile_rows / (16 * MT), tile = block / sub, at = block % sub * 16 * MT;
+  __device__ __forceinline__ Tile(const LoraArgs& a, int tile) {
     const int4 t = *(const int4*)(a.plan + a.p.tiles + 4L * tile);
     const bool live = tile < a.plan[LH_TILES];
     l = min(max(__builtin_amdgcn_readfirstlane(t.x), 0), a.p.L - 1);
-    first = min(max(__builtin_amdgcn_readfirstlane(t.y) + at, 0), a.p.T - 1);
-    n = live ? min(__builtin_amdgcn_readfirstlane(t.z) - at, 16 * MT) : 0;
+    first = min(max(__builtin_amdgcn_readfirstlane(t.y), 0), a.p.T - 1);
+    n = live ? min(min(__builtin_amdgcn_readfirstlane(t.z), a.p.tile_rows), a.p.T - first) : 0;
     if (n <= 0) return;
     rank = min(a.ranks[l], a.R);
     if (rank <= 0) n = 0;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int i = min(first + min(16 * m + (lane & 15), max(n, 1) - 1), a.p.T - 1);
-      row[m] = min(max(a.plan[a.p.rows + i], 0), a.p.T - 1);
-    }
+  }
+  __device__ __forceinline__ int row(const LoraArgs& a, int i) const {  // of entry first + i
+    return min(max(a.plan[a.p.rows + first + min(i, n - 1)], 0), a.p.T - 1);
   }
 };
-
-// u of 16 MT rows and 16 NG ranks of a part, over the k steps (of 32) k0 .. k1: lane l holds ranks 16 g + 4 (l / 16) + i
-// of row 16 m + l % 16.  kAhead steps' loads are in flight together.
-template <int MT, int NG, int kAhead>
-__device__ __forceinline__ void shrink(const LoraArgs& a, const Rows<MT>& r, int part, int k0, int k1, int lane, v4f (&u)[MT][NG]) {
-  const int lr = lane & 15, lg = lane >> 4;
-  const uint16_t *xr[MT], *ar[NG];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) xr[m] = a.x + r.row[m] * a.x_stride + 8 * lg;
-#pragma unroll
-  for (int g = 0; g < NG; ++g) ar[g] = a.a + (((long)r.l * a.parts + part) * a.R + min(kGroup * g + lr, a.R - 1)) * a.K + 8 * lg;
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int g = 0; g < NG; ++g) u[m][g] = (v4f){0.f, 0.f, 0.f, 0.f};
-  auto steps = [&](int k, auto count) __attribute__((always_inline)) {
-    constexpr int n = decltype(count)::value;
-    uint4 xv[n][MT], av[n][NG];
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) xv[i][m] = *(const uint4*)(xr[m] + 32 * (k + i));
-#pragma unroll
-      for (int g = 0; g < NG; ++g) av[i][g] = *(const uint4*)(ar[g] + 32 * (k + i));
-    }
-#pragma unroll
-    for (int i = 0; i < n; ++i)
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          u[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, av[i][g]), __builtin_bit_cast(v8bf, xv[i][m]),
-                                                            u[m][g], 0, 0, 0);
-  };
-  int k = k0;
-  for (; k + kAhead <= k1; k += kAhead) steps(k, std::integral_constant<int, kAhead>());
-  for (; k < k1; ++k) steps(k, std::integral_constant<int, 1>());
-}
-
-// 4 ranks' u as they enter the second product
-__device__ __forceinline__ void split_u(v4f s, float scale, int live, uint2* hi, uint2* lo) {
-  float v[4], rest[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = e < live ? s[e] * scale : 0.f;
-    const float top = round_bf16(v[e]);
-    rest[e] = fabsf(top) < INFINITY ? v[e] - top : 0.f;  // not inf - inf
-  }
-  *hi = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-  *lo = make_uint2(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]));
-}
-
-template <int MT, int RG>
-struct ULds {
-  uint16_t u[16 * MT][RG][2][kGroup];  // hi, lo
-};
-
-// The columns c0 .. c1 (in one part), 32 at a time for each of kWaves waves
-template <int MT, int NG, int RG, int kWaves>
-__device__ __forceinline__ void expand(const LoraArgs& a, const Rows<MT>& r, const ULds<MT, RG>& lds, int c0, int c1, int lane,
-                                       int wave) {
-  const int lr = lane & 15, lg = lane >> 4;
-  v8bf uv[MT][NG];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int g = 0; g < NG; ++g) uv[m][g] = *(const v8bf*)&lds.u[16 * m + lr][g][lg >> 1][8 * (lg & 1)];
-  // lane l holds columns 4 (l / 16) + i of row l % 16 of each product: two with their columns in turns of 4 make 8
-  // in a row
-  const uint16_t* bl = a.b + ((long)r.l * a.N + 8 * (lr >> 2) + (lr & 3)) * a.R + 8 * (lg & 1);
-  for (int c = c0 + kCols * wave; c < c1; c += kCols * kWaves) {
-    uint4 yv[MT], bv[2][NG];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) yv[m] = *(const uint4*)(a.y + r.row[m] * a.y_stride + c + 8 * lg);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) bv[j][g] = *(const uint4*)(bl + (long)(c + 4 * j) * a.R + min(kGroup * g, a.R - kGroup));
-    v4f acc[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      acc[m][0] = (v4f){lo_of(yv[m].x), hi_of(yv[m].x), lo_of(yv[m].y), hi_of(yv[m].y)};
-      acc[m][1] = (v4f){lo_of(yv[m].z), hi_of(yv[m].z), lo_of(yv[m].w), hi_of(yv[m].w)};
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint4 v = bv[j][g];
-        if (kGroup * (g + 1) > r.rank) v = mask8(v, r.rank - kGroup * g - 8 * (lg & 1));
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, v), uv[m][g], acc[m][j], 0, 0, 0);
-      }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      if (16 * m + lr < r.n)
-        *(uint4*)(a.y + r.row[m] * a.y_stride + c + 8 * lg) =
-            make_uint4(pack2(acc[m][0][0], acc[m][0][1]), pack2(acc[m][0][2], acc[m][0][3]),
-                       pack2(acc[m][1][0], acc[m][1][1]), pack2(acc[m][1][2], acc[m][1][3]));
-  }
-}
 
 // The part and the columns of run `run` (every part has its own runs)
 __device__ __forceinline__ void run_of(const LoraArgs& a, int run, int* part, int* c0, int* c1) {
@@ -185,7 +79,7 @@ __device__ __forceinline__ void run_of(const LoraArgs& a, int run, int* part, in
   *c1 = min(*c0 + a.chunk, a.col[p + 1]);
 }
 
-// fn of the number of 16-rank groups that the adapter has: 1, 2, 4 or 8 as a constant
+// fn of the number of 16-rank groups that `rank` takes, 1, 2, 4 or 8 (RG at most), as a constant
 template <int RG, typename F>
 __device__ __forceinline__ void by_groups(int rank, F fn) {
   if (RG == 1 || rank <= 16) return fn(std::integral_constant<int, 1>());
@@ -196,94 +90,414 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
   if constexpr (RG >= 8) return fn(std::integral_constant<int, 8>());
 }
 
+// ---------------------------------------------------------------------------
+// few rows.  u: a wave takes every eighth rank, its lanes 8 values of a row each; the sums over the lanes go to LDS.
+// Columns: kLanes lanes have 8 ranks of a column each, a wave 64 columns at a time; over kLanes turns lane i
+// ends with the sum of column i.
+// ---------------------------------------------------------------------------
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+constexpr int kFewRows = 4;
+
+__device__ __forceinline__ float dot8(v4i a, v4i b, float c) {
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, (int)a[i]), __builtin_bit_cast(v2bf, (int)b[i]), c, false);
+  return c;
+}
+
+// Sum over kLanes adjacent lanes
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float s) {
+  return s + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(s), CTRL, 0xf, 0xf, false));
+}
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float s) {
+  s = dpp_add<0xb1>(s);                              // of a pair
+  if constexpr (kLanes >= 4) s = dpp_add<0x4e>(s);   // of 4: the other pair
+  if constexpr (kLanes >= 8) s = dpp_add<0x141>(s);  // of 8, mirrored
+  if constexpr (kLanes >= 16) s = dpp_add<0x140>(s);  // of 16, mirrored
+  return s;
+}
+
+// 64 columns' operands: lane's 8 ranks of kLanes columns, and its own column of each row
+template <int NR, int kLanes>
+struct FewColumns {
+  v4i b[kLanes];
+  uint16_t y[NR];
+
+  __device__ __forceinline__ void load(const LoraArgs& a, const Tile& t, const int (&row)[NR], int c, int end, int lane) {
+    const int sub = lane % kLanes, group = lane / kLanes * kLanes;
+    const uint16_t* src = a.b + (long)t.l * a.N * a.R + (8 * sub < t.rank ? 8 * sub : 0);
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) b[i] = *(const v4i*)(src + (long)min(c + group + i, end - 1) * a.R);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) y[r] = a.y[row[r] * a.y_stride + min(c + lane, end - 1)];
+  }
+  // mask: of the lane's 8 ranks those that the adapter has
+  __device__ __forceinline__ void add(const LoraArgs& a, const Tile& t, const int (&row)[NR], int c, int end, int lane, uint4 mask,
+                                      const float (&u)[NR][8]) {
+    const int sub = lane % kLanes;
+    float sum[NR];
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) {
+      const uint32_t w[4] = {(uint32_t)b[i][0] & mask.x, (uint32_t)b[i][1] & mask.y, (uint32_t)b[i][2] & mask.z,
+                             (uint32_t)b[i][3] & mask.w};
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fmaf(hi_of(w[e]), u[r][2 * e + 1], fmaf(lo_of(w[e]), u[r][2 * e], s));
+        s = lanes_sum<kLanes>(s);
+        sum[r] = i == 0 || sub == i ? s : sum[r];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+      if (r < t.n && c + lane < end) a.y[row[r] * a.y_stride + c + lane] = f32_to_bf16(bf16_to_f32(y[r]) + sum[r]);
+  }
+};
+
+// kLanes: of a column; 8 kLanes ranks at most, kLanes of them a wave's
+template <int NR, int kLanes>
+__device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, int part, int c0, int c1, int lane, int wave,
+                                         float (&s_u)[kFewRows][8 * kLanes]) {
+  int row[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) row[r] = __builtin_amdgcn_readfirstlane(t.row(a, r));
+  const float scale = a.scales[t.l];
+  // a wave's columns side by side; the first 64 on their way before u
+  const int per = (c1 - c0 + 64 * kFewWaves - 1) / (64 * kFewWaves) * 64, end = min(c0 + (wave + 1) * per, c1);
+  int c = c0 + wave * per;
+  constexpr bool kEarly = NR * kLanes <= 16;  // where there are registers for them
+  FewColumns<NR, kLanes> now;
+  if (kEarly && c < end) now.load(a, t, row, c, end, lane);
+
+  float acc[kLanes][NR];
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) acc[i][r] = 0.f;
+  // kTogether ranks by kBlock times 512 values are in flight together
+  constexpr int kTogether = kLanes < 4 ? kLanes : 4, kBlock = NR * kLanes <= 4 ? 8 : 4;
+  const uint16_t* ap = a.a + ((long)t.l * a.parts + part) * a.R * a.K;
+  // No branch around a load: the compiler waits where it joins.  Behind K (`whole` is false) both operands are zeros.
+  auto block = [&](int k0, auto whole) __attribute__((always_inline)) {
+    auto load = [&](const uint16_t* row, int j) __attribute__((always_inline)) {
+      const int k = k0 + 512 * j + 8 * lane;
+      if (whole) return *(const v4i*)(row + k);
+      const v4i v = *(const v4i*)(row + min(k, a.K - 8));
+      const int keep = k < a.K ? -1 : 0;
+      return (v4i){v[0] & keep, v[1] & keep, v[2] & keep, v[3] & keep};
+    };
+    v4i xv[kBlock][NR];
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) xv[j][r] = load(a.x + row[r] * a.x_stride, j);
+#pragma unroll
+    for (int i0 = 0; i0 < kLanes; i0 += kTogether) {
+      if (wave + kFewWaves * i0 < t.rank) {
+        v4i av[kTogether][kBlock];
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j) av[i][j] = load(ap + (long)min(wave + kFewWaves * (i0 + i), t.rank - 1) * a.K, j);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i)
+#pragma unroll
+          for (int j = 0; j < kBlock; ++j)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) acc[i0 + i][r] = dot8(av[i][j], xv[j][r], acc[i0 + i][r]);
+      }
+    }
+  };
+  int k0 = 0;
+  for (; k0 + 512 * kBlock <= a.K; k0 += 512 * kBlock) block(k0, std::true_type());
+  if (k0 < a.K) block(k0, std::false_type());
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) {
+    const int rank = wave + kFewWaves * i;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float s = rank < t.rank ? wave_sum_uniform(acc[i][r]) * scale : 0.f;
+      if (lane == 0) s_u[r][rank] = s;
+    }
+  }
+  __syncthreads();
+  float u[NR][8];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const v4f lo = *(const v4f*)&s_u[r][8 * (lane % kLanes)], hi = *(const v4f*)&s_u[r][8 * (lane % kLanes) + 4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[r][e] = lo[e], u[r][4 + e] = hi[e];
+  }
+  const uint4 mask = mask8(make_uint4(~0u, ~0u, ~0u, ~0u), t.rank - 8 * (lane % kLanes));
+  for (; c < end; c += 64) {
+    if constexpr (kEarly) {
+      FewColumns<NR, kLanes> next;
+      if (c + 64 < end) next.load(a, t, row, c + 64, end, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      now.add(a, t, row, c, end, lane, mask, u);
+      now = next;
+    } else {
+      now.load(a, t, row, c, end, lane);
+      now.add(a, t, row, c, end, lane, mask, u);
+    }
+  }
+}
+
+template <int kLanes>
+__global__ __launch_bounds__(kFewThreads, kLanes <= 4 ? 4 : 2) void lora_few_kernel(LoraArgs a) {
+  __shared__ __attribute__((aligned(16))) float s_u[kFewRows][8 * kLanes];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Tile t(a, blockIdx.y);
+  if (t.n <= 0) return;
+  int part, c0, c1;
+  run_of(a, blockIdx.x, &part, &c0, &c1);
+  if (t.n == 1)
+    few_rows<1, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+  else if (t.n == 2)
+    few_rows<2, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+  else
+    few_rows<4, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+}
+
+// ---------------------------------------------------------------------------
+// many rows: u.  64 rows by up to 64 ranks, 128 k at a time through LDS, of which each of the 4 waves multiplies 32; the
+// next 128 are on their way meanwhile.  In LDS a row has 16 pieces of 8 values, piece c at c ^ (row % 16), so that
+// the 16 rows of an operand lie in different banks.
+// ---------------------------------------------------------------------------
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kRowsM = 64, kMT = kRowsM / 16;
+constexpr int kSlice = 128;
+constexpr int kRanksM = 64;  // of a workgroup
+
+template <int NG>
+struct ShrinkLds {
+  union {
+    struct {
+      v4i a[16 * NG][16], x[kRowsM][16];
+    } slice[2];
+    v4f part[kWaves][kMT][NG][64];
+  };
+};
+
+template <int NG, int RG>
+__device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, int part, int rank0, int s0, int s1, int share, int lane,
+                                       int wave, ShrinkLds<RG>& lds) {
+  const int lr = lane & 15, lg = lane >> 4;
+  const int q = threadIdx.x >> 4, piece = threadIdx.x & 15, to = piece ^ (q & 15);  // rows q + 16 i of both
+  const uint16_t *xr[kMT], *ar[NG];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i) xr[i] = a.x + t.row(a, q + 16 * i) * a.x_stride;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) ar[i] = a.a + (((long)t.l * a.parts + part) * a.R + min(rank0 + q + 16 * i, t.rank - 1)) * a.K;
+  struct Slice {
+    v4i a[NG], x[kMT];
+  } r0, r1, r2, r3;
+  // No branch around a load: the compiler waits where it joins.  Rows and ranks that there are not repeat the last one, and
+  // are not stored; k behind K repeat the last 8, and are not multiplied.
+  auto load = [&](int s, Slice& into) __attribute__((always_inline)) {
+    const int k = min(kSlice * min(s, s1 - 1) + 8 * piece, a.K - 8);
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) into.x[i] = *(const v4i*)(xr[i] + k);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) into.a[i] = *(const v4i*)(ar[i] + k);
+  };
+  auto store = [&](int buf, const Slice& from) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) lds.slice[buf].a[q + 16 * i][to] = from.a[i];
+#pragma unroll
+    for (int i = 0; i < kMT; ++i) lds.slice[buf].x[q + 16 * i][to] = from.x[i];
+  };
+  v4f u[kMT][NG];
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) u[m][g] = (v4f){0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int buf) __attribute__((always_inline)) {
+    const int at = (4 * wave + lg) ^ lr;
+    v8bf xf[kMT], af[NG];
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) xf[m] = __builtin_bit_cast(v8bf, lds.slice[buf].x[16 * m + lr][at]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) af[g] = __builtin_bit_cast(v8bf, lds.slice[buf].a[16 * g + lr][at]);
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) u[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[g], xf[m], u[m][g], 0, 0, 0);
+  };
+  // slice s + 4 is loaded while slice s is multiplied, and goes to LDS during slice s + 3
+  auto turn = [&](int s, int buf, Slice& mine, Slice& after) __attribute__((always_inline)) {
+    load(s + 4, mine);  // these registers went to LDS in the last turn
+    __builtin_amdgcn_sched_barrier(0);
+    if (s < s1 && kSlice * s + 32 * wave < a.K) multiply(buf);
+    store(buf ^ 1, after);  // last read a slice ago, before the last barrier
+    __syncthreads();
+  };
+  load(s0, r0);
+  load(s0 + 1, r1);
+  load(s0 + 2, r2);
+  load(s0 + 3, r3);
+  store(0, r0);
+  __syncthreads();
+  for (int s = s0; s < s1; s += 4) {
+    turn(s, 0, r0, r1);
+    turn(s + 1, 1, r1, r2);
+    turn(s + 2, 0, r2, r3);
+    turn(s + 3, 1, r3, r0);
+  }
+  // lane l has ranks 4 (l / 16) + i of row l % 16 of each: joined over the waves
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) lds.part[wave][m][g][lane] = u[m][g];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kMT * NG * 64; i += kThreads) {
+    const int m = i / (64 * NG), g = i / 64 % NG, row = 16 * m + i % 16, rank = rank0 + kGroup * g + 4 * (i % 64 / 16);
+    v4f sum = lds.part[0][m][g][i % 64];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += lds.part[w][m][g][i % 64];
+    if (row < t.n && rank < a.R) *(v4f*)(a.u + (((long)share * a.p.T + t.first + row) * a.parts + part) * a.R + rank) = sum;
+  }
+}
+
 template <int RG>
-__global__ __launch_bounds__(512) void lora_one_kernel(LoraArgs a) {
-  constexpr int kWaves = 8, kThreads = 64 * kWaves;
-  __shared__ __attribute__((aligned(16))) struct {
-    v4f part[kWaves][RG][64];
-    ULds<1, RG> u;
-  } lds;
+__global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
+  __shared__ __attribute__((aligned(16))) ShrinkLds<RG> lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Rows<1> r(a, blockIdx.y, lane);
-  if (r.n <= 0) return;
-  int part, c0, c1;
-  run_of(a, blockIdx.x, &part, &c0, &c1);
-  const float scale = a.scales[r.l];
-  by_groups<RG>(r.rank, [&](auto groups) __attribute__((always_inline)) {
-    constexpr int NG = decltype(groups)::value;
-    v4f u[1][NG];
-    const int steps = a.K / 32, per = (steps + kWaves - 1) / kWaves;
-    shrink<1, NG, (NG <= 2 ? 8 : NG <= 4 ? 4 : 2)>(a, r, part, min(wave * per, steps), min((wave + 1) * per, steps), lane, u);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) lds.part[wave][g][lane] = u[0][g];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NG * 64; i += kThreads) {
-      const int g = i / 64, r0 = 4 * (i % 64 / 16);
-      v4f s = lds.part[0][g][i % 64];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) s += lds.part[w][g][i % 64];
-      split_u(s, scale, r.rank - kGroup * g - r0, (uint2*)&lds.u.u[i % 16][g][0][r0], (uint2*)&lds.u.u[i % 16][g][1][r0]);
-    }
-    __syncthreads();
-    expand<1, NG, RG, kWaves>(a, r, lds.u, c0, c1, lane, wave);
+  const Tile t(a, blockIdx.y);
+  if (t.n <= 0) return;
+  const int part = blockIdx.x % a.parts, share = blockIdx.x / a.parts % a.shares, rank0 = blockIdx.x / a.parts / a.shares * kRanksM;
+  if (rank0 >= t.rank) return;
+  const int slices = (a.K + kSlice - 1) / kSlice, per = (slices + a.shares - 1) / a.shares;
+  const int s0 = min(share * per, slices), s1 = min(s0 + per, slices);
+  if (s0 >= s1) return;
+  by_groups<RG>(t.rank - rank0, [&](auto groups) __attribute__((always_inline)) {
+    shrink<decltype(groups)::value, RG>(a, t, part, rank0, s0, s1, share, lane, wave, lds);
   });
 }
 
-template <int MT, int RG>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
-  constexpr int kWaves = 4, kThreads = 64 * kWaves;
-  __shared__ __attribute__((aligned(16))) v4f lds[kWaves][MT][RG][64];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Rows<MT> r(a, blockIdx.y, lane);
-  if (r.n <= 0) return;
-  const int part = blockIdx.x % a.parts, share = blockIdx.x / a.parts;
-  by_groups<RG>(r.rank, [&](auto groups) __attribute__((always_inline)) {
-    constexpr int NG = decltype(groups)::value;
-    v4f u[MT][NG];
-    const int steps = a.K / 32, per = (steps + a.shares * kWaves - 1) / (a.shares * kWaves), at = (share * kWaves + wave) * per;
-    shrink<MT, NG, (MT + NG <= 3 ? 8 : MT + NG <= 6 ? 4 : 2)>(a, r, part, min(at, steps), min(at + per, steps), lane, u);
+// ---------------------------------------------------------------------------
+// many rows: columns.  A wave has 16 of the 64 rows, all of them 128 columns of B at a time, through LDS.  Lane l has 8
+// columns in a row, from 8 (l % 16), of rows 4 (l / 16) + i: column 8 (l % 16) + j is column l % 16 of product j,
+// and B's columns lie in LDS in that order.
+// ---------------------------------------------------------------------------
+constexpr int kPiece = 128;
+
+// 4 ranks' u as they enter the product
+__device__ __forceinline__ void split_u(v4f s, float scale, int live, uint2* hi, uint2* lo) {
+  float v[4], rest[4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) lds[wave][m][g][lane] = u[m][g];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * NG * 64; i += kThreads) {
-      const int m = i / (64 * NG), g = i / 64 % NG, row = 16 * m + i % 16;
-      v4f s = lds[0][m][g][i % 64];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) s += lds[w][m][g][i % 64];
-      const int rank0 = kGroup * g + 4 * (i % 64 / 16);
-      if (row < r.n && rank0 < a.R)
-        *(v4f*)(a.u + (((long)share * a.p.T + r.first + row) * a.parts + part) * a.R + rank0) = s;
-    }
-  });
+  for (int e = 0; e < 4; ++e) {
+    v[e] = e < live ? s[e] * scale : 0.f;
+    const float top = round_bf16(v[e]);
+    rest[e] = fabsf(top) < INFINITY ? v[e] - top : 0.f;  // not inf - inf
+  }
+  *hi = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+  *lo = make_uint2(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]));
 }
 
-template <int MT, int RG>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
-  constexpr int kWaves = 4, kThreads = 64 * kWaves;
-  __shared__ __attribute__((aligned(16))) ULds<MT, RG> lds;
+template <int NG>
+struct ExpandLds {
+  static constexpr int kRow = 32 * NG + 16;  // bytes of a column, 16 of them so that 8 columns' banks differ
+  uint16_t u[kRowsM][2][16 * NG + 8];        // hi, lo
+  uint8_t b[kPiece * kRow];
+};
+
+template <int NG>
+__device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, int part, int c0, int c1, int lane, int wave,
+                                       ExpandLds<NG>& lds) {
+  constexpr int kRow = ExpandLds<NG>::kRow;
+  const int lr = lane & 15, lg = lane >> 4;
+  const float scale = a.scales[t.l];
+  const uint16_t* bl = a.b + (long)t.l * a.N * a.R;
+  uint16_t* yr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) yr[i] = a.y + t.row(a, 16 * wave + 4 * lg + i) * a.y_stride;
+
+  // No branch around a load: columns behind the run repeat its last ones, and are not stored
+  uint4 bv[NG], yv[4];
+  auto load = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) yv[i] = *(const uint4*)(yr[i] + min(c + 8 * lr, c1 - 8));
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int at = threadIdx.x + kThreads * i, n = at / (2 * NG), r = at % (2 * NG) * 8;
+      bv[i] = *(const uint4*)(bl + (long)min(c + n, c1 - 1) * a.R + (r < t.rank ? r : 0));
+    }
+  };
+  auto store_b = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int at = threadIdx.x + kThreads * i, n = at / (2 * NG), r = at % (2 * NG) * 8;
+      *(uint4*)(lds.b + (n % 8 * 16 + n / 8) * kRow + 2 * r) = mask8(bv[i], t.rank - r);
+    }
+  };
+  load(c0);
+  for (int i = threadIdx.x; i < kRowsM * NG * 4; i += kThreads) {
+    const int row = min(i / (NG * 4), t.n - 1), r0 = 4 * (i % (NG * 4));
+    const float* src = a.u + (((long)t.first + row) * a.parts + part) * a.R + (r0 < t.rank ? r0 : 0);
+    v4f s = *(const v4f*)src;
+    for (int z = 1; z < a.shares; ++z) s += *(const v4f*)(src + (long)z * a.p.T * a.parts * a.R);
+    split_u(s, scale, t.rank - r0, (uint2*)&lds.u[i / (NG * 4)][0][r0], (uint2*)&lds.u[i / (NG * 4)][1][r0]);
+  }
+  store_b();
+  __syncthreads();
+  // 16 ranks: hi and lo fill the 32 of one MFMA, against B twice; more: 32 ranks of hi, then of lo
+  constexpr int kSteps = NG == 1 ? 1 : NG / 2;
+  v8bf uv[kSteps][2];
+#pragma unroll
+  for (int g = 0; g < kSteps; ++g)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      uv[g][h] = NG == 1 ? *(const v8bf*)&lds.u[16 * wave + lr][lg >> 1][8 * (lg & 1)] : *(const v8bf*)&lds.u[16 * wave + lr][h][32 * g + 8 * lg];
+  for (int c = c0; c < c1; c += kPiece) {
+    v4f acc[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j][i] = j % 2 ? hi_of(w[j / 2]) : lo_of(w[j / 2]);
+    }
+    load(min(c + kPiece, c1 - 1));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int g = 0; g < kSteps; ++g) {
+        const v8bf b = *(const v8bf*)(lds.b + (16 * j + lr) * kRow + (NG == 1 ? 16 * (lg & 1) : 64 * g + 16 * lg));
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][0], b, acc[j], 0, 0, 0);
+        if (NG > 1) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][1], b, acc[j], 0, 0, 0);
+      }
+    __syncthreads();  // B's columns are read
+    if (c + 8 * lr < c1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * wave + 4 * lg + i < t.n)
+          *(uint4*)(yr[i] + c + 8 * lr) = make_uint4(pack2(acc[0][i], acc[1][i]), pack2(acc[2][i], acc[3][i]),
+                                                     pack2(acc[4][i], acc[5][i]), pack2(acc[6][i], acc[7][i]));
+    store_b();
+    __syncthreads();
+  }
+}
+
+template <int RG>
+__global__ __launch_bounds__(kThreads, RG <= 4 ? 4 : 2) void lora_expand_kernel(LoraArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[sizeof(ExpandLds<RG>)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Rows<MT> r(a, blockIdx.y, lane);
-  if (r.n <= 0) return;
+  const Tile t(a, blockIdx.y);
+  if (t.n <= 0) return;
   int part, c0, c1;
   run_of(a, blockIdx.x, &part, &c0, &c1);
-  const float scale = a.scales[r.l];
-  by_groups<RG>(r.rank, [&](auto groups) __attribute__((always_inline)) {
+  by_groups<RG>(t.rank, [&](auto groups) __attribute__((always_inline)) {
     constexpr int NG = decltype(groups)::value;
-    for (int i = threadIdx.x; i < 16 * MT * NG * 4; i += kThreads) {
-      const int row = i / (NG * 4), r0 = 4 * (i % (NG * 4)), from = min(row, r.n - 1);
-      v4f s = {0.f, 0.f, 0.f, 0.f};
-      const float* src = a.u + (((long)r.first + from) * a.parts + part) * a.R + min(r0, a.R - 4);
-      for (int z = 0; z < a.shares; ++z) s += *(const v4f*)(src + (long)z * a.p.T * a.parts * a.R);
-      uint16_t* dst = &lds.u[row][r0 / kGroup][0][r0 % kGroup];
-      split_u(s, scale, r.rank - r0, (uint2*)dst, (uint2*)(dst + kGroup));
-    }
-    __syncthreads();
-    expand<MT, NG, RG, kWaves>(a, r, lds, c0, c1, lane, wave);
+    expand<NG>(a, t, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
   });
 }
 
@@ -292,57 +506,45 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
          parts <= kMaxParts;
 }
 
-// Which form a call takes, and its shape
-struct LoraForm {
-  bool one;
-  int shares, mt, chunk;
-};
-#ifndef LORA_ONE
-#define LORA_ONE 0
-#endif
+// How a call is cut up
 #ifndef LORA_CHUNK
 #define LORA_CHUNK 512
 #endif
-#ifndef LORA_MT
-#define LORA_MT 4
+#ifndef LORA_FEW
+#define LORA_FEW 1024
 #endif
 #ifndef LORA_WGS
 #define LORA_WGS 256
 #endif
+struct LoraForm {
+  bool few;
+  int shares, chunk;
+};
 LoraForm lora_form(const LoraLayout& p, int K, int R, int parts, int N) {
-  LoraForm f{};
-  f.one = p.tile_rows == 16 && LORA_ONE;
-  f.mt = p.tile_rows == 16 ? 1 : R > 64 ? 2 : LORA_MT;
-  f.shares = 1;
-  if (!f.one)
+  LoraForm f{p.tile_rows == kFewRows, 1, LORA_CHUNK};
+  if (f.few)
+    for (f.chunk = 512; f.chunk < 4096 && (long)p.N * N / f.chunk > LORA_FEW; f.chunk *= 2) {
+    }
+  else
     while (f.shares < 8 && p.N * parts * f.shares < LORA_WGS && K / (2 * f.shares) >= 512) f.shares *= 2;
-  f.chunk = LORA_CHUNK;
-  if (f.mt == 1) f.chunk = p.N * N / 256 > 1024 ? 512 : 256;
-  if (f.mt == 1 && !f.one) f.chunk /= 2;
   return f;
 }
 
 size_t lora_ws(const LoraLayout& p, const LoraForm& f, int R, int parts) {
-  return f.one ? 0 : moe_align_up((size_t)f.shares * p.T * parts * R * sizeof(float), 256);
+  return f.few ? 0 : moe_align_up((size_t)f.shares * p.T * parts * R * sizeof(float), 256);
 }
 
 template <int RG>
 void launch(const LoraArgs& g, const LoraForm& f, int runs, hipStream_t s) {
-  if (f.one) {
-    hipLaunchKernelGGL((lora_one_kernel<RG>), dim3(runs, g.p.N), dim3(512), 0, s, g);
+  const dim3 columns(runs, g.p.N);
+  if (f.few) {
+    hipLaunchKernelGGL((lora_few_kernel<2 * RG>), columns, dim3(kFewThreads), 0, s, g);
     return;
   }
-  const int blocks = g.p.N * (g.p.tile_rows / (16 * f.mt));
-  const dim3 first(g.parts * g.shares, blocks), second(runs, blocks);
-#define LORA_LAUNCH(MT)                                                                       \
-  do {                                                                                        \
-    hipLaunchKernelGGL((lora_shrink_kernel<MT, RG>), first, dim3(256), 0, s, g);              \
-    hipLaunchKernelGGL((lora_expand_kernel<MT, RG>), second, dim3(256), 0, s, g);             \
-  } while (0)
-  if (f.mt == 1) LORA_LAUNCH(1);
-  else if (f.mt == 2) LORA_LAUNCH(2);
-  else if constexpr (RG <= 4) LORA_LAUNCH(4);
-#undef LORA_LAUNCH
+  constexpr int NG = RG < 4 ? RG : 4;
+  const dim3 first(g.parts * g.shares * ((g.R + kRanksM - 1) / kRanksM), g.p.N);
+  hipLaunchKernelGGL((lora_shrink_kernel<NG>), first, dim3(kThreads), 0, s, g);
+  hipLaunchKernelGGL((lora_expand_kernel<RG>), columns, dim3(kThreads), 0, s, g);
 }
 
 }  // namespace
@@ -364,7 +566,7 @@ extern "C" int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, l
   LoraArgs g{};
   long n = 0;
   for (int p = 0; p < parts; ++p) {
-    MOE_RETURN_IF(columns[p] <= 0 || columns[p] % kCols, MOE_ERR_INVALID_ARG);
+    MOE_RETURN_IF(columns[p] <= 0 || columns[p] % 32, MOE_ERR_INVALID_ARG);
     n += columns[p];
     MOE_RETURN_IF(n > (1 << 24), MOE_ERR_INVALID_ARG);
     g.col[p + 1] = (int)n;
