@@ -24,7 +24,8 @@ struct LoraLayout {
 static inline bool lora_plan_ok(int T, int L) { return T >= 0 && T <= kLoraMaxRows && L >= 1 && L <= kLoraMaxAdapters; }
 
 // Rows of a tile: few, where each may have an adapter of its own, or many, which share the reading of theirs.
-static inline int lora_tile_rows(int T) { return T <= 256 ? 4 : 64; }
+constexpr int kLoraFewRows = 2;
+static inline int lora_tile_rows(int T) { return T <= 256 ? kLoraFewRows : 64; }
 
 static inline LoraLayout lora_layout(int T, int L) {
   LoraLayout p{};

@@ -28,7 +28,7 @@ struct LoraArgs {
   const int32_t* plan;
   float* u;               // [shares][T][P][R], rows in the plan's order
   LoraLayout p;
-  int K, R, N, parts, shares, chunk;  // chunk: columns of a workgroup, in one part
+  int K, R, N, parts, shares, chunk, runs;  // chunk: columns of a workgroup, in one part; runs: of them in all parts
   int col[kMaxParts + 1];             // where the parts begin
 };
 
@@ -51,8 +51,8 @@ struct Tile {
   int l, first, n, rank;  // adapter, first entry of the sorted rows, rows (0: nothing to do), rank
 
   __device__ __forceinline__ Tile(const LoraArgs& a, int tile) {
-    const int4 t = *(const int4*)(a.plan + a.p.tiles + 4L * tile);
-    const bool live = tile < a.plan[LH_TILES];
+    const int4 t = *(const int4*)(a.plan + a.p.tiles + 4L * min(tile, a.p.N - 1));
+    const bool live = tile < min(a.plan[LH_TILES], a.p.N);
     l = min(max(__builtin_amdgcn_readfirstlane(t.x), 0), a.p.L - 1);
     first = min(max(__builtin_amdgcn_readfirstlane(t.y), 0), a.p.T - 1);
     n = live ? min(min(__builtin_amdgcn_readfirstlane(t.z), a.p.tile_rows), a.p.T - first) : 0;
@@ -64,6 +64,12 @@ struct Tile {
     return min(max(a.plan[a.p.rows + first + min(i, n - 1)], 0), a.p.T - 1);
   }
 };
+
+// Workgroups that follow each other go to different XCDs (8): those of one tile, which share its rows of x and its
+// adapter, are 8 apart, so that they find them in one L2.
+__device__ __forceinline__ int tile_of(int per_tile) { return blockIdx.x / 8 / per_tile * 8 + blockIdx.x % 8; }
+__device__ __forceinline__ int turn_of(int per_tile) { return blockIdx.x / 8 % per_tile; }
+unsigned lora_grid(int tiles, int per_tile) { return (unsigned)((tiles + 7) / 8 * 8 * per_tile); }
 
 // The part and the columns of run `run` (every part has its own runs)
 __device__ __forceinline__ void run_of(const LoraArgs& a, int run, int* part, int* c0, int* c1) {
@@ -95,8 +101,17 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
 // Columns: kLanes lanes have 8 ranks of a column each, a wave 64 columns at a time; over kLanes turns lane i
 // ends with the sum of column i.
 // ---------------------------------------------------------------------------
+#ifndef LORA_KB
+#define LORA_KB 4
+#endif
+#ifndef LORA_TG
+#define LORA_TG 4
+#endif
+#ifndef LORA_LB
+#define LORA_LB
+#endif
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
-constexpr int kFewRows = 4;
+constexpr int kFewRows = kLoraFewRows;
 
 __device__ __forceinline__ float dot8(v4i a, v4i b, float c) {
   typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -179,7 +194,7 @@ __device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, int p
 #pragma unroll
     for (int r = 0; r < NR; ++r) acc[i][r] = 0.f;
   // kTogether ranks by kBlock times 512 values are in flight together
-  constexpr int kTogether = kLanes < 4 ? kLanes : 4, kBlock = NR * kLanes <= 4 ? 8 : 4;
+  constexpr int kTogether = kLanes < LORA_TG ? kLanes : LORA_TG, kBlock = LORA_KB;
   const uint16_t* ap = a.a + ((long)t.l * a.parts + part) * a.R * a.K;
   // No branch around a load: the compiler waits where it joins.  Behind K (`whole` is false) both operands are zeros.
   auto block = [&](int k0, auto whole) __attribute__((always_inline)) {
@@ -249,20 +264,18 @@ __device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, int p
 }
 
 template <int kLanes>
-__global__ __launch_bounds__(kFewThreads, kLanes <= 4 ? 4 : 2) void lora_few_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kFewThreads LORA_LB) void lora_few_kernel(LoraArgs a) {
   __shared__ __attribute__((aligned(16))) float s_u[kFewRows][8 * kLanes];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile t(a, blockIdx.y);
+  const Tile t(a, tile_of(a.runs));
   if (t.n <= 0) return;
   int part, c0, c1;
-  run_of(a, blockIdx.x, &part, &c0, &c1);
+  run_of(a, turn_of(a.runs), &part, &c0, &c1);
   if (t.n == 1)
     few_rows<1, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
-  else if (t.n == 2)
-    few_rows<2, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
   else
-    few_rows<4, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+    few_rows<kFewRows, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
 }
 
 // ---------------------------------------------------------------------------
@@ -370,9 +383,10 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   __shared__ __attribute__((aligned(16))) ShrinkLds<RG> lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile t(a, blockIdx.y);
+  const int blocks = a.parts * a.shares * ((a.R + kRanksM - 1) / kRanksM), at = turn_of(blocks);
+  const Tile t(a, tile_of(blocks));
   if (t.n <= 0) return;
-  const int part = blockIdx.x % a.parts, share = blockIdx.x / a.parts % a.shares, rank0 = blockIdx.x / a.parts / a.shares * kRanksM;
+  const int part = at % a.parts, share = at / a.parts % a.shares, rank0 = at / a.parts / a.shares * kRanksM;
   if (rank0 >= t.rank) return;
   const int slices = (a.K + kSlice - 1) / kSlice, per = (slices + a.shares - 1) / a.shares;
   const int s0 = min(share * per, slices), s1 = min(s0 + per, slices);
@@ -491,10 +505,10 @@ __global__ __launch_bounds__(kThreads, RG <= 4 ? 4 : 2) void lora_expand_kernel(
   __shared__ __attribute__((aligned(16))) uint8_t lds[sizeof(ExpandLds<RG>)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile t(a, blockIdx.y);
+  const Tile t(a, tile_of(a.runs));
   if (t.n <= 0) return;
   int part, c0, c1;
-  run_of(a, blockIdx.x, &part, &c0, &c1);
+  run_of(a, turn_of(a.runs), &part, &c0, &c1);
   by_groups<RG>(t.rank, [&](auto groups) __attribute__((always_inline)) {
     constexpr int NG = decltype(groups)::value;
     expand<NG>(a, t, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
@@ -535,15 +549,14 @@ size_t lora_ws(const LoraLayout& p, const LoraForm& f, int R, int parts) {
 }
 
 template <int RG>
-void launch(const LoraArgs& g, const LoraForm& f, int runs, hipStream_t s) {
-  const dim3 columns(runs, g.p.N);
+void launch(const LoraArgs& g, const LoraForm& f, hipStream_t s) {
+  const dim3 columns(lora_grid(g.p.N, g.runs));
   if (f.few) {
     hipLaunchKernelGGL((lora_few_kernel<2 * RG>), columns, dim3(kFewThreads), 0, s, g);
     return;
   }
-  constexpr int NG = RG < 4 ? RG : 4;
-  const dim3 first(g.parts * g.shares * ((g.R + kRanksM - 1) / kRanksM), g.p.N);
-  hipLaunchKernelGGL((lora_shrink_kernel<NG>), first, dim3(kThreads), 0, s, g);
+  const dim3 first(lora_grid(g.p.N, g.parts * g.shares * ((g.R + kRanksM - 1) / kRanksM)));
+  hipLaunchKernelGGL((lora_shrink_kernel<(RG < 4 ? RG : 4)>), first, dim3(kThreads), 0, s, g);
   hipLaunchKernelGGL((lora_expand_kernel<RG>), columns, dim3(kThreads), 0, s, g);
 }
 
@@ -586,17 +599,17 @@ extern "C" int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, l
   g.a = (const uint16_t*)a, g.b = (const uint16_t*)b, g.ranks = ranks, g.scales = scales;
   g.plan = (const int32_t*)plan, g.u = (float*)workspace;
   g.K = K, g.R = R, g.N = (int)n, g.parts = parts, g.shares = f.shares, g.chunk = f.chunk;
-  int runs = 0;
-  for (int p = 0; p < parts; ++p) runs += (columns[p] + f.chunk - 1) / f.chunk;
+  for (int p = 0; p < parts; ++p) g.runs += (columns[p] + f.chunk - 1) / f.chunk;
+  MOE_RETURN_IF(!moe_grid_fits((long)(g.p.N + 7) * g.runs), MOE_ERR_INVALID_ARG);
   hipStream_t s = (hipStream_t)stream;
   if (R <= 16)
-    launch<1>(g, f, runs, s);
+    launch<1>(g, f, s);
   else if (R <= 32)
-    launch<2>(g, f, runs, s);
+    launch<2>(g, f, s);
   else if (R <= 64)
-    launch<4>(g, f, runs, s);
+    launch<4>(g, f, s);
   else
-    launch<8>(g, f, runs, s);
+    launch<8>(g, f, s);
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }

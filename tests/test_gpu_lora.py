@@ -47,7 +47,7 @@ def test_plan_by_row(pkg, dev, T, L):
     rows, offsets = plan_ref(ids, L)
     assert np.array_equal(plan.rows.cpu().numpy(), rows) and np.array_equal(plan.offsets.cpu().numpy(), offsets)
     tiles, room = tiles_of(pkg, plan)
-    height = 4 if T <= 256 else 64
+    height = 2 if T <= 256 else 64
     want = [(l, o, min(height, offsets[l + 1] - o), 0) for l in range(L) for o in range(offsets[l], offsets[l + 1], height)]
     assert len(want) <= room and np.array_equal(tiles, np.asarray(want).reshape(-1, 4))
 
