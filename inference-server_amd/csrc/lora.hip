@@ -46,23 +46,27 @@ __device__ __forceinline__ uint4 mask8(uint4 v, int live) {
   return make_uint4(keep(v.x, 0), keep(v.y, 2), keep(v.z, 4), keep(v.w, 6));
 }
 
-// A workgroup's tile.  What the plan says is kept within the step and the pool, whatever it holds.
+// A workgroup's tile.  What the plan says is kept within the step and the pool, whatever it holds (behind its last tile,
+// anything), so that the rows and the adapter can be asked for before it is known whether there is work: `n` > 0.
 struct Tile {
-  int l, first, n, rank;  // adapter, first entry of the sorted rows, rows (0: nothing to do), rank
+  int l, first, n, rank;  // adapter, first entry of the sorted rows, rows, rank
 
   __device__ __forceinline__ Tile(const LoraArgs& a, int tile) {
     const int4 t = *(const int4*)(a.plan + a.p.tiles + 4L * min(tile, a.p.N - 1));
-    const bool live = tile < min(a.plan[LH_TILES], a.p.N);
+    const int tiles = min(a.plan[LH_TILES], a.p.N);
     l = min(max(__builtin_amdgcn_readfirstlane(t.x), 0), a.p.L - 1);
     first = min(max(__builtin_amdgcn_readfirstlane(t.y), 0), a.p.T - 1);
-    n = live ? min(min(__builtin_amdgcn_readfirstlane(t.z), a.p.tile_rows), a.p.T - first) : 0;
-    if (n <= 0) return;
     rank = min(a.ranks[l], a.R);
-    if (rank <= 0) n = 0;
+    const int rows = min(min(__builtin_amdgcn_readfirstlane(t.z), a.p.tile_rows), a.p.T - first);
+    n = tile < tiles && rank > 0 ? rows : 0;
+    last = max(rows, 1) - 1;
   }
-  __device__ __forceinline__ int row(const LoraArgs& a, int i) const {  // of entry first + i
-    return min(max(a.plan[a.p.rows + first + min(i, n - 1)], 0), a.p.T - 1);
+  __device__ __forceinline__ int row(const LoraArgs& a, int i) const {  // of entry first + i, or of the last one
+    return min(max(a.plan[a.p.rows + first + min(i, last)], 0), a.p.T - 1);
   }
+
+ private:
+  int last;
 };
 
 // Workgroups that follow each other go to different XCDs (8): those of one tile, which share its rows of x and its
@@ -105,7 +109,7 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
 #define LORA_KB 4
 #endif
 #ifndef LORA_TG
-#define LORA_TG 4
+#define LORA_TG 2
 #endif
 #ifndef LORA_LB
 #define LORA_LB
@@ -175,11 +179,11 @@ struct FewColumns {
 
 // kLanes: of a column; 8 kLanes ranks at most, kLanes of them a wave's
 template <int NR, int kLanes>
-__device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, int part, int c0, int c1, int lane, int wave,
-                                         float (&s_u)[kFewRows][8 * kLanes]) {
+__device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, const int (&rows)[kFewRows], int part, int c0, int c1,
+                                         int lane, int wave, float (&s_u)[kFewRows][8 * kLanes]) {
   int row[NR];
 #pragma unroll
-  for (int r = 0; r < NR; ++r) row[r] = __builtin_amdgcn_readfirstlane(t.row(a, r));
+  for (int r = 0; r < NR; ++r) row[r] = rows[r];
   const float scale = a.scales[t.l];
   // a wave's columns side by side; the first 64 on their way before u
   const int per = (c1 - c0 + 64 * kFewWaves - 1) / (64 * kFewWaves) * 64, end = min(c0 + (wave + 1) * per, c1);
@@ -269,13 +273,16 @@ __global__ __launch_bounds__(kFewThreads LORA_LB) void lora_few_kernel(LoraArgs 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile t(a, tile_of(a.runs));
-  if (t.n <= 0) return;
+  int row[kFewRows];
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r) row[r] = __builtin_amdgcn_readfirstlane(t.row(a, r));
   int part, c0, c1;
   run_of(a, turn_of(a.runs), &part, &c0, &c1);
+  if (t.n <= 0) return;
   if (t.n == 1)
-    few_rows<1, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+    few_rows<1, kLanes>(a, t, row, part, c0, c1, lane, wave, s_u);
   else
-    few_rows<kFewRows, kLanes>(a, t, part, c0, c1, lane, wave, s_u);
+    few_rows<kFewRows, kLanes>(a, t, row, part, c0, c1, lane, wave, s_u);
 }
 
 // ---------------------------------------------------------------------------
@@ -299,13 +306,11 @@ struct ShrinkLds {
 };
 
 template <int NG, int RG>
-__device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, int part, int rank0, int s0, int s1, int share, int lane,
+__device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const uint16_t* const (&xr)[kMT], int part, int rank0, int s0, int s1, int share, int lane,
                                        int wave, ShrinkLds<RG>& lds) {
   const int lr = lane & 15, lg = lane >> 4;
   const int q = threadIdx.x >> 4, piece = threadIdx.x & 15, to = piece ^ (q & 15);  // rows q + 16 i of both
-  const uint16_t *xr[kMT], *ar[NG];
-#pragma unroll
-  for (int i = 0; i < kMT; ++i) xr[i] = a.x + t.row(a, q + 16 * i) * a.x_stride;
+  const uint16_t* ar[NG];
 #pragma unroll
   for (int i = 0; i < NG; ++i) ar[i] = a.a + (((long)t.l * a.parts + part) * a.R + min(rank0 + q + 16 * i, t.rank - 1)) * a.K;
   struct Slice {
@@ -385,6 +390,9 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int blocks = a.parts * a.shares * ((a.R + kRanksM - 1) / kRanksM), at = turn_of(blocks);
   const Tile t(a, tile_of(blocks));
+  const uint16_t* xr[kMT];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i) xr[i] = a.x + t.row(a, threadIdx.x / 16 + 16 * i) * a.x_stride;
   if (t.n <= 0) return;
   const int part = at % a.parts, share = at / a.parts % a.shares, rank0 = at / a.parts / a.shares * kRanksM;
   if (rank0 >= t.rank) return;
@@ -392,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   const int s0 = min(share * per, slices), s1 = min(s0 + per, slices);
   if (s0 >= s1) return;
   by_groups<RG>(t.rank - rank0, [&](auto groups) __attribute__((always_inline)) {
-    shrink<decltype(groups)::value, RG>(a, t, part, rank0, s0, s1, share, lane, wave, lds);
+    shrink<decltype(groups)::value, RG>(a, t, xr, part, rank0, s0, s1, share, lane, wave, lds);
   });
 }
 
@@ -424,16 +432,12 @@ struct ExpandLds {
 };
 
 template <int NG>
-__device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, int part, int c0, int c1, int lane, int wave,
+__device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_t* const (&yr)[4], int part, int c0, int c1, int lane, int wave,
                                        ExpandLds<NG>& lds) {
   constexpr int kRow = ExpandLds<NG>::kRow;
   const int lr = lane & 15, lg = lane >> 4;
   const float scale = a.scales[t.l];
   const uint16_t* bl = a.b + (long)t.l * a.N * a.R;
-  uint16_t* yr[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) yr[i] = a.y + t.row(a, 16 * wave + 4 * lg + i) * a.y_stride;
-
   // No branch around a load: columns behind the run repeat its last ones, and are not stored
   uint4 bv[NG], yv[4];
   auto load = [&](int c) __attribute__((always_inline)) {
@@ -506,12 +510,15 @@ __global__ __launch_bounds__(kThreads, RG <= 4 ? 4 : 2) void lora_expand_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Tile t(a, tile_of(a.runs));
-  if (t.n <= 0) return;
+  uint16_t* yr[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) yr[i] = a.y + t.row(a, 16 * wave + 4 * (lane >> 4) + i) * a.y_stride;
   int part, c0, c1;
   run_of(a, turn_of(a.runs), &part, &c0, &c1);
+  if (t.n <= 0) return;
   by_groups<RG>(t.rank, [&](auto groups) __attribute__((always_inline)) {
     constexpr int NG = decltype(groups)::value;
-    expand<NG>(a, t, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
+    expand<NG>(a, t, yr, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
   });
 }
 
@@ -528,7 +535,7 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
 #define LORA_FEW 1024
 #endif
 #ifndef LORA_WGS
-#define LORA_WGS 256
+#define LORA_WGS 512
 #endif
 struct LoraForm {
   bool few;
