@@ -230,6 +230,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   __shared__ __attribute__((aligned(16))) TopLds lds;
   __shared__ Sums s_sums[kWaves];
   __shared__ float s_max[kWaves];
+  __shared__ int s_odd[kWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
@@ -244,7 +245,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const int tail0 = head + vecs * kVec;
   const int n_head = split == 0 ? head : 0, n_edge = wave == 0 ? n_head + (split == a.splits - 1 ? a.V - tail0 : 0) : 0;
   const int edge = lane < n_head ? lane : tail0 + lane - n_head;
-  const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
   const int per_wave = (a.k + kWaves - 1) / kWaves;
 
   Top top{lds.buf[wave], 0, 0, -INFINITY, -INFINITY, 0};
@@ -280,16 +280,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     raise(top, (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(b) << 32);
   };
 
-  // the edges, then two vectors a turn, those of the next one on their way; the first gives a bound to go by
-  if (TOP) top.lane_max = edge_value;
-  reference(edge_value);
-  add(edge_value);
+  // Two vectors a turn, those of the next one on their way, and before them the edges; the first turn gives a bound to go by.
   const int first = v0 + wave * MOE_WAVE;
   auto load = [&](int i) __attribute__((always_inline)) { return xv[min(i, max(v1, 1) - 1)]; };
   uint4 now[2], next[2];
   if (vecs > 0) {
     now[0] = load(first + lane);
     now[1] = load(first + kThreads + lane);
+  }
+  const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
+  if (wave == 0) {  // the other waves' is -inf
+    if (TOP) top.lane_max = edge_value;
+    reference(edge_value);
+    add(edge_value);
   }
   int turn = 0, renewal = 2;
   bool full = false;  // more candidates than there is room for
@@ -339,15 +342,21 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     now[0] = next[0];
     now[1] = next[1];
   }
-  // from the reference as the sums used it, m log2(e) rounded, to m itself
+  // from the reference as the sums used it, m log2(e) rounded, to m itself; all lanes' is the same
   const float off = m == -INFINITY ? 0.f : fmaf(m, kLog2e, -m2), undo = __builtin_amdgcn_exp2f(-off);
+  s = wave_sum_uniform(s);
+  t = wave_sum_uniform(t);
   Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
 
   if (lane == 0) s_max[wave] = m;
   if (TOP && threadIdx.x == 0) lds.n_vecs = lds.n_list = 0;
   if (TOP) renew();
   uint64_t* list = lds.buf[0];
-  bool again = __syncthreads_or(full || !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar));
+  if (lane == 0) s_odd[wave] = full || !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar);
+  __syncthreads();
+  bool again = false;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) again |= s_odd[w] != 0;
   if (TOP && !again) {
     take_bound();
     auto keep = [&](float v, int index) __attribute__((always_inline)) {
@@ -418,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         }
       }
     }
-    sum = Sums{m, s, t};
+    sum = Sums{m, wave_sum_uniform(s), wave_sum_uniform(t)};
     if (TOP) {  // the waves' candidates in one list, which takes the place of their buffers
       uint64_t key[kKeep / MOE_WAVE];
 #pragma unroll
@@ -429,7 +438,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         if (key[j] != 0) list[atomicAdd(&lds.n_list, 1)] = key[j];
     }
   }
-  sum = join_wave(sum);
   if (lane == 0) s_sums[wave] = sum;
   __syncthreads();
   sum = s_sums[0];
