@@ -6,7 +6,7 @@
 // 16 bytes a clock for each CU; so here consecutive lanes read consecutive bytes everywhere, and operands go through LDS.
 //
 // Two forms over the plan's tiles (rows of one adapter, lora.h):
-//   few rows (tiles of 4): one launch, a workgroup per (tile, run of columns), which forms the u of its part by
+//   few rows (tiles of 2): one launch, a workgroup per (tile, run of columns), which forms the u of its part by
 //     itself; dot products over the lanes, no MFMA;
 //   many (tiles of 64): u of every (tile, part, share of K) to the workspace in fp32, then the columns, both on MFMAs.
 //     For the second product u is split in two bf16 values, u = hi + lo to 2^-17 of it.
@@ -51,19 +51,26 @@ __device__ __forceinline__ uint4 mask8(uint4 v, int live) {
 struct Tile {
   int l, first, n, rank;  // adapter, first entry of the sorted rows, rows, rank
 
-  __device__ __forceinline__ Tile(const LoraArgs& a, int tile) {
-    const int4 t = *(const int4*)(a.plan + a.p.tiles + 4L * min(tile, a.p.N - 1));
-    const int tiles = min(a.plan[LH_TILES], a.p.N);
-    l = min(max(__builtin_amdgcn_readfirstlane(t.x), 0), a.p.L - 1);
-    first = min(max(__builtin_amdgcn_readfirstlane(t.y), 0), a.p.T - 1);
-    rank = min(a.ranks[l], a.R);
-    const int rows = min(min(__builtin_amdgcn_readfirstlane(t.z), a.p.tile_rows), a.p.T - first);
-    n = tile < tiles && rank > 0 ? rows : 0;
-    last = max(rows, 1) - 1;
+  // tile `tile` of the plan's list of kRows ones
+  template <int kRows>
+  __device__ __forceinline__ static Tile of(const LoraArgs& a, int tile) {
+    constexpr bool pair = kRows == kLoraPair;
+    const int room = pair ? a.p.M : a.p.N;
+    const int4 e = *(const int4*)(a.plan + (pair ? a.p.pairs : a.p.tiles) + 4L * min(tile, room - 1));
+    const int tiles = min(a.plan[pair ? LH_PAIRS : LH_TILES], room);
+    Tile t;
+    t.l = min(max(__builtin_amdgcn_readfirstlane(e.x), 0), a.p.L - 1);
+    t.first = min(max(__builtin_amdgcn_readfirstlane(e.y), 0), a.p.T - 1);
+    t.rank = min(a.ranks[t.l], a.R);
+    const int rows = min(min(__builtin_amdgcn_readfirstlane(e.z), kRows), a.p.T - t.first);
+    t.n = tile < tiles && t.rank > 0 ? rows : 0;
+    t.last = max(rows, 1) - 1;
+    return t;
   }
   __device__ __forceinline__ int row(const LoraArgs& a, int i) const {  // of entry first + i, or of the last one
     return min(max(a.plan[a.p.rows + first + min(i, last)], 0), a.p.T - 1);
   }
+  __device__ __forceinline__ bool narrow() const { return last < 16; }
 
  private:
   int last;
@@ -115,7 +122,7 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
 #define LORA_LB
 #endif
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
-constexpr int kFewRows = kLoraFewRows;
+constexpr int kFewRows = kLoraPair;
 
 __device__ __forceinline__ float dot8(v4i a, v4i b, float c) {
   typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -272,7 +279,7 @@ __global__ __launch_bounds__(kFewThreads LORA_LB) void lora_few_kernel(LoraArgs 
   __shared__ __attribute__((aligned(16))) float s_u[kFewRows][8 * kLanes];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile t(a, tile_of(a.runs));
+  const Tile t = Tile::of<kLoraPair>(a, tile_of(a.runs));
   int row[kFewRows];
 #pragma unroll
   for (int r = 0; r < kFewRows; ++r) row[r] = __builtin_amdgcn_readfirstlane(t.row(a, r));
@@ -291,7 +298,7 @@ __global__ __launch_bounds__(kFewThreads LORA_LB) void lora_few_kernel(LoraArgs 
 // the 16 rows of an operand lie in different banks.
 // ---------------------------------------------------------------------------
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kRowsM = 64, kMT = kRowsM / 16;
+constexpr int kRowsM = kLoraRows, kMT = kRowsM / 16;
 constexpr int kSlice = 128;
 constexpr int kRanksM = 64;  // of a workgroup
 
@@ -305,23 +312,23 @@ struct ShrinkLds {
   };
 };
 
-template <int NG, int RG>
-__device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const uint16_t* const (&xr)[kMT], int part, int rank0, int s0, int s1, int share, int lane,
-                                       int wave, ShrinkLds<RG>& lds) {
+template <int MT, int NG, int RG>
+__device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const uint16_t* const (&xr)[kMT], int part, int rank0,
+                                       int s0, int s1, int share, int lane, int wave, ShrinkLds<RG>& lds) {
   const int lr = lane & 15, lg = lane >> 4;
   const int q = threadIdx.x >> 4, piece = threadIdx.x & 15, to = piece ^ (q & 15);  // rows q + 16 i of both
   const uint16_t* ar[NG];
 #pragma unroll
   for (int i = 0; i < NG; ++i) ar[i] = a.a + (((long)t.l * a.parts + part) * a.R + min(rank0 + q + 16 * i, t.rank - 1)) * a.K;
   struct Slice {
-    v4i a[NG], x[kMT];
+    v4i a[NG], x[MT];
   } r0, r1, r2, r3;
   // No branch around a load: the compiler waits where it joins.  Rows and ranks that there are not repeat the last one, and
   // are not stored; k behind K repeat the last 8, and are not multiplied.
   auto load = [&](int s, Slice& into) __attribute__((always_inline)) {
     const int k = min(kSlice * min(s, s1 - 1) + 8 * piece, a.K - 8);
 #pragma unroll
-    for (int i = 0; i < kMT; ++i) into.x[i] = *(const v4i*)(xr[i] + k);
+    for (int i = 0; i < MT; ++i) into.x[i] = *(const v4i*)(xr[i] + k);
 #pragma unroll
     for (int i = 0; i < NG; ++i) into.a[i] = *(const v4i*)(ar[i] + k);
   };
@@ -329,22 +336,22 @@ __device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const u
 #pragma unroll
     for (int i = 0; i < NG; ++i) lds.slice[buf].a[q + 16 * i][to] = from.a[i];
 #pragma unroll
-    for (int i = 0; i < kMT; ++i) lds.slice[buf].x[q + 16 * i][to] = from.x[i];
+    for (int i = 0; i < MT; ++i) lds.slice[buf].x[q + 16 * i][to] = from.x[i];
   };
-  v4f u[kMT][NG];
+  v4f u[MT][NG];
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int g = 0; g < NG; ++g) u[m][g] = (v4f){0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](int buf) __attribute__((always_inline)) {
     const int at = (4 * wave + lg) ^ lr;
-    v8bf xf[kMT], af[NG];
+    v8bf xf[MT], af[NG];
 #pragma unroll
-    for (int m = 0; m < kMT; ++m) xf[m] = __builtin_bit_cast(v8bf, lds.slice[buf].x[16 * m + lr][at]);
+    for (int m = 0; m < MT; ++m) xf[m] = __builtin_bit_cast(v8bf, lds.slice[buf].x[16 * m + lr][at]);
 #pragma unroll
     for (int g = 0; g < NG; ++g) af[g] = __builtin_bit_cast(v8bf, lds.slice[buf].a[16 * g + lr][at]);
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int g = 0; g < NG; ++g) u[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[g], xf[m], u[m][g], 0, 0, 0);
   };
@@ -370,11 +377,11 @@ __device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const u
   }
   // lane l has ranks 4 (l / 16) + i of row l % 16 of each: joined over the waves
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int g = 0; g < NG; ++g) lds.part[wave][m][g][lane] = u[m][g];
   __syncthreads();
-  for (int i = threadIdx.x; i < kMT * NG * 64; i += kThreads) {
+  for (int i = threadIdx.x; i < MT * NG * 64; i += kThreads) {
     const int m = i / (64 * NG), g = i / 64 % NG, row = 16 * m + i % 16, rank = rank0 + kGroup * g + 4 * (i % 64 / 16);
     v4f sum = lds.part[0][m][g][i % 64];
 #pragma unroll
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int blocks = a.parts * a.shares * ((a.R + kRanksM - 1) / kRanksM), at = turn_of(blocks);
-  const Tile t(a, tile_of(blocks));
+  const Tile t = Tile::of<kLoraRows>(a, tile_of(blocks));
   const uint16_t* xr[kMT];
 #pragma unroll
   for (int i = 0; i < kMT; ++i) xr[i] = a.x + t.row(a, threadIdx.x / 16 + 16 * i) * a.x_stride;
@@ -398,9 +405,12 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
   if (rank0 >= t.rank) return;
   const int slices = (a.K + kSlice - 1) / kSlice, per = (slices + a.shares - 1) / a.shares;
   const int s0 = min(share * per, slices), s1 = min(s0 + per, slices);
-  if (s0 >= s1) return;
   by_groups<RG>(t.rank - rank0, [&](auto groups) __attribute__((always_inline)) {
-    shrink<decltype(groups)::value, RG>(a, t, xr, part, rank0, s0, s1, share, lane, wave, lds);
+    constexpr int NG = decltype(groups)::value;
+    if (t.narrow())
+      shrink<1, NG, RG>(a, t, xr, part, rank0, s0, s1, share, lane, wave, lds);
+    else
+      shrink<kMT, NG, RG>(a, t, xr, part, rank0, s0, s1, share, lane, wave, lds);
   });
 }
 
@@ -431,33 +441,38 @@ struct ExpandLds {
   uint8_t b[kPiece * kRow];
 };
 
-template <int NG>
-__device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_t* const (&yr)[4], int part, int c0, int c1, int lane, int wave,
-                                       ExpandLds<NG>& lds) {
-  constexpr int kRow = ExpandLds<NG>::kRow;
+template <int J, int NG>
+__device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_t* const (&yr)[4], int part, int c0, int c1,
+                                       int lane, int wave, ExpandLds<NG>& lds) {
+  constexpr int kRow = ExpandLds<NG>::kRow, kRows = J == 8 ? kRowsM : 16;
+  constexpr int kY = J / 2;  // 32-bit words of a row's columns
   const int lr = lane & 15, lg = lane >> 4;
+  const int row0 = J == 8 ? 16 * wave : 0, tile0 = J == 8 ? 0 : J * wave, mine = J * lr + 16 * tile0;  // of the piece
   const float scale = a.scales[t.l];
   const uint16_t* bl = a.b + (long)t.l * a.N * a.R;
   // No branch around a load: columns behind the run repeat its last ones, and are not stored
-  uint4 bv[NG], yv[4];
+  typedef uint32_t Words __attribute__((ext_vector_type(kY)));
+  v4i bv[NG];
+  Words yv[4];
   auto load = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) yv[i] = *(const uint4*)(yr[i] + min(c + 8 * lr, c1 - 8));
+    for (int i = 0; i < 4; ++i) yv[i] = *(const Words*)(yr[i] + min(c + mine, c1 - J));
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const int at = threadIdx.x + kThreads * i, n = at / (2 * NG), r = at % (2 * NG) * 8;
-      bv[i] = *(const uint4*)(bl + (long)min(c + n, c1 - 1) * a.R + (r < t.rank ? r : 0));
+      bv[i] = *(const v4i*)(bl + (long)min(c + n, c1 - 1) * a.R + (r < t.rank ? r : 0));
     }
   };
   auto store_b = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const int at = threadIdx.x + kThreads * i, n = at / (2 * NG), r = at % (2 * NG) * 8;
-      *(uint4*)(lds.b + (n % 8 * 16 + n / 8) * kRow + 2 * r) = mask8(bv[i], t.rank - r);
+      const uint4 v = mask8(__builtin_bit_cast(uint4, bv[i]), t.rank - r);
+      *(uint4*)(lds.b + ((n / (16 * J) * J + n % J) * 16 + n % (16 * J) / J) * kRow + 2 * r) = v;
     }
   };
   load(c0);
-  for (int i = threadIdx.x; i < kRowsM * NG * 4; i += kThreads) {
+  for (int i = threadIdx.x; i < kRows * NG * 4; i += kThreads) {
     const int row = min(i / (NG * 4), t.n - 1), r0 = 4 * (i % (NG * 4));
     const float* src = a.u + (((long)t.first + row) * a.parts + part) * a.R + (r0 < t.rank ? r0 : 0);
     v4f s = *(const v4f*)src;
@@ -473,32 +488,32 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
   for (int g = 0; g < kSteps; ++g)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      uv[g][h] = NG == 1 ? *(const v8bf*)&lds.u[16 * wave + lr][lg >> 1][8 * (lg & 1)] : *(const v8bf*)&lds.u[16 * wave + lr][h][32 * g + 8 * lg];
+      uv[g][h] = NG == 1 ? *(const v8bf*)&lds.u[row0 + lr][lg >> 1][8 * (lg & 1)] : *(const v8bf*)&lds.u[row0 + lr][h][32 * g + 8 * lg];
   for (int c = c0; c < c1; c += kPiece) {
-    v4f acc[8];
+    v4f acc[J];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j][i] = j % 2 ? hi_of(w[j / 2]) : lo_of(w[j / 2]);
-    }
+      for (int j = 0; j < J; ++j) acc[j][i] = j % 2 ? hi_of(yv[i][j / 2]) : lo_of(yv[i][j / 2]);
     load(min(c + kPiece, c1 - 1));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int g = 0; g < kSteps; ++g) {
-        const v8bf b = *(const v8bf*)(lds.b + (16 * j + lr) * kRow + (NG == 1 ? 16 * (lg & 1) : 64 * g + 16 * lg));
+        const v8bf b = *(const v8bf*)(lds.b + (16 * (tile0 + j) + lr) * kRow + (NG == 1 ? 16 * (lg & 1) : 64 * g + 16 * lg));
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][0], b, acc[j], 0, 0, 0);
         if (NG > 1) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][1], b, acc[j], 0, 0, 0);
       }
     __syncthreads();  // B's columns are read
-    if (c + 8 * lr < c1)
+    if (c + mine < c1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (16 * wave + 4 * lg + i < t.n)
-          *(uint4*)(yr[i] + c + 8 * lr) = make_uint4(pack2(acc[0][i], acc[1][i]), pack2(acc[2][i], acc[3][i]),
-                                                     pack2(acc[4][i], acc[5][i]), pack2(acc[6][i], acc[7][i]));
+      for (int i = 0; i < 4; ++i) {
+        Words out;
+#pragma unroll
+        for (int w = 0; w < kY; ++w) out[w] = pack2(acc[2 * w][i], acc[2 * w + 1][i]);
+        if (row0 + 4 * lg + i < t.n) *(Words*)(yr[i] + c + mine) = out;
+      }
     store_b();
     __syncthreads();
   }
@@ -509,16 +524,19 @@ __global__ __launch_bounds__(kThreads, RG <= 4 ? 4 : 2) void lora_expand_kernel(
   __shared__ __attribute__((aligned(16))) uint8_t lds[sizeof(ExpandLds<RG>)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Tile t(a, tile_of(a.runs));
+  const Tile t = Tile::of<kLoraRows>(a, tile_of(a.runs));
   uint16_t* yr[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) yr[i] = a.y + t.row(a, 16 * wave + 4 * (lane >> 4) + i) * a.y_stride;
+  for (int i = 0; i < 4; ++i) yr[i] = a.y + t.row(a, (t.narrow() ? 0 : 16 * wave) + 4 * (lane >> 4) + i) * a.y_stride;
   int part, c0, c1;
   run_of(a, turn_of(a.runs), &part, &c0, &c1);
   if (t.n <= 0) return;
   by_groups<RG>(t.rank, [&](auto groups) __attribute__((always_inline)) {
     constexpr int NG = decltype(groups)::value;
-    expand<NG>(a, t, yr, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
+    if (t.narrow())
+      expand<2, NG>(a, t, yr, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
+    else
+      expand<8, NG>(a, t, yr, part, c0, c1, lane, wave, *(ExpandLds<NG>*)lds);
   });
 }
 
@@ -528,8 +546,14 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
 }
 
 // How a call is cut up
+#ifndef LORA_FORM
+#define LORA_FORM (p.M > 0 && (long)R * K <= 1 << 18 && (long)p.T * R * K <= 1 << 23)
+#endif
 #ifndef LORA_CHUNK
 #define LORA_CHUNK 512
+#endif
+#ifndef LORA_MINK
+#define LORA_MINK 512
 #endif
 #ifndef LORA_FEW
 #define LORA_FEW 1024
@@ -539,15 +563,18 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
 #endif
 struct LoraForm {
   bool few;
-  int shares, chunk;
+  int tiles, shares, chunk;
 };
 LoraForm lora_form(const LoraLayout& p, int K, int R, int parts, int N) {
-  LoraForm f{p.tile_rows == kFewRows, 1, LORA_CHUNK};
-  if (f.few)
-    for (f.chunk = 512; f.chunk < 4096 && (long)p.N * N / f.chunk > LORA_FEW; f.chunk *= 2) {
+  LoraForm f{LORA_FORM, p.N, 1, LORA_CHUNK};
+  if (f.few) {
+    f.tiles = p.M;
+    for (f.chunk = 512; f.chunk < 4096 && (long)f.tiles * N / f.chunk > LORA_FEW; f.chunk *= 2) {
     }
-  else
-    while (f.shares < 8 && p.N * parts * f.shares < LORA_WGS && K / (2 * f.shares) >= 512) f.shares *= 2;
+  } else {
+    while (f.shares < 8 && f.tiles * parts * f.shares < LORA_WGS && K / (2 * f.shares) >= LORA_MINK) f.shares *= 2;
+    while (f.chunk > 128 && (long)f.tiles * N / f.chunk < LORA_WGS) f.chunk /= 2;
+  }
   return f;
 }
 
@@ -557,12 +584,12 @@ size_t lora_ws(const LoraLayout& p, const LoraForm& f, int R, int parts) {
 
 template <int RG>
 void launch(const LoraArgs& g, const LoraForm& f, hipStream_t s) {
-  const dim3 columns(lora_grid(g.p.N, g.runs));
+  const dim3 columns(lora_grid(f.tiles, g.runs));
   if (f.few) {
     hipLaunchKernelGGL((lora_few_kernel<2 * RG>), columns, dim3(kFewThreads), 0, s, g);
     return;
   }
-  const dim3 first(lora_grid(g.p.N, g.parts * g.shares * ((g.R + kRanksM - 1) / kRanksM)));
+  const dim3 first(lora_grid(f.tiles, g.parts * g.shares * ((g.R + kRanksM - 1) / kRanksM)));
   hipLaunchKernelGGL((lora_shrink_kernel<(RG < 4 ? RG : 4)>), first, dim3(kThreads), 0, s, g);
   hipLaunchKernelGGL((lora_expand_kernel<RG>), columns, dim3(kThreads), 0, s, g);
 }
@@ -607,7 +634,7 @@ extern "C" int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, l
   g.plan = (const int32_t*)plan, g.u = (float*)workspace;
   g.K = K, g.R = R, g.N = (int)n, g.parts = parts, g.shares = f.shares, g.chunk = f.chunk;
   for (int p = 0; p < parts; ++p) g.runs += (columns[p] + f.chunk - 1) / f.chunk;
-  MOE_RETURN_IF(!moe_grid_fits((long)(g.p.N + 7) * g.runs), MOE_ERR_INVALID_ARG);
+  MOE_RETURN_IF(!moe_grid_fits((long)(f.tiles + 7) * g.runs), MOE_ERR_INVALID_ARG);
   hipStream_t s = (hipStream_t)stream;
   if (R <= 16)
     launch<1>(g, f, s);

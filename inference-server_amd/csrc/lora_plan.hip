@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void lora_plan_kernel(LoraPlanArgs a) {
   __shared__ int s_cu[kLoraMaxSeqs + 1];
   __shared__ int s_total[kBins], s_before[kBins];  // rows of each adapter: all, and those in front of this workgroup's
   __shared__ int s_wave[kWaves][kBins];
-  __shared__ int s_first[kBins + 1], s_tile[kBins + 1];
+  __shared__ int s_first[kBins + 1], s_tile[kBins + 1], s_pair[kBins + 1];
   const LoraLayout& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int T = p.T, L = p.L, bins = L + 1;
@@ -90,26 +90,26 @@ __global__ __launch_bounds__(kThreads) void lora_plan_kernel(LoraPlanArgs a) {
   __syncthreads();
 
   if (wave == 0) {  // where each adapter's rows and tiles begin
-    int n[kPerLane], t[kPerLane], rows = 0, tiles = 0;
+    int n[kPerLane], rows = 0, tiles = 0, pairs = 0;
+    auto of = [&](int i, int height) { return lane * kPerLane + i < L ? (n[i] + height - 1) / height : 0; };
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int b = lane * kPerLane + i;
       n[i] = b < bins ? s_total[b] : 0;
-      t[i] = b < L ? (n[i] + p.tile_rows - 1) / p.tile_rows : 0;
-      rows += n[i], tiles += t[i];
+      rows += n[i], tiles += of(i, kLoraRows), pairs += of(i, kLoraPair);
     }
-    int rows_to = rows, tiles_to = tiles;
+    int rows_to = rows, tiles_to = tiles, pairs_to = pairs;
 #pragma unroll
     for (int d = 1; d < MOE_WAVE; d *= 2) {
-      const int r = __shfl_up(rows_to, d), s = __shfl_up(tiles_to, d);
-      if (lane >= d) rows_to += r, tiles_to += s;
+      const int r = __shfl_up(rows_to, d), s = __shfl_up(tiles_to, d), q = __shfl_up(pairs_to, d);
+      if (lane >= d) rows_to += r, tiles_to += s, pairs_to += q;
     }
-    rows_to -= rows, tiles_to -= tiles;
+    rows_to -= rows, tiles_to -= tiles, pairs_to -= pairs;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int b = lane * kPerLane + i;
-      if (b <= bins) s_first[b] = rows_to, s_tile[b] = tiles_to;
-      rows_to += n[i], tiles_to += t[i];
+      if (b <= bins) s_first[b] = rows_to, s_tile[b] = tiles_to, s_pair[b] = pairs_to;
+      rows_to += n[i], tiles_to += of(i, kLoraRows), pairs_to += of(i, kLoraPair);
     }
   }
   __syncthreads();
@@ -120,18 +120,22 @@ __global__ __launch_bounds__(kThreads) void lora_plan_kernel(LoraPlanArgs a) {
   }
   if (blockIdx.x == 0) {
     for (int i = tid; i <= bins; i += kThreads) a.plan[p.offsets + i] = s_first[i];
-    if (tid == 0) a.plan[LH_TILES] = s_tile[L];
+    if (tid == 0) a.plan[LH_TILES] = s_tile[L], a.plan[LH_PAIRS] = s_pair[L];
   }
-  for (int t = blockIdx.x * kThreads + tid; t < min(s_tile[L], p.N); t += gridDim.x * kThreads) {
-    int lo = 0, hi = L - 1;  // the last adapter whose tiles begin at t or before
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (s_tile[mid] <= t) lo = mid;
-      else hi = mid - 1;
+  auto list = [&](const int* from, int height, int room, long to) {
+    for (int t = blockIdx.x * kThreads + tid; t < min(from[L], room); t += gridDim.x * kThreads) {
+      int lo = 0, hi = L - 1;  // the last adapter whose tiles begin at t or before
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (from[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int at = (t - from[lo]) * height;
+      *(int4*)(a.plan + to + 4L * t) = make_int4(lo, s_first[lo] + at, min(s_total[lo] - at, height), 0);
     }
-    const int at = (t - s_tile[lo]) * p.tile_rows;
-    *(int4*)(a.plan + p.tiles + 4L * t) = make_int4(lo, s_first[lo] + at, min(s_total[lo] - at, p.tile_rows), 0);
-  }
+  };
+  list(s_tile, kLoraRows, p.N, p.tiles);
+  if (p.M > 0) list(s_pair, kLoraPair, p.M, p.pairs);
 }
 
 }  // namespace

@@ -29,11 +29,14 @@ def i32(a, dev):
     return torch.tensor(np.asarray(a), dtype=torch.int32, device=dev)
 
 
-def tiles_of(pkg, plan):
-    """The plan's tiles, as the kernels read them."""
+def lists_of(plan):
+    """The plan's tiles of 64 rows and of 2, as the kernels read them, and the room for each."""
     buf = plan.buffer.cpu().numpy()
-    at = (plan._at[1] + plan.num_rows + 3) // 4 * 4
-    return buf[at:at + 4 * buf[0]].reshape(-1, 4), len(buf[at:]) // 4
+    T, some = plan.num_rows, min(plan.num_rows, plan.num_adapters)
+    at = (plan._at[1] + T + 3) // 4 * 4
+    rooms = (T // 64 + some, T // 2 + some if T <= 256 else 0)
+    assert len(buf) == at + 4 * sum(rooms)
+    return [(buf[a:a + 4 * n].reshape(-1, 4), n, room) for a, n, room in ((at, buf[0], rooms[0]), (at + 4 * rooms[0], buf[1] if rooms[1] else 0, rooms[1]))]
 
 
 @pytest.mark.parametrize("T,L", [(0, 1), (1, 1), (1, 256), (5, 3), (63, 2), (64, 256), (65, 100), (1000, 7), (1024, 1),
@@ -46,10 +49,9 @@ def test_plan_by_row(pkg, dev, T, L):
     plan = pkg.lora_plan(i32(ids, dev), L)
     rows, offsets = plan_ref(ids, L)
     assert np.array_equal(plan.rows.cpu().numpy(), rows) and np.array_equal(plan.offsets.cpu().numpy(), offsets)
-    tiles, room = tiles_of(pkg, plan)
-    height = 2 if T <= 256 else 64
-    want = [(l, o, min(height, offsets[l + 1] - o), 0) for l in range(L) for o in range(offsets[l], offsets[l + 1], height)]
-    assert len(want) <= room and np.array_equal(tiles, np.asarray(want).reshape(-1, 4))
+    for height, (tiles, n, room) in zip((64, 2), lists_of(plan)):
+        want = [(l, o, min(height, offsets[l + 1] - o), 0) for l in range(L) for o in range(offsets[l], offsets[l + 1], height)]
+        assert n <= room and (not room or np.array_equal(tiles, np.asarray(want).reshape(-1, 4)))
 
 
 @pytest.mark.parametrize("lens,T", [([3], 3), ([0, 5, 0, 0, 7, 1], 13), ([1] * 64, 64), ([700, 1, 1300, 64], 3000),
