@@ -112,15 +112,6 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
 // Columns: kLanes lanes have 8 ranks of a column each, a wave 64 columns at a time; over kLanes turns lane i
 // ends with the sum of column i.
 // ---------------------------------------------------------------------------
-#ifndef LORA_KB
-#define LORA_KB 4
-#endif
-#ifndef LORA_TG
-#define LORA_TG 2
-#endif
-#ifndef LORA_LB
-#define LORA_LB
-#endif
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
 constexpr int kFewRows = kLoraPair;
 
@@ -204,8 +195,9 @@ __device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, const
   for (int i = 0; i < kLanes; ++i)
 #pragma unroll
     for (int r = 0; r < NR; ++r) acc[i][r] = 0.f;
-  // kTogether ranks by kBlock times 512 values are in flight together
-  constexpr int kTogether = kLanes < LORA_TG ? kLanes : LORA_TG, kBlock = LORA_KB;
+  // kTogether ranks by kBlock times 512 values are in flight together.  (Four ranks, or twice the values, take registers that
+  // another workgroup of the CU misses: 24 rows of up to 64 ranks beside q/k/v 11.0 us with two, 11.3 with four.)
+  constexpr int kTogether = 2, kBlock = 4;
   const uint16_t* ap = a.a + ((long)t.l * a.parts + part) * a.R * a.K;
   // No branch around a load: the compiler waits where it joins.  Behind K (`whole` is false) both operands are zeros.
   auto block = [&](int k0, auto whole) __attribute__((always_inline)) {
@@ -275,7 +267,7 @@ __device__ __forceinline__ void few_rows(const LoraArgs& a, const Tile& t, const
 }
 
 template <int kLanes>
-__global__ __launch_bounds__(kFewThreads LORA_LB) void lora_few_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kFewThreads) void lora_few_kernel(LoraArgs a) {
   __shared__ __attribute__((aligned(16))) float s_u[kFewRows][8 * kLanes];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -357,10 +349,10 @@ __device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const u
   };
   // slice s + 4 is loaded while slice s is multiplied, and goes to LDS during slice s + 3
   auto turn = [&](int s, int buf, Slice& mine, Slice& after) __attribute__((always_inline)) {
-    load(s + 4, mine);  // these registers went to LDS in the last turn
+    if (s + 4 < s1) load(s + 4, mine);  // these registers went to LDS in the last turn
     __builtin_amdgcn_sched_barrier(0);
-    if (s < s1 && kSlice * s + 32 * wave < a.K) multiply(buf);
-    store(buf ^ 1, after);  // last read a slice ago, before the last barrier
+    if (kSlice * s + 32 * wave < a.K) multiply(buf);
+    if (s + 1 < s1) store(buf ^ 1, after);  // last read a slice ago, before the last barrier
     __syncthreads();
   };
   load(s0, r0);
@@ -371,8 +363,11 @@ __device__ __forceinline__ void shrink(const LoraArgs& a, const Tile& t, const u
   __syncthreads();
   for (int s = s0; s < s1; s += 4) {
     turn(s, 0, r0, r1);
+    if (s + 1 >= s1) break;
     turn(s + 1, 1, r1, r2);
+    if (s + 2 >= s1) break;
     turn(s + 2, 0, r2, r3);
+    if (s + 3 >= s1) break;
     turn(s + 3, 1, r3, r0);
   }
   // lane l has ranks 4 (l / 16) + i of row l % 16 of each: joined over the waves
@@ -472,12 +467,32 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
     }
   };
   load(c0);
-  for (int i = threadIdx.x; i < kRows * NG * 4; i += kThreads) {
-    const int row = min(i / (NG * 4), t.n - 1), r0 = 4 * (i % (NG * 4));
-    const float* src = a.u + (((long)t.first + row) * a.parts + part) * a.R + (r0 < t.rank ? r0 : 0);
-    v4f s = *(const v4f*)src;
-    for (int z = 1; z < a.shares; ++z) s += *(const v4f*)(src + (long)z * a.p.T * a.parts * a.R);
-    split_u(s, scale, t.rank - r0, (uint2*)&lds.u[i / (NG * 4)][0][r0], (uint2*)&lds.u[i / (NG * 4)][1][r0]);
+  // u: the shares' sums, some shares of all this thread's values in flight together
+  constexpr int kMine = (kRows * NG * 4 + kThreads - 1) / kThreads, kShares = kMine >= 8 ? 1 : kMine >= 4 ? 2 : 4;
+  v4f su[kMine];
+  const float* src[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = threadIdx.x + kThreads * i, r0 = 4 * (at % (NG * 4));
+    src[i] = a.u + (((long)t.first + min(at / (NG * 4), t.n - 1)) * a.parts + part) * a.R + (r0 < t.rank ? r0 : 0);
+    su[i] = (v4f){0.f, 0.f, 0.f, 0.f};
+  }
+  const long share = (long)a.p.T * a.parts * a.R;
+  for (int z = 0; z < a.shares; z += kShares) {
+    v4f v[kShares][kMine];
+#pragma unroll
+    for (int e = 0; e < kShares; ++e)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) v[e][i] = *(const v4f*)(src[i] + min(z + e, a.shares - 1) * share);
+#pragma unroll
+    for (int e = 0; e < kShares; ++e)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) su[i] += z + e < a.shares ? v[e][i] : (v4f){0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = threadIdx.x + kThreads * i, row = at / (NG * 4), r0 = 4 * (at % (NG * 4));
+    if (row < kRows) split_u(su[i], scale, t.rank - r0, (uint2*)&lds.u[row][0][r0], (uint2*)&lds.u[row][1][r0]);
   }
   store_b();
   __syncthreads();
@@ -489,14 +504,14 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       uv[g][h] = NG == 1 ? *(const v8bf*)&lds.u[row0 + lr][lg >> 1][8 * (lg & 1)] : *(const v8bf*)&lds.u[row0 + lr][h][32 * g + 8 * lg];
-  for (int c = c0; c < c1; c += kPiece) {
-    v4f acc[J];
+  v4f acc[J];
+  auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < J; ++j) acc[j][i] = j % 2 ? hi_of(yv[i][j / 2]) : lo_of(yv[i][j / 2]);
-    load(min(c + kPiece, c1 - 1));
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -505,7 +520,8 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][0], b, acc[j], 0, 0, 0);
         if (NG > 1) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][1], b, acc[j], 0, 0, 0);
       }
-    __syncthreads();  // B's columns are read
+  };
+  auto store_y = [&](int c) __attribute__((always_inline)) {
     if (c + mine < c1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -514,9 +530,23 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
         for (int w = 0; w < kY; ++w) out[w] = pack2(acc[2 * w][i], acc[2 * w + 1][i]);
         if (row0 + 4 * lg + i < t.n) *(Words*)(yr[i] + c + mine) = out;
       }
+  };
+  // The last piece apart, so that no branch lies around a load, and y's stores behind B's: a wait for a load waits for
+  // every store in front of it.
+  int c = c0;
+  for (; c + kPiece < c1; c += kPiece) {
+    begin();
+    load(c + kPiece);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply();
+    __syncthreads();  // B's columns are read
     store_b();
+    store_y(c);
     __syncthreads();
   }
+  begin();
+  multiply();
+  store_y(c);
 }
 
 template <int RG>
@@ -545,35 +575,30 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
          parts <= kMaxParts;
 }
 
-// How a call is cut up
-#ifndef LORA_FORM
-#define LORA_FORM (p.M > 0 && (long)R * K <= 1 << 18 && (long)p.T * R * K <= 1 << 23)
-#endif
-#ifndef LORA_CHUNK
-#define LORA_CHUNK 512
-#endif
-#ifndef LORA_MINK
-#define LORA_MINK 512
-#endif
-#ifndef LORA_FEW
-#define LORA_FEW 1024
-#endif
-#ifndef LORA_WGS
-#define LORA_WGS 512
-#endif
+// How a call is cut up.
+// Few rows: each pair of rows reads its adapter for itself, once for each run, so this pays while rows times rank times K
+// is small.  (us in a graph, few / many rows' form.  2048 to q/k/v 5120, rank 16: 1 row 4.2 / 6.4, 64 rows of 64 adapters
+// 6.3 / 10.0, 256 of 8 10.8 / 11.4; rank 64: 1 row 6.4 / 8.0, 32 of 8 9.6 / 8.9, 64 of 64 17.2 / 16.6, 128 of 64 25.2 / 21.3.
+// 8192 to 4096, rank 64: 1 row 12.0 / 9.1, 64 of 64 31.0 / 20.4.)
+constexpr long kFewWork = 1 << 23, kFewAdapter = 1 << 18;
+// Runs of 512 columns at least, 64 for each wave, and more where that makes more workgroups than this: each forms u again.
+// (128 rows of 100 adapters, 4096 to q/k/v 9216: 17.2 us for 512, 13.7 for 1024, 15.6 for 2048.)
+constexpr int kFewGroups = 1024;
+// Many rows: at least two workgroups a CU, by shares of K and by shorter runs of columns.
+constexpr int kManyGroups = 512, kShareK = 512, kManyRun = 512;
+
 struct LoraForm {
   bool few;
   int tiles, shares, chunk;
 };
 LoraForm lora_form(const LoraLayout& p, int K, int R, int parts, int N) {
-  LoraForm f{LORA_FORM, p.N, 1, LORA_CHUNK};
+  LoraForm f{p.M > 0 && (long)R * K <= kFewAdapter && (long)p.T * R * K <= kFewWork, p.N, 1, kManyRun};
   if (f.few) {
     f.tiles = p.M;
-    for (f.chunk = 512; f.chunk < 4096 && (long)f.tiles * N / f.chunk > LORA_FEW; f.chunk *= 2) {
-    }
+    for (f.chunk = 512; f.chunk < 4096 && (long)f.tiles * N / f.chunk > kFewGroups;) f.chunk *= 2;
   } else {
-    while (f.shares < 8 && f.tiles * parts * f.shares < LORA_WGS && K / (2 * f.shares) >= LORA_MINK) f.shares *= 2;
-    while (f.chunk > 128 && (long)f.tiles * N / f.chunk < LORA_WGS) f.chunk /= 2;
+    while (f.shares < 8 && f.tiles * parts * f.shares < kManyGroups && K / (2 * f.shares) >= kShareK) f.shares *= 2;
+    while (f.chunk > kPiece && (long)f.tiles * N / f.chunk < kManyGroups) f.chunk /= 2;
   }
   return f;
 }
