@@ -10,6 +10,7 @@ Layers:
   ``experts``  drop-in modules, the transformers experts-interface registration, and the
                HIP-graph replay of a block per decode batch bucket
   ``checkpoint`` FP8 expert layers from a local safetensors checkpoint
+  ``decode``   the decoder layers of a step, captured or not, with adapters, and the output head
   ``build``    hipcc build of the library
 """
 

@@ -28,6 +28,10 @@ tokens in one call: ``DecodeModel.plan`` (``moe_mi355x_paged_plan``) builds the 
 on the GPU from the sequences' lengths, and each layer runs ``moe_mi355x_qk_norm_rope_append_fp8`` and
 ``moe_mi355x_paged_attn_fp8`` in the place of the bf16 cache's pair.  ``DecodeModel.capture_run`` records plan and layers
 as one graph, which replays on lengths that change on the GPU.
+
+Sequences may bring adapters (``LayerAdapters``): ``DecodeModel.lora_plan`` sorts a step's rows by them once
+(``moe_mi355x_lora_plan``), and in each layer ``moe_mi355x_lora_add`` adds what they contribute to the q/k/v projection and to
+o_proj's.  ``OutputHead`` ends a step: the model's last norm, lm_head and ``moe_mi355x_token_logprobs``.
 """
 
 from __future__ import annotations
@@ -152,31 +156,56 @@ class DecoderLayerWeights:
                    e.down_proj_scale_inv)
 
 
+@dataclass(frozen=True)
+class LayerAdapters:
+    """The adapters of a layer's attention projections: pools of the same number of adapters (None: no adapter changes that
+    projection).  ``qkv`` has the parts q, k and v (``qkv_columns``), ``o`` one."""
+
+    qkv: kernels.LoraPool | None = None
+    o: kernels.LoraPool | None = None
+
+    @staticmethod
+    def qkv_columns(cfg: DecoderConfig) -> tuple[int, int, int]:
+        return cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
+
+    @classmethod
+    def empty(cls, cfg: DecoderConfig, num_adapters: int, max_rank: int, device) -> LayerAdapters:
+        """Pools without adapters, to ``LoraPool.load`` into."""
+        return cls(kernels.LoraPool.empty(num_adapters, cfg.hidden, cls.qkv_columns(cfg), max_rank, device),
+                   kernels.LoraPool.empty(num_adapters, cfg.heads * cfg.head_dim, (cfg.hidden,), max_rank, device))
+
+
+def _project(x, weight, pool: kernels.LoraPool | None, lora: kernels.LoraPlan | None):
+    """The shared projection, and what the rows' adapters add to it."""
+    y = _linear(x, weight)
+    return y if pool is None or lora is None else kernels.lora_add(y, x, pool, lora)
+
+
 def attention_sublayer(w: DecoderLayerWeights, h, positions, context_lens, block_tables, inv_freq, k_cache,
-                       v_cache):
+                       v_cache, adapters: LayerAdapters = LayerAdapters(), lora: kernels.LoraPlan | None = None):
     """``o_proj(attention(input_layernorm(h)))`` for one new token per sequence, appending the
     token's k, v to the cache (modeling_qwen3_moe.py:329-340 with :151-191).  The residual add
     of :341 is left to the caller (the MoE sublayer forms it)."""
     cfg = w.cfg
     B = h.shape[0]
     x = kernels.rms_norm(h, w.ln1, cfg.rms_eps)
-    qkv = _linear(x, w.wqkv)
+    qkv = _project(x, w.wqkv, adapters.qkv, lora)
     q = kernels.qk_norm_rope_append(qkv, w.q_norm, w.k_norm, inv_freq, positions, cfg.heads, cfg.kv_heads,
                                     cfg.rms_eps, k_cache, v_cache, block_tables)
     a = kernels.paged_attention_decode(q, k_cache, v_cache, block_tables, context_lens, cfg.head_dim ** -0.5)
-    return _linear(a.view(B, cfg.heads * cfg.head_dim), w.wo)
+    return _project(a.view(B, cfg.heads * cfg.head_dim), w.wo, adapters.o, lora)
 
 
 def attention_sublayer_fp8(w: DecoderLayerWeights, h, plan: kernels.PagedPlan, inv_freq, k_cache, v_cache, k_scale,
-                           v_scale):
+                           v_scale, adapters: LayerAdapters = LayerAdapters(), lora: kernels.LoraPlan | None = None):
     """``attention_sublayer`` over the 8-bit cache, for the rows of a plan: prompts and single tokens."""
     cfg = w.cfg
     x = kernels.rms_norm(h, w.ln1, cfg.rms_eps)
     cache = (k_cache, v_cache, k_scale, v_scale)
-    q = kernels.qk_norm_rope_append_fp8(_linear(x, w.wqkv), w.q_norm, w.k_norm, inv_freq, cfg.heads, cfg.kv_heads,
-                                        cfg.rms_eps, *cache, plan)
+    q = kernels.qk_norm_rope_append_fp8(_project(x, w.wqkv, adapters.qkv, lora), w.q_norm, w.k_norm, inv_freq, cfg.heads,
+                                        cfg.kv_heads, cfg.rms_eps, *cache, plan)
     a = kernels.paged_attention_fp8(q, *cache, plan, cfg.head_dim ** -0.5)
-    return _linear(a.view(h.shape[0], cfg.heads * cfg.head_dim), w.wo)
+    return _project(a.view(h.shape[0], cfg.heads * cfg.head_dim), w.wo, adapters.o, lora)
 
 
 def moe_sublayer(w: DecoderLayerWeights, h, attn_out=None):
@@ -203,13 +232,24 @@ class DecodeModel:
     then call the graph's ``replay()``.
 
     With a ``PagedKVCacheFp8``, ``plan`` and ``run`` take the place of ``step``, and ``capture_run`` of ``capture``.
+
+    ``adapters``: a ``LayerAdapters`` for each layer, all of the same number of adapters.  ``step`` and ``run`` then take
+    the step's ``lora_plan``, the capturing calls the adapters' numbers, which become the last of their static inputs.
     """
 
     def __init__(self, cfg: DecoderConfig, layers: list[DecoderLayerWeights],
-                 cache: PagedKVCache | PagedKVCacheFp8):
+                 cache: PagedKVCache | PagedKVCacheFp8, adapters: list[LayerAdapters] | None = None):
         self.cfg = cfg
         self.layers = layers
         self.cache = cache
+        self.adapters = adapters
+        self.num_adapters = 0
+        if adapters is not None:
+            pools = [p for a in adapters for p in (a.qkv, a.o) if p is not None]
+            if len(adapters) != len(layers) or not pools or len({p.num_adapters for p in pools}) != 1:
+                raise ValueError(f"adapters must be one LayerAdapters for each of the {len(layers)} layers, with pools of one "
+                                 "number of adapters")
+            self.num_adapters = pools[0].num_adapters
         dev = layers[0].wqkv.device
         self.inv_freq = default_inv_freq(cfg, dev)
         self._graph = None
@@ -218,32 +258,55 @@ class DecodeModel:
         if not isinstance(self.cache, PagedKVCacheFp8):
             raise TypeError(f"this call needs a PagedKVCacheFp8, the model has a {type(self.cache).__name__}")
 
+    def _need_adapters(self) -> None:
+        if self.adapters is None:
+            raise ValueError("the model was made without adapters")
+
+    def _lora_args(self, i: int, lora: kernels.LoraPlan | None) -> dict:
+        return {} if lora is None else {"adapters": self.adapters[i], "lora": lora}
+
+    def lora_plan(self, adapter_ids, plan: kernels.PagedPlan | None = None,
+                  out: kernels.LoraPlan | None = None) -> kernels.LoraPlan:
+        """The rows of a step by adapter (``kernels.lora_plan``): ``adapter_ids`` int32 [B], each sequence's adapter (-1:
+        none), for ``step``, or with the step's ``plan`` for ``run``."""
+        self._need_adapters()
+        if plan is None:
+            return kernels.lora_plan(adapter_ids, self.num_adapters, out=out)
+        return kernels.lora_plan(adapter_ids, self.num_adapters, cu_rows=plan.cu_tokens, num_rows=plan.sizes[1], out=out)
+
     def plan(self, cached_lens, new_lens, block_tables, free_pages, num_tokens: int, max_new_tokens: int,
              out: kernels.PagedPlan | None = None) -> kernels.PagedPlan:
         """The plan of a step over the 8-bit cache (``kernels.paged_plan`` with this model's heads)."""
         return kernels.paged_plan(cached_lens, new_lens, block_tables, free_pages, num_tokens, max_new_tokens,
                                   self.cfg.heads, self.cfg.kv_heads, out=out)
 
-    def run(self, h, plan: kernels.PagedPlan):
+    def run(self, h, plan: kernels.PagedPlan, lora: kernels.LoraPlan | None = None):
         """Every layer on the hidden states [T, hidden] of a plan's rows, over the 8-bit cache; returns theirs after
         the last layer (padding rows: of no use)."""
         self._need_fp8_cache()
+        if lora is not None:
+            self._need_adapters()
         for i, w in enumerate(self.layers):
-            h = moe_sublayer(w, h, attention_sublayer_fp8(w, h, plan, self.inv_freq, *self.cache.layer(i)))
+            h = moe_sublayer(w, h, attention_sublayer_fp8(w, h, plan, self.inv_freq, *self.cache.layer(i),
+                                                          **self._lora_args(i, lora)))
         return h
 
-    def capture_run(self, h, cached_lens, new_lens, block_tables, free_pages, max_new_tokens: int):
+    def capture_run(self, h, cached_lens, new_lens, block_tables, free_pages, max_new_tokens: int, adapter_ids=None):
         """Records a step's plan and ``run`` on copies of the given inputs; returns (graph, static inputs, static
         output, plan).  ``block_tables`` is among the static inputs: a replay enters the new pages there."""
         self._need_fp8_cache()
         dev = h.device
         statics = [t.clone() for t in (h, cached_lens, new_lens, block_tables, free_pages)]
+        if adapter_ids is not None:
+            self._need_adapters()
+            statics.append(adapter_ids.clone())
         lens = statics[2]
         real = lens.clone()
 
         def step():
-            plan = self.plan(*statics[1:], h.shape[0], max_new_tokens)
-            return self.run(statics[0], plan), plan
+            plan = self.plan(*statics[1:5], h.shape[0], max_new_tokens)
+            lora = None if adapter_ids is None else self.lora_plan(statics[5], plan)
+            return self.run(statics[0], plan, lora), plan
 
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -258,32 +321,64 @@ class DecodeModel:
             out, plan = step()
         return graph, statics, out, plan
 
-    def step(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True):
+    def step(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True,
+             lora: kernels.LoraPlan | None = None):
         if attention and isinstance(self.cache, PagedKVCacheFp8):
             raise TypeError("step's attention reads a bf16 cache (PagedKVCache), the model has a PagedKVCacheFp8")
+        if lora is not None:
+            self._need_adapters()
         for i, w in enumerate(self.layers):
             o = None
             if attention:
                 o = attention_sublayer(w, h, positions, context_lens, block_tables, self.inv_freq, self.cache.k[i],
-                                       self.cache.v[i])
+                                       self.cache.v[i], **self._lora_args(i, lora))
             if moe:
                 h = moe_sublayer(w, h, o)
             elif o is not None:
                 h = h + o
         return h
 
-    def capture(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True):
+    def capture(self, h, positions, context_lens, block_tables, moe: bool = True, attention: bool = True,
+                adapter_ids=None):
         """Records one step on copies of the given inputs; returns the graph handle
         (graph, static inputs, static output)."""
         dev = h.device
         statics = [t.clone() for t in (h, positions, context_lens, block_tables)]
+        if adapter_ids is not None:
+            self._need_adapters()
+            statics.append(adapter_ids.clone())
+
+        def step():
+            more = {} if adapter_ids is None else {"lora": self.lora_plan(statics[4])}
+            return self.step(*statics[:4], moe=moe, attention=attention, **more)
+
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):  # warm the allocator and the library outside the capture
-            self.step(*statics, moe=moe, attention=attention)
+            step()
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):  # a stream of dev, whichever device is the current one
-            out = self.step(*statics, moe=moe, attention=attention)
+            out = step()
         return graph, statics, out
+
+
+class OutputHead:
+    """What follows the layers: the model's last RMSNorm (``norm`` bf16 [hidden]) and lm_head (``weight`` bf16 [vocab,
+    hidden]), ``Qwen3MoeModel.norm`` and ``Qwen3MoeForCausalLM.lm_head``."""
+
+    def __init__(self, norm: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6):
+        self.norm, self.weight, self.eps = norm, weight, eps
+
+    def logits(self, h: torch.Tensor) -> torch.Tensor:
+        """bf16 [T, vocab] of hidden states [T, hidden]."""
+        x = kernels.rms_norm(h, self.norm, self.eps)
+        if self.weight.shape[0] % 64 or self.weight.shape[1] % 128:  # the library's linear kernel takes no such sizes
+            return torch.nn.functional.linear(x, self.weight)
+        return _linear(x, self.weight)
+
+    def token_logprobs(self, h: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> kernels.TokenLogprobs:
+        """Log probabilities of ``tokens`` [T] as what comes after the hidden states' own tokens, with entropy and the
+        ``top_k`` most likely ones (``kernels.token_logprobs``)."""
+        return kernels.token_logprobs(self.logits(h), tokens, top_k)
