@@ -109,13 +109,25 @@ __device__ __forceinline__ Row row_of(Sums v) {
 }
 __device__ __forceinline__ float logprob(const Row& r, float x) { return (float)((double)x - r.m - r.ln_z); }
 
-// Entropy and the given token's logprob, by one thread
+// A row's given token, asked for at a kernel's start: at its end the number and then the value would each be a wait for
+// memory (1 row 10.0 -> GIVEN1 us, 64 rows with 20 alternatives 16.9 -> GIVEN64).
+struct Given {
+  int64_t token;
+  float x;
+};
 template <typename E>
-__device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r) {
+__device__ __forceinline__ Given given_of(const LpArgs& a, int row) {
+  Given g{-1, 0.f};
+  if (a.tokens) {
+    g.token = a.id_bytes == 8 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
+    g.x = value_at((const E*)a.x + row * a.stride, g.token < 0 || g.token >= a.V ? 0 : g.token);
+  }
+  return g;
+}
+// Entropy and the given token's logprob, by one thread
+__device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r, const Given& g) {
   a.entropy[row] = r.entropy;
-  if (!a.tokens) return;
-  const int64_t g = a.id_bytes == 8 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
-  a.logprobs[row] = g < 0 ? 0.f : g < a.V ? logprob(r, value_at((const E*)a.x + row * a.stride, g)) : NAN;
+  if (a.tokens) a.logprobs[row] = g.token < 0 ? 0.f : g.token < a.V ? logprob(r, g.x) : NAN;
 }
 
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return ~wave_max_u32_uniform(~v); }
@@ -289,6 +301,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     now[1] = load(first + kThreads + lane);
   }
   const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
+  Given given{};
+  if (a.splits == 1) given = given_of<E>(a, row);
   if (wave == 0) {  // the other waves' is -inf
     if (TOP) top.lane_max = edge_value;
     reference(edge_value);
@@ -464,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     a.sums[blockIdx.x] = make_float4(sum.m, sum.s, sum.t, 0.f);
     return;
   }
-  finish<E>(a, row, r);
+  finish(a, row, r, given);
 }
 
 // Joins a row's splits: their sums, and the k largest of their lists
@@ -474,22 +488,28 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   __shared__ int s_count;
   __shared__ uint32_t s_bound[kWaves];
   const int row = blockIdx.x, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float4* parts = a.sums + (long)row * a.splits;
   const uint64_t* keys = a.keys + (long)row * a.splits * a.k;
-  if (threadIdx.x == 0) s_count = 0;
-  __syncthreads();
+  const int n = a.splits * a.k;
+  // everything asked for at once
   const float4 v = lane < a.splits ? parts[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  const Row r = row_of(join_wave(Sums{v.x, v.y, v.z}));
+  const int j = min(1 << wave, a.k), c = a.k > 0 ? (a.k + j - 1) / j : 0;
+  const uint64_t mine = a.k > 0 && lane < a.splits ? keys[(long)lane * a.k + j - 1] : 0;
+  const uint64_t first = (int)threadIdx.x < n ? keys[threadIdx.x] : 0;
+  const Given given = given_of<E>(a, row);
+  if (threadIdx.x == 0) s_count = 0;
   if (a.k > 0) {
     // Where c splits have j values of at least b each, with c j >= k, the k largest are all >= b: wave w looks at j = 1, 2, 4, 8.
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = min(1 << wave, a.k), c = (a.k + j - 1) / j;
-    const uint32_t mine = lane < a.splits ? (uint32_t)(keys[(long)lane * a.k + j - 1] >> 32) : 0;
-    const uint32_t b = c <= a.splits ? bound_of(mine, c) : 0;
+    const uint32_t b = c <= a.splits ? bound_of((uint32_t)(mine >> 32), c) : 0;
     if (lane == 0) s_bound[wave] = b;
+  }
+  const Row r = row_of(join_wave(Sums{v.x, v.y, v.z}));
+  if (a.k > 0) {
     __syncthreads();
     const uint64_t least = (uint64_t)max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])) << 32;
-    for (int i = threadIdx.x; i < a.splits * a.k; i += kThreads) {
-      const uint64_t key = keys[i];
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint64_t key = i < kThreads ? first : keys[i];
       if (key >= least && key != 0) list[atomicAdd(&s_count, 1)] = key;
     }
     __syncthreads();
@@ -498,8 +518,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
       a.top_logprobs[(long)row * a.k + place] = logprob(r, value_of(key));
     });
   }
-  if (threadIdx.x != 0) return;
-  finish<E>(a, row, r);
+  if (threadIdx.x == 0) finish(a, row, r, given);
 }
 
 bool lp_ok(int T, int V, int k) { return T >= 0 && V >= 1 && k >= 0 && k <= kMaxTop && k <= V && T < (1 << 24); }
