@@ -24,7 +24,6 @@ constexpr int kMaxTop = 64;
 constexpr int kBuf = 512;      // candidates that a wave keeps
 constexpr int kKeep = 128;     // ... after they are cut down, at most
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
-constexpr int kVecs = 256;             // vectors whose values a workgroup looks at at the end
 constexpr int kMaxSplits = 64;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -110,7 +109,7 @@ __device__ __forceinline__ Row row_of(Sums v) {
 __device__ __forceinline__ float logprob(const Row& r, float x) { return (float)((double)x - r.m - r.ln_z); }
 
 // A row's given token, asked for at a kernel's start: at its end the number and then the value would each be a wait for
-// memory (1 row 10.0 -> GIVEN1 us, 64 rows with 20 alternatives 16.9 -> GIVEN64).
+// memory (64 rows with 20 alternatives 16.9 -> 16.5 us).
 struct Given {
   int64_t token;
   float x;
@@ -154,28 +153,18 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
 }
 
 struct TopLds {
-  uint64_t buf[kWaves][kBuf];  // at the end the list of all waves, kList + 3 at most
-  int vecs[kVecs];
+  uint64_t buf[kWaves][kBuf];
+  uint64_t list[kList + 4];  // of all waves, at the end
   uint32_t bound[kWaves];
-  int n_vecs, n_list;
+  int n_list;
 };
 
-// A wave's candidates
+// A wave's candidates in the plain scan
 struct Top {
   uint64_t* buf;
-  int count;          // wave-uniform
-  uint64_t least;     // keys below are not among the k largest; wave-uniform
-  float least_value;
-  float lane_max;
-  uint32_t bound;  // of the wave's lanes
+  int count;       // wave-uniform
+  uint64_t least;  // keys below are not among the k largest; wave-uniform
 };
-
-__device__ __forceinline__ void raise(Top& t, uint64_t least) {
-  if (least > t.least) {
-    t.least = least;
-    t.least_value = value_of(least);
-  }
-}
 
 // There is room for 64 more.
 __device__ __forceinline__ void offer(Top& t, float x, int index, bool valid) {
@@ -209,7 +198,7 @@ __device__ __forceinline__ void cut(Top& t, int k, int lane) {
       hi = mid - 1;
     }
   }
-  raise(t, lo);
+  t.least = lo;
   t.count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -259,7 +248,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const int edge = lane < n_head ? lane : tail0 + lane - n_head;
   const int per_wave = (a.k + kWaves - 1) / kWaves;
 
-  Top top{lds.buf[wave], 0, 0, -INFINITY, -INFINITY, 0};
+  // candidates: vectors, as {bits of the maximum, index}
+  uint64_t* buf = lds.buf[wave];
+  int count = 0;
+  uint32_t bound = 0;                          // that the wave's lanes give
+  float lane_max = -INFINITY, least = -INFINITY;  // values below `least` are not among the k largest
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
   auto reference = [&](float pm) __attribute__((always_inline)) {
     if (__any(pm > limit)) {
@@ -282,14 +275,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     t = fmaf(e, fmaxf(d, kNoTerm), t);
   };
   auto renew = [&]() __attribute__((always_inline)) {
-    top.bound = max(bound_of(ordered(top.lane_max), per_wave), top.bound);
-    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = top.bound;
+    bound = max(bound_of(ordered(lane_max), per_wave), bound);
+    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = bound;
   };
   auto take_bound = [&]() __attribute__((always_inline)) {
     uint32_t b = ~0u;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
-    raise(top, (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(b) << 32);
+    least = from_ordered(__builtin_amdgcn_readfirstlane(b));
+  };
+  auto offer_vec = [&](float most, int index, bool valid) __attribute__((always_inline)) {
+    const bool pass = valid && !(most < least);
+    const uint64_t mask = __ballot(pass);
+    if (pass) buf[count + __popcll(mask & lanemask_lt())] = (uint64_t)__float_as_uint(most) << 32 | (uint32_t)index;
+    count += __popcll(mask);
+  };
+  auto drop = [&]() __attribute__((always_inline)) {  // candidates that the bound has passed
+    const int n = count;
+    count = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; j += MOE_WAVE) {
+      const uint64_t e = buf[min(j + lane, n - 1)];
+      offer_vec(__uint_as_float((uint32_t)(e >> 32)), (int)(uint32_t)e, j + lane < n);
+    }
   };
 
   // Two vectors a turn, those of the next one on their way, and before them the edges; the first turn gives a bound to go by.
@@ -304,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   Given given{};
   if (a.splits == 1) given = given_of<E>(a, row);
   if (wave == 0) {  // the other waves' is -inf
-    if (TOP) top.lane_max = edge_value;
+    if (TOP) lane_max = edge_value;
     reference(edge_value);
     add(edge_value);
   }
@@ -337,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) add(v[h][e]);
     if (TOP) {
-      top.lane_max = fmaxf(top.lane_max, most);
+      lane_max = fmaxf(lane_max, most);
       if (brief) break;
       if (turn == 0 || turn == renewal) {
         renew();
@@ -345,12 +353,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         else renewal = 4 * renewal + 3;
         take_bound();
       }
-      if (__any(!(most < top.least_value))) {
+      if (__any(!(most < least))) {
         take_bound();  // the other waves may have renewed theirs
-        full |= top.count > kBuf - 2 * MOE_WAVE;
-        if (full) top.count = 0;
+        if (count > kBuf - 2 * MOE_WAVE) {
+          renew();
+          take_bound();
+          drop();
+          full |= count > kBuf - 2 * MOE_WAVE;
+          if (full) count = 0;
+        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) offer(top, pm[h], i + h * kThreads, i + h * kThreads < v1);
+        for (int h = 0; h < 2; ++h) offer_vec(pm[h], i + h * kThreads, i + h * kThreads < v1);
       }
     }
     now[0] = next[0];
@@ -363,9 +376,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
 
   if (lane == 0) s_max[wave] = m;
-  if (TOP && threadIdx.x == 0) lds.n_vecs = lds.n_list = 0;
+  if (TOP && threadIdx.x == 0) lds.n_list = 0;
   if (TOP) renew();
-  uint64_t* list = lds.buf[0];
+  uint64_t* list = lds.list;
   if (lane == 0) s_odd[wave] = full || !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar);
   __syncthreads();
   bool again = false;
@@ -373,38 +386,42 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   for (int w = 0; w < kWaves; ++w) again |= s_odd[w] != 0;
   if (TOP && !again) {
     take_bound();
-    auto keep = [&](float v, int index) __attribute__((always_inline)) {
-      const uint64_t key = key_of(v, index);
-      if (key < top.least) return;
-      const int at = atomicAdd(&lds.n_list, 1);
-      if (at < kList) list[at] = key;
-    };
-    if (!brief) {
-      for (int j = lane; j < top.count; j += MOE_WAVE) {
-        const uint64_t key = top.buf[j];
-        if (key < top.least) continue;
-        const int at = atomicAdd(&lds.n_vecs, 1);
-        if (at < kVecs) lds.vecs[at] = index_of(key);
-      }
-      __syncthreads();
-      const int n = lds.n_vecs;
-      again = n > kVecs;
-      if ((int)threadIdx.x < min(n, kVecs)) {
-        const int at = lds.vecs[threadIdx.x];
-        unpack(xv[at], v[0]);
+    // The values that reach the bound go to the list, a wave asking once for places; value e is index + e.
+    auto keep = [&](const float* v, int n, int index, bool valid) __attribute__((always_inline)) {
+      uint64_t mask[kVec];
+      int found = 0;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) keep(v[0][e], head + at * kVec + e);
+      for (int e = 0; e < n; ++e) {
+        mask[e] = __ballot(valid && !(v[e] < least));
+        found += __popcll(mask[e]);
       }
-    } else {
+      if (found == 0) return;
+      int to = 0;
+      if (lane == 0) to = atomicAdd(&lds.n_list, found);
+      to = __builtin_amdgcn_readfirstlane(to);
+#pragma unroll
+      for (int e = 0; e < n; ++e) {
+        const int at = to + __popcll(mask[e] & lanemask_lt());
+        if ((mask[e] >> lane & 1) && at < kList) list[at] = key_of(v[e], index + e);
+        to += __popcll(mask[e]);
+      }
+    };
+    if (brief) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = first + lane + h * kThreads;
-        if (at < v1 && !(pm[h] < top.least_value))
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) keep(v[h][e], head + at * kVec + e);
+        keep(v[h], kVec, head + at * kVec, at < v1);
+      }
+    } else {
+      drop();
+#pragma unroll 1
+      for (int j = 0; j < count; j += MOE_WAVE) {  // their other values are read again
+        const int at = (int)(uint32_t)buf[min(j + lane, count - 1)];
+        unpack(xv[at], v[0]);
+        keep(v[0], kVec, head + at * kVec, j + lane < count);
       }
     }
-    if (lane < n_edge) keep(edge_value, edge);
+    keep(&edge_value, 1, edge, lane < n_edge);
     __syncthreads();
     again |= lds.n_list > kList;
   }
@@ -424,9 +441,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       t = fmaf(e, fmaxf(d, kNoTerm), t);
     };
     term(edge_value);
+    Top top{buf, 0, 0};
     if (TOP) {
       if (threadIdx.x == 0) lds.n_list = 0;
-      top.count = 0, top.least = 0;
       offer(top, edge_value, edge, lane < n_edge);
     }
     for (int i0 = first; i0 < v1; i0 += kThreads) {
@@ -442,14 +459,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       }
     }
     sum = Sums{m, wave_sum_uniform(s), wave_sum_uniform(t)};
-    if (TOP) {  // the waves' candidates in one list, which takes the place of their buffers
-      uint64_t key[kKeep / MOE_WAVE];
-#pragma unroll
-      for (int j = 0; j < kKeep / MOE_WAVE; ++j) key[j] = j * MOE_WAVE + lane < top.count ? top.buf[j * MOE_WAVE + lane] : 0;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kKeep / MOE_WAVE; ++j)
-        if (key[j] != 0) list[atomicAdd(&lds.n_list, 1)] = key[j];
+    if (TOP) {
+      __syncthreads();  // the list is empty
+      for (int j = lane; j < top.count; j += MOE_WAVE) list[atomicAdd(&lds.n_list, 1)] = top.buf[j];
     }
   }
   if (lane == 0) s_sums[wave] = sum;
