@@ -401,7 +401,7 @@ int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, long long x_
  * has NaN for logprobs and entropy.  fp32 sums.  No counterpart in the reference.
  *   logits  bf16 (dtype 0) or fp32 (1) [T, V], rows `stride` values apart    tokens [T] (id_bytes 4 or 8) or NULL, then
  *   logprobs may be NULL    entropy fp32 [T]    top_ids int64, top_logprobs fp32 [T, k] (k 0: may be NULL)
- * 1 <= V, 0 <= k <= min(V, 64), T < 2^24.
+ * 1 <= V <= 2^30, 0 <= k <= min(V, 64), T < 2^24.
  */
 size_t moe_mi355x_token_logprobs_workspace_bytes(int T, int V, int k);
 int moe_mi355x_token_logprobs(const void* logits, int dtype, long long stride, const void* tokens, int id_bytes, int T,

@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / MOE_WAVE;
 constexpr int kMaxTop = 64;
+constexpr int kMaxV = 1 << 30;  // places in a row, and a little past it, are ints
 constexpr int kBuf = 512;      // candidates that a wave keeps
 constexpr int kKeep = 128;     // ... after they are cut down, at most
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
@@ -128,8 +129,6 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r, c
   a.entropy[row] = r.entropy;
   if (a.tokens) a.logprobs[row] = g.token < 0 ? 0.f : g.token < a.V ? logprob(r, g.x) : NAN;
 }
-
-__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) { return ~wave_max_u32_uniform(~v); }
 
 // A bound that at least n of the wave's 64 values reach, close to the n-th largest: down from the largest by growing
 // steps, of 1/32 of a binade at first, then back by three halvings of the last one.
@@ -533,7 +532,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   if (threadIdx.x == 0) finish(a, row, r, given);
 }
 
-bool lp_ok(int T, int V, int k) { return T >= 0 && V >= 1 && k >= 0 && k <= kMaxTop && k <= V && T < (1 << 24); }
+bool lp_ok(int T, int V, int k) { return T >= 0 && T < (1 << 24) && V >= 1 && V <= kMaxV && k >= 0 && k <= kMaxTop && k <= V; }
 
 // Workgroups of a row: for three workgroups a CU in all, each with 4096 values at least.  (us in a graph, for 512 / 768 /
 // 1024 / 2048 workgroups, 151936 bf16 values a row: 64 rows with 20 alternatives 17.7 / 17.7 / 18.4 / 21.1, 256 rows 35.1 /

@@ -1026,8 +1026,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise ValueError(f"logits must be on a ROCm GPU device, got {logits.device}")
     T, V = logits.shape
     stride = logits.stride(0) if T > 1 else V
-    if V < 1 or T >= 1 << 24:
-        raise ValueError(f"logits must have at least one column and fewer than 2^24 rows, got {tuple(logits.shape)}")
+    if not 1 <= V <= 1 << 30 or T >= 1 << 24:
+        raise ValueError(f"logits must have 1 to 2^30 columns and fewer than 2^24 rows, got {tuple(logits.shape)}")
     if (V > 1 and logits.stride(1) != 1) or stride < V:
         raise ValueError(f"logits: rows must be contiguous and not overlap, got strides {logits.stride()}")
     if not 0 <= top_k <= min(V, TOP_MAX):

@@ -152,3 +152,12 @@ def test_projections_add_where_there_is_a_pool_and_a_plan(dec, monkeypatch):
     x = torch.ones(2)
     assert dec._project(x, 3.0, None, "plan").tolist() == [3, 3] and dec._project(x, 3.0, "pool", None).tolist() == [3, 3]
     assert not calls and dec._project(x, 3.0, "pool", "plan").tolist() == [4, 4] and calls == [("pool", "plan")]
+
+
+def test_rows_of_logits_end_at_2_30(lib):
+    """A place in a row, and a vector's past its end, stay ints; the split of one row over workgroups too."""
+    ws = lib.moe_mi355x_token_logprobs_workspace_bytes
+    assert ws(1, 1 << 30, 5) > 0
+    for V in ((1 << 30) + 1, (1 << 31) - 4096, (1 << 31) - 1):
+        assert ws(1, V, 5) == 0
+        assert lib.moe_mi355x_token_logprobs(FAKE, 0, 1 << 32, FAKE, 8, 1, V, 5, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == -1
