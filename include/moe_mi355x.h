@@ -385,7 +385,8 @@ int moe_mi355x_lora_plan(const int32_t* adapter_ids, const int32_t* cu_rows, int
  * are left as they are; what a and b hold past an adapter's rank reaches nothing.
  *   y bf16 [T, N], N = sum of columns, and x bf16 [T, K]; rows y_stride and x_stride values apart (multiples of 8)
  *   a bf16 [L, parts R, K]    b bf16 [L, N, R]    ranks int32 [L]    scales fp32 [L]    columns: host array [parts]
- * K % 32 == 0, R % 16 == 0, R <= 128, 1 <= parts <= 4, columns[p] % 32 == 0; x and y must not overlap.
+ * K % 32 == 0, R % 16 == 0, R <= 128, 1 <= parts <= 4, columns[p] % 32 == 0; x and y share no value (-1; side by
+ * side in wider rows is fine).
  */
 size_t moe_mi355x_lora_add_workspace_bytes(int T, int L, int K, int R, int parts, const int* columns);
 int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, long long x_stride, const void* a, const void* b,

@@ -604,6 +604,15 @@ LoraForm lora_form(const LoraLayout& p, int K, int R, int parts, int N) {
   return f;
 }
 
+// Whether rows of y and of x share no value: they lie in different ranges, or side by side in rows of one length.  (What a
+// workgroup adds to y is not ordered against what another reads of x.)
+bool rows_disjoint(const uint16_t* y, long y_stride, long N, const uint16_t* x, long x_stride, long K, long T) {
+  if (x + (T - 1) * x_stride + K <= y || y + (T - 1) * y_stride + N <= x) return true;
+  if (y_stride != x_stride || T == 1) return false;
+  const long at = ((x - y) % y_stride + y_stride) % y_stride;
+  return at >= N && at + K <= y_stride;
+}
+
 size_t lora_ws(const LoraLayout& p, const LoraForm& f, int R, int parts) {
   return f.few ? 0 : moe_align_up((size_t)f.shares * p.T * parts * R * sizeof(float), 256);
 }
@@ -655,6 +664,7 @@ extern "C" int moe_mi355x_lora_add(void* y, long long y_stride, const void* x, l
   const size_t need = lora_ws(g.p, f, R, parts);
   MOE_RETURN_IF(need > 0 && (!workspace || workspace_bytes < need), MOE_ERR_WORKSPACE);
   MOE_RETURN_IF(need > 0 && !moe_aligned16(workspace), MOE_ERR_ALIGNMENT);
+  MOE_RETURN_IF(!rows_disjoint((const uint16_t*)y, y_stride, n, (const uint16_t*)x, x_stride, K, T), MOE_ERR_INVALID_ARG);
   g.y = (uint16_t*)y, g.x = (const uint16_t*)x, g.y_stride = y_stride, g.x_stride = x_stride;
   g.a = (const uint16_t*)a, g.b = (const uint16_t*)b, g.ranks = ranks, g.scales = scales;
   g.plan = (const int32_t*)plan, g.u = (float*)workspace;

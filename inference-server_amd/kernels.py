@@ -973,7 +973,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, pool: LoraPool, plan: LoraPlan) -
     """Adds to ``y``, the shared projection of ``x``, in place what each row's adapter contributes:
     ``y[t] += scale_l * B_l (A_l x[t])``, part by part.  Prompts and single tokens of any number of requests in
     one call; rows without an adapter are left as they are.  ``y`` bf16 [T, N], ``x`` bf16 [T, K] (rows may lie
-    apart); returns ``y``.  fp32 sums, one rounding of the result; ``A x`` is kept to 2^-17 of its value."""
+    apart, but x and y share no value); returns ``y``.  fp32 sums, one rounding of the result; ``A x`` is kept to 2^-17 of its value."""
     if not isinstance(pool, LoraPool) or not isinstance(plan, LoraPlan):
         raise TypeError("pool must be a LoraPool and plan a LoraPlan (lora_plan)")
     if pool.num_adapters != plan.num_adapters:

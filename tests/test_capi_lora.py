@@ -161,3 +161,14 @@ def test_rows_of_logits_end_at_2_30(lib):
     for V in ((1 << 30) + 1, (1 << 31) - 4096, (1 << 31) - 1):
         assert ws(1, V, 5) == 0
         assert lib.moe_mi355x_token_logprobs(FAKE, 0, 1 << 32, FAKE, 8, 1, V, 5, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == -1
+
+
+@pytest.mark.parametrize("at,ys,xs,T", [
+    (0, 96, 256, 5000), (64, 96, 256, 5000), (-256, 96, 256, 5000), (5000 * 96 - 8, 96, 256, 5000), (88, 352, 352, 5000),
+    (104, 352, 352, 5000), (-248, 352, 352, 5000), (7 * 352, 352, 352, 5000), (88, 352, 352, 1), (-248, 96, 256, 1)])
+def test_add_refuses_an_x_that_it_would_change(lib, at, ys, xs, T):
+    """x `at` values behind y, K 256 and N 96."""
+    y = 1 << 30
+    n = lib.moe_mi355x_lora_add_workspace_bytes(T, 4, 256, 16, 2, ints(64, 32))
+    assert lib.moe_mi355x_lora_add(y, ys, y + 2 * at, xs, FAKE, FAKE, FAKE, FAKE, FAKE, T, 4, 256, 16, 2, ints(64, 32), FAKE, n,
+                                   None) == -1
