@@ -212,3 +212,46 @@ def test_refusals(pkg, dev):
     for args in ((x.half(),), (None,), (x, t.float()), (x, [0])):
         with pytest.raises(TypeError):
             pkg.token_logprobs(*args)
+
+
+@pytest.mark.parametrize("T,k", [(3, 7), (900, 20)])
+def test_rows_that_rise_and_fall(pkg, dev, T, k):
+    """Candidates keep coming along a row that rises, in one wave's places alone, or in steps; none after the first values of
+    one that falls."""
+    V = 60000
+    at = torch.arange(V, dtype=torch.float32)
+    wave = torch.where(at // 512 % 4 == 1, at / V * 9, -5.0)
+    rows = torch.stack([at / V * 9 + at % 7 * 1e-3, wave, (at // 4096) * 0.75 - at % 3, 9 - at / V * 9])
+    x = torch.cat([rows.to(torch.bfloat16), rows[:, torch.randperm(V, generator=torch.Generator().manual_seed(1))].to(torch.bfloat16)]).to(dev)
+    x = x.repeat((T + 7) // 8, 1)[:T].contiguous()
+    r = check(pkg, x[:8].contiguous(), tokens_of(dev, min(T, 8), V), k)
+    many = pkg.token_logprobs(x, None, k)
+    assert torch.equal(many.top_ids[:8], r.top_ids) and torch.equal(many.top_ids[-1], r.top_ids[(T - 1) % 8])
+    check(pkg, x.float()[:8].contiguous(), None, k)
+
+
+@pytest.mark.parametrize("dtype,stride", [(torch.bfloat16, (1 << 31) + 8), (torch.float32, (1 << 30) + 3)])
+def test_rows_2_31_apart(pkg, dev, dtype, stride):
+    T, V = 3, 5000
+    whole = torch.empty((T - 1) * stride + V, dtype=dtype, device=dev)
+    x = whole.as_strided((T, V), (stride, 1))
+    x.copy_(logits_of(dev, T, V, dtype))
+    check(pkg, x, tokens_of(dev, T, V), 6)
+
+
+def test_a_row_of_2_27(pkg, dev):
+    """One row in 64 parts, its largest at the edges and in the middle.  Tolerances as above, for a lane's 2^13 values."""
+    V = (1 << 27) + 5
+    x = logits_of(dev, 1, V)
+    for at, v in ((V - 1, 24.0), (0, 23.0), (V // 2, 22.0), (V - 6, 21.0)):
+        x[0, at] = v
+    r = pkg.token_logprobs(x, torch.tensor([V - 1], device=dev), 4)
+    d = x[0].double()
+    ln_z = d.logsumexp(0)
+    entropy = ln_z - ((d - ln_z).exp() * d).sum()
+    z = (60 + V / 64 / 256) * 2.0 ** -24
+    assert r.top_ids.tolist() == [[V - 1, 0, V // 2, V - 6]]
+    assert (r.top_logprobs[0].double() - torch.tensor([24.0, 23, 22, 21], device=dev) + ln_z).abs().max() <= z + 2.0 ** -22
+    assert r.logprobs[0] == r.top_logprobs[0, 0]
+    dist = (24 * torch.ones((), device=dev) - (ln_z - entropy)).abs().double()
+    assert (r.entropy[0].double() - entropy).abs() <= z * (1 + 2 * (dist + 11)) + 2.0 ** -23 * entropy.abs()

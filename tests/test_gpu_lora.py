@@ -293,3 +293,56 @@ def test_refusals(pkg, dev):
     for args in ((ids.long(), 2), ([0], 2)):
         with pytest.raises(TypeError):
             pkg.lora_plan(*args)
+
+
+@pytest.mark.parametrize("T,K,columns,R,ranks", [
+    (16, 8192, (256,), 64, [64]),           # tiles of up to 16 rows, and of more
+    (17, 8192, (256,), 64, [64]),
+    (65, 8224, (160,), 64, [33]),           # a row over a tile; k past whole slices
+    (130, 4128, (288, 32), 80, [80, 1]),
+    (256, 2080, (224,), 16, [16] * 256),    # the last step with small tiles, an adapter a row
+    (257, 2080, (224,), 16, [16] * 256),
+    (128, 2048, (576,), 32, [32, 15]),      # at the limit of the form of few rows, and past it
+    (129, 2048, (576,), 32, [32, 15]),
+    (90, 8192, (672,), 16, [9] * 40),
+    (600, 1312, (96, 96, 96, 96), 112, [112, 97, 65, 64, 63]),
+])
+def test_edges_of_forms_and_tiles(pkg, dev, T, K, columns, R, ranks):
+    Case(pkg, dev, T, K, columns, R, ranks, seed=T + R, ids=[t * len(ranks) // T for t in range(T)]).run(pkg)
+    Case(pkg, dev, T, K, columns, R, ranks, seed=T + R, poison=True).run(pkg)
+
+
+@pytest.mark.parametrize("T,stride", [(40, 512), (1000, 512), (2100, 1 << 21)])
+def test_x_and_y_side_by_side(pkg, dev, T, stride):
+    """In rows of one buffer, in either order; the longest past 2^32 values."""
+    c = Case(pkg, dev, T, 256, (64, 32), 32, [32, 7, 20], seed=2)
+    want = pkg.lora_add(c.y.clone(), c.x, c.pool, c.plan)
+    whole = torch.empty((T, stride), dtype=torch.bfloat16, device=dev)
+    for x, y in ((whole[:, :256], whole[:, 256:352]), (whole[:, -256:], whole[:, -352:-256]), (whole[:, :256], whole[:, -96:])):
+        x.copy_(c.x)
+        y.copy_(c.y)
+        assert torch.equal(pkg.lora_add(y, x, c.pool, c.plan), want) and torch.equal(x, c.x)
+
+
+@pytest.mark.parametrize("K,N", [(64, 131104), (131104, 64)])
+@pytest.mark.parametrize("T", [2, 300])
+def test_the_last_adapter_of_a_pool_past_2_32(pkg, dev, K, N, T):
+    L, R = 256, 128
+    one = Case(pkg, dev, T, K, (N,), R, [128], seed=4, ids=[0] * T)
+    a, b = (torch.empty((L, *t.shape[1:]), dtype=t.dtype, device=dev) for t in (one.a, one.b))
+    a[-1], b[-1] = one.a[0], one.b[0]
+    scales = torch.zeros(L, device=dev)
+    scales[-1] = one.scales[0]
+    pool = pkg.LoraPool(a, b, i32([0] * (L - 1) + [128], dev), scales, (N,))
+    got = pkg.lora_add(one.y.clone(), one.x, pool, pkg.lora_plan(i32([L - 1] * T, dev), L))
+    one.run(pkg)
+    one.check(got)
+
+
+def test_an_x_that_it_would_change_is_refused(pkg, dev):
+    c = Case(pkg, dev, 8, 64, (64,), 16, [16])
+    wide = torch.zeros((9, 192), dtype=torch.bfloat16, device=dev)
+    same = torch.zeros((8, 64), dtype=torch.bfloat16, device=dev)
+    for y, x in ((same, same), (wide[:8, :64], wide[:8, 56:120]), (wide[:8, :64], wide[1:, :64]), (wide[:8, 128:], wide[:8].flatten()[:512].view(8, 64))):
+        with pytest.raises(Exception, match="invalid"):
+            pkg.lora_add(y, x, c.pool, c.plan)
