@@ -577,11 +577,12 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
 }
 
 // How a call is cut up.
-// Few rows: each pair of rows reads its adapter for itself, once for each run, so this pays while rows times rank times K
-// is small.  (us in a graph, few / many rows' form.  2048 to q/k/v 5120, rank 16: 1 row 4.2 / 6.4, 64 rows of 64 adapters
-// 6.3 / 10.0, 256 of 8 10.8 / 11.4; rank 64: 1 row 6.4 / 8.0, 32 of 8 9.6 / 8.9, 64 of 64 17.2 / 16.6, 128 of 64 25.2 / 21.3.
-// 8192 to 4096, rank 64: 1 row 12.0 / 9.1, 64 of 64 31.0 / 20.4.)
-constexpr long kFewWork = 1 << 23, kFewAdapter = 1 << 18;
+// Few rows: every run of columns of each pair of rows reads the part's A for itself, which one CU takes 1.2 us for 64 KB
+// to do, so this pays where rank times K is small, and for the fewer rows the larger it is.  (us in a graph, few / many rows'
+// form, "rows/adapters".  2048 to q/k/v 5120, rank 16: 1/1 3.7 / 5.4, 32/32 5.0 / 7.4, 128/64 9.4 / 11.7, 256/64 13.9 /
+// 12.1; rank 32: 1/1 4.4 / 6.2, 64/64 10.6 / 13.5, 128/64 13.9 / 15.0, 256/64 20.7 / 16.0; rank 64: 1/1 7.3 / 7.7, 8/8 9.4 /
+// 8.3, 32/32 11.3 / 12.6, 48/48 16.0 / 13.7, 128/64 23.5 / 20.7.  4096 to 2048, rank 64: 1/1 7.8 / 6.7, 32/32 12.6 / 10.7.)
+constexpr long kFewAdapter = 1 << 17, kFewRead = 160L << 32;
 // Runs of 512 columns at least, 64 for each wave, and more where that makes more workgroups than this: each forms u again.
 // (128 rows of 100 adapters, 4096 to q/k/v 9216: 17.2 us for 512, 13.7 for 1024, 15.6 for 2048.)
 constexpr int kFewGroups = 1024;
@@ -593,7 +594,8 @@ struct LoraForm {
   int tiles, shares, chunk;
 };
 LoraForm lora_form(const LoraLayout& p, int K, int R, int parts, int N) {
-  LoraForm f{p.M > 0 && (long)R * K <= kFewAdapter && (long)p.T * R * K <= kFewWork, p.N, 1, kManyRun};
+  const long part = (long)R * K;
+  LoraForm f{p.M > 0 && part <= kFewAdapter && p.T * part * part <= kFewRead, p.N, 1, kManyRun};
   if (f.few) {
     f.tiles = p.M;
     for (f.chunk = 512; f.chunk < 4096 && (long)f.tiles * N / f.chunk > kFewGroups;) f.chunk *= 2;
