@@ -1008,6 +1008,11 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace_bytes(rows: int, columns: int, top_k: int) -> int:
+    return _lib.load().moe_mi355x_token_logprobs_workspace_bytes(rows, columns, top_k)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenLogprobs:
     """Log probabilities of ``tokens`` (int32 or int64 [T]) under ``logits`` (bf16 or fp32 [T, V], rows may lie
     apart), the entropy of each row and its ``top_k`` most likely tokens with their log probabilities, descending, the
@@ -1033,17 +1038,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     if not 0 <= top_k <= min(V, TOP_MAX):
         raise ValueError(f"top_k must be in [0, min(V, {TOP_MAX})], got {top_k}")
     if tokens is not None:
-        _need(tokens, "tokens", (torch.int32, torch.int64), 1)
-        _same_device(logits, tokens=tokens)
+        if not _fits(tokens, torch.int64, dev, 1) and not _fits(tokens, torch.int32, dev, 1):
+            _need(tokens, "tokens", (torch.int32, torch.int64), 1)
+            _same_device(logits, tokens=tokens)
         if tokens.shape[0] != T:
             raise ValueError(f"tokens must be [{T}], got {tuple(tokens.shape)}")
-    lib = _lib.load()
     f32 = logits.new_empty((T * (2 + top_k),), dtype=torch.float32)
     entropy, logprobs, top = f32.split_with_sizes([T, T, T * top_k])
     ids = logits.new_empty((T, top_k), dtype=torch.int64)
-    nws = lib.moe_mi355x_token_logprobs_workspace_bytes(T, V, top_k)
+    nws = _logprobs_workspace_bytes(T, V, top_k)
     ws = logits.new_empty(nws, dtype=torch.uint8) if nws else None
-    _launch("token_logprobs", dev, lib.moe_mi355x_token_logprobs, logits.data_ptr(),
+    _launch("token_logprobs", dev, _lib.load().moe_mi355x_token_logprobs, logits.data_ptr(),
             0 if logits.dtype == torch.bfloat16 else 1, stride, None if tokens is None else tokens.data_ptr(),
             8 if tokens is None else _id_bytes(tokens), T, V, top_k, logprobs.data_ptr(), entropy.data_ptr(),
             ids.data_ptr(), top.data_ptr(), ws.data_ptr() if nws else None, nws, _stream(logits))
