@@ -4,7 +4,8 @@
 // A counting sort in one launch.  Each workgroup places 1024 rows; where they go it works out by itself, from
 // counts over all rows (by sequence, where the numbers are the sequences'), which costs less than a second launch.
 // Within a wave the rows of one adapter find each other by the bits of its number (9 ballots), so that neither the
-// order nor the time depends on atomics or on how many adapters meet.
+// order nor the time depends on atomics or on how many adapters meet.  Bound by latency: 4.2 us in a graph for 64 rows of 100
+// adapters, 4.4 for 9044 rows of 12 sequences, of which a launch is 1.7; the rest are four phases between barriers.
 #include "lora.h"
 
 namespace {
@@ -114,28 +115,26 @@ __global__ __launch_bounds__(kThreads) void lora_plan_kernel(LoraPlanArgs a) {
   }
   __syncthreads();
   if (live) {
-    int to = s_first[bin] + s_before[bin] + in_wave;
-    for (int w = 0; w < wave; ++w) to += s_wave[w][bin];
+    int at = s_before[bin] + in_wave;  // among its adapter's rows
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) at += w < wave ? s_wave[w][bin] : 0;
+    const int to = s_first[bin] + at;
     if (to < T) a.plan[p.rows + to] = row;
+    // the row that begins a tile writes its record
+    auto record = [&](const int* from, int height, int room, long list) {
+      const int tile = from[bin] + at / height;
+      if (at % height == 0 && tile < room)
+        *(int4*)(a.plan + list + 4L * tile) = make_int4(bin, to, min(s_total[bin] - at, height), 0);
+    };
+    if (bin < L) {
+      record(s_tile, kLoraRows, p.N, p.tiles);
+      if (p.M > 0) record(s_pair, kLoraPair, p.M, p.pairs);
+    }
   }
   if (blockIdx.x == 0) {
     for (int i = tid; i <= bins; i += kThreads) a.plan[p.offsets + i] = s_first[i];
     if (tid == 0) a.plan[LH_TILES] = s_tile[L], a.plan[LH_PAIRS] = s_pair[L];
   }
-  auto list = [&](const int* from, int height, int room, long to) {
-    for (int t = blockIdx.x * kThreads + tid; t < min(from[L], room); t += gridDim.x * kThreads) {
-      int lo = 0, hi = L - 1;  // the last adapter whose tiles begin at t or before
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (from[mid] <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      const int at = (t - from[lo]) * height;
-      *(int4*)(a.plan + to + 4L * t) = make_int4(lo, s_first[lo] + at, min(s_total[lo] - at, height), 0);
-    }
-  };
-  list(s_tile, kLoraRows, p.N, p.tiles);
-  if (p.M > 0) list(s_pair, kLoraPair, p.M, p.pairs);
 }
 
 }  // namespace
