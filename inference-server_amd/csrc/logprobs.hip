@@ -25,7 +25,9 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / MOE_WAVE;
 constexpr int kMaxTop = 64;
 constexpr int kMaxV = 1 << 30;  // places in a row, and a little past it, are ints
-constexpr int kBuf = 512;      // candidates that a wave keeps
+constexpr int kBatch = 8;      // turns whose vectors' maxima are looked through together
+constexpr int kCand = 192;     // vectors that a wave keeps as candidates
+constexpr int kBuf = 512;      // values that it does in the plain scan
 constexpr int kKeep = 128;     // ... after they are cut down, at most
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
 constexpr int kMaxSplits = 64;
@@ -155,7 +157,11 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
 }
 
 struct TopLds {
-  uint64_t buf[kWaves][kBuf];
+  union {
+    float2 most[kBatch][kThreads];  // maxima of a batch's vectors
+    uint64_t buf[kWaves][kBuf];
+  };
+  uint64_t cand[kWaves][kCand];
   uint64_t list[kList + 4];  // of all waves, at the end
   uint32_t bound[kWaves];
   int n_list;
@@ -251,8 +257,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const int per_wave = (a.k + kWaves - 1) / kWaves;
 
   // candidates: vectors, as {bits of the maximum, index}
-  uint64_t* buf = lds.buf[wave];
+  uint64_t* cand = lds.cand[wave];
   int count = 0;
+  bool full = false;  // more of them than there is room for
   uint32_t bound = 0;                          // that the wave's lanes give
   float lane_max = -INFINITY, least = -INFINITY;  // values below `least` are not among the k largest
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
@@ -289,7 +296,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   auto offer_vec = [&](float most, int index, bool valid) __attribute__((always_inline)) {
     const bool pass = valid && !(most < least);
     const uint64_t mask = __ballot(pass);
-    if (pass) buf[count + __popcll(mask & lanemask_lt())] = (uint64_t)__float_as_uint(most) << 32 | (uint32_t)index;
+    if (mask == 0) return;
+    if (count > kCand - MOE_WAVE) full = true, count = 0;
+    if (pass) cand[count + __popcll(mask & lanemask_lt())] = (uint64_t)__float_as_uint(most) << 32 | (uint32_t)index;
     count += __popcll(mask);
   };
   auto drop = [&]() __attribute__((always_inline)) {  // candidates that the bound has passed
@@ -297,12 +306,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     count = 0;
 #pragma unroll 1
     for (int j = 0; j < n; j += MOE_WAVE) {
-      const uint64_t e = buf[min(j + lane, n - 1)];
+      const uint64_t e = cand[min(j + lane, n - 1)];
       offer_vec(__uint_as_float((uint32_t)(e >> 32)), (int)(uint32_t)e, j + lane < n);
     }
   };
-
-  // Two vectors a turn, those of the next one on their way, and before them the edges; the first turn gives a bound to go by.
+  // Two vectors a turn, those of the next one on their way, and before them the edges.
   const int first = v0 + wave * MOE_WAVE;
   auto load = [&](int i) __attribute__((always_inline)) { return xv[min(i, max(v1, 1) - 1)]; };
   uint4 now[2], next[2];
@@ -318,14 +326,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     reference(edge_value);
     add(edge_value);
   }
-  int turn = 0, renewal = 2;
-  bool full = false;  // more candidates than there is room for
+  // a batch's vectors, of turns from `turn0` on
+  auto offer_batch = [&](int turn0, int turns) __attribute__((always_inline)) {
+    float2 most[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) most[b] = lds.most[b][threadIdx.x];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = first + lane + (turn0 + b) * 2 * kThreads;
+      offer_vec(most[b].x, i, b < turns && i < v1);
+      offer_vec(most[b].y, i + kThreads, b < turns && i + kThreads < v1);
+    }
+  };
   const bool brief = v1 - v0 <= 2 * kThreads;  // all in the first turn's registers
+  const int turns = max((v1 - v0 + 2 * kThreads - 1) / (2 * kThreads), 1);
   float v[2][kVec], pm[2];
 #pragma unroll 1
-  for (int i0 = first; i0 < v1 || turn == 0; i0 += 2 * kThreads, ++turn) {
+  for (int turn = 0; turn < turns; ++turn) {
+    const int i0 = first + turn * 2 * kThreads;
     const int i = i0 + lane;
-    if (i0 + 2 * kThreads < v1) {
+    if (turn + 1 < turns) {
       next[0] = load(i + 2 * kThreads);
       next[1] = load(i + 3 * kThreads);
     }
@@ -348,24 +368,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       for (int e = 0; e < kVec; ++e) add(v[h][e]);
     if (TOP) {
       lane_max = fmaxf(lane_max, most);
-      if (brief) break;
-      if (turn == 0 || turn == renewal) {
+      if (!brief) lds.most[turn % kBatch][threadIdx.x] = make_float2(pm[0], pm[1]);
+      if (turn % kBatch == kBatch - 1 && turn + 1 < turns) {
         renew();
-        if (turn == 0) __syncthreads();
-        else renewal = 4 * renewal + 3;
+        if (turn < kBatch) __syncthreads();  // later the other waves' may be a batch old
         take_bound();
-      }
-      if (__any(!(most < least))) {
-        take_bound();  // the other waves may have renewed theirs
-        if (count > kBuf - 2 * MOE_WAVE) {
-          renew();
-          take_bound();
-          drop();
-          full |= count > kBuf - 2 * MOE_WAVE;
-          if (full) count = 0;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) offer_vec(pm[h], i + h * kThreads, i + h * kThreads < v1);
+        offer_batch(turn + 1 - kBatch, kBatch);
       }
     }
     now[0] = next[0];
@@ -381,7 +389,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   if (TOP && threadIdx.x == 0) lds.n_list = 0;
   if (TOP) renew();
   uint64_t* list = lds.list;
-  if (lane == 0) s_odd[wave] = full || !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar);
+  if (lane == 0) s_odd[wave] = !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar);
   __syncthreads();
   bool again = false;
 #pragma unroll
@@ -416,9 +424,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       }
     } else {
       drop();
+      offer_batch((turns - 1) / kBatch * kBatch, (turns - 1) % kBatch + 1);
+      if (full && lane == 0) atomicAdd(&lds.n_list, kList + 1);
 #pragma unroll 1
       for (int j = 0; j < count; j += MOE_WAVE) {  // their other values are read again
-        const int at = (int)(uint32_t)buf[min(j + lane, count - 1)];
+        const int at = (int)(uint32_t)cand[min(j + lane, count - 1)];
         unpack(xv[at], v[0]);
         keep(v[0], kVec, head + at * kVec, j + lane < count);
       }
@@ -443,7 +453,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       t = fmaf(e, fmaxf(d, kNoTerm), t);
     };
     term(edge_value);
-    Top top{buf, 0, 0};
+    Top top{lds.buf[wave], 0, 0};
     if (TOP) {
       if (threadIdx.x == 0) lds.n_list = 0;
       offer(top, edge_value, edge, lane < n_edge);
