@@ -35,6 +35,8 @@ constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 5.5f;  // 8 ln 2: what a value may be above the reference
 constexpr float kFar = 1 << 20;  // a reference up to here, times log2(e), is off by 2^-5 at most, which is undone exactly
+constexpr float kFarSlack = 300.f;  // log2 of what weighs nothing next to a maximum within kFar of zero
+constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kNoTerm = -200.f;  // log2 of a term that is zero in fp32, in the place of -inf times zero
 
 struct LpArgs {
@@ -268,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       const float old = m2;
       const bool first = m == -INFINITY;
       m = wave_max_uniform(fmaxf(m, pm));
-      m2 = m * kLog2e;
+      m2 = fmaxf(m * kLog2e, -kFar);  // values below leave nothing
       asm("" : "+v"(m2));  // rounded: as an operand of a fused difference it would not be what the terms were formed with
       limit = m + kSlack;
       if (!first) {  // before the first value that is not -inf the sums are 0, or NaN
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     uint32_t b = ~0u;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
-    least = from_ordered(__builtin_amdgcn_readfirstlane(b));
+    least = fmaxf(from_ordered(__builtin_amdgcn_readfirstlane(b)), kLowest);  // -inf: only where there is nothing else
   };
   auto offer_vec = [&](float most, int index, bool valid) __attribute__((always_inline)) {
     const bool pass = valid && !(most < least);
@@ -384,16 +386,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   s = wave_sum_uniform(s);
   t = wave_sum_uniform(t);
   Sums sum{m, s * undo, fmaf(-off, s, t) * undo};
+  if (m * kLog2e < -kFar) sum.s = sum.t = 0.f;  // to another wave's maximum, or the row is gone over again
 
   if (lane == 0) s_max[wave] = m;
   if (TOP && threadIdx.x == 0) lds.n_list = 0;
   if (TOP) renew();
   uint64_t* list = lds.list;
-  if (lane == 0) s_odd[wave] = !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY) || !(fabsf(m2) < kFar);
+  if (lane == 0) s_odd[wave] = !(fabsf(s) < INFINITY) || !(fabsf(t) < INFINITY);
   __syncthreads();
   bool again = false;
+  m = s_max[0];
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) again |= s_odd[w] != 0;
+  for (int w = 0; w < kWaves; ++w) {
+    again |= s_odd[w] != 0;
+    m = fmaxf(m, s_max[w]);
+  }
+  again |= m != -INFINITY && !(fabsf(m * kLog2e) < kFar - kFarSlack);
   if (TOP && !again) {
     take_bound();
     // The values that reach the bound go to the list, a wave asking once for places; value e is index + e.
@@ -435,16 +443,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     }
     keep(&edge_value, 1, edge, lane < n_edge);
     __syncthreads();
-    again |= lds.n_list > kList;
+    const int found = lds.n_list;
+    again |= found > kList;
+    if (!again && found < a.k) {  // all others are -inf: the first of them
+      __syncthreads();
+      if (wave == 0) {
+        const int i = (split == 0 ? 0 : head + v0 * kVec) + lane, end = split == a.splits - 1 ? a.V : head + v1 * kVec;
+        const bool more = lane < a.k && i < end && value_at(x, min(i, a.V - 1)) == -INFINITY;
+        const uint64_t mask = __ballot(more);
+        if (more) list[found + __popcll(mask & lanemask_lt())] = key_of(-INFINITY, i);
+        if (lane == 0) lds.n_list = found + __popcll(mask);
+      }
+    }
   }
 
   // NaN, +inf, a reference so far out that its product with log2(e) is rounded by much, more candidates than there is
   // room for (values that rise along the row, or nearly all equal): again, from the maximum and value by value.
   if (again) {
     __syncthreads();  // the counts are read
-    m = s_max[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_max[w]);
     s = t = 0.f;
     const float ref = m == -INFINITY ? 0.f : m;
     auto term = [&](float v) __attribute__((always_inline)) {
@@ -458,18 +474,27 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       if (threadIdx.x == 0) lds.n_list = 0;
       offer(top, edge_value, edge, lane < n_edge);
     }
+    if (first < v1) now[0] = load(first + lane);
     for (int i0 = first; i0 < v1; i0 += kThreads) {
-      const int j = i0 + lane;
+      const int j = i0 + lane, index = head + j * kVec;
+      unpack(now[0], v[0]);
+      now[0] = load(j + kThreads);
+      // whether a value may be among the largest; later ones lose against equal earlier ones
+      const float bound_value = value_of(top.least);
+      bool maybe = top.least == 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        term(j < v1 ? v[0][e] : -INFINITY);
+        maybe |= !(v[0][e] <= bound_value) || (v[0][e] == bound_value && index < index_of(top.least));
+      }
+      if (!TOP || !__any(maybe && j < v1)) continue;
 #pragma unroll 1
       for (int e = 0; e < kVec; ++e) {
-        const float v = j < v1 ? value_at(x, head + (long)j * kVec + e) : -INFINITY;
-        term(v);
-        if (TOP) {
-          offer(top, v, head + j * kVec + e, j < v1);
-          if (top.count > (i0 + kThreads < v1 || e + 1 < kVec ? kBuf - MOE_WAVE : kKeep)) cut(top, a.k, lane);
-        }
+        offer(top, j < v1 ? value_at(x, index + e) : 0.f, index + e, j < v1);
+        if (top.count > kBuf - MOE_WAVE) cut(top, a.k, lane);
       }
     }
+    if (TOP && top.count > kKeep) cut(top, a.k, lane);
     sum = Sums{m, wave_sum_uniform(s), wave_sum_uniform(t)};
     if (TOP) {
       __syncthreads();  // the list is empty

@@ -255,3 +255,38 @@ def test_a_row_of_2_27(pkg, dev):
     assert r.logprobs[0] == r.top_logprobs[0, 0]
     dist = (24 * torch.ones((), device=dev) - (ln_z - entropy)).abs().double()
     assert (r.entropy[0].double() - entropy).abs() <= z * (1 + 2 * (dist + 11)) + 2.0 ** -23 * entropy.abs()
+
+
+@pytest.mark.parametrize("mask", [-INF, -1e9, -3.3895313892515355e38])
+@pytest.mark.parametrize("T,V,k", [(1, 151936, 20), (40, 20001, 5), (900, 9000, 64)])
+def test_masked_rows(pkg, dev, T, V, k, mask):
+    """A mask that leaves 3, k - 1, k or many tokens, at the row's start, its end or anywhere; among equals the first ones."""
+    g = torch.Generator().manual_seed(T)
+    x = torch.full((8, V), mask)
+    for i, n in enumerate((3, k - 1, k, 1000)):
+        places = torch.randperm(V, generator=g)[:n]
+        x[i, places] = torch.randn(n, generator=g) * 3
+        at = n if i % 2 else V - n
+        x[4 + i, at - n if i % 2 else at:at if i % 2 else V] = torch.randn(n, generator=g) * 3
+    x = x.to(torch.bfloat16).to(dev)
+    tokens = torch.stack([row.argmax() for row in x])
+    few = check(pkg, x[:min(T, 8)].contiguous(), tokens[:min(T, 8)], k)
+    check(pkg, x[:2].float().contiguous(), None, k)
+    if T > 8:
+        many = pkg.token_logprobs(x.repeat((T + 7) // 8, 1)[:T].contiguous(), None, k)
+        for i in range(8):
+            assert torch.equal(many.top_ids[i::8], few.top_ids[i:i + 1].expand(many.top_ids[i::8].shape))
+
+
+def test_rows_far_below_zero(pkg, dev):
+    """Maxima on both sides of where a reference times log2(e) is no longer held closely, and parts of a row far below the rest."""
+    V = 9001
+    g = torch.Generator().manual_seed(3)
+    near = torch.randn(V, generator=g)
+    at = torch.arange(V)
+    rows = [near - 726817 + off for off in (-400, -200, -3, 0, 3, 200, 400)]
+    rows += [torch.where(at // 512 % 4 == 1, near, near - 1e6), torch.where(at < V // 2, near - 5e8, near),
+             torch.where(at % 2 == 0, near - 726600, near - 726900), torch.where(at == V - 1, 0.0, near - 3e38)]
+    x = torch.stack(rows).to(dev)
+    check(pkg, x, tokens_of(dev, len(rows), V), 9)
+    check(pkg, x.repeat(80, 1), tokens_of(dev, 80 * len(rows), V), 9)
