@@ -7,17 +7,21 @@
 // of the about nine issue slots that a value costs).  A wave keeps a reference near its maximum instead of the
 // maximum: the sums are scaled only where a value passes it by 2^8, which after the first values happens rarely.
 //
-// The largest are found on the way.  Each lane's running maximum gives a bound: where j lanes of each of the four waves
-// have seen a value of at least b, with 4 j >= k, the k largest are all >= b.  The bound is renewed at growing
-// distances.  Of a 16-byte vector with a value that passes it the maximum and the place are kept in LDS; those that pass
-// the bound at the end are read again, and their values that do sorted by counting.
+// The largest are found on the way.  The maxima of the 16-byte vectors are kept in LDS and looked through a batch of turns at a
+// time, the last batch at the end.  Each lane's running maximum gives a bound: where j lanes of each of the four waves have
+// seen a value of at least b, with 4 j >= k, the k largest are all >= b.  Vectors that reach it are candidates; those that
+// do so at the end are read again, and their values that reach it sorted by counting.  What only equals the bound (the value that
+// a mask has left nearly everywhere, say) is taken up to the k-th in the order of the row; -inf not at all, for where fewer
+// than k values are above it the first of the rest are at the row's start.
 //
-// Few rows are split over workgroups, whose sums and lists a second kernel joins.  Rows with NaN or +inf, with a maximum
-// of a size past 7 * 10^5 (the type's lowest everywhere, say) or with more candidates than there is room for (values
-// that rise along the row, or nearly all equal) are gone over again by a plainer scan.
+// Few rows are split over workgroups, whose sums and lists a second kernel joins.  Rows with NaN or +inf, whose maximum is
+// of a size past 7 * 10^5 (the type's lowest everywhere, say) or with more candidates than there is room for (values that rise
+// along the row) are gone over again by a plainer scan.
 //
-// (151936 bf16 values a row, in a graph: one row with 5 alternatives 9.0 us, 64 with 20 17.5; 6000 rows without 315, 5.8
-// TB/s.  777 fp32 rows of 50257 with 8 38.6, 4.05 TB/s: all start and end together, with nothing to load at either end.)
+// (151936 bf16 values a row, in a graph: one row with 5 alternatives 9.4 us, 64 with 20 16.9; 6000 rows without 315, 5.8
+// TB/s.  777 fp32 rows of 50257 with 8 38.6, 4.05 TB/s: all start and end together, with nothing to load at either end.  777
+// bf16 rows with 5 alternatives, the same logits again and again: 56 us, and with all but 10 tokens masked by -inf 57, by
+// -10^9 73; before equals and far parts were told apart, 289 and 282.)
 #include "common.h"
 
 namespace {
@@ -29,6 +33,7 @@ constexpr int kBatch = 8;      // turns whose vectors' maxima are looked through
 constexpr int kCand = 192;     // vectors that a wave keeps as candidates
 constexpr int kBuf = 512;      // values that it does in the plain scan
 constexpr int kKeep = 128;     // ... after they are cut down, at most
+constexpr int kFewFound = 24;  // values found at a time that are taken without a look for those that only equal the bound
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
 constexpr int kMaxSplits = 64;
 
@@ -155,7 +160,7 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
     const uint32_t mid = lo + step / 2;
     if (mid > lo && reached(mid)) lo = mid;
   }
-  return lo;
+  return ~wave_max_u32_uniform(mine >= lo ? ~mine : 0);  // the least of them, so that what only equals it is known as such
 }
 
 struct TopLds {
@@ -258,10 +263,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const int edge = lane < n_head ? lane : tail0 + lane - n_head;
   const int per_wave = (a.k + kWaves - 1) / kWaves;
 
+  const int first = v0 + wave * MOE_WAVE;
   // candidates: vectors, as {bits of the maximum, index}
   uint64_t* cand = lds.cand[wave];
   int count = 0;
-  bool full = false;  // more of them than there is room for
+  bool full = false;   // more of them than there is room for
+  bool stale = false;  // of which some the bound may have passed
   uint32_t bound = 0;                          // that the wave's lanes give
   float lane_max = -INFINITY, least = -INFINITY;  // values below `least` are not among the k largest
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
@@ -294,12 +301,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
     least = fmaxf(from_ordered(__builtin_amdgcn_readfirstlane(b)), kLowest);  // -inf: only where there is nothing else
+    stale = true;
   };
-  auto offer_vec = [&](float most, int index, bool valid) __attribute__((always_inline)) {
-    const bool pass = valid && !(most < least);
-    const uint64_t mask = __ballot(pass);
-    if (mask == 0) return;
-    if (count > kCand - MOE_WAVE) full = true, count = 0;
+  // Candidates come in the order of the row: behind k of them a vector that only equals the bound has none of the largest.
+  // That is looked at where there are many (the bound is what a mask has left, say).
+  auto push = [&](float most, int index, bool pass, bool many) __attribute__((always_inline)) {
+    uint64_t mask = __ballot(pass);
+    if (many) {
+      pass = pass && (most != least || count + __popcll(mask & lanemask_lt()) < a.k);
+      mask = __ballot(pass);
+    }
     if (pass) cand[count + __popcll(mask & lanemask_lt())] = (uint64_t)__float_as_uint(most) << 32 | (uint32_t)index;
     count += __popcll(mask);
   };
@@ -309,11 +320,32 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 #pragma unroll 1
     for (int j = 0; j < n; j += MOE_WAVE) {
       const uint64_t e = cand[min(j + lane, n - 1)];
-      offer_vec(__uint_as_float((uint32_t)(e >> 32)), (int)(uint32_t)e, j + lane < n);
+      const float most = __uint_as_float((uint32_t)(e >> 32));
+      push(most, (int)(uint32_t)e, j + lane < n && !(most < least), true);
+    }
+    stale = false;
+  };
+  // a batch's vectors, of turns from `turn0` on
+  auto offer_batch = [&](int turn0, int turns) __attribute__((always_inline)) {
+    float2 most[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) most[b] = lds.most[b][threadIdx.x];
+#pragma unroll
+    for (int b = 0; b < 2 * kBatch; ++b) {
+      const int index = first + lane + (2 * turn0 + b) * kThreads;
+      const float value = b % 2 ? most[b / 2].y : most[b / 2].x;
+      const bool pass = b / 2 < turns && index < v1 && !(value < least);
+      const int n = __popcll(__ballot(pass));
+      if (n == 0) continue;
+      bool many = count + n > kCand / 2;
+      if (many) {
+        if (stale) drop();
+        if (count > kCand - MOE_WAVE) full = true, count = 0;
+      }
+      push(value, index, pass, many);
     }
   };
   // Two vectors a turn, those of the next one on their way, and before them the edges.
-  const int first = v0 + wave * MOE_WAVE;
   auto load = [&](int i) __attribute__((always_inline)) { return xv[min(i, max(v1, 1) - 1)]; };
   uint4 now[2], next[2];
   if (vecs > 0) {
@@ -328,18 +360,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     reference(edge_value);
     add(edge_value);
   }
-  // a batch's vectors, of turns from `turn0` on
-  auto offer_batch = [&](int turn0, int turns) __attribute__((always_inline)) {
-    float2 most[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) most[b] = lds.most[b][threadIdx.x];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = first + lane + (turn0 + b) * 2 * kThreads;
-      offer_vec(most[b].x, i, b < turns && i < v1);
-      offer_vec(most[b].y, i + kThreads, b < turns && i + kThreads < v1);
-    }
-  };
   const bool brief = v1 - v0 <= 2 * kThreads;  // all in the first turn's registers
   const int turns = max((v1 - v0 + 2 * kThreads - 1) / (2 * kThreads), 1);
   float v[2][kVec], pm[2];
@@ -401,11 +421,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     again |= s_odd[w] != 0;
     m = fmaxf(m, s_max[w]);
   }
+  bool redo = again;  // the largest too
   again |= m != -INFINITY && !(fabsf(m * kLog2e) < kFar - kFarSlack);
-  if (TOP && !again) {
+  if (TOP && !redo) {
     take_bound();
-    // The values that reach the bound go to the list, a wave asking once for places; value e is index + e.
-    auto keep = [&](const float* v, int n, int index, bool valid) __attribute__((always_inline)) {
+    // The values that reach the bound go to the list, a wave asking once for places; value e is index + e, and `before` of them
+    // came earlier in the row: behind k of them none that only equals the bound.
+    auto keep = [&](const float* v, int n, int index, bool valid, int& before) __attribute__((always_inline)) {
       uint64_t mask[kVec];
       int found = 0;
 #pragma unroll
@@ -414,6 +436,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         found += __popcll(mask[e]);
       }
       if (found == 0) return;
+      if (found > kFewFound) {
+        int rank = before;
+#pragma unroll
+        for (int e = 0; e < n; ++e) rank += __popcll(mask[e] & lanemask_lt());
+        before += found;
+        found = 0;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          const bool reach = mask[e] >> lane & 1;
+          mask[e] = __ballot(reach && (v[e] != least || rank < a.k));
+          rank += reach;
+          found += __popcll(mask[e]);
+        }
+      } else {
+        before += found;
+      }
       int to = 0;
       if (lane == 0) to = atomicAdd(&lds.n_list, found);
       to = __builtin_amdgcn_readfirstlane(to);
@@ -424,11 +462,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         to += __popcll(mask[e]);
       }
     };
+    int before = 0, edges = 0;
     if (brief) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = first + lane + h * kThreads;
-        keep(v[h], kVec, head + at * kVec, at < v1);
+        keep(v[h], kVec, head + at * kVec, at < v1, before);
       }
     } else {
       drop();
@@ -438,14 +477,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       for (int j = 0; j < count; j += MOE_WAVE) {  // their other values are read again
         const int at = (int)(uint32_t)cand[min(j + lane, count - 1)];
         unpack(xv[at], v[0]);
-        keep(v[0], kVec, head + at * kVec, j + lane < count);
+        keep(v[0], kVec, head + at * kVec, j + lane < count, before);
       }
     }
-    keep(&edge_value, 1, edge, lane < n_edge);
+    keep(&edge_value, 1, edge, lane < n_edge, edges);
     __syncthreads();
     const int found = lds.n_list;
-    again |= found > kList;
-    if (!again && found < a.k) {  // all others are -inf: the first of them
+    redo = found > kList;
+    again |= redo;
+    if (!redo && found < a.k) {  // all others are -inf: the first of them
       __syncthreads();
       if (wave == 0) {
         const int i = (split == 0 ? 0 : head + v0 * kVec) + lane, end = split == a.splits - 1 ? a.V : head + v1 * kVec;
@@ -457,8 +497,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     }
   }
 
-  // NaN, +inf, a reference so far out that its product with log2(e) is rounded by much, more candidates than there is
-  // room for (values that rise along the row, or nearly all equal): again, from the maximum and value by value.
+  // NaN, +inf, a maximum so far out that its product with log2(e) is rounded by much, more candidates than there is
+  // room for (values that rise along the row): again, from the maximum and, for the largest, value by value.
   if (again) {
     __syncthreads();  // the counts are read
     s = t = 0.f;
@@ -470,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     };
     term(edge_value);
     Top top{lds.buf[wave], 0, 0};
-    if (TOP) {
+    if (TOP && redo) {
       if (threadIdx.x == 0) lds.n_list = 0;
       offer(top, edge_value, edge, lane < n_edge);
     }
@@ -487,16 +527,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         term(j < v1 ? v[0][e] : -INFINITY);
         maybe |= !(v[0][e] <= bound_value) || (v[0][e] == bound_value && index < index_of(top.least));
       }
-      if (!TOP || !__any(maybe && j < v1)) continue;
+      if (!TOP || !redo || !__any(maybe && j < v1)) continue;
 #pragma unroll 1
       for (int e = 0; e < kVec; ++e) {
         offer(top, j < v1 ? value_at(x, index + e) : 0.f, index + e, j < v1);
         if (top.count > kBuf - MOE_WAVE) cut(top, a.k, lane);
       }
     }
-    if (TOP && top.count > kKeep) cut(top, a.k, lane);
+    if (TOP && redo && top.count > kKeep) cut(top, a.k, lane);
     sum = Sums{m, wave_sum_uniform(s), wave_sum_uniform(t)};
-    if (TOP) {
+    if (TOP && redo) {
       __syncthreads();  // the list is empty
       for (int j = lane; j < top.count; j += MOE_WAVE) list[atomicAdd(&lds.n_list, 1)] = top.buf[j];
     }
@@ -556,10 +596,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   const Row r = row_of(join_wave(Sums{v.x, v.y, v.z}));
   if (a.k > 0) {
     __syncthreads();
-    const uint64_t least = (uint64_t)max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3])) << 32;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t key = i < kThreads ? first : keys[i];
-      if (key >= least && key != 0) list[atomicAdd(&s_count, 1)] = key;
+    const uint32_t least = max(max(s_bound[0], s_bound[1]), max(s_bound[2], s_bound[3]));
+    int equal = 0;  // keys of the wave that only equal the bound: of those the first k, which the splits' order is
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+      const int i = i0 + (int)threadIdx.x;
+      const uint64_t key = i0 == 0 ? first : i < n ? keys[i] : 0;
+      const uint32_t value = (uint32_t)(key >> 32);
+      const uint64_t mask = __ballot(key != 0 && value == least);
+      if (key != 0 && (value > least || (value == least && equal + __popcll(mask & lanemask_lt()) < a.k)))
+        list[atomicAdd(&s_count, 1)] = key;
+      equal += __popcll(mask);
     }
     __syncthreads();
     write_top(list, s_count, a.k, [&](int place, uint64_t key) __attribute__((always_inline)) {

@@ -290,3 +290,23 @@ def test_rows_far_below_zero(pkg, dev):
     x = torch.stack(rows).to(dev)
     check(pkg, x, tokens_of(dev, len(rows), V), 9)
     check(pkg, x.repeat(80, 1), tokens_of(dev, 80 * len(rows), V), 9)
+
+
+@pytest.mark.parametrize("T,V,k", [(1, 151936, 20), (3, 3000, 64), (40, 20001, 5), (900, 9000, 64)])
+def test_rows_of_few_values(pkg, dev, T, V, k):
+    """Among thousands of equals the first ones: all the same, of two or five values, the larger ones at the end alone, a step
+    down, runs along the row."""
+    g = torch.Generator().manual_seed(V)
+    at = torch.arange(V)
+    x = torch.stack([torch.zeros(V), torch.randint(0, 2, (V,), generator=g).float(), torch.randint(-2, 3, (V,), generator=g).float(),
+                     (at > V - k // 2 - 2).float(), (at < V // 3).float(), (at // 777 % 3).float(),
+                     torch.where(at // 512 % 4 == 2, 1.0, 0.0), torch.where(torch.rand(V, generator=g) < 2 * k / V, 1.0, 0.0)])
+    x = x.to(torch.bfloat16).to(dev)
+    n = min(T, 8)
+    few = check(pkg, x[:n].contiguous(), tokens_of(dev, n, V), k)
+    check(pkg, x[-n:].float().contiguous(), None, k)
+    check(pkg, x[-n:].contiguous(), None, 1)
+    if T > 8:
+        many = pkg.token_logprobs(x.repeat((T + 7) // 8, 1)[:T].contiguous(), None, k)
+        for i in range(8):
+            assert torch.equal(many.top_ids[i::8], few.top_ids[i:i + 1].expand(many.top_ids[i::8].shape))
