@@ -29,7 +29,10 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / MOE_WAVE;
 constexpr int kMaxTop = 64;
 constexpr int kMaxV = 1 << 30;  // places in a row, and a little past it, are ints
-constexpr int kBatch = 8;      // turns whose vectors' maxima are looked through together
+constexpr int kPer = 2;        // vectors of a lane's turn (4: 777 fp32 rows level, one row with 5 alternatives 9.4 -> 10.0 us)
+constexpr int kTurn = kPer * kThreads;
+constexpr int kBatch = 16;     // vectors of a lane whose maxima are looked through together
+constexpr int kBatchTurns = kBatch / kPer;
 constexpr int kCand = 192;     // vectors that a wave keeps as candidates
 constexpr int kBuf = 512;      // values that it does in the plain scan
 constexpr int kKeep = 128;     // ... after they are cut down, at most
@@ -165,7 +168,7 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
 
 struct TopLds {
   union {
-    float2 most[kBatch][kThreads];  // maxima of a batch's vectors
+    float most[kBatchTurns][kThreads][kPer];  // maxima of a batch's vectors
     uint64_t buf[kWaves][kBuf];
   };
   uint64_t cand[kWaves][kCand];
@@ -327,14 +330,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   };
   // a batch's vectors, of turns from `turn0` on
   auto offer_batch = [&](int turn0, int turns) __attribute__((always_inline)) {
-    float2 most[kBatch];
+    typedef float Maxima __attribute__((ext_vector_type(kPer)));
+    Maxima most[kBatchTurns];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) most[b] = lds.most[b][threadIdx.x];
+    for (int b = 0; b < kBatchTurns; ++b) most[b] = *(const Maxima*)lds.most[b][threadIdx.x];
 #pragma unroll
-    for (int b = 0; b < 2 * kBatch; ++b) {
-      const int index = first + lane + (2 * turn0 + b) * kThreads;
-      const float value = b % 2 ? most[b / 2].y : most[b / 2].x;
-      const bool pass = b / 2 < turns && index < v1 && !(value < least);
+    for (int b = 0; b < kBatch; ++b) {
+      const int index = first + lane + (kPer * turn0 + b) * kThreads;
+      const float value = most[b / kPer][b % kPer];
+      const bool pass = b / kPer < turns && index < v1 && !(value < least);
       const int n = __popcll(__ballot(pass));
       if (n == 0) continue;
       bool many = count + n > kCand / 2;
@@ -345,12 +349,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       push(value, index, pass, many);
     }
   };
-  // Two vectors a turn, those of the next one on their way, and before them the edges.
+  // kPer vectors a turn, those of the next one on their way, and before them the edges.
   auto load = [&](int i) __attribute__((always_inline)) { return xv[min(i, max(v1, 1) - 1)]; };
-  uint4 now[2], next[2];
+  uint4 now[kPer], next[kPer];
   if (vecs > 0) {
-    now[0] = load(first + lane);
-    now[1] = load(first + kThreads + lane);
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) now[h] = load(first + h * kThreads + lane);
   }
   const float edge_value = lane < n_edge ? value_at(x, edge) : -INFINITY;
   Given given{};
@@ -360,19 +364,20 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     reference(edge_value);
     add(edge_value);
   }
-  const bool brief = v1 - v0 <= 2 * kThreads;  // all in the first turn's registers
-  const int turns = max((v1 - v0 + 2 * kThreads - 1) / (2 * kThreads), 1);
-  float v[2][kVec], pm[2];
+  const bool brief = v1 - v0 <= kTurn;  // all in the first turn's registers
+  const int turns = max((v1 - v0 + kTurn - 1) / kTurn, 1);
+  float v[kPer][kVec], pm[kPer];
 #pragma unroll 1
   for (int turn = 0; turn < turns; ++turn) {
-    const int i0 = first + turn * 2 * kThreads;
+    const int i0 = first + turn * kTurn;
     const int i = i0 + lane;
     if (turn + 1 < turns) {
-      next[0] = load(i + 2 * kThreads);
-      next[1] = load(i + 3 * kThreads);
-    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kPer; ++h) next[h] = load(i + kTurn + h * kThreads);
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
       unpack(now[h], v[h]);
       if (i0 + h * kThreads + MOE_WAVE > v1) {
 #pragma unroll
@@ -381,25 +386,30 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       pm[h] = v[h][0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) pm[h] = fmaxf(pm[h], v[h][e]);
+      most = fmaxf(most, pm[h]);
     }
-    const float most = fmaxf(pm[0], pm[1]);
     reference(most);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < kPer; ++h) {
+      if (i0 + h * kThreads >= v1) continue;  // nothing but -inf
 #pragma unroll
       for (int e = 0; e < kVec; ++e) add(v[h][e]);
+    }
     if (TOP) {
       lane_max = fmaxf(lane_max, most);
-      if (!brief) lds.most[turn % kBatch][threadIdx.x] = make_float2(pm[0], pm[1]);
-      if (turn % kBatch == kBatch - 1 && turn + 1 < turns) {
+      if (!brief) {
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) lds.most[turn % kBatchTurns][threadIdx.x][h] = pm[h];
+      }
+      if (turn % kBatchTurns == kBatchTurns - 1 && turn + 1 < turns) {
         renew();
-        if (turn < kBatch) __syncthreads();  // later the other waves' may be a batch old
+        if (turn < kBatchTurns) __syncthreads();  // later the other waves' may be a batch old
         take_bound();
-        offer_batch(turn + 1 - kBatch, kBatch);
+        offer_batch(turn + 1 - kBatchTurns, kBatchTurns);
       }
     }
-    now[0] = next[0];
-    now[1] = next[1];
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) now[h] = next[h];
   }
   // from the reference as the sums used it, m log2(e) rounded, to m itself; all lanes' is the same
   const float off = m == -INFINITY ? 0.f : fmaf(m, kLog2e, -m2), undo = __builtin_amdgcn_exp2f(-off);
@@ -465,13 +475,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     int before = 0, edges = 0;
     if (brief) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kPer; ++h) {
         const int at = first + lane + h * kThreads;
         keep(v[h], kVec, head + at * kVec, at < v1, before);
       }
     } else {
       drop();
-      offer_batch((turns - 1) / kBatch * kBatch, (turns - 1) % kBatch + 1);
+      offer_batch((turns - 1) / kBatchTurns * kBatchTurns, (turns - 1) % kBatchTurns + 1);
       if (full && lane == 0) atomicAdd(&lds.n_list, kList + 1);
 #pragma unroll 1
       for (int j = 0; j < count; j += MOE_WAVE) {  // their other values are read again
