@@ -18,7 +18,7 @@
 // of a size past 7 * 10^5 (the type's lowest everywhere, say) or with more candidates than there is room for (values that rise
 // along the row) are gone over again by a plainer scan.
 //
-// (151936 bf16 values a row, in a graph: one row with 5 alternatives 9.4 us, 64 with 20 16.9; 6000 rows without 315, 5.8
+// (151936 bf16 values a row, in a graph: one row with 5 alternatives 9.4 us, 64 with 20 16.5; 6000 rows without 315, 5.8
 // TB/s.  777 fp32 rows of 50257 with 8 38.6, 4.05 TB/s: all start and end together, with nothing to load at either end.  777
 // bf16 rows with 5 alternatives, the same logits again and again: 56 us, and with all but 10 tokens masked by -inf 57, by
 // -10^9 73; before equals and far parts were told apart, 289 and 282.)
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   finish(a, row, r, given);
 }
 
-// Joins a row's splits: their sums, and the k largest of their lists.  (3.4 us for one row's 38, 4.3 for 64 rows' 12.)
+// Joins a row's splits: their sums, and the k largest of their lists.  (3.6 us for one row's 38, 4.0 for 64 rows' 12.)
 template <typename E>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   __shared__ __attribute__((aligned(16))) uint64_t list[kMaxSplits * kMaxTop + 4];
