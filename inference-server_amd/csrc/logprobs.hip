@@ -36,7 +36,9 @@ constexpr int kBatchTurns = kBatch / kPer;
 constexpr int kCand = 192;     // vectors that a wave keeps as candidates
 constexpr int kBuf = 512;      // values that it does in the plain scan
 constexpr int kKeep = 128;     // ... after they are cut down, at most
-constexpr int kFewFound = 24;  // values found at a time that are taken without a look for those that only equal the bound
+constexpr int kFewCand = 48;   // candidates that are taken without a look for those that only equal the bound
+constexpr int kFewLanes = 12;  // lanes with values for the list that are taken without a look for those that only equal the bound
+constexpr int kBoundRows = kThreads / 16;
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
 constexpr int kMaxSplits = 64;
 
@@ -145,23 +147,40 @@ __device__ __forceinline__ void finish(const LpArgs& a, int row, const Row& r, c
   if (a.tokens) a.logprobs[row] = g.token < 0 ? 0.f : g.token < a.V ? logprob(r, g.x) : NAN;
 }
 
-// A bound that at least n of the wave's 64 values reach, close to the n-th largest: down from the largest by growing
-// steps, of 1/32 of a binade at first, then back by three halvings of the last one.
+template <int D>
+__device__ __forceinline__ float ror(float v) {
+  return __uint_as_float(row_ror<D>(__float_as_uint(v)));
+}
+// of the D next lanes of the 16 those with more
+template <int D>
+__device__ __forceinline__ void count_more(float mine, int& more) {
+  more += ror<D>(mine) > mine;
+  if constexpr (D > 1) count_more<D - 1>(mine, more);
+}
+
+// A bound that at least n of the wave's 64 values reach, close to the n-th largest: down from the largest by growing steps,
+// of 1/32 of a binade at first, then the last one in 16 parts.  Some thresholds at a time, for each is a wait of the scalar unit
+// for the vector unit and back.
 __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
   const uint32_t most = wave_max_u32_uniform(mine);
   auto reached = [&](uint32_t b) __attribute__((always_inline)) { return __popcll(__ballot(mine >= b)) >= n; };
-  uint32_t step = 1u << 18, lo = most, down = 0;
+  auto below = [&](uint32_t by) __attribute__((always_inline)) { return most > by ? most - by : 0; };  // 0 is reached by all
+  uint32_t lo = most, step = 1u << 18, from = 0, width = 0;
 #pragma unroll 1
-  while (!reached(lo)) {  // 0 is reached by all
-    down = down + step;
-    lo = most > down ? most - down : 0;
-    step *= 2;
+  while (!reached(lo)) {
+    const uint32_t a = below(from + step), b = below(from + 3 * step), c = below(from + 7 * step), d = below(from + 15 * step);
+    const bool ra = reached(a), rb = reached(b), rc = reached(c);
+    lo = ra ? a : rb ? b : rc ? c : d;
+    width = ra ? step : rb ? 2 * step : rc ? 4 * step : 8 * step;
+    from += 15 * step;
+    step *= 16;
   }
-#pragma unroll 1
-  for (int i = 0; i < 3 && down != 0; ++i) {
-    step = max(step / 2, 2u);
-    const uint32_t mid = lo + step / 2;
-    if (mid > lo && reached(mid)) lo = mid;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    width /= 4;
+    const uint32_t a = lo + width, b = a + width, c = b + width;
+    const bool ra = reached(a), rb = reached(b), rc = reached(c);
+    lo = rc ? c : rb ? b : ra ? a : lo;
   }
   return ~wave_max_u32_uniform(mine >= lo ? ~mine : 0);  // the least of them, so that what only equals it is known as such
 }
@@ -173,7 +192,7 @@ struct TopLds {
   };
   uint64_t cand[kWaves][kCand];
   uint64_t list[kList + 4];  // of all waves, at the end
-  uint32_t bound[kWaves];
+  float bound[kBoundRows];  // of 16 lanes each
   int n_list;
 };
 
@@ -264,7 +283,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   const int tail0 = head + vecs * kVec;
   const int n_head = split == 0 ? head : 0, n_edge = wave == 0 ? n_head + (split == a.splits - 1 ? a.V - tail0 : 0) : 0;
   const int edge = lane < n_head ? lane : tail0 + lane - n_head;
-  const int per_wave = (a.k + kWaves - 1) / kWaves;
+  // where `rows` of the workgroup's rows of 16 lanes have per_row values of at least b, there are k of them
+  const int per_row = (a.k + kBoundRows - 1) / kBoundRows, rows = (a.k + max(per_row, 1) - 1) / max(per_row, 1);
 
   const int first = v0 + wave * MOE_WAVE;
   // candidates: vectors, as {bits of the maximum, index}
@@ -272,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   int count = 0;
   bool full = false;   // more of them than there is room for
   bool stale = false;  // of which some the bound may have passed
-  uint32_t bound = 0;                          // that the wave's lanes give
+  bool ordered = true;
   float lane_max = -INFINITY, least = -INFINITY;  // values below `least` are not among the k largest
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
   auto reference = [&](float pm) __attribute__((always_inline)) {
@@ -295,25 +315,33 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     s += e;
     t = fmaf(e, fmaxf(d, kNoTerm), t);
   };
-  auto renew = [&]() __attribute__((always_inline)) {
-    bound = max(bound_of(ordered(lane_max), per_wave), bound);
-    if (lane == 0) ((volatile uint32_t*)lds.bound)[wave] = bound;
+  auto row_max = [&](float v) __attribute__((always_inline)) {
+    v = fmaxf(v, ror<1>(v));
+    v = fmaxf(v, ror<2>(v));
+    v = fmaxf(v, ror<4>(v));
+    return fmaxf(v, ror<8>(v));
   };
-  auto take_bound = [&]() __attribute__((always_inline)) {
-    uint32_t b = ~0u;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) b = min(b, ((volatile uint32_t*)lds.bound)[w]);
-    least = fmaxf(from_ordered(__builtin_amdgcn_readfirstlane(b)), kLowest);  // -inf: only where there is nothing else
+  auto renew = [&]() __attribute__((always_inline)) {
+    float rest = lane_max, best = row_max(rest);
+#pragma unroll 1
+    for (int i = 1; i < per_row; ++i) {
+      const uint32_t at = (uint32_t)(__ballot(rest == best) >> (lane & 48)) & 0xffffu;  // the row's lanes that have it
+      rest = 1u << (lane & 15) == (at & -at) ? -INFINITY : rest;
+      best = row_max(rest);
+    }
+    if (lane % 16 == 0) ((volatile float*)lds.bound)[wave * 4 + lane / 16] = best;
+  };
+  auto take_bound = [&]() __attribute__((always_inline)) {  // the rows' `rows`-th largest
+    const float mine = ((volatile float*)lds.bound)[lane % 16];
+    int more = 0;
+    count_more<15>(mine, more);
+    const float b = -row_max(more < rows ? -mine : -INFINITY);
+    least = fmaxf(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(b))), kLowest);  // -inf: only where there is nothing else
     stale = true;
   };
-  // Candidates come in the order of the row: behind k of them a vector that only equals the bound has none of the largest.
-  // That is looked at where there are many (the bound is what a mask has left, say).
-  auto push = [&](float most, int index, bool pass, bool many) __attribute__((always_inline)) {
-    uint64_t mask = __ballot(pass);
-    if (many) {
-      pass = pass && (most != least || count + __popcll(mask & lanemask_lt()) < a.k);
-      mask = __ballot(pass);
-    }
+  auto push = [&](float most, int index, bool pass) __attribute__((always_inline)) {
+    const uint64_t mask = __ballot(pass);
+    if (count > kCand - MOE_WAVE) full = true, count = 0;
     if (pass) cand[count + __popcll(mask & lanemask_lt())] = (uint64_t)__float_as_uint(most) << 32 | (uint32_t)index;
     count += __popcll(mask);
   };
@@ -324,29 +352,35 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     for (int j = 0; j < n; j += MOE_WAVE) {
       const uint64_t e = cand[min(j + lane, n - 1)];
       const float most = __uint_as_float((uint32_t)(e >> 32));
-      push(most, (int)(uint32_t)e, j + lane < n && !(most < least), true);
+      push(most, (int)(uint32_t)e, j + lane < n && !(most < least));
     }
     stale = false;
   };
-  // a batch's vectors, of turns from `turn0` on
+  // A batch's vectors, of turns from `turn0` on.  Few are taken a lane's at a time, many in the order of the row: then behind k
+  // candidates those that only equal the bound have none of the largest.
   auto offer_batch = [&](int turn0, int turns) __attribute__((always_inline)) {
-    typedef float Maxima __attribute__((ext_vector_type(kPer)));
-    Maxima most[kBatchTurns];
+    uint32_t mine = 0;
 #pragma unroll
-    for (int b = 0; b < kBatchTurns; ++b) most[b] = *(const Maxima*)lds.most[b][threadIdx.x];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int index = first + lane + (kPer * turn0 + b) * kThreads;
-      const float value = most[b / kPer][b % kPer];
-      const bool pass = b / kPer < turns && index < v1 && !(value < least);
-      const int n = __popcll(__ballot(pass));
-      if (n == 0) continue;
-      bool many = count + n > kCand / 2;
-      if (many) {
-        if (stale) drop();
-        if (count > kCand - MOE_WAVE) full = true, count = 0;
+    for (int b = 0; b < kBatch; ++b) mine |= lds.most[b / kPer][threadIdx.x][b % kPer] < least ? 0u : 1u << b;
+    mine &= (2u << (kPer * turns - 1)) - 1;
+    auto value = [&](int b) __attribute__((always_inline)) { return lds.most[b / kPer][threadIdx.x][b % kPer]; };
+    auto place = [&](int b) __attribute__((always_inline)) { return first + lane + (kPer * turn0 + b) * kThreads; };
+    if (count + __popcll(__ballot(mine != 0)) <= kFewCand) {
+#pragma unroll 1
+      while (__any(mine != 0)) {
+        const int b = __builtin_ctz(mine | 1u << 31) % kBatch;
+        push(value(b), place(b), mine != 0);
+        mine &= mine - 1;
+        ordered = false;
       }
-      push(value, index, pass, many);
+      return;
+    }
+    if (stale) drop();
+#pragma unroll 1
+    for (int b = 0; b < kPer * turns; ++b) {
+      const float most = value(b);
+      const uint64_t mask = __ballot(!(most < least));
+      push(most, place(b), !(most < least) && (most != least || count + __popcll(mask & lanemask_lt()) < a.k));
     }
   };
   // kPer vectors a turn, those of the next one on their way, and before them the edges.
@@ -435,41 +469,42 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   again |= m != -INFINITY && !(fabsf(m * kLog2e) < kFar - kFarSlack);
   if (TOP && !redo) {
     take_bound();
-    // The values that reach the bound go to the list, a wave asking once for places; value e is index + e, and `before` of them
-    // came earlier in the row: behind k of them none that only equals the bound.
+    // The values that reach the bound go to the list: value e is index + e, and `before` of them came earlier in the row; behind
+    // k of them none that only equals the bound, which is looked at where there are many.
     auto keep = [&](const float* v, int n, int index, bool valid, int& before) __attribute__((always_inline)) {
-      uint64_t mask[kVec];
-      int found = 0;
+      uint32_t reach = 0, over = 0;  // bit e: value e reaches the bound, passes it
 #pragma unroll
       for (int e = 0; e < n; ++e) {
-        mask[e] = __ballot(valid && !(v[e] < least));
-        found += __popcll(mask[e]);
+        reach |= v[e] < least ? 0u : 1u << e;
+        over |= v[e] > least ? 1u << e : 0u;
       }
-      if (found == 0) return;
-      if (found > kFewFound) {
+      reach = valid ? reach : 0u;
+      const int lanes = __popcll(__ballot(reach != 0));
+      if (lanes > kFewLanes && ordered) {
         int rank = before;
-#pragma unroll
-        for (int e = 0; e < n; ++e) rank += __popcll(mask[e] & lanemask_lt());
-        before += found;
-        found = 0;
-#pragma unroll
+#pragma unroll 1
+        for (int e = 0; e < n; ++e) rank += __popcll(__ballot(reach >> e & 1) & lanemask_lt());
+        const uint32_t all = reach;
+#pragma unroll 1
         for (int e = 0; e < n; ++e) {
-          const bool reach = mask[e] >> lane & 1;
-          mask[e] = __ballot(reach && (v[e] != least || rank < a.k));
-          rank += reach;
-          found += __popcll(mask[e]);
+          if (!(over >> e & 1) && rank >= a.k) reach &= ~(1u << e);
+          rank += all >> e & 1;
         }
-      } else {
-        before += found;
       }
-      int to = 0;
-      if (lane == 0) to = atomicAdd(&lds.n_list, found);
-      to = __builtin_amdgcn_readfirstlane(to);
+      before += lanes;
+#pragma unroll 1
+      for (;;) {
+        const uint64_t mask = __ballot(reach != 0);
+        if (mask == 0) break;
+        const int e = __builtin_ctz(reach | 1u << 31);
+        float value = v[0];
 #pragma unroll
-      for (int e = 0; e < n; ++e) {
-        const int at = to + __popcll(mask[e] & lanemask_lt());
-        if ((mask[e] >> lane & 1) && at < kList) list[at] = key_of(v[e], index + e);
-        to += __popcll(mask[e]);
+        for (int o = 1; o < n; ++o) value = e == o ? v[o] : value;
+        int to = 0;
+        if (lane == 0) to = atomicAdd(&lds.n_list, __popcll(mask));
+        to = __builtin_amdgcn_readfirstlane(to) + __popcll(mask & lanemask_lt());
+        if (reach != 0 && to < kList) list[to] = key_of(value, index + e);
+        reach &= reach - 1;
       }
     };
     int before = 0, edges = 0;
