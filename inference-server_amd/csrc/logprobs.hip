@@ -8,8 +8,8 @@
 // maximum: the sums are scaled only where a value passes it by 2^8, which after the first values happens rarely.
 //
 // The largest are found on the way.  The maxima of the 16-byte vectors are kept in LDS and looked through a batch of turns at a
-// time, the last batch at the end.  Each lane's running maximum gives a bound: where j lanes of each of the four waves have
-// seen a value of at least b, with 4 j >= k, the k largest are all >= b.  Vectors that reach it are candidates; those that
+// time, the last batch at the end.  The lanes' running maxima give a bound: where j of the lanes of each of c rows of 16 lanes have
+// seen a value of at least b, with c j >= k, the k largest are all >= b.  Vectors that reach it are candidates; those that
 // do so at the end are read again, and their values that reach it sorted by counting.  What only equals the bound (the value that
 // a mask has left nearly everywhere, say) is taken up to the k-th in the order of the row; -inf not at all, for where fewer
 // than k values are above it the first of the rest are at the row's start.
@@ -18,10 +18,10 @@
 // of a size past 7 * 10^5 (the type's lowest everywhere, say) or with more candidates than there is room for (values that rise
 // along the row) are gone over again by a plainer scan.
 //
-// (151936 bf16 values a row, in a graph: one row with 5 alternatives 9.4 us, 64 with 20 16.5; 6000 rows without 315, 5.8
-// TB/s.  777 fp32 rows of 50257 with 8 38.6, 4.05 TB/s: all start and end together, with nothing to load at either end.  777
-// bf16 rows with 5 alternatives, the same logits again and again: 56 us, and with all but 10 tokens masked by -inf 57, by
-// -10^9 73; before equals and far parts were told apart, 289 and 282.)
+// (151936 bf16 values a row, in a graph: one row with 5 alternatives 8.4 us, 64 with 20 15.4; 6000 rows without 317, 5.75
+// TB/s.  777 fp32 rows of 50257 with 8 36.3, 4.3 TB/s: all start and end together, with nothing to load at either end.  777
+// bf16 rows with 5 alternatives, the same logits again and again: 53 us, and with all but 10 tokens masked by -inf 53, by
+// -10^9 62; before equals and far parts were told apart, 289 and 282.)
 #include "common.h"
 
 namespace {
@@ -182,7 +182,7 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t mine, int n) {
     const bool ra = reached(a), rb = reached(b), rc = reached(c);
     lo = rc ? c : rb ? b : ra ? a : lo;
   }
-  return ~wave_max_u32_uniform(mine >= lo ? ~mine : 0);  // the least of them, so that what only equals it is known as such
+  return ~wave_max_u32_uniform(mine >= lo ? ~mine : 0);  // the least of them, so that what only equals it is known
 }
 
 struct TopLds {
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   int count = 0;
   bool full = false;   // more of them than there is room for
   bool stale = false;  // of which some the bound may have passed
-  bool ordered = true;
+  bool ordered = true;  // in the order of the row
   float lane_max = -INFINITY, least = -INFINITY;  // values below `least` are not among the k largest
   float m = -INFINITY, m2 = 0.f, limit = -INFINITY, s = 0.f, t = 0.f;
   auto reference = [&](float pm) __attribute__((always_inline)) {
