@@ -845,9 +845,10 @@ class LoraPool:
                    torch.zeros(num_adapters, dtype=torch.int32, device=device),
                    torch.zeros(num_adapters, dtype=torch.float32, device=device), columns)
 
+    @torch.no_grad()
     def load(self, index: int, parts, scale: float) -> None:
         """Adapter ``index`` from ``parts``: an ``(A [r, K], B [columns, r])`` for each part, of one rank r, or None for a
-        part that it leaves alone.  Copied, on the current stream."""
+        part that it leaves alone.  Values are copied, on the current stream; gradients do not pass."""
         if not 0 <= index < self.num_adapters:
             raise ValueError(f"index must be in [0, {self.num_adapters}), got {index}")
         if len(parts) != len(self.columns):

@@ -172,3 +172,27 @@ def test_add_refuses_an_x_that_it_would_change(lib, at, ys, xs, T):
     n = lib.moe_mi355x_lora_add_workspace_bytes(T, 4, 256, 16, 2, ints(64, 32))
     assert lib.moe_mi355x_lora_add(y, ys, y + 2 * at, xs, FAKE, FAKE, FAKE, FAKE, FAKE, T, 4, 256, 16, 2, ints(64, 32), FAKE, n,
                                    None) == -1
+
+
+# ---- loading adapters, over CPU tensors (a pool's own constructor takes GPU tensors alone) ----
+
+
+def pool_on_cpu(pkg, L, K, columns, R):
+    pool = object.__new__(pkg.LoraPool)
+    pool.a, pool.b = torch.zeros((L, len(columns) * R, K)), torch.zeros((L, sum(columns), R))
+    pool.ranks, pool.scales = torch.zeros(L, dtype=torch.int32), torch.zeros(L)
+    pool.columns, pool.in_features, pool.out_features, pool.max_rank, pool.num_adapters = columns, K, sum(columns), R, L
+    return pool
+
+
+def test_trained_weights_are_loaded_as_values(pkg):
+    """Parameters that take gradients leave none of their graph in the pool, whose own tensors may take them too."""
+    pool = pool_on_cpu(pkg, 2, 32, (32,), 16)
+    a, b = (torch.nn.Parameter(torch.randn(s)) for s in ((4, 32), (32, 4)))
+    pool.load(0, [(a, b)], 1.0)
+    assert not pool.a.requires_grad and not pool.b.requires_grad
+    pool.a, pool.b = pool.a.requires_grad_(), pool.b.requires_grad_()
+    pool.load(1, [(a, b)], 1.0)
+    assert pool.a.is_leaf and pool.b.is_leaf
+    for i in range(2):
+        assert torch.equal(pool.a[i, :4], a) and torch.equal(pool.b[i, :, :4], b)
