@@ -861,14 +861,15 @@ class LoraPool:
             if p is not None and (tuple(p[0].shape) != (rank, self.in_features) or tuple(p[1].shape) != (n, rank)):
                 raise ValueError(f"a part of rank {rank} must be [{rank}, {self.in_features}] and [{n}, {rank}], got "
                                  f"{tuple(p[0].shape)} and {tuple(p[1].shape)}")
-        self.a[index].zero_()
-        self.b[index].zero_()
-        at = 0
+        # put together apart: the parts may be views of the slot
+        a, b, at = torch.zeros_like(self.a[index]), torch.zeros_like(self.b[index]), 0
         for i, (p, n) in enumerate(zip(parts, self.columns)):
             if p is not None:
-                self.a[index, i * self.max_rank:i * self.max_rank + rank].copy_(p[0])
-                self.b[index, at:at + n, :rank].copy_(p[1])
+                a[i * self.max_rank:i * self.max_rank + rank].copy_(p[0])
+                b[at:at + n, :rank].copy_(p[1])
             at += n
+        self.a[index].copy_(a)
+        self.b[index].copy_(b)
         self.ranks[index] = rank
         self.scales[index] = float(scale)
 

@@ -196,3 +196,30 @@ def test_trained_weights_are_loaded_as_values(pkg):
     assert pool.a.is_leaf and pool.b.is_leaf
     for i in range(2):
         assert torch.equal(pool.a[i, :4], a) and torch.equal(pool.b[i, :, :4], b)
+
+
+def test_an_adapter_is_loaded_from_the_pool_itself(pkg):
+    """From its own slot with another scale, its parts changed over, cut to a lower rank; and from another slot."""
+    pool = pool_on_cpu(pkg, 2, 32, (32, 32), 16)
+    parts = [(torch.randn(4, 32), torch.randn(32, 4)) for _ in range(2)]
+
+    def held(slot, r):
+        return [(pool.a[slot, 16 * p:16 * p + r], pool.b[slot, 32 * p:32 * p + 32, :r]) for p in range(2)]
+
+    def check(slot, want):
+        for p, (a, b) in enumerate(want):
+            r = len(a)
+            mine_a, mine_b = pool.a[slot, 16 * p:16 * p + 16], pool.b[slot, 32 * p:32 * p + 32]
+            assert torch.equal(mine_a[:r], a) and torch.equal(mine_b[:, :r], b)
+            assert not mine_a[r:].any() and not mine_b[:, r:].any()
+
+    pool.load(0, parts, 1.0)
+    pool.load(0, held(0, 4), 0.5)
+    check(0, parts)
+    pool.load(0, held(0, 4)[::-1], 0.5)
+    check(0, parts[::-1])
+    pool.load(1, held(0, 4), 2.0)
+    check(1, parts[::-1])
+    pool.load(0, held(0, 3), 1.0)
+    check(0, [(a[:3], b[:, :3]) for a, b in parts[::-1]])
+    assert pool.ranks.tolist() == [3, 4] and pool.scales.tolist() == [1.0, 2.0]
