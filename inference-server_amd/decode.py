@@ -168,6 +168,15 @@ class LayerAdapters:
     def qkv_columns(cfg: DecoderConfig) -> tuple[int, int, int]:
         return cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
 
+    def check(self, cfg: DecoderConfig) -> None:
+        """Raises where a pool is not of this projection of ``cfg``: with the columns in another order or in other parts, of the
+        same sum, what one part's adapters add would go to another's."""
+        for name, pool, want in (("qkv", self.qkv, (cfg.hidden, self.qkv_columns(cfg))),
+                                 ("o", self.o, (cfg.heads * cfg.head_dim, (cfg.hidden,)))):
+            if isinstance(pool, kernels.LoraPool) and (pool.in_features, pool.columns) != want:  # others: lora_add's to refuse
+                raise ValueError(f"{name} pool: needs {want[0]} features to parts of {want[1]} columns, has {pool.in_features} "
+                                 f"to {pool.columns}")
+
     @classmethod
     def empty(cls, cfg: DecoderConfig, num_adapters: int, max_rank: int, device) -> LayerAdapters:
         """Pools without adapters, to ``LoraPool.load`` into."""
@@ -187,6 +196,8 @@ def attention_sublayer(w: DecoderLayerWeights, h, positions, context_lens, block
     token's k, v to the cache (modeling_qwen3_moe.py:329-340 with :151-191).  The residual add
     of :341 is left to the caller (the MoE sublayer forms it)."""
     cfg = w.cfg
+    if lora is not None:
+        adapters.check(cfg)
     B = h.shape[0]
     x = kernels.rms_norm(h, w.ln1, cfg.rms_eps)
     qkv = _project(x, w.wqkv, adapters.qkv, lora)
@@ -200,6 +211,8 @@ def attention_sublayer_fp8(w: DecoderLayerWeights, h, plan: kernels.PagedPlan, i
                            v_scale, adapters: LayerAdapters = LayerAdapters(), lora: kernels.LoraPlan | None = None):
     """``attention_sublayer`` over the 8-bit cache, for the rows of a plan: prompts and single tokens."""
     cfg = w.cfg
+    if lora is not None:
+        adapters.check(cfg)
     x = kernels.rms_norm(h, w.ln1, cfg.rms_eps)
     cache = (k_cache, v_cache, k_scale, v_scale)
     q = kernels.qk_norm_rope_append_fp8(_project(x, w.wqkv, adapters.qkv, lora), w.q_norm, w.k_norm, inv_freq, cfg.heads,
@@ -250,6 +263,11 @@ class DecodeModel:
                 raise ValueError(f"adapters must be one LayerAdapters for each of the {len(layers)} layers, with pools of one "
                                  "number of adapters")
             self.num_adapters = pools[0].num_adapters
+            for a, w in zip(adapters, layers):
+                a.check(cfg)
+                for name, p in (("qkv", a.qkv), ("o", a.o)):
+                    if isinstance(p, kernels.LoraPool) and p.device != w.wqkv.get_device():
+                        raise ValueError(f"{name} pool: must be on the layer's device, {w.wqkv.device}")
         dev = layers[0].wqkv.device
         self.inv_freq = default_inv_freq(cfg, dev)
         self._graph = None

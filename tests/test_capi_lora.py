@@ -223,3 +223,29 @@ def test_an_adapter_is_loaded_from_the_pool_itself(pkg):
     pool.load(0, held(0, 3), 1.0)
     check(0, [(a[:3], b[:, :3]) for a, b in parts[::-1]])
     assert pool.ranks.tolist() == [3, 4] and pool.scales.tolist() == [1.0, 2.0]
+
+
+def test_models_take_pools_of_their_own_projections(pkg, dec):
+    """Columns in another order or in other parts, of the same sum, would be added to other columns."""
+    cfg = dec.DecoderConfig(hidden=64, heads=2, kv_heads=1)
+    q, k, v = dec.LayerAdapters.qkv_columns(cfg)
+    layers = [SimpleNamespace(wqkv=torch.zeros(1), cfg=cfg)]
+
+    def pool(K, columns, device=-1):
+        p = pool_on_cpu(pkg, 2, K, columns, 16)
+        p.device = device
+        return p
+
+    def make(qkv=pool(64, (q, k, v)), o=pool(q, (64,))):
+        return dec.DecodeModel(cfg, layers, dec.PagedKVCache(1, 1, 1, "cpu"), [dec.LayerAdapters(qkv, o)])
+
+    make(), make(qkv=None), make(o=None)
+    for bad in ({"qkv": pool(64, (k, v, q))}, {"qkv": pool(64, (q + k + v,))}, {"qkv": pool(64, (q, k + v))},
+                {"qkv": pool(96, (q, k, v))}, {"qkv": pool(64, (q, k, v), device=0)}, {"o": pool(q, (32, 32))}, {"o": pool(64, (q,))},
+                {"o": pool(q, (64,), device=1)}):
+        with pytest.raises(ValueError, match="qkv|o "):
+            make(**bad)
+    wrong = dec.LayerAdapters(pool(64, (k, v, q)))
+    for sublayer, n in ((dec.attention_sublayer, 6), (dec.attention_sublayer_fp8, 6)):
+        with pytest.raises(ValueError, match="qkv"):
+            sublayer(layers[0], torch.zeros((1, 64)), *[None] * n, adapters=wrong, lora=object())
