@@ -419,14 +419,16 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 128;
 
-// 4 ranks' u as they enter the product
+// 4 ranks' u as they enter the product.  A finite one past bf16's largest value is that and a rest, not an infinity.
 __device__ __forceinline__ void split_u(v4f s, float scale, int live, uint2* hi, uint2* lo) {
+  constexpr float kMost = 0x1.fep127f;
   float v[4], rest[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    v[e] = e < live ? s[e] * scale : 0.f;
-    const float top = round_bf16(v[e]);
-    rest[e] = fabsf(top) < INFINITY ? v[e] - top : 0.f;  // not inf - inf
+    const float u = e < live ? s[e] * scale : 0.f;
+    const bool finite = fabsf(u) < INFINITY;
+    v[e] = finite ? __builtin_amdgcn_fmed3f(round_bf16(u), -kMost, kMost) : u;
+    rest[e] = finite ? u - v[e] : 0.f;  // not inf - inf
   }
   *hi = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
   *lo = make_uint2(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]));

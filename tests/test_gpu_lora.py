@@ -346,3 +346,22 @@ def test_an_x_that_it_would_change_is_refused(pkg, dev):
     for y, x in ((same, same), (wide[:8, :64], wide[:8, 56:120]), (wide[:8, :64], wide[1:, :64]), (wide[:8, 128:], wide[:8].flatten()[:512].view(8, 64))):
         with pytest.raises(Exception, match="invalid"):
             pkg.lora_add(y, x, c.pool, c.plan)
+
+
+@pytest.mark.parametrize("T,R", [(40, 16), (40, 64), (300, 16), (300, 64), (300, 128)])
+def test_a_finite_intermediate_past_bf16(pkg, dev, T, R):
+    """scale * A x = +-1.999 * 2^127: finite in fp32, past bf16's largest.  Against b of 0, 2^-20, and 1 the result is the formula's,
+    whose bf16 is no near tie (1.999 lies 2^-8.4 from the next one)."""
+    ids = [0] * (T - 7) + [1] * 7  # tiles of many rows and of few
+    c = Case(pkg, dev, T, 32, (96,), R, [R, 1], ids=ids)
+    c.x.zero_()
+    c.a.zero_()
+    c.b.zero_()
+    c.x[:, 0] = torch.where(torch.arange(T, device=dev) % 2 == 0, 2.0 ** 64, -(2.0 ** 64))
+    c.a[:, 0, 0] = 2.0 ** 63
+    c.scales.fill_(1.999)
+    c.b[:, 1::3, 0] = 2.0 ** -20
+    c.b[:, 2::3, 0] = 1.0
+    want = c.expected()[0].float().to(torch.bfloat16)
+    got = pkg.lora_add(c.y, c.x, c.pool, c.plan).cpu()
+    assert want[:, 2::3].isinf().all() and want[:, 1::3].isfinite().all() and torch.equal(got, want)
