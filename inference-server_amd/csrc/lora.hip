@@ -117,11 +117,13 @@ __device__ __forceinline__ void by_groups(int rank, F fn) {
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
 constexpr int kFewRows = kLoraPair;
 
-__device__ __forceinline__ float dot8(v4i a, v4i b, float c) {
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
   typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, a), __builtin_bit_cast(v2bf, b), c, false);
+}
+__device__ __forceinline__ float dot8(v4i a, v4i b, float c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, (int)a[i]), __builtin_bit_cast(v2bf, (int)b[i]), c, false);
+  for (int i = 0; i < 4; ++i) c = dot2((uint32_t)a[i], (uint32_t)b[i], c);
   return c;
 }
 
@@ -419,6 +421,16 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 128;
 
+// 8 values of B, infinite ones as zeros
+__device__ __forceinline__ v8bf finite8(v8bf b) {
+  const v4i w = __builtin_bit_cast(v4i, b);
+  v4i keep;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    keep[i] = ((w[i] & 0x7fff) == 0x7f80 ? 0 : w[i] & 0xffff) | ((w[i] & 0x7fff0000) == 0x7f800000 ? 0 : w[i] & (int)0xffff0000);
+  return __builtin_bit_cast(v8bf, keep);
+}
+
 // 4 ranks' u as they enter the product.  A finite one past bf16's largest value is that and a rest, not an infinity.
 __device__ __forceinline__ void split_u(v4f s, float scale, int live, uint2* hi, uint2* lo) {
   constexpr float kMost = 0x1.fep127f;
@@ -526,18 +538,26 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
         if (NG > 1) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][1], b, acc[j], 0, 0, 0);
       }
   };
-  auto store_y = [&](int c) __attribute__((always_inline)) {
+  auto store_y = [&](int c, auto check) __attribute__((always_inline)) {
+    Words out[4];
+    float odd = 0.f;  // NaN where something is not finite
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < kY; ++w) {
+        out[i][w] = pack2(acc[2 * w][i], acc[2 * w + 1][i]);
+        if (check) odd = dot2(out[i][w], 0, odd);
+      }
+    if (check && __any(odd != 0.f)) return false;
     if (c + mine < c1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        Words out;
-#pragma unroll
-        for (int w = 0; w < kY; ++w) out[w] = pack2(acc[2 * w][i], acc[2 * w + 1][i]);
-        if (row0 + 4 * lg + i < t.n) *(Words*)(yr[i] + c + mine) = out;
-      }
+      for (int i = 0; i < 4; ++i)
+        if (row0 + 4 * lg + i < t.n) *(Words*)(yr[i] + c + mine) = out[i];
+    return true;
   };
   // The last piece apart, so that no branch lies around a load, and y's stores behind B's: a wait for a load waits for
   // every store in front of it.
+  uint32_t left = 0;  // pieces that were not stored
   int c = c0;
   for (; c + kPiece < c1; c += kPiece) {
     begin();
@@ -546,12 +566,32 @@ __device__ __forceinline__ void expand(const LoraArgs& a, const Tile& t, uint16_
     multiply();
     __syncthreads();  // B's columns are read
     store_b();
-    store_y(c);
+    left |= store_y(c, std::true_type()) ? 0u : 1u << (c - c0) / kPiece;
     __syncthreads();
   }
   begin();
   multiply();
-  store_y(c);
+  left |= store_y(c, std::true_type()) ? 0u : 1u << (c - c0) / kPiece;
+  // An infinite value of B makes NaN of lo's zeros, and of a lo of the other sign than hi.  Pieces with something that is not
+  // finite once more, hi with B and lo with what is finite of it, from memory: each wave for itself.
+  while (__builtin_expect(left != 0, 0)) {
+    c = c0 + kPiece * __builtin_ctz(left);
+    left &= left - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) yv[i] = *(const Words*)(yr[i] + min(c + mine, c1 - J));
+    begin();
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int g = 0; g < kSteps; ++g) {
+        const int r = NG == 1 ? 8 * (lg & 1) : 32 * g + 8 * lg;
+        const uint4 w = mask8(*(const uint4*)(bl + (long)min(c + mine + j, c1 - 1) * a.R + (r < t.rank ? r : 0)), t.rank - r);
+        const v8bf b = __builtin_bit_cast(v8bf, w), rest = finite8(b);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][0], NG == 1 && lg >= 2 ? rest : b, acc[j], 0, 0, 0);
+        if (NG > 1) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[g][1], rest, acc[j], 0, 0, 0);
+      }
+    store_y(c, std::false_type());
+  }
 }
 
 template <int RG>
@@ -592,6 +632,7 @@ constexpr long kFewAdapter = 1 << 17, kFewRead = 160L << 32;
 constexpr int kFewGroups = 1024;
 // Many rows: at least two workgroups a CU, by shares of K and by shorter runs of columns.
 constexpr int kManyGroups = 512, kShareK = 512, kManyRun = 512;
+static_assert(kManyRun / kPiece <= 32);  // bits of `left`
 
 struct LoraForm {
   bool few;

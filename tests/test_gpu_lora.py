@@ -365,3 +365,44 @@ def test_a_finite_intermediate_past_bf16(pkg, dev, T, R):
     want = c.expected()[0].float().to(torch.bfloat16)
     got = pkg.lora_add(c.y, c.x, c.pool, c.plan).cpu()
     assert want[:, 2::3].isinf().all() and want[:, 1::3].isfinite().all() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T", [40, 300, 1500])
+@pytest.mark.parametrize("R,ranks", [(16, [16, 3]), (32, [20, 32]), (64, [64, 17]), (128, [128, 70])])
+def test_infinities_in_b(pkg, dev, T, R, ranks):
+    """An infinite value of B makes infinities of its column alone, of the sign of A x, whatever the size of the step; two of
+    different signs, and one against a zero, NaN."""
+    c = Case(pkg, dev, T, 128, QKV, R, ranks, seed=R, ids=[0] * (T - 9) + [1] * 8 + [-1])
+    INF = float("inf")
+    c.b[0, 5, 1], c.b[0, 300, 12], c.b[0, 517, 0] = INF, -INF, INF
+    c.b[0, 77, 0], c.b[0, 77, 2] = INF, INF
+    c.b[1, 6, 2], c.b[1, 767, 0] = -INF, INF
+    c.x[4] = 0
+    c.y[3, 9], c.y[T - 2, 5], c.y[3, 11] = INF, float("nan"), -INF
+    before = c.y.clone()
+    want, size = c.expected()
+    got = pkg.lora_add(c.y, c.x, c.pool, c.plan).double().cpu()
+    odd = ~want.isfinite()
+    # per row of the first adapter 4 columns, of the second 2; 3 values of y
+    assert odd.sum() == (T - 9) * 4 + 8 * 2 + 3
+    assert torch.equal(got[odd].nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
+    tol = 2.0 ** -8 * want.abs() + (c.K + 2 * R + 2) * 2.0 ** -24 * (size + before.double().cpu().abs()) + 2.0 ** -17 * size
+    assert ((got - want).abs() <= tol)[~odd].all()
+    assert torch.equal(got[-1], before[-1].double().cpu())
+
+
+@pytest.mark.parametrize("R", [16, 64, 128])
+def test_infinities_in_some_pieces_of_a_run(pkg, dev, R):
+    """Runs of 512 columns of a long step, some of whose pieces of 128 hold an infinity; tiles of many rows and of few."""
+    T = 4200
+    c = Case(pkg, dev, T, 128, (4096, 544), R, [R, 7], seed=R, ids=[0] * (T - 9) + [1] * 9)
+    INF = float("inf")
+    for n, r, v in ((200, 0, INF), (511, 3, -INF), (4095, 6, INF), (4096 + 130, 2, INF), (4096 + 543, 1, -INF)):
+        c.b[:, n, r] = v
+    before = c.y.double().cpu()
+    want, size = c.expected()
+    got = pkg.lora_add(c.y, c.x, c.pool, c.plan).double().cpu()
+    odd = ~want.isfinite()
+    assert odd.sum() == T * 5 and torch.equal(got[odd].nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
+    tol = 2.0 ** -8 * want.abs() + (c.K + 2 * R + 2) * 2.0 ** -24 * (size + before.abs()) + 2.0 ** -17 * size
+    assert ((got - want).abs() <= tol)[~odd].all()
