@@ -406,3 +406,37 @@ def test_infinities_in_some_pieces_of_a_run(pkg, dev, R):
     assert odd.sum() == T * 5 and torch.equal(got[odd].nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
     tol = 2.0 ** -8 * want.abs() + (c.K + 2 * R + 2) * 2.0 ** -24 * (size + before.abs()) + 2.0 ** -17 * size
     assert ((got - want).abs() <= tol)[~odd].all()
+
+
+def form_of(pkg, T, L, K, columns, R):
+    """Few rows or many: the form of few rows needs no workspace."""
+    import ctypes
+
+    n = pkg._lib.load().moe_mi355x_lora_add_workspace_bytes(T, L, K, R, len(columns), (ctypes.c_int * len(columns))(*columns))
+    return "many" if n else "few"
+
+
+@pytest.mark.parametrize("R", [16, 32, 64, 128])
+@pytest.mark.parametrize("paired", [False, True])
+def test_few_rows_over_long_runs_of_columns(pkg, dev, R, paired):
+    """Runs of 2048 columns, in which a wave has four turns of 64, and a part's last run of fewer; tiles of one row and of two."""
+    T, K, columns = 128, 128, (8192, 544, 32)
+    ranks = [R, 1, R - 1, 9] * 25
+    ids = [t // 2 if paired else t for t in range(T)]
+    ids = [i if i < 100 else 99 - i % 100 for i in ids]
+    assert form_of(pkg, T, len(ranks), K, columns, R) == "few"
+    Case(pkg, dev, T, K, columns, R, ranks, seed=R, ids=ids).run(pkg)
+    Case(pkg, dev, T, K, columns, R, ranks, seed=R + 1, ids=ids, x_pad=8, y_pad=24, poison=True).run(pkg)
+
+
+@pytest.mark.parametrize("R,ranks", [(16, [16, 5]), (32, [32, 17]), (64, [64, 33]), (64, [30, 16]), (128, [128, 65]), (128, [64, 20])])
+def test_many_rows_over_long_runs_of_columns(pkg, dev, R, ranks):
+    """Runs of 512 columns in four pieces of 128, and a part's last run of fewer; tiles of many rows and of up to 16."""
+    T, K, columns = 4100, 256, (4096, 544, 32)
+    L = 40
+    ranks = (ranks * L)[:L]
+    ids = [0] * 2000 + [1] * 1613 + [2 + t // 13 for t in range(494 - 13)]  # the narrow ones of 13 rows
+    ids = np.asarray((ids + [-1] * T)[:T])
+    assert form_of(pkg, T, L, K, columns, R) == "many"
+    Case(pkg, dev, T, K, columns, R, ranks, seed=R, ids=ids).run(pkg)
+    Case(pkg, dev, T, K, columns, R, ranks, seed=R + 1, ids=np.random.default_rng(R).permutation(ids), x_pad=8, y_pad=24, poison=True).run(pkg)
