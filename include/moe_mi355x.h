@@ -380,7 +380,7 @@ int moe_mi355x_lora_plan(const int32_t* adapter_ids, const int32_t* cu_rows, int
 /*
  * What the rows' adapters add to a shared projection, in place: for row t with adapter l, column n in part p of the
  * projection (the q, k and v of a fused one are its parts; columns[p] columns each), r < min(ranks[l], R):
- *   u = sum_k x[t, k] a[l, p R + r, k]      y[t, n] = bf16( y[t, n] + scales[l] sum_r u[t, p, r] b[l, n, r] )
+ *   u = scales[l] sum_k x[t, k] a[l, p R + r, k]      y[t, n] = bf16( y[t, n] + sum_r u[t, p, r] b[l, n, r] )
  * with fp32 sums, u kept to 2^-17 of its value, one rounding.  Rows without an adapter, and with one of rank 0 or less,
  * are left as they are; what a and b hold past an adapter's rank reaches nothing.
  *   y bf16 [T, N], N = sum of columns, and x bf16 [T, K]; rows y_stride and x_stride values apart (multiples of 8)

@@ -4,7 +4,7 @@
 // and the k largest by (value, lower index first) with their logprobs.
 //
 // One pass over the logits, bound by their bytes and, for bf16, nearly by the vector unit (an exponential takes four
-// of the about nine issue slots that a value costs).  A wave keeps a reference near its maximum instead of the
+// of the nine and a half issue slots that a value costs).  A wave keeps a reference near its maximum instead of the
 // maximum: the sums are scaled only where a value passes it by 2^8, which after the first values happens rarely.
 //
 // The largest are found on the way.  The maxima of the 16-byte vectors are kept in LDS and looked through a batch of turns at a
@@ -20,8 +20,8 @@
 //
 // (151936 bf16 values a row, in a graph: one row with 5 alternatives 8.4 us, 64 with 20 15.4; 6000 rows without 317, 5.75
 // TB/s.  777 fp32 rows of 50257 with 8 36.3, 4.3 TB/s: all start and end together, with nothing to load at either end.  777
-// bf16 rows with 5 alternatives, the same logits again and again: 53 us, and with all but 10 tokens masked by -inf 53, by
-// -10^9 62; before equals and far parts were told apart, 289 and 282.)
+// bf16 rows with 5 alternatives: 59 us, 4.0 TB/s, and with all but 10 tokens masked by -inf 58.5, by -10^9 67; before equals and far
+// parts were told apart, 289 and 282, on the same logits again and again.)
 #include "common.h"
 
 namespace {
@@ -33,11 +33,13 @@ constexpr int kPer = 2;        // vectors of a lane's turn (4: 777 fp32 rows lev
 constexpr int kTurn = kPer * kThreads;
 constexpr int kBatch = 16;     // vectors of a lane whose maxima are looked through together
 constexpr int kBatchTurns = kBatch / kPer;
-constexpr int kCand = 192;     // vectors that a wave keeps as candidates
+constexpr int kCand = 192;     // vectors that a wave keeps as candidates (128 or 256: 777 rows with 5 alternatives 1% more)
 constexpr int kBuf = 512;      // values that it does in the plain scan
 constexpr int kKeep = 128;     // ... after they are cut down, at most
-constexpr int kFewCand = 48;   // candidates that are taken without a look for those that only equal the bound
-constexpr int kFewLanes = 12;  // lanes with values for the list that are taken without a look for those that only equal the bound
+// Candidates that are taken without a look for those that only equal the bound.  (16: 64 rows with 20 alternatives 15.7 -> 16.8 us,
+// 256 rows 25.5 -> 27.6; 96: level, but 777 rows masked by -10^9 67 -> 161.)
+constexpr int kFewCand = 48;
+constexpr int kFewLanes = 12;  // lanes with values for the list that are (4 or 32: level, the masked rows 67 -> 68)
 constexpr int kBoundRows = kThreads / 16;
 constexpr int kList = kWaves * kKeep;  // ... and a workgroup at the end
 constexpr int kMaxSplits = 64;
@@ -664,9 +666,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
 bool lp_ok(int T, int V, int k) { return T >= 0 && T < (1 << 24) && V >= 1 && V <= kMaxV && k >= 0 && k <= kMaxTop && k <= V; }
 
 // Workgroups of a row: for three workgroups a CU in all, each with 4096 values at least.  (us in a graph, for 512 / 768 /
-// 1024 / 1280 workgroups, 151936 bf16 values a row: 64 rows with 20 alternatives 15.9 / 16.0 / 16.6 / 16.1, 256 rows 32.1 /
-// 29.4 / 27.9 / 28.0, 777 rows without alternatives 43.6 / 43.5 / 46.1 / 46.1; 777 fp32 rows of 50257 with 8 32.1 / 33.2 / 37.5 /
-// 37.6.  The same logits again and again, so partly from the cache behind L2.)
+// 1024 / 1280 workgroups, 151936 bf16 values a row: 64 rows with 20 alternatives 15.0 / 15.7 / 16.6 / 16.5, 256 rows 27.7 /
+// 25.5 / 26.1 / 25.5, 777 rows without alternatives 50 / 50 / 53 / 53, with 5 59 / 59 / 67 / 67; 777 fp32 rows of 50257 with 8 36.3 /
+// 36.3 / 48 / 48.  Three sets of logits in turn, those of 256 rows and fewer partly from the cache behind L2.)
 constexpr int kGroups = 768, kMinValues = 4096;
 int lp_splits(int T, int V) {
   const int most = (V + kMinValues - 1) / kMinValues, want = (kGroups + T - 1) / (T > 0 ? T : 1);

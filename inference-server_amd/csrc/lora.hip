@@ -1,10 +1,10 @@
 // What the adapters of a step's rows add to a shared projection: for row t with adapter l, column n in part p of the
 // projection (q, k and v are parts of one), r < rank_l,
-//   u[t, p, r] = sum_k x[t, k] A_l[p R + r, k]          y[t, n] = bf16( y[t, n] + scale_l sum_r u[t, p, r] B_l[n, r] )
+//   u[t, p, r] = scale_l sum_k x[t, k] A_l[p R + r, k]          y[t, n] = bf16( y[t, n] + sum_r u[t, p, r] B_l[n, r] )
 // with fp32 sums and one rounding, of y.  Bound by bytes: x, y and the adapters in use once each.  Consecutive lanes read
 // consecutive bytes everywhere, MFMA operands go through LDS, and no branch lies around a load, for the compiler waits
 // where it joins.  (4642 rows beside q/k/v, 2048 to 5120, ranks up to 64: 49 us with operands straight from memory, a lane a
-// row; 45 through LDS; 39 without the branches, 33 now: 117 MB at 3.5 TB/s, u's launch 12 us and the columns' 20.5.)
+// row; 45 through LDS; 39 without the branches, 33.5 now: 117 MB at 3.5 TB/s, u's launch 12 us and the columns' 20.8.)
 //
 // Two forms over the plan's tiles (rows of one adapter, lora.h):
 //   few rows (tiles of 2): one launch, a workgroup per (tile, run of columns), which forms the u of its part by
@@ -27,7 +27,7 @@ struct LoraArgs {
   const int32_t* ranks;   // [L]
   const float* scales;    // [L]
   const int32_t* plan;
-  float* u;               // [shares][T][P][R], rows in the plan's order
+  float* u;               // before the scale; [shares][T][P][R], rows in the plan's order
   LoraLayout p;
   int K, R, N, parts, shares, chunk, runs;  // chunk: columns of a workgroup, in one part; runs: of them in all parts
   int col[kMaxParts + 1];             // where the parts begin
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kThreads) void lora_shrink_kernel(LoraArgs a) {
 // ---------------------------------------------------------------------------
 // many rows: columns.  A wave has 16 of the 64 rows, all of them 128 columns of B at a time, through LDS.  Lane l has 8
 // columns in a row, from 8 (l % 16), of rows 4 (l / 16) + i: column 8 (l % 16) + j is column l % 16 of product j,
-// and B's columns lie in LDS in that order.  (4642 rows, 2048 to 5120, ranks up to 64: 20.5 us, y read and written at 4.6 TB/s.)
+// and B's columns lie in LDS in that order.  (4642 rows, 2048 to 5120, ranks up to 64: 20.8 us, y read and written at 4.6 TB/s.)
 // ---------------------------------------------------------------------------
 constexpr int kPiece = 128;
 
@@ -622,13 +622,19 @@ bool lora_ok(int T, int L, int K, int R, int parts) {
 
 // How a call is cut up.
 // Few rows: every run of columns of each pair of rows reads the part's A for itself, which one CU takes 1.2 us for 64 KB
-// to do, so this pays where rank times K is small, and for the fewer rows the larger it is.  (us in a graph, few / many rows'
-// form, "rows/adapters".  2048 to q/k/v 5120, rank 16: 1/1 3.7 / 5.4, 32/32 5.0 / 7.4, 128/64 9.4 / 11.7, 256/64 13.9 /
-// 12.1; rank 32: 1/1 4.4 / 6.2, 64/64 10.6 / 13.5, 128/64 13.9 / 15.0, 256/64 20.7 / 16.0; rank 64: 1/1 7.3 / 7.7, 8/8 9.4 /
-// 8.3, 32/32 11.3 / 12.6, 48/48 16.0 / 13.7, 128/64 23.5 / 20.7.  4096 to 2048, rank 64: 1/1 7.8 / 6.7, 32/32 12.6 / 10.7.)
+// to do, so this pays where rank times K is small, and for the fewer rows the larger it is.  By the pool's rank: what its
+// adapters' are is known on the GPU alone.  (us in a graph, few / many rows' form, "rows/adapters", as many rows for each adapter, of the
+// pool's rank.  2048 to q/k/v 5120, rank 16: 1/1 3.8 / 5.6, 32/32 5.5 / 9.1, 128/64 8.5 / 11.9, 256/64 12.0 / 12.2; rank 32: 1/1
+// 4.4 / 6.4, 64/64 11.8 / 15.7, 128/64 12.3 / 15.9, 192/64 17.6 / 16.0; rank 64: 1/1 7.1 / 7.8, 8/8 8.0 / 8.4, 32/32 13.8 / 13.9, 48/48
+// 15.3 / 18.5, 64/64 22.5 / 22.5, 192/64 30.8 / 23.5; rank 128: 1/1 11.5 / 10.0, 16/16 14.5 / 16.2, 32/32 30.2 / 25.5.  4096 to 9216,
+// rank 16: 128/64 13.1 / 17.6, 192/64 20.5 / 18.0.  4096 to 2048, rank 64: 1/1 7.8 / 6.9, 32/32 11.1 / 11.5, 64/64 12.7 / 15.1,
+// 256/64 24.4 / 15.6.  8192 to 4096, rank 16: 32/32 7.2 / 10.0, 64/64 10.6 / 12.9, 192/64 15.3 / 13.3.)
+// The rule sees neither the runs of columns nor how many rows share an adapter, and in between it gives up some us: it takes the
+// form of many rows for 48/48 of rank 64 and 16/16 of rank 128 beside q/k/v, and for 48/48 to 64/64 of the last two projections.
 constexpr long kFewAdapter = 1 << 17, kFewRead = 160L << 32;
 // Runs of 512 columns at least, 64 for each wave, and more where that makes more workgroups than this: each forms u again.
-// (128 rows of 100 adapters, 4096 to q/k/v 9216: 17.2 us for 512, 13.7 for 1024, 15.6 for 2048.)
+// (128 rows of 100 adapters, 4096 to q/k/v 9216, for 512, 1024, 2048 and 4096 workgroups, which are runs of 4096 to 512 columns: 16.8,
+// 13.4, 15.4 and 19.3 us.)
 constexpr int kFewGroups = 1024;
 // Many rows: at least two workgroups a CU, by shares of K and by shorter runs of columns.
 constexpr int kManyGroups = 512, kShareK = 512, kManyRun = 512;

@@ -973,9 +973,10 @@ def _rows_apart(t: torch.Tensor, name: str, rows: int, columns: int, device: int
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, pool: LoraPool, plan: LoraPlan) -> torch.Tensor:
     """Adds to ``y``, the shared projection of ``x``, in place what each row's adapter contributes:
-    ``y[t] += scale_l * B_l (A_l x[t])``, part by part.  Prompts and single tokens of any number of requests in
+    ``y[t] += B_l (scale_l * (A_l x[t]))``, part by part.  Prompts and single tokens of any number of requests in
     one call; rows without an adapter are left as they are.  ``y`` bf16 [T, N], ``x`` bf16 [T, K] (rows may lie
-    apart, but x and y share no value); returns ``y``.  fp32 sums, one rounding of the result; ``A x`` is kept to 2^-17 of its value."""
+    apart, but x and y share no value); returns ``y``.  fp32 sums, one rounding of the result; ``scale * A x`` is kept to
+    2^-17 of its value."""
     if not isinstance(pool, LoraPool) or not isinstance(plan, LoraPlan):
         raise TypeError("pool must be a LoraPool and plan a LoraPlan (lora_plan)")
     if pool.num_adapters != plan.num_adapters:
