@@ -638,6 +638,7 @@ constexpr long kFewAdapter = 1 << 17, kFewRead = 160L << 32;
 constexpr int kFewGroups = 1024;
 // Many rows: at least two workgroups a CU, by shares of K and by shorter runs of columns.
 constexpr int kManyGroups = 512, kShareK = 512, kManyRun = 512;
+static_assert(kManyRun / kPiece <= 32, "a bit for each piece of a run");
 static_assert(kManyRun / kPiece <= 32);  // bits of `left`
 
 struct LoraForm {

@@ -395,7 +395,7 @@ def test_infinities_in_b(pkg, dev, T, R, ranks):
 def test_infinities_in_some_pieces_of_a_run(pkg, dev, R):
     """Runs of 512 columns of a long step, some of whose pieces of 128 hold an infinity; tiles of many rows and of few."""
     T = 4200
-    c = Case(pkg, dev, T, 128, (4096, 544), R, [R, 7], seed=R, ids=[0] * (T - 9) + [1] * 9)
+    c = Case(pkg, dev, T, 128, (4096, 544), R, [R, 7], seed=R, ids=[0] * (T - 9) + [1] * 9, poison=True)
     INF = float("inf")
     for n, r, v in ((200, 0, INF), (511, 3, -INF), (4095, 6, INF), (4096 + 130, 2, INF), (4096 + 543, 1, -INF)):
         c.b[:, n, r] = v
